@@ -58,6 +58,7 @@ extern "C" {
 #define MOE_ERR_TIMEOUT_GRID 0x106
 #define MOE_ERR_BAD_EXPERT 0x201
 #define MOE_ERR_BAD_ROW 0x202
+#define MOE_ERR_BAD_CODE 0x203
 
 /* Rows per M-tile of the grouped GEMMs (the C9 BLOCK_M), and the taller
  * tile of the 2-CTA cluster-pair GEMMs that large batches use (ABI 2). */
@@ -349,6 +350,106 @@ MOE_API int moe_last_cuda_error(void);
  */
 MOE_API int moe_add_rmsnorm(const void* x, const void* delta, const float* weight, int T, int H,
                             float eps, void* h_out, void* y, cudaStream_t stream);
+
+/*
+ * The norms around a decoder block that norms its output too, with the gate
+ * and the residual scale between them (the block of C8/python/solution.py:
+ * 318-325 with a norm behind each sub-block):
+ *   n = delta * rsqrt(mean(delta^2) + eps) * post_weight
+ *   h_out = x + residual_scale * act(gate) * n
+ *   y = h * rsqrt(mean(h^2) + eps) * pre_weight    (of h before its rounding)
+ * in one pass over the rows; x, delta, h_out, y bf16 [T, H] (h_out may be x,
+ * y may be delta), weights fp32 [H], H % 8 == 0, H <= 32768.  gate: none, one
+ * per token [T], per channel [H] or per element [T, H], bf16 or fp32
+ * (gate_f32), through the identity, the sigmoid or tanh.
+ */
+#define MOE_GATE_NONE 0
+#define MOE_GATE_TOKEN 1
+#define MOE_GATE_CHANNEL 2
+#define MOE_GATE_ELEMENT 3
+#define MOE_GATE_ACT_NONE 0
+#define MOE_GATE_ACT_SIGMOID 1
+#define MOE_GATE_ACT_TANH 2
+MOE_API int moe_block_norm(const void* x, const void* delta, const float* post_weight,
+                           const float* pre_weight, const void* gate, int gate_kind, int gate_f32,
+                           int gate_act, float residual_scale, int T, int H, float eps,
+                           void* h_out, void* y, cudaStream_t stream);
+
+/*
+ * Expert weights in 4 bits.  Every row of a projection is cut into groups of
+ * `group` (32, 64 or 128) columns with a bf16 scale and, optionally, a zero
+ * point each:  w[n, c] = s[n, c/group] * (q[n, c] - z[n, c/group]), q and z in
+ * 0..15, z = 8 throughout where zero points are absent.
+ *
+ * moe_w4_pack lays one projection out for the kernels (once, when the weights
+ * are loaded): codes uint8 [E, N, K] (one code per byte), scales bf16
+ * [E, N, K/group], zeros uint8 [E, N, K/group] or NULL.  With a second matrix
+ * (codes1, scales1, zeros1) the two are interleaved by eight rows: the packed
+ * gate (0) and up (1) projections.  q takes E*M*K/2 bytes, s E*M*(K/group)*2
+ * and z E*M*(K/group), M = N, or 2N for two matrices.  A code or zero point
+ * above 15 records MOE_ERR_BAD_CODE and is taken modulo 16.  K % 64 == 0,
+ * K % group == 0, K <= 8192; N % 16 == 0 (N % 8 for two matrices); all
+ * pointers to codes and packed data 16-byte aligned.
+ *
+ * moe_w4_bank: a layer's packed projections (host struct, read during the
+ * call): w13 gate and up [E, I, H], w2 down [E, H, I].
+ */
+typedef struct moe_w4_bank {
+  const void* w13_q;
+  const void* w13_s;
+  const void* w13_z; /* NULL without zero points (then w2_z too) */
+  const void* w2_q;
+  const void* w2_s;
+  const void* w2_z;
+  int32_t E, H, I, group;
+} moe_w4_bank;
+MOE_API int moe_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros0,
+                        const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E,
+                        int N, int K, int group, void* q, void* s, void* z, int32_t* status,
+                        cudaStream_t stream);
+
+/*
+ * moe_grouped_w13_swiglu_gather and moe_grouped_w2 on a 4-bit bank: the same
+ * tile tables (of either height), row index (NULL: row r itself), row map and
+ * slot scale.  H % 64 == 0, I % 64 == 0, both <= 8192 and multiples of the
+ * group; E <= 1024.
+ */
+MOE_API int moe_grouped_w13_swiglu_w4(const void* src, int src_rows, const int32_t* index,
+                                      int index_div, int M, const int32_t* tiles,
+                                      const int32_t* num_tiles, int max_tiles,
+                                      const moe_w4_bank* bank, void* h, int32_t* status,
+                                      cudaStream_t stream);
+MOE_API int moe_grouped_w2_w4(const void* h, int M, const int32_t* tiles,
+                              const int32_t* num_tiles, int max_tiles, const moe_w4_bank* bank,
+                              const int32_t* row_map, const float* slot_scale, void* out,
+                              int out_rows, int32_t* status, cudaStream_t stream);
+
+/*
+ * The 4-bit experts for routed tokens: y[n] = sum_j weights[n, j] *
+ * MLP_{ids[n, j]}(x[n]) over the experts the bank holds, which are
+ * [e_begin, e_begin + bank->E) of num_experts; records of other experts add
+ * nothing (a token without any gets a zero row).  ids int32 [T, k] in
+ * [0, num_experts), weights fp32 [T, k], 1 <= k <= 8.  Sort, both grouped
+ * products and the k-way sum; no host sync (C5/python/solution.py:131-160,
+ * C6/python/solution.py:137-176).
+ */
+MOE_API size_t moe_w4_experts_workspace_bytes(int T, int top_k, const moe_w4_bank* bank);
+MOE_API int moe_w4_experts_forward(const void* x, const int32_t* ids, const float* weights, int T,
+                                   int top_k, int num_experts, int e_begin,
+                                   const moe_w4_bank* bank, void* workspace,
+                                   size_t workspace_bytes, void* y, int32_t* status,
+                                   cudaStream_t stream);
+
+/*
+ * moe_layer_forward on a 4-bit bank that holds all E experts.  The router as
+ * in moe_router_topk (E % 16 == 0, 16 <= E <= 256).
+ */
+MOE_API size_t moe_w4_layer_workspace_bytes(int T, int top_k, const moe_w4_bank* bank);
+MOE_API int moe_w4_layer_forward(const void* x, const void* router_weight,
+                                 const float* router_bias, const moe_w4_bank* bank, int T,
+                                 int top_k, int norm_topk_prob, void* workspace,
+                                 size_t workspace_bytes, void* y, int32_t* status,
+                                 cudaStream_t stream);
 
 /*
  * Send plan of the all_to_all expert-parallel schedule (C7/python/solution.py:

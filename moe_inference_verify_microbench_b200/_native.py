@@ -94,7 +94,32 @@ SIGNATURES: dict[str, tuple] = {
     "moe_decode_layer_split": (_c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int,
                                         _c_int, _c_int, _c_int, _ptr, _c_size, _ptr, _ptr, _ptr]),
     "moe_last_cuda_error": (_c_int, []),
+    # norms around a block; 4-bit expert weights
+    "moe_block_norm": (_c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int,
+                                ctypes.c_float, _c_int, _c_int, ctypes.c_float, _ptr, _ptr,
+                                _ptr]),
+    "moe_w4_pack": (_c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int,
+                             _ptr, _ptr, _ptr, _ptr, _ptr]),
+    "moe_grouped_w13_swiglu_w4": (_c_int, [_ptr, _c_int, _ptr, _c_int, _c_int, _ptr, _ptr, _c_int,
+                                           _ptr, _ptr, _ptr, _ptr]),
+    "moe_grouped_w2_w4": (_c_int, [_ptr, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr, _ptr, _ptr,
+                                   _c_int, _ptr, _ptr]),
+    "moe_w4_experts_workspace_bytes": (_c_size, [_c_int, _c_int, _ptr]),
+    "moe_w4_experts_forward": (_c_int, [_ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr,
+                                        _ptr, _c_size, _ptr, _ptr, _ptr]),
+    "moe_w4_layer_workspace_bytes": (_c_size, [_c_int, _c_int, _ptr]),
+    "moe_w4_layer_forward": (_c_int, [_ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _ptr,
+                                      _c_size, _ptr, _ptr, _ptr]),
 }
+
+
+class W4BankStruct(ctypes.Structure):
+    """``moe_w4_bank`` of the header."""
+
+    _fields_ = [("w13_q", _ptr), ("w13_s", _ptr), ("w13_z", _ptr), ("w2_q", _ptr),
+                ("w2_s", _ptr), ("w2_z", _ptr), ("E", ctypes.c_int32), ("H", ctypes.c_int32),
+                ("I", ctypes.c_int32), ("group", ctypes.c_int32)]
+
 
 ABI_VERSION = 5
 

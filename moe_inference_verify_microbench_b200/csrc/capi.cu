@@ -87,6 +87,65 @@ size_t layer_layout(int T, int H, int I, int E, int k, int mode, void* ws, Body&
   return c.used;
 }
 
+W4Bank w4_bank(const moe_w4_bank& b) {
+  return {b.w13_q, b.w13_s, b.w13_z, b.w2_q, b.w2_s, b.w2_z, b.E, b.H, b.I, b.group};
+}
+
+// Buffers of one pass over the 4-bit experts; with `routed`, also the router's
+// ids and weights.
+struct W4Layout {
+  int* ids;
+  float* w;
+  void* sort_ws;
+  size_t sort_bytes;
+  int *counts, *offsets, *perm;
+  int4* tiles;
+  int max_tiles;
+  int* num_tiles;
+  void *h, *slots;
+  size_t bytes;
+};
+
+W4Layout w4_layout(void* ws, int T, int k, const W4Bank& b, bool routed) {
+  const long long R = static_cast<long long>(T) * k;
+  W4Layout l{};
+  Carver c(ws);
+  if (routed) {
+    l.ids = c.take<int>(R);
+    l.w = c.take<float>(R);
+  }
+  l.sort_bytes = sort_workspace_bytes(static_cast<int>(R), b.E);
+  l.sort_ws = c.take<uint8_t>(l.sort_bytes);
+  l.counts = c.take<int>(b.E);
+  l.offsets = c.take<int>(b.E + 1);
+  l.perm = c.take<int>(R);
+  l.max_tiles = max_tiles_bound(R, b.E, MOE_BLOCK_M);
+  l.tiles = c.take<int4>(l.max_tiles);
+  l.num_tiles = c.take<int>(1);
+  l.h = c.take<__nv_bfloat16>(R * b.I);
+  l.slots = c.take<__nv_bfloat16>(R * b.H);
+  l.bytes = c.used;
+  return l;
+}
+
+bool w4_count_ok(int T, int k) {
+  return static_cast<long long>(T) * k <= 0x7fffffffLL;
+}
+
+// The experts' products of sorted records and the weighted sum per token.
+int w4_products(const W4Bank& b, const W4Layout& l, const void* x, const int* ids, const float* w,
+                int T, int k, int e_begin, void* y, int* status, cudaStream_t stream) {
+  const int R = T * k;
+  int rc = launch_w4_w13(b, x, T, l.perm, k, R, l.tiles, l.num_tiles, l.max_tiles, l.h, status,
+                         stream);
+  if (rc != kRcOk) return rc;
+  rc = launch_w4_w2(b, l.h, R, l.tiles, l.num_tiles, l.max_tiles, l.perm, w, l.slots, R, status,
+                    stream);
+  if (rc != kRcOk) return rc;
+  return launch_combine(l.slots, R, nullptr, nullptr, ids, e_begin, e_begin + b.E, T, k, b.H, y,
+                        status, stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -109,6 +168,7 @@ const char* moe_error_string(int code) {
     case kErrTimeoutGrid: return "device: timed out in a grid-wide barrier of the single-launch decode layer";
     case kErrBadExpert: return "device: expert id out of range";
     case kErrBadRow: return "device: row index out of range";
+    case kErrBadCode: return "device: 4-bit weight code or zero point above 15";
     default: return "unknown code";
   }
 }
@@ -310,6 +370,32 @@ int moe_add_rmsnorm(const void* x, const void* delta, const float* weight, int T
   return launch_add_rmsnorm(x, delta, weight, T, H, eps, h_out, y, stream);
 }
 
+int moe_block_norm(const void* x, const void* delta, const float* post_weight,
+                   const float* pre_weight, const void* gate, int gate_kind, int gate_f32,
+                   int gate_act, float residual_scale, int T, int H, float eps, void* h_out,
+                   void* y, cudaStream_t stream) {
+  if (gate_kind < MOE_GATE_NONE || gate_kind > MOE_GATE_ELEMENT ||
+      (gate_kind != MOE_GATE_NONE && T > 0 && gate == nullptr))
+    return kRcBadArgument;
+  BlockNormArgs a{};
+  a.x = x;
+  a.delta = delta;
+  a.post = post_weight;
+  a.pre = pre_weight;
+  a.gate = gate_kind == MOE_GATE_NONE ? nullptr : gate;
+  a.gate_row = gate_kind == MOE_GATE_TOKEN ? 1 : gate_kind == MOE_GATE_ELEMENT ? H : 0;
+  a.gate_col = gate_kind == MOE_GATE_CHANNEL || gate_kind == MOE_GATE_ELEMENT ? 1 : 0;
+  a.gate_f32 = gate_f32 != 0;
+  a.act = gate_act;
+  a.T = T;
+  a.H = H;
+  a.eps = eps;
+  a.scale = residual_scale;
+  a.h = h_out;
+  a.y = y;
+  return launch_block_norm(a, stream);
+}
+
 int moe_cast_f32_to_bf16(const float* src, long long n, void* y, cudaStream_t stream) {
   return launch_cast_f32_bf16(src, n, y, stream);
 }
@@ -468,6 +554,105 @@ int moe_layer_forward_ex(const void* x, const void* router_weight, const float* 
                                        status, stream);
                });
   return rc;
+}
+
+int moe_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros0,
+                const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E, int N,
+                int K, int group, void* q, void* s, void* z, int32_t* status,
+                cudaStream_t stream) {
+  return launch_w4_pack(codes0, scales0, zeros0, codes1, scales1, zeros1, E, N, K, group, q, s, z,
+                        status, stream);
+}
+
+int moe_grouped_w13_swiglu_w4(const void* src, int src_rows, const int32_t* index, int index_div,
+                              int M, const int32_t* tiles, const int32_t* num_tiles,
+                              int max_tiles, const moe_w4_bank* bank, void* h, int32_t* status,
+                              cudaStream_t stream) {
+  if (bank == nullptr) return kRcBadArgument;
+  return launch_w4_w13(w4_bank(*bank), src, src_rows, index, index_div, M,
+                       reinterpret_cast<const int4*>(tiles), num_tiles, max_tiles, h, status,
+                       stream);
+}
+
+int moe_grouped_w2_w4(const void* h, int M, const int32_t* tiles, const int32_t* num_tiles,
+                      int max_tiles, const moe_w4_bank* bank, const int32_t* row_map,
+                      const float* slot_scale, void* out, int out_rows, int32_t* status,
+                      cudaStream_t stream) {
+  if (bank == nullptr) return kRcBadArgument;
+  return launch_w4_w2(w4_bank(*bank), h, M, reinterpret_cast<const int4*>(tiles), num_tiles,
+                      max_tiles, row_map, slot_scale, out, out_rows, status, stream);
+}
+
+size_t moe_w4_experts_workspace_bytes(int T, int top_k, const moe_w4_bank* bank) {
+  if (T < 0 || top_k <= 0 || bank == nullptr || bank->E <= 0 || bank->H <= 0 || bank->I <= 0 ||
+      !w4_count_ok(T, top_k))
+    return 0;
+  return w4_layout(nullptr, T, top_k, w4_bank(*bank), false).bytes;
+}
+
+int moe_w4_experts_forward(const void* x, const int32_t* ids, const float* weights, int T,
+                           int top_k, int num_experts, int e_begin, const moe_w4_bank* bank,
+                           void* workspace, size_t workspace_bytes, void* y, int32_t* status,
+                           cudaStream_t stream) {
+  if (bank == nullptr || T < 0 || top_k <= 0) return kRcBadArgument;
+  const W4Bank b = w4_bank(*bank);
+  int rc = w4_check_bank(b);
+  if (rc != kRcOk) return rc;
+  if (e_begin < 0 || num_experts <= 0 || b.E > num_experts - e_begin) return kRcBadArgument;
+  if (top_k > 8 || !w4_count_ok(T, top_k)) return kRcUnsupported;
+  if (T == 0) return kRcOk;
+  if (x == nullptr || ids == nullptr || weights == nullptr || y == nullptr ||
+      workspace == nullptr || (reinterpret_cast<uintptr_t>(y) & 15u) != 0 ||
+      (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+    return kRcBadArgument;
+  const W4Layout l = w4_layout(workspace, T, top_k, b, false);
+  if (workspace_bytes < l.bytes) return kRcWorkspace;
+  rc = launch_sort_align(ids, T * top_k, num_experts, e_begin, b.E, MOE_BLOCK_M, l.sort_ws,
+                         l.counts, l.offsets, nullptr, l.perm, nullptr, l.tiles, l.max_tiles,
+                         l.num_tiles, status, stream);
+  if (rc != kRcOk) return rc;
+  return w4_products(b, l, x, ids, weights, T, top_k, e_begin, y, status, stream);
+}
+
+size_t moe_w4_layer_workspace_bytes(int T, int top_k, const moe_w4_bank* bank) {
+  if (T < 0 || top_k <= 0 || bank == nullptr || bank->E <= 0 || bank->H <= 0 || bank->I <= 0 ||
+      !w4_count_ok(T, top_k))
+    return 0;
+  return w4_layout(nullptr, T, top_k, w4_bank(*bank), true).bytes;
+}
+
+int moe_w4_layer_forward(const void* x, const void* router_weight, const float* router_bias,
+                         const moe_w4_bank* bank, int T, int top_k, int norm_topk_prob,
+                         void* workspace, size_t workspace_bytes, void* y, int32_t* status,
+                         cudaStream_t stream) {
+  if (bank == nullptr || router_weight == nullptr || T < 0 || top_k <= 0) return kRcBadArgument;
+  const W4Bank b = w4_bank(*bank);
+  int rc = w4_check_bank(b);
+  if (rc != kRcOk) return rc;
+  if (top_k > b.E) return kRcBadArgument;
+  if (top_k > 8 || !w4_count_ok(T, top_k)) return kRcUnsupported;
+  if (T == 0) return kRcOk;
+  if (x == nullptr || y == nullptr || workspace == nullptr ||
+      (reinterpret_cast<uintptr_t>(y) & 15u) != 0 ||
+      (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+    return kRcBadArgument;
+  const W4Layout l = w4_layout(workspace, T, top_k, b, true);
+  if (workspace_bytes < l.bytes) return kRcWorkspace;
+  if (use_router_small(T, b.H, b.E, top_k)) {
+    rc = launch_router_sort_small(x, router_weight, router_bias, T, b.H, b.E, top_k,
+                                  norm_topk_prob, l.ids, l.w, nullptr, l.counts, l.offsets, l.perm,
+                                  l.tiles, l.max_tiles, l.num_tiles, status, stream);
+    if (rc != kRcOk) return rc;
+  } else {
+    rc = launch_router(x, router_weight, router_bias, T, b.H, b.E, top_k, norm_topk_prob, l.ids,
+                       l.w, nullptr, status, stream);
+    if (rc != kRcOk) return rc;
+    rc = launch_sort_align(l.ids, T * top_k, b.E, 0, b.E, MOE_BLOCK_M, l.sort_ws, l.counts,
+                           l.offsets, nullptr, l.perm, nullptr, l.tiles, l.max_tiles, l.num_tiles,
+                           status, stream);
+    if (rc != kRcOk) return rc;
+  }
+  return w4_products(b, l, x, l.ids, l.w, T, top_k, 0, y, status, stream);
 }
 
 }  // extern "C"

@@ -168,6 +168,36 @@ int launch_w2_atomic(const void* h, int M, const int4* tiles, const int* num_til
                      int max_tiles, const void* w_down, int E, int H, int I, const int* row_map,
                      const float* row_scale, int n_slots, int red_div, float* out_f32,
                      int* status, cudaStream_t stream, int tile_rows = 128);
+// 4-bit expert weights (w4.cu; layout in w4.cuh): the packed bank of a layer.
+struct W4Bank {
+  const void *w13_q, *w13_s, *w13_z;  // gate and up rows interleaved by eights
+  const void *w2_q, *w2_s, *w2_z;     // down; zero points null: 8 throughout
+  int E, H, I, group;
+};
+constexpr int kW4MaxK = 8192;
+int w4_check_bank(const W4Bank& bank);
+int launch_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros0,
+                   const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E, int N,
+                   int K, int group, void* q, void* s, void* z, int* status, cudaStream_t stream);
+int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* index,
+                  int index_div, int M, const int4* tiles, const int* num_tiles, int max_tiles,
+                  void* h_out, int* status, cudaStream_t stream);
+int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
+                 int max_tiles, const int* row_map, const float* row_scale, void* out,
+                 int out_rows, int* status, cudaStream_t stream);
+
+// Norms around a block: n = RMSNorm(delta) * post, h = x + scale * act(gate) * n,
+// y = RMSNorm(h) * pre.  gate[t * gate_row + c * gate_col], bf16 or fp32, null: 1.
+struct BlockNormArgs {
+  const void *x, *delta, *gate;
+  const float *post, *pre;
+  long long gate_row;
+  int gate_col, gate_f32, act;  // act: 0 none, 1 sigmoid, 2 tanh
+  int T, H;
+  float eps, scale;
+  void *h, *y;
+};
+int launch_block_norm(const BlockNormArgs& a, cudaStream_t stream);
 // Block glue: h = delta ? bf16(x + delta) : x; y = bf16(h * rsqrt(mean(h^2) + eps) * w).
 int launch_add_rmsnorm(const void* x, const void* delta, const float* w, int T, int H, float eps,
                        void* h_out, void* y, cudaStream_t stream);

@@ -25,6 +25,7 @@ enum StatusCode : int {
   kErrTimeoutGrid = 0x106,     // a grid-wide barrier of a single-launch layer never completed
   kErrBadExpert = 0x201,       // an expert id outside [0, E)
   kErrBadRow = 0x202,          // a tile row range outside the A operand
+  kErrBadCode = 0x203,         // a 4-bit weight code or zero point above 15
 };
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s

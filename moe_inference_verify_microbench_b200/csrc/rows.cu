@@ -252,6 +252,139 @@ __global__ void __launch_bounds__(kRowsThreads) add_rmsnorm_rows(
   }
 }
 
+// The norm after a block, its gate and residual scale, and the norm before the
+// next block, in one pass over the row:
+//   n = delta * rsqrt(mean(delta^2) + eps) * post
+//   h = x + scale * act(gate) * n
+//   y = h * rsqrt(mean(h^2) + eps) * pre
+// HBM bounds it: 4 H bytes read and 4 H written per row (and the gate).  One
+// CTA per row keeps x, delta and then h in registers (VPT 16-byte vectors per
+// thread), so nothing is read twice; both sums of squares and h are fp32, and y
+// is the norm of the unrounded h.
+template <int ACT>
+__device__ __forceinline__ float gate_act(float g) {
+  if (ACT == 1) return 1.0f / (1.0f + __expf(-g));
+  if (ACT == 2) return tanhf(g);
+  return g;
+}
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float2 p = __bfloat1622float2(h[q]);
+    f[2 * q] = p.x;
+    f[2 * q + 1] = p.y;
+  }
+}
+
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+  const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
+  f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+
+// Sum over the CTA; every thread gets it.  `sh` holds one float per warp.
+__device__ __forceinline__ float cta_sum(float v, float* sh) {
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int nw = blockDim.x >> 5;
+  if (nw == 1) return v;
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = static_cast<int>(threadIdx.x & 31) < nw ? sh[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+constexpr int kBlockNormMaxH = 4 * 8 * 1024;
+
+template <int VPT, int ACT>
+__global__ void __launch_bounds__(1024) block_norm_rows(const BlockNormArgs a) {
+  __shared__ float sh[2][32];
+  pdl_wait();
+  pdl_trigger();
+  const int vec = a.H / 8;
+  const size_t n = blockIdx.x;
+  const uint4* xr = static_cast<const uint4*>(a.x) + n * vec;
+  const uint4* dr = static_cast<const uint4*>(a.delta) + n * vec;
+  uint4 xv[VPT], dv[VPT];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    xv[i] = dv[i] = make_uint4(0, 0, 0, 0);
+    if (v < vec) {
+      dv[i] = __ldg(dr + v);
+      xv[i] = __ldg(xr + v);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    float d[8];
+    unpack8(dv[i], d);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) ss = fmaf(d[q], d[q], ss);
+  }
+  const float inv_h = 1.0f / static_cast<float>(a.H);
+  const float r1 = rsqrtf(cta_sum(ss, sh[0]) * inv_h + a.eps) * a.scale;
+  float token_gate = 1.0f;  // one gate for the row
+  if (a.gate != nullptr && a.gate_col == 0) {
+    const float g = a.gate_f32 ? static_cast<const float*>(a.gate)[n * a.gate_row]
+                               : __bfloat162float(static_cast<const __nv_bfloat16*>(
+                                     a.gate)[n * a.gate_row]);
+    token_gate = gate_act<ACT>(g);
+  }
+  float h[VPT][8];
+  ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) h[i][q] = 0.0f;
+    if (v < vec) {
+      float d[8], w[8], gt[8];
+      unpack8(xv[i], h[i]);
+      unpack8(dv[i], d);
+      load8(a.post + 8 * v, w);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) gt[q] = token_gate;
+      if (a.gate != nullptr && a.gate_col != 0) {
+        const size_t o = n * a.gate_row + 8 * v;
+        if (a.gate_f32) load8(static_cast<const float*>(a.gate) + o, gt);
+        else unpack8(__ldg(reinterpret_cast<const uint4*>(
+                 static_cast<const __nv_bfloat16*>(a.gate) + o)), gt);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) gt[q] = gate_act<ACT>(gt[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        h[i][q] = fmaf(d[q] * r1 * w[q], gt[q], h[i][q]);
+        ss = fmaf(h[i][q], h[i][q], ss);
+      }
+      static_cast<uint4*>(a.h)[n * vec + v] =
+          make_uint4(pack_bf16x2(h[i][0], h[i][1]), pack_bf16x2(h[i][2], h[i][3]),
+                     pack_bf16x2(h[i][4], h[i][5]), pack_bf16x2(h[i][6], h[i][7]));
+    }
+  }
+  const float r2 = rsqrtf(cta_sum(ss, sh[1]) * inv_h + a.eps);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < vec) {
+      float w[8];
+      load8(a.pre + 8 * v, w);
+      uint32_t o[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        o[q] = pack_bf16x2(h[i][2 * q] * r2 * w[2 * q], h[i][2 * q + 1] * r2 * w[2 * q + 1]);
+      static_cast<uint4*>(a.y)[n * vec + v] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+}
+
 static int rows_grid(long long rows) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -309,6 +442,37 @@ int launch_add_rmsnorm(const void* x, const void* delta, const float* w, int T, 
                                    static_cast<const uint4*>(delta), w, T, H / 8, eps,
                                    static_cast<uint4*>(h_out), static_cast<uint4*>(y));
   return e == cudaSuccess ? kRcOk : kRcCudaError;
+}
+
+template <int VPT>
+static cudaError_t block_norm_launch(const BlockNormArgs& a, cudaStream_t stream) {
+  const int vec = a.H / 8;
+  const int threads = ((vec + VPT - 1) / VPT + 31) / 32 * 32;
+  auto kern = a.act == 1 ? block_norm_rows<VPT, 1>
+              : a.act == 2 ? block_norm_rows<VPT, 2>
+                           : block_norm_rows<VPT, 0>;
+  return launch_pdl(kern, dim3(a.T), dim3(threads), 0, stream, a);
+}
+
+int launch_block_norm(const BlockNormArgs& a, cudaStream_t stream) {
+  if (a.T < 0 || a.H <= 0 || !(a.eps >= 0.0f) || a.act < 0 || a.act > 2 || a.gate_row < 0 ||
+      (a.gate_col != 0 && a.gate_col != 1) ||
+      (a.T > 0 && (a.x == nullptr || a.delta == nullptr || a.post == nullptr ||
+                   a.pre == nullptr || a.h == nullptr || a.y == nullptr)))
+    return kRcBadArgument;
+  if (a.H % 8 != 0 || a.H > kBlockNormMaxH) return kRcUnsupported;
+  for (const void* p : {a.x, a.delta, static_cast<const void*>(a.post),
+                        static_cast<const void*>(a.pre), static_cast<const void*>(a.h),
+                        static_cast<const void*>(a.y)})
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return kRcBadArgument;
+  if (a.gate != nullptr && a.gate_col != 0 &&
+      ((reinterpret_cast<uintptr_t>(a.gate) & 15u) != 0 || a.gate_row % 8 != 0))
+    return kRcBadArgument;
+  if (a.T == 0) return kRcOk;
+  const int vec = a.H / 8;
+  const cudaError_t e = vec <= 2 * 1024 ? block_norm_launch<2>(a, stream)
+                                        : block_norm_launch<4>(a, stream);
+  return note_cuda_error(e) == cudaSuccess ? kRcOk : kRcCudaError;
 }
 
 int launch_cast_f32_bf16(const float* src, long long n, void* y, cudaStream_t stream) {

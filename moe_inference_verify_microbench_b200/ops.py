@@ -8,6 +8,7 @@ word that ``check_status`` reads (tests and debugging only).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import NamedTuple
 
@@ -85,6 +86,23 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, ndim: int | None = Non
 def _rc(rc: int, what: str) -> None:
     if rc != 0:
         raise MoEKernelError(f"{what}: {_native.error_string(rc)} (rc={rc})", rc)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Makes ``device`` the current one for a launch on its stream (nothing to do
+    where it is already)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+def _same_device(device: torch.device, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on {device}, got {t.device}")
 
 
 # --------------------------------------------------------------------------- router
@@ -374,6 +392,58 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float,
     return (h, y) if delta is not None else y
 
 
+_GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}  # MOE_GATE_ACT_*
+
+
+def block_norm(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor,
+               pre_weight: torch.Tensor, eps: float, gate: torch.Tensor | None = None,
+               gate_act: str = "none", residual_scale: float = 1.0):
+    """The norm after a block, its gate and residual scale, and the norm before the
+    next block, in one pass over the rows:
+    ``h = x + residual_scale * act(gate) * RMSNorm(delta) * post_weight`` and
+    ``y = RMSNorm(h) * pre_weight``, both sums of squares in fp32 and ``y`` taken from
+    ``h`` before its rounding.  ``x``, ``delta`` bf16 [..., H], H a multiple of 8 up to
+    32768; ``gate`` (bf16 or fp32) one value per channel [H], per token [..., 1] or
+    per element [..., H], through ``gate_act`` ("none", "sigmoid" or "tanh").
+    Returns ``(h, y)``."""
+    _need(x, "x", torch.bfloat16)
+    _need(delta, "delta", torch.bfloat16)
+    if x.dim() == 0 or delta.shape != x.shape:
+        raise ValueError("delta must have the shape of x, [..., H]")
+    if gate_act not in _GATE_ACTS:
+        raise ValueError(f"gate_act must be one of {tuple(_GATE_ACTS)}, got {gate_act!r}")
+    H = x.shape[-1]
+    T = x.numel() // max(H, 1)
+    dev = x.device
+    w = []
+    for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if t.device != dev or t.numel() != H:
+            raise ValueError(f"{name} must be [H] on the device of x")
+        w.append(t.detach().float().contiguous())
+    kind = 0
+    if gate is not None:
+        if gate.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"gate must be bfloat16 or float32, got {gate.dtype}")
+        _need(gate, "gate", gate.dtype)
+        if gate.dim() == 1 and x.dim() > 1 and gate.shape[0] == H:
+            kind = 2
+        elif gate.shape == x.shape:
+            kind = 3
+        elif gate.shape == x.shape[:-1] + (1,):
+            kind = 1
+        else:
+            raise ValueError(f"gate must be [H], [..., 1] or [..., H] for x {tuple(x.shape)}, got "
+                             f"{tuple(gate.shape)}")
+    _same_device(dev, delta=delta, gate=gate)
+    h, y = torch.empty_like(x), torch.empty_like(x)
+    with _on(dev):
+        _rc(_native.load().moe_block_norm(
+            _p(x), _p(delta), _p(w[0]), _p(w[1]), _p(gate), kind,
+            int(gate is not None and gate.dtype == torch.float32), _GATE_ACTS[gate_act],
+            float(residual_scale), T, H, float(eps), _p(h), _p(y), _stream(dev)), "moe_block_norm")
+    return h, y
+
+
 # --------------------------------------------------------------------------- EP send plan
 
 
@@ -512,3 +582,176 @@ def layer_workspace_bytes(T: int, H: int, I: int, E: int, top_k: int,
                           index_add: str = "deterministic") -> int:
     return int(_native.load().moe_layer_workspace_bytes_ex(T, H, I, E, top_k,
                                                            _combine_mode(index_add)))
+
+
+# --------------------------------------------------------------------------- 4-bit experts
+
+
+def _bank_of(bank, device: torch.device, hidden: int | None = None):
+    from .w4 import W4Experts
+    if not isinstance(bank, W4Experts):
+        raise TypeError(f"bank must be a W4Experts, got {type(bank).__name__}")
+    if bank.device != device:
+        raise ValueError(f"the 4-bit bank is on {bank.device}, the activations on {device}")
+    if hidden is not None and hidden != bank.hidden:
+        raise ValueError(f"x must have {bank.hidden} columns for this bank, got {hidden}")
+    return bank
+
+
+def _workspace(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor:
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {device}")
+    return workspace
+
+
+def _output(out: torch.Tensor | None, shape, device: torch.device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
+    _need(out, "out", torch.bfloat16)
+    if tuple(out.shape) != tuple(shape) or out.device != device:
+        raise ValueError(f"out must be {tuple(shape)} on {device}, got {tuple(out.shape)} on "
+                         f"{out.device}")
+    return out
+
+
+def grouped_w13_swiglu_w4(a: torch.Tensor, tiles: torch.Tensor, num_tiles: torch.Tensor,
+                          max_tiles_: int, bank, index: torch.Tensor | None = None,
+                          index_div: int = 1, M: int | None = None,
+                          out: torch.Tensor | None = None) -> torch.Tensor:
+    """``grouped_w13_swiglu`` on a 4-bit bank (``W4Experts``); with ``index`` the row
+    gather of ``grouped_w13_swiglu_gather`` (row r is ``a[index[r] // index_div]``)."""
+    _need(a, "a", torch.bfloat16, 2)
+    _need(tiles, "tiles", torch.int32)
+    _need(num_tiles, "num_tiles", torch.int32)
+    dev = a.device
+    _bank_of(bank, dev, a.shape[1])
+    if tiles.numel() < 4 * max_tiles_:
+        raise ValueError(f"tiles must hold max_tiles = {max_tiles_} entries")
+    if index is not None:
+        _need(index, "index", torch.int32)
+        M = index.numel() if M is None else M
+        if index.numel() < M:
+            raise ValueError("index must hold at least M entries")
+    else:
+        M = a.shape[0] if M is None else M
+        if M > a.shape[0]:
+            raise ValueError("a must hold at least M rows")
+    _same_device(dev, tiles=tiles, num_tiles=num_tiles, index=index)
+    h = _output(out, (M, bank.intermediate), dev)
+    with _on(dev):
+        _rc(_native.load().moe_grouped_w13_swiglu_w4(
+            _p(a), a.shape[0], _p(index), index_div, M, _p(tiles), _p(num_tiles), max_tiles_,
+            bank.native, _p(h), _p(status_word(dev)), _stream(dev)), "moe_grouped_w13_swiglu_w4")
+    return h
+
+
+def grouped_w2_w4(h: torch.Tensor, tiles: torch.Tensor, num_tiles: torch.Tensor, max_tiles_: int,
+                  bank, row_map: torch.Tensor | None = None,
+                  slot_scale: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                  out_rows: int | None = None) -> torch.Tensor:
+    """``grouped_w2`` on a 4-bit bank (``W4Experts``)."""
+    _need(h, "h", torch.bfloat16, 2)
+    _need(tiles, "tiles", torch.int32)
+    _need(num_tiles, "num_tiles", torch.int32)
+    dev = h.device
+    _bank_of(bank, dev)
+    M, I = h.shape
+    if I != bank.intermediate:
+        raise ValueError(f"h must have {bank.intermediate} columns for this bank, got {I}")
+    if tiles.numel() < 4 * max_tiles_:
+        raise ValueError(f"tiles must hold max_tiles = {max_tiles_} entries")
+    rows = out.shape[0] if out is not None else out_rows if out_rows is not None else M
+    if row_map is not None:
+        _need(row_map, "row_map", torch.int32)
+        if row_map.numel() < M:
+            raise ValueError("row_map must hold an entry for every row of h")
+    if slot_scale is not None:
+        _need(slot_scale, "slot_scale", torch.float32)
+        if slot_scale.numel() < rows:
+            raise ValueError("slot_scale must hold an entry for every row of out")
+    _same_device(dev, tiles=tiles, num_tiles=num_tiles, row_map=row_map, slot_scale=slot_scale)
+    out = _output(out, (rows, bank.hidden), dev)
+    with _on(dev):
+        _rc(_native.load().moe_grouped_w2_w4(
+            _p(h), M, _p(tiles), _p(num_tiles), max_tiles_, bank.native, _p(row_map),
+            _p(slot_scale), _p(out), rows, _p(status_word(dev)), _stream(dev)),
+            "moe_grouped_w2_w4")
+    return out
+
+
+def experts_w4_workspace_bytes(T: int, top_k: int, bank) -> int:
+    """Workspace bytes of ``experts_w4``."""
+    return int(_native.load().moe_w4_experts_workspace_bytes(T, top_k, bank.native))
+
+
+def experts_w4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, bank,
+               num_experts: int | None = None, e_begin: int = 0,
+               out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """The 4-bit experts for routed tokens: ``y[n] = sum_j weights[n, j] *
+    MLP_{ids[n, j]}(x[n])`` (C5/python/solution.py:131-160).  The bank holds experts
+    [e_begin, e_begin + bank.num_experts) of ``num_experts`` (default: all of them are
+    held); records of other experts add nothing, as in C6's local-expert filter
+    (C6/python/solution.py:137-176).  ``ids`` int32 [T, k], ``weights`` fp32 [T, k], k <= 8."""
+    _need(x, "x", torch.bfloat16, 2)
+    _need(ids, "ids", torch.int32, 2)
+    _need(weights, "weights", torch.float32, 2)
+    dev = x.device
+    T, H = x.shape
+    _bank_of(bank, dev, H)
+    k = ids.shape[1]
+    if ids.shape[0] != T or weights.shape != ids.shape:
+        raise ValueError(f"ids and weights must be [T, k] with T = {T}, got {tuple(ids.shape)} and "
+                         f"{tuple(weights.shape)}")
+    if num_experts is None:
+        num_experts = e_begin + bank.num_experts
+    if e_begin < 0 or e_begin + bank.num_experts > num_experts:
+        raise ValueError(f"experts [{e_begin}, {e_begin + bank.num_experts}) of the bank are not "
+                         f"among {num_experts}")
+    _same_device(dev, ids=ids, weights=weights)
+    lib = _native.load()
+    y = _output(out, (T, H), dev)
+    ws = _workspace(workspace, int(lib.moe_w4_experts_workspace_bytes(T, k, bank.native)), dev)
+    with _on(dev):
+        _rc(lib.moe_w4_experts_forward(_p(x), _p(ids), _p(weights), T, k, num_experts, e_begin,
+                                       bank.native, _p(ws), ws.numel() * ws.element_size(), _p(y),
+                                       _p(status_word(dev)), _stream(dev)),
+            "moe_w4_experts_forward")
+    return y
+
+
+def moe_layer_w4_workspace_bytes(T: int, top_k: int, bank) -> int:
+    """Workspace bytes of ``moe_layer_w4``."""
+    return int(_native.load().moe_w4_layer_workspace_bytes(T, top_k, bank.native))
+
+
+def moe_layer_w4(x: torch.Tensor, router_weight: torch.Tensor, bank, top_k: int,
+                 norm_topk_prob: bool = True, bias: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None,
+                 workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``moe_layer`` on a 4-bit bank (``W4Experts``) that holds all experts: router,
+    top-k, experts and the weighted sum in one C-ABI call."""
+    _need(x, "x", torch.bfloat16, 2)
+    _need(router_weight, "router_weight", torch.bfloat16, 2)
+    dev = x.device
+    T, H = x.shape
+    _bank_of(bank, dev, H)
+    if tuple(router_weight.shape) != (bank.num_experts, H):
+        raise ValueError(f"router_weight must be [E, H] = {(bank.num_experts, H)}, got "
+                         f"{tuple(router_weight.shape)}")
+    if bias is not None:
+        _need(bias, "bias", torch.float32, 1)
+        if bias.numel() != bank.num_experts:
+            raise ValueError(f"bias must hold E = {bank.num_experts} entries")
+    _same_device(dev, router_weight=router_weight, bias=bias)
+    lib = _native.load()
+    y = _output(out, (T, H), dev)
+    ws = _workspace(workspace, int(lib.moe_w4_layer_workspace_bytes(T, top_k, bank.native)), dev)
+    with _on(dev):
+        _rc(lib.moe_w4_layer_forward(_p(x), _p(router_weight), _p(bias), bank.native, T, top_k,
+                                     int(bool(norm_topk_prob)), _p(ws),
+                                     ws.numel() * ws.element_size(), _p(y), _p(status_word(dev)),
+                                     _stream(dev)), "moe_w4_layer_forward")
+    return y
