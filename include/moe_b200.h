@@ -385,8 +385,9 @@ MOE_API int moe_block_norm(const void* x, const void* delta, const float* post_w
  * are loaded): codes uint8 [E, N, K] (one code per byte), scales bf16
  * [E, N, K/group], zeros uint8 [E, N, K/group] or NULL.  With a second matrix
  * (codes1, scales1, zeros1) the two are interleaved by eight rows: the packed
- * gate (0) and up (1) projections.  q takes E*M*K/2 bytes, s E*M*(K/group)*2
- * and z E*M*(K/group), M = N, or 2N for two matrices.  A code or zero point
+ * gate (0) and up (1) projections.  q takes E*M*K/2 bytes and s, which holds
+ * the scales and the zero points, E*M*(K/group) * 2 (4 with zero points),
+ * M = N, or 2N for two matrices.  A code or zero point
  * above 15 records MOE_ERR_BAD_CODE and is taken modulo 16.  K % 64 == 0,
  * K % group == 0, K <= 8192; N % 16 == 0 (N % 8 for two matrices); all
  * pointers to codes and packed data 16-byte aligned.
@@ -397,15 +398,13 @@ MOE_API int moe_block_norm(const void* x, const void* delta, const float* post_w
 typedef struct moe_w4_bank {
   const void* w13_q;
   const void* w13_s;
-  const void* w13_z; /* NULL without zero points (then w2_z too) */
   const void* w2_q;
   const void* w2_s;
-  const void* w2_z;
-  int32_t E, H, I, group;
+  int32_t E, H, I, group, has_zeros;
 } moe_w4_bank;
 MOE_API int moe_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros0,
                         const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E,
-                        int N, int K, int group, void* q, void* s, void* z, int32_t* status,
+                        int N, int K, int group, void* q, void* s, int32_t* status,
                         cudaStream_t stream);
 
 /*

@@ -99,7 +99,7 @@ SIGNATURES: dict[str, tuple] = {
                                 ctypes.c_float, _c_int, _c_int, ctypes.c_float, _ptr, _ptr,
                                 _ptr]),
     "moe_w4_pack": (_c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int,
-                             _ptr, _ptr, _ptr, _ptr, _ptr]),
+                             _ptr, _ptr, _ptr, _ptr]),
     "moe_grouped_w13_swiglu_w4": (_c_int, [_ptr, _c_int, _ptr, _c_int, _c_int, _ptr, _ptr, _c_int,
                                            _ptr, _ptr, _ptr, _ptr]),
     "moe_grouped_w2_w4": (_c_int, [_ptr, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr, _ptr, _ptr,
@@ -116,9 +116,9 @@ SIGNATURES: dict[str, tuple] = {
 class W4BankStruct(ctypes.Structure):
     """``moe_w4_bank`` of the header."""
 
-    _fields_ = [("w13_q", _ptr), ("w13_s", _ptr), ("w13_z", _ptr), ("w2_q", _ptr),
-                ("w2_s", _ptr), ("w2_z", _ptr), ("E", ctypes.c_int32), ("H", ctypes.c_int32),
-                ("I", ctypes.c_int32), ("group", ctypes.c_int32)]
+    _fields_ = [("w13_q", _ptr), ("w13_s", _ptr), ("w2_q", _ptr), ("w2_s", _ptr),
+                ("E", ctypes.c_int32), ("H", ctypes.c_int32), ("I", ctypes.c_int32),
+                ("group", ctypes.c_int32), ("has_zeros", ctypes.c_int32)]
 
 
 ABI_VERSION = 5

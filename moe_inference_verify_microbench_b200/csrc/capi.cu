@@ -88,7 +88,7 @@ size_t layer_layout(int T, int H, int I, int E, int k, int mode, void* ws, Body&
 }
 
 W4Bank w4_bank(const moe_w4_bank& b) {
-  return {b.w13_q, b.w13_s, b.w13_z, b.w2_q, b.w2_s, b.w2_z, b.E, b.H, b.I, b.group};
+  return {b.w13_q, b.w13_s, b.w2_q, b.w2_s, b.E, b.H, b.I, b.group, b.has_zeros};
 }
 
 // Buffers of one pass over the 4-bit experts; with `routed`, also the router's
@@ -558,9 +558,8 @@ int moe_layer_forward_ex(const void* x, const void* router_weight, const float* 
 
 int moe_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros0,
                 const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E, int N,
-                int K, int group, void* q, void* s, void* z, int32_t* status,
-                cudaStream_t stream) {
-  return launch_w4_pack(codes0, scales0, zeros0, codes1, scales1, zeros1, E, N, K, group, q, s, z,
+                int K, int group, void* q, void* s, int32_t* status, cudaStream_t stream) {
+  return launch_w4_pack(codes0, scales0, zeros0, codes1, scales1, zeros1, E, N, K, group, q, s,
                         status, stream);
 }
 

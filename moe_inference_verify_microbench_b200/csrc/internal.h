@@ -170,15 +170,15 @@ int launch_w2_atomic(const void* h, int M, const int4* tiles, const int* num_til
                      int* status, cudaStream_t stream, int tile_rows = 128);
 // 4-bit expert weights (w4.cu; layout in w4.cuh): the packed bank of a layer.
 struct W4Bank {
-  const void *w13_q, *w13_s, *w13_z;  // gate and up rows interleaved by eights
-  const void *w2_q, *w2_s, *w2_z;     // down; zero points null: 8 throughout
-  int E, H, I, group;
+  const void *w13_q, *w13_s;  // gate and up rows interleaved by eights
+  const void *w2_q, *w2_s;    // down
+  int E, H, I, group, zeros;
 };
 constexpr int kW4MaxK = 8192;
 int w4_check_bank(const W4Bank& bank);
 int launch_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros0,
                    const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E, int N,
-                   int K, int group, void* q, void* s, void* z, int* status, cudaStream_t stream);
+                   int K, int group, void* q, void* s, int* status, cudaStream_t stream);
 int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* index,
                   int index_div, int M, const int4* tiles, const int* num_tiles, int max_tiles,
                   void* h_out, int* status, cudaStream_t stream);

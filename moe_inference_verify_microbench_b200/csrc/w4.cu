@@ -6,21 +6,24 @@
 //
 // At few records per expert these are a stream of weights: 0.5 byte and the
 // group's share of a scale per weight, so HBM bounds them and everything else
-// has to stay below 23 bytes of weights per cycle and SM.  One persistent CTA per SM; a
-// producer thread copies whole 16-row tiles (contiguous, with their scales) into a
-// ring of shared-memory stages; eight consumer warps turn codes into bf16
-// operands in registers (28 integer instructions per 1024 weights and warp, no
-// conversion) and multiply them on the tensor cores as the 16-row operand of
-// mma.m16n8k16, with up to 32 records as its columns.  The records' rows are
-// held in registers for all tiles of an expert, so shared memory sees each
-// weight once and no activation at all.  Up to eight warps share a tile along
-// K and add their fp32 partials through shared memory.
+// has to stay below 23 bytes of weights per cycle and SM.  One persistent CTA of
+// sixteen warps per SM.  Every warp copies the part of a 16-row tile that it will
+// use itself (contiguous, in the order its lanes consume) into shared memory
+// with cp.async, several tiles ahead, so the stream needs no barrier; it turns
+// codes into fp16 operands in registers (20 integer instructions per 1024
+// weights, no conversion) and multiplies them on the tensor cores as the 16-row
+// operand of mma.m16n8k16, with up to 16 records as its columns.  The records'
+// rows stay in registers for all tiles of an expert.  The warps that share a
+// tile along K add their fp32 partials through shared memory.
 //
-// Numerics: products of bf16 activations with (q - z) are exact in fp32; each
-// 64-column block (32 where the group is 32) is summed on the tensor cores in
-// fp32 and then scaled in fp32, so no weight is ever rounded to bf16.
+// Numerics: products of activations with (q - z) are exact in fp32; each
+// group (or a warp's share of it) is summed on the tensor cores in fp32 and
+// then scaled in fp32, so no weight is ever rounded to bf16.
 #include <algorithm>
 #include <atomic>
+#include <cuda_fp16.h>
+#include <initializer_list>
+#include <type_traits>
 
 #include "grouped_gemm.cuh"
 #include "internal.h"
@@ -37,19 +40,19 @@ struct W4PackArgs {
   int E, N, K, group;
   uint8_t* q;
   uint16_t* s;
-  uint8_t* z;
   int* status;
 };
 
+// The word of a lane's eight columns 8i + {0, 1} from `codes`.
 __device__ __forceinline__ uint32_t w4_word(const uint8_t* codes, bool& bad) {
-  const uint2 v = *reinterpret_cast<const uint2*>(codes);  // columns 0..3, 4..7
-  bad |= ((v.x | v.y) & 0xf0f0f0f0u) != 0;
-  uint32_t w = 0;
+  uint32_t w = 0, seen = 0;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    const uint32_t q = ((c < 4 ? v.x : v.y) >> (8 * (c & 3))) & 0xfu;
-    w |= q << (4 * ((c >> 1) + 4 * (c & 1)));
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t v = *reinterpret_cast<const uint16_t*>(codes + 8 * i);
+    seen |= v;
+    w |= (v & 0xfu) << (4 * i) | ((v >> 8) & 0xfu) << (4 * i + 16);
   }
+  bad |= (seen & 0xf0f0u) != 0;
   return w;
 }
 
@@ -73,7 +76,7 @@ __global__ void __launch_bounds__(256) w4_pack(const W4PackArgs a) {
     const long long e = et / tiles;
     const int g = lane >> 2, t = lane & 3;
     const size_t row = static_cast<size_t>(e) * a.N + static_cast<size_t>(tile) * rows + g;
-    const size_t col = static_cast<size_t>(kb) * 64 + 8 * t;
+    const size_t col = static_cast<size_t>(kb) * 64 + 2 * t;
     const uint8_t* p0 = a.codes[0] + row * a.K + col;
     const uint8_t* p1 = pair ? a.codes[1] + row * a.K + col : p0 + static_cast<size_t>(8) * a.K;
     uint4 w;
@@ -94,13 +97,15 @@ __global__ void __launch_bounds__(256) w4_pack(const W4PackArgs a) {
     const size_t row = static_cast<size_t>(e) * a.N + static_cast<size_t>(tile) * rows + g;
     const size_t o0 = row * ng + grp;
     const size_t o1 = pair ? o0 : o0 + static_cast<size_t>(8) * ng;
-    a.s[2 * i] = a.scales[0][o0];
-    a.s[2 * i + 1] = a.scales[pair ? 1 : 0][o1];
-    if (a.z != nullptr) {
+    const bool zp = a.zeros[0] != nullptr;
+    uint16_t* rec = a.s + (zp ? 4 : 2) * i;
+    rec[0] = a.scales[0][o0];
+    rec[1] = a.scales[pair ? 1 : 0][o1];
+    if (zp) {
       const uint8_t z0 = a.zeros[0][o0], z1 = a.zeros[pair ? 1 : 0][o1];
       bad |= z0 > 15 || z1 > 15;
-      a.z[2 * i] = z0 & 15;
-      a.z[2 * i + 1] = z1 & 15;
+      rec[2] = 0x6400u | (z0 & 15u);  // fp16 1024 + z
+      rec[3] = 0x6400u | (z1 & 15u);
     }
   }
   if (bad) record_status(a.status, kErrBadCode);
@@ -111,7 +116,7 @@ __global__ void __launch_bounds__(256) w4_pack(const W4PackArgs a) {
 struct W4Args {
   W4Matrix m;
   W4Plan p;
-  const uint4* act;     // A rows [act_rows][K]
+  const uint32_t* act;  // A rows [act_rows][K], bf16 pairs
   int act_rows;
   const int* index;     // A row of record p = act[index[p] / index_div] (null = p)
   int index_div;
@@ -128,232 +133,237 @@ struct W4Args {
   int* status;
 };
 
-// Work of a tile-table entry: its records in chunks of p.nr, each chunk one
-// pass over the expert's stages (units).  A bad entry has none and is
-// reported.
-__device__ __forceinline__ int w4_units(const W4Args& a, const int4& t) {
+// Work of a tile-table entry: its records in chunks of 8 NT, each chunk one pass
+// over the expert's tiles (units).  A bad entry has none and is reported.
+template <int NT>
+__device__ __forceinline__ int w4_chunks(const W4Args& a, const int4& t) {
   if (t.x < 0 || t.x >= a.E || t.y < 0 || t.z > a.M || t.z <= t.y) {
     if (t.z != t.y || t.x < 0 || t.x >= a.E)
       record_status(a.status, t.x < 0 || t.x >= a.E ? kErrBadExpert : kErrBadRow);
     return 0;
   }
-  return (t.z - t.y + a.p.nr - 1) / a.p.nr * a.p.groups;
+  return static_cast<int>(static_cast<unsigned>(t.z - t.y + 8 * NT - 1) / (8u * NT));
 }
 
 // Cost of a unit: the stream of its weights, and a share for every eight
 // records multiplied with them.
-__device__ __forceinline__ int w4_unit_cost(const W4Args& a, const int4& t) {
-  return 6 + (min(t.z - t.y, a.p.nr) + 7) / 8;
+template <int NT>
+__device__ __forceinline__ int w4_unit_cost(const int4& t) {
+  return NT > 1 && t.z - t.y > 8 ? 5 : 4;
 }
 
+// A position in the work: tile-table entry, unit within it.
 struct W4Pos {
   int entry, unit;
 };
 
 // This CTA's contiguous range of units [lo, hi), the summed cost split evenly
 // over the grid.  Every thread of the CTA calls it.
+template <int NT>
 __device__ __forceinline__ void w4_range(const W4Args& a, int nt, W4Pos* lo, W4Pos* hi) {
-  __shared__ long long sh_scan[32];
-  __shared__ W4Pos sh_pos[2];
-  __shared__ long long sh_total;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  auto cost = [&](int i) -> long long {
+  __shared__ long long sums[kW4Warps];
+  __shared__ W4Pos pos[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto cost = [&](int i, int* per) -> long long {
+    *per = 1;
     if (i >= nt) return 0;
     const int4 t = a.tiles[i];
-    const int u = w4_units(a, t);
-    return u > 0 ? static_cast<long long>(u) * w4_unit_cost(a, t) : 0;
+    *per = w4_unit_cost<NT>(t);
+    return static_cast<long long>(w4_chunks<NT>(a, t)) * (a.m.tiles * *per);
   };
-  auto scan = [&](long long v, long long* total) {  // inclusive, over the block
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += y;
-    }
-    if (lane == 31) sh_scan[warp] = v;
-    __syncthreads();
-    long long before = 0, all = 0;
-    for (int w = 0; w < nw; ++w) {
-      const long long s = sh_scan[w];
-      if (w < warp) before += s;
-      all += s;
-    }
-    __syncthreads();
-    *total = all;
-    return before + v;
-  };
-  if (threadIdx.x == 0) {
-    sh_pos[0] = sh_pos[1] = {0, 0};
-    sh_total = 0;
+  int per0;
+  const long long first = cost(threadIdx.x, &per0);  // most tables fit the CTA
+  long long mine = first;
+  for (int i = threadIdx.x + kW4Threads; i < nt; i += kW4Threads) {
+    int per;
+    mine += cost(i, &per);
   }
-  long long total = 0;
-  for (int base = 0; base < nt; base += blockDim.x) {
-    long long part;
-    scan(cost(base + static_cast<int>(threadIdx.x)), &part);
-    total += part;
-  }
-  long long carry = 0;
-  for (int base = 0; base < nt; base += blockDim.x) {
-    const int i = base + static_cast<int>(threadIdx.x);
-    const long long c = cost(i);
-    long long part;
-    const long long incl = scan(c, &part) + carry;
-    carry += part;
-    if (c > 0) {
-      const int per = w4_unit_cost(a, a.tiles[i]);
+  if (threadIdx.x < 2) pos[threadIdx.x] = {0, 0};
+  long long total = 0, carry = 0;
+  for (int base = 0; base < nt; base += kW4Threads) {
+    int per = per0;
+    const long long c = base == 0 ? first : cost(base + static_cast<int>(threadIdx.x), &per);
+    long long incl = c;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const long long want = total * (static_cast<long long>(blockIdx.x) + k) / gridDim.x;
-        if (want > incl - c && want <= incl)
-          sh_pos[k] = {i, static_cast<int>((want - (incl - c) + per - 1) / per)};
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (base == 0) {  // the grand total, once
+      long long all = nt <= kW4Threads ? incl : mine;
+      if (nt > kW4Threads) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
       }
+      if (lane == 31) sums[warp] = all;
+      __syncthreads();
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < kW4Warps; ++w) total += sums[w];
+    }
+    if (nt > kW4Threads) {
+      __syncthreads();
+      if (lane == 31) sums[warp] = incl;
+      __syncthreads();
+    }
+    long long before = carry;
+#pragma unroll
+    for (int w = 0; w < kW4Warps; ++w) {
+      if (w < warp) before += sums[w];
+      carry += sums[w];
+    }
+    incl += before;
+    const long long excl = incl - c;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const long long want = total * (static_cast<long long>(blockIdx.x) + k) / gridDim.x;
+      if (want > excl && want <= incl)
+        pos[k] = {base + static_cast<int>(threadIdx.x),
+                  static_cast<int>((want - excl + per - 1) / per)};
     }
   }
   __syncthreads();
-  *lo = sh_pos[0];
-  *hi = sh_pos[1];
+  *lo = pos[0];
+  *hi = pos[1];
 }
 
-// The ring of stages in shared memory.
-struct W4Ring {
-  uint8_t* base;
-  uint64_t* full;
-  uint64_t* empty;
-  volatile int* abort_flag;
-  int s;
-  uint32_t ph;
-  __device__ __forceinline__ void next(int stages) {
-    if (++s == stages) {
-      s = 0;
-      ph ^= 1u;
+// Walks the units of a range, every tl-th from a first one on, in runs of tiles
+// that share their expert and records.
+template <int NT>
+struct W4Walk {
+  int entry, chunk, tile;  // next unit
+  int chunks;              // of the entry
+  int4 t;
+  __device__ __forceinline__ void open(const W4Args& a, int nt) {
+    for (chunks = 0; entry < nt; ++entry) {
+      t = a.tiles[entry];
+      chunks = w4_chunks<NT>(a, t);
+      if (chunks > 0) return;
     }
+  }
+  __device__ __forceinline__ void start(const W4Args& a, int nt, const W4Pos& lo, int skip) {
+    entry = lo.entry;
+    chunk = 0;
+    tile = lo.unit + skip;
+    open(a, nt);
+  }
+  // Tiles of the run that starts at the next unit: 0 at the end of the range.
+  __device__ __forceinline__ int run(const W4Args& a, int nt, const W4Pos& hi) {
+    while (tile >= a.m.tiles && entry < nt) {
+      tile -= a.m.tiles;
+      if (++chunk >= chunks) {
+        chunk = 0;
+        ++entry;
+        open(a, nt);
+      }
+    }
+    if (entry >= nt || entry > hi.entry) return 0;
+    const int end =
+        entry == hi.entry ? min(a.m.tiles, hi.unit - chunk * a.m.tiles) : a.m.tiles;
+    return end > tile ? (end - tile + a.p.tl - 1) >> a.p.tl_shift : 0;
   }
 };
-
-// Copies tiles [tile0, tile0 + n) of expert e into the next stage (one thread).
-__device__ __forceinline__ bool w4_produce(const W4Matrix& m, const W4Plan& p, W4Ring& r, int e,
-                                           int tile0, int n, int* status) {
-  if (!mbar_wait(&r.empty[r.s], r.ph ^ 1u, r.abort_flag, status, kErrTimeoutEmpty)) return false;
-  const uint32_t qb = static_cast<uint32_t>(n) * m.nb * kW4BlockBytes;
-  const uint32_t sb = static_cast<uint32_t>(n) * m.ng * 32, zb = m.z != nullptr ? sb / 2 : 0u;
-  const size_t et = static_cast<size_t>(e) * m.tiles + tile0;
-  uint8_t* dst = r.base + r.s * p.stage_bytes;
-  mbar_arrive_expect_tx(&r.full[r.s], qb + sb + zb);
-  bulk_load(dst, m.q + et * m.nb * kW4BlockBytes, qb, &r.full[r.s]);
-  bulk_load(dst + p.s_off, m.s + et * m.ng * 32, sb, &r.full[r.s]);
-  if (zb != 0) bulk_load(dst + p.z_off, m.z + et * m.ng * 16, zb, &r.full[r.s]);
-  r.next(p.stages);
-  return true;
-}
-
-// After an abort: every copy of the last `issued` stages lands before the CTA exits.
-__device__ __forceinline__ void w4_drain(uint64_t* full, int stages, uint32_t issued) {
-  const uint32_t n = static_cast<uint32_t>(stages);
-  for (uint32_t i = issued > n ? issued - n : 0u; i < issued; ++i) {
-    const unsigned long long t0 = globaltimer_ns();
-    while (!mbar_try_wait(&full[i % n], (i / n) & 1u)) {
-      if (globaltimer_ns() - t0 > kWaitLimitNs) break;
-    }
-  }
-}
 
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-__device__ __forceinline__ uint4 lds128(const uint8_t* p) {
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(smem_u32(p))
-               : "memory");
+               : "r"(addr));
   return v;
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES)
+               : "memory");
 }
 
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-// acc += scale * (codes of one 16 x 64 block - zero points) . records.
-// FOLD (no zero points, group >= 64): the operand is 128 + q and the sum starts
-// at -136 * (sum of the block's activations), `fold`, so the subtraction of
-// 128 + 8 costs nothing; it cancels to within 2^-23 * 136 * sum|x| of the block.
-// Otherwise 128 + z is subtracted from every operand, which is exact.
+// d += (codes of a half block's two words) . records, two of the block's four
+// 16-column steps.  Without FOLD the zero points come off the operands first:
+// z holds 1024 + z of rows g and g + 8 in the halves.
 template <int NT, bool FOLD>
-__device__ __forceinline__ void w4_block(float (&acc)[NT][4], const uint4& w,
-                                         const uint32_t (&b)[NT][8], const float (&fold)[NT][2],
-                                         const uint8_t* sp, const uint8_t* zp, int sg0, int sg1) {
-  uint32_t z0[2] = {0x43084308u, 0x43084308u}, z1[2] = {0x43084308u, 0x43084308u};
-  const uint32_t sc0 = *reinterpret_cast<const uint32_t*>(sp + sg0 * 32);
-  uint32_t sc1 = sc0;
+__device__ __forceinline__ void w4_half(float (&d)[NT][4], uint32_t wl, uint32_t wh, int h,
+                                        const uint32_t (&b)[NT][8], uint32_t z) {
+  uint32_t lo[4], hi[4];
+  w4_pairs(wl, lo);
+  w4_pairs(wh, hi);
   if constexpr (!FOLD) {
-    if (sg1 != sg0) sc1 = *reinterpret_cast<const uint32_t*>(sp + sg1 * 32);
-    if (zp != nullptr) {
-      const uint32_t v0 = *reinterpret_cast<const uint16_t*>(zp + sg0 * 16);
-      const uint32_t v1 = *reinterpret_cast<const uint16_t*>(zp + sg1 * 16);
-      z0[0] = (0x4300u | (v0 & 0xffu)) * 0x10001u;
-      z0[1] = (0x4300u | (v0 >> 8)) * 0x10001u;
-      z1[0] = (0x4300u | (v1 & 0xffu)) * 0x10001u;
-      z1[1] = (0x4300u | (v1 >> 8)) * 0x10001u;
+    const uint32_t zl = __byte_perm(z, 0, 0x1010), zh = __byte_perm(z, 0, 0x3232);
+    const uint32_t yl = (zl & 0x000f000fu) << 4 | 0x54005400u;  // 64 + z
+    const uint32_t yh = (zh & 0x000f000fu) << 4 | 0x54005400u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo[i] = sub_f16x2(lo[i], (i & 1) ? yl : zl);
+      hi[i] = sub_f16x2(hi[i], (i & 1) ? yh : zh);
     }
   }
-  float d[NT][4];
 #pragma unroll
-  for (int st = 0; st < 4; ++st) {
-    const uint32_t wl = st < 2 ? w.x : w.y, wh = st < 2 ? w.z : w.w;
-    const int i = 2 * (st & 1);
-    uint32_t a[4] = {w4_pair(wl, i), w4_pair(wh, i), w4_pair(wl, i + 1), w4_pair(wh, i + 1)};
-    if constexpr (!FOLD) {
-      const uint32_t zl = st < 2 ? z0[0] : z1[0], zh = st < 2 ? z0[1] : z1[1];
-      a[0] = sub_bf16x2(a[0], zl);
-      a[1] = sub_bf16x2(a[1], zh);
-      a[2] = sub_bf16x2(a[2], zl);
-      a[3] = sub_bf16x2(a[3], zh);
-    }
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      if (st == 0 || (!FOLD && st == 2 && sg1 != sg0)) {
-        if (!FOLD && st == 2) {  // group 32: the first half is complete
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            acc[j][c] = fmaf(c < 2 ? bf16_lo(sc0) : bf16_hi(sc0), d[j][c], acc[j][c]);
-        }
-        float c0[4];
-        c0[0] = c0[2] = FOLD ? fold[j][0] : 0.0f;
-        c0[1] = c0[3] = FOLD ? fold[j][1] : 0.0f;
-        mma_16816(d[j], a, b[j][2 * st], b[j][2 * st + 1], c0);
-      } else {
-        mma_16816(d[j], a, b[j][2 * st], b[j][2 * st + 1], d[j]);
-      }
-    }
-  }
+    for (int j = 0; j < NT; ++j)
+      mma_16816(d[j], lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], b[j][4 * h + 2 * s],
+                b[j][4 * h + 2 * s + 1]);
+}
+
+// acc += scale * d: the end of a group (or of the warp's share of it).
+template <int NT>
+__device__ __forceinline__ void w4_flush(float (&acc)[NT][4], const float (&d)[NT][4],
+                                         uint32_t sc) {
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      acc[j][c] = fmaf(c < 2 ? bf16_lo(sc1) : bf16_hi(sc1), d[j][c], acc[j][c]);
+      acc[j][c] = fmaf(c < 2 ? bf16_lo(sc) : bf16_hi(sc), d[j][c], acc[j][c]);
 }
 
-// Record columns (in eights) a warp can hold next to KBT blocks: 128 registers
-// of operands either way.
-template <int KBT>
-constexpr int w4_max_nt() {
-  return KBT <= 4 ? 4 : KBT <= 8 ? 2 : 1;
+// What of a tile is this warp's.
+struct W4Share {
+  int ks, tl;    // its place along K, its place among the tiles worked on at once
+  int kb0, myb;  // its blocks
+  int g0;        // the first group they touch
+};
+
+template <int KB>
+__device__ __forceinline__ W4Share w4_share(const W4Args& a) {
+  // the shuffle tells the compiler that these are the same for the whole warp
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  W4Share s;
+  s.ks = warp & (a.p.ks - 1);
+  s.tl = warp >> a.p.ks_shift;
+  s.myb = max(0, min(KB, a.m.nb - s.ks * KB));
+  s.kb0 = s.myb > 0 ? s.ks * KB : 0;  // a warp without blocks multiplies with zeros
+  s.g0 = (2 * s.kb0) >> a.m.gshift;
+  return s;
 }
 
-// One record chunk's pass over units [u0, u1) of an entry (u counts stages
-// within the chunk): records t.y + rec0 .. + n, n <= 8 NT.  Every consumer
-// warp calls it; a warp whose wait gave up goes on without reading or storing, so the
-// others never wait for it at a barrier.
-template <bool SWIGLU, int KBT, int NT, bool FOLD>
-__device__ __forceinline__ void w4_consume(const W4Args& a, W4Ring& r, float* part, uint32_t& round,
-                                           int rec0, int n, int g0, int g1, bool& ok) {
-  const W4Plan& p = a.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ks = warp % p.ks, tl = warp / p.ks;
-  const int g = lane >> 2, t = lane & 3;
-  const int kb0 = ks * p.kbn;
-  const int myb = max(0, min(p.kbn, a.m.nb - kb0));
-  const int vec = a.m.nb * 8;  // 16-byte vectors per A row
-  uint32_t b[KBT][NT][8];
-  float fold[KBT][NT][2];
+// A chunk's activations as this warp's matrix operand in fp16: its blocks of
+// records rec0 .. rec0 + n (zeros past n and past the last block).  A record's
+// part is scaled by the power of two that puts its largest magnitude in [2^15,
+// 2^16), and `inv` takes it back: a bf16 value within 2^-32 of the largest keeps
+// all its bits, a smaller one loses at most 2^-40 of the largest.
+//
+// Without zero points the weight operand stays 1024 + q or 64 + q, and a group's
+// sum starts at -(1032 or 72) times its activations (`fold`), so the subtraction
+// costs nothing per weight; it cancels to within 2^-23 * 1032 * sum|x|.
+// kW4Half subtracts from every operand instead, which is exact.
+template <int KB, int NT, int MODE>
+__device__ __forceinline__ void w4_load_records(const W4Args& a, const W4Share& sh, int rec0,
+                                                int n, uint32_t (&b)[KB][NT][8],
+                                                float (&fold)[KB][NT][2], float (&inv)[NT][2]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     int row = -1;
@@ -365,206 +375,274 @@ __device__ __forceinline__ void w4_consume(const W4Args& a, W4Ring& r, float* pa
         row = -1;
       }
     }
-    const uint4* src = a.act + static_cast<size_t>(max(row, 0)) * vec + kb0 * 8 + t;
+    const uint32_t* src = a.act + (static_cast<size_t>(max(row, 0)) * a.m.nb + sh.kb0) * 32 + t;
+    uint32_t most = 0;
 #pragma unroll
-    for (int k = 0; k < KBT; ++k) {
-      uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
-      if (row >= 0 && k < myb) {
-        v0 = __ldg(src + k * 8);
-        v1 = __ldg(src + k * 8 + 4);
+    for (int k = 0; k < KB; ++k) {
+      const bool have = row >= 0 && k < sh.myb;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[k][j][i] = have ? __ldg(src + k * 32 + 4 * i) : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = __vmaxu2(most, b[k][j][i] & 0x7fff7fffu);
+    most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int e = static_cast<int>(max(most & 0xffffu, most >> 16) >> 7);  // biased exponent
+    const int up = min(142 - e, 110);
+    const float scale = __int_as_float((127 + up) << 23);
+    const float back = __int_as_float((127 - up) << 23);
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t v = b[k][j][i];
+        const __half2 h = __floats2half2_rn(bf16_lo(v) * scale, bf16_hi(v) * scale);
+        b[k][j][i] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      b[k][j][0] = v0.x, b[k][j][1] = v0.y, b[k][j][2] = v0.z, b[k][j][3] = v0.w;
-      b[k][j][4] = v1.x, b[k][j][5] = v1.y, b[k][j][6] = v1.z, b[k][j][7] = v1.w;
+    // of this lane's columns: records 8j + 2t and 8j + 2t + 1
+    inv[j][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+    inv[j][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+  }
+  if constexpr (MODE != kW4Half) {
+    // a product with the operand of codes 8, per group: kept at its first block
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = KB - 1; k >= 0; --k) {
+        if (MODE == kW4Block || (k & 1)) d[0] = d[1] = d[2] = d[3] = 0.0f;
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+          mma_16816(d, 0x64086408u, 0x64086408u, 0x54805480u, 0x54805480u, b[k][j][2 * st],
+                    b[k][j][2 * st + 1]);
+        fold[k][j][0] = -d[0];
+        fold[k][j][1] = -d[1];
+      }
     }
   }
-  if constexpr (FOLD) {
-    // sums of a block's activations for this lane's columns, as a product with ones
-    const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+}
+
+// acc = this warp's share of a tile (its codes at `slot`, its group records at
+// slot + KB blocks) times the records.
+template <int KB, int NT, int MODE>
+__device__ __forceinline__ void w4_tile(const W4Args& a, const W4Share& sh, uint32_t slot,
+                                        const uint32_t (&b)[KB][NT][8],
+                                        const float (&fold)[KB][NT][2],
+                                        const float (&inv)[NT][2], float (&acc)[NT][4]) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t qp = slot + lane * 16;
+  const uint32_t rec = slot + KB * kW4BlockBytes + (lane >> 2) * a.m.rec;
+  const uint32_t step = 8 * a.m.rec;
+  float d[NT][4];
 #pragma unroll
-    for (int k = 0; k < KBT; ++k)
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
 #pragma unroll
-        for (int st = 0; st < 4; ++st) mma_16816(d, one, b[k][j][2 * st], b[k][j][2 * st + 1], d);
-        fold[k][j][0] = -136.0f * d[0];
-        fold[k][j][1] = -136.0f * d[1];
-      }
-  }
-  for (int gi = g0; gi < g1; ++gi) {
-    const int tile0 = gi * p.ts;
-    const int nt = min(p.ts, a.m.tiles - tile0);
-    if (ok && !mbar_wait(&r.full[r.s], r.ph, r.abort_flag, a.status, kErrTimeoutFull)) ok = false;
-    ok = __all_sync(0xffffffffu, ok);
-    const uint8_t* stage = r.base + r.s * p.stage_bytes;
-    for (int tt = tl; tt < nt; tt += p.tl) {
-      float acc[NT][4];
+  for (int k = 0; k < KB; ++k) {
+    const uint4 w = lds128(qp + k * kW4BlockBytes);
+    if (MODE != kW4TwoBlocks || (k & 1) == 0) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
-      const uint8_t* qp = stage + (tt * a.m.nb + kb0) * kW4BlockBytes + lane * 16;
-      const uint8_t* sp = stage + p.s_off + tt * a.m.ng * 32 + g * 4;
-      const uint8_t* zp = a.m.z != nullptr ? stage + p.z_off + tt * a.m.ng * 16 + g * 2 : nullptr;
-      if (ok) {
+        for (int c = 0; c < 4; ++c) d[j][c] = MODE != kW4Half ? fold[k][j][c & 1] : 0.0f;
+    }
+    if constexpr (MODE != kW4Half) {
+      w4_half<NT, true>(d, w.x, w.z, 0, b[k], 0u);
+      w4_half<NT, true>(d, w.y, w.w, 1, b[k], 0u);
+      if (MODE == kW4TwoBlocks && (k & 1)) w4_flush<NT>(acc, d, lds32(rec + (k >> 1) * step));
+      // a group of 128 may span two of an odd number of blocks: its record serves both
+      if (MODE == kW4Block)
+        w4_flush<NT>(acc, d, lds32(rec + (((2 * (sh.kb0 + k)) >> a.m.gshift) - sh.g0) * step));
+    } else {
 #pragma unroll
-        for (int k = 0; k < KBT; ++k) {
-          if (k < myb) {
-            const int half = 2 * (kb0 + k);
-            w4_block<NT, FOLD>(acc, lds128(qp + k * kW4BlockBytes), b[k], fold[k], sp, zp,
-                               half >> a.m.gshift, (half + 1) >> a.m.gshift);
-          }
-        }
-      }
-      if (p.ks > 1) {
-        // partials of the ks warps: [buffer][warp][value][lane]
-        constexpr int kStride = w4_max_nt<KBT>() * 128;  // the same for every NT
-        float* pw = part + ((round & 1u) * kW4Warps + warp) * kStride + lane;
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t r = rec + (((2 * (sh.kb0 + k) + h) >> a.m.gshift) - sh.g0) * step;
+        const uint32_t z = a.m.rec == 8 ? lds32(r + 4) : 0x64086408u;
+        w4_half<NT, false>(d, h == 0 ? w.x : w.y, h == 0 ? w.z : w.w, h, b[k], z);
+        w4_flush<NT>(acc, d, lds32(r));
+        if (h == 0) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+          for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) pw[(4 * j + c) * 32] = acc[j][c];
-        named_barrier(1 + tl, p.ks * 32);
-        const float* pr = part + ((round & 1u) * kW4Warps + tl * p.ks) * kStride + lane;
-#pragma unroll
-        for (int u = 0; u < 2 * NT; ++u) {
-          if ((u & (p.ks - 1)) == ks) {
-            float s0 = 0.0f, s1 = 0.0f;
-            for (int w = 0; w < p.ks; ++w) {
-              s0 += pr[w * kStride + (4 * (u >> 1) + (u & 1)) * 32];
-              s1 += pr[w * kStride + (4 * (u >> 1) + (u & 1) + 2) * 32];
-            }
-            acc[u >> 1][u & 1] = s0;
-            acc[u >> 1][(u & 1) + 2] = s1;
-          }
-        }
-        ++round;
-      }
-#pragma unroll
-      for (int u = 0; u < 2 * NT; ++u) {
-        const int rec = 8 * (u >> 1) + 2 * t + (u & 1);
-        if ((u & (p.ks - 1)) == ks && rec < n && ok) {
-          const float v0 = acc[u >> 1][u & 1], v1 = acc[u >> 1][(u & 1) + 2];
-          const int tile = tile0 + tt;
-          if constexpr (SWIGLU) {
-            a.out[static_cast<size_t>(rec0 + rec) * a.out_ld + tile * 8 + g] =
-                __float2bfloat16_rn(silu_f(v0) * v1);
-          } else {
-            const int o = a.row_map != nullptr ? __ldg(a.row_map + rec0 + rec) : rec0 + rec;
-            if (o >= 0 && o < a.out_rows) {
-              const float sc = a.row_scale != nullptr ? __ldg(a.row_scale + o) : 1.0f;
-              __nv_bfloat16* dst = a.out + static_cast<size_t>(o) * a.out_ld + tile * 16 + g;
-              dst[0] = __float2bfloat16_rn(v0 * sc);
-              dst[8] = __float2bfloat16_rn(v1 * sc);
-            } else {
-              record_status(a.status, kErrBadRow);
-            }
-          }
+            for (int c = 0; c < 4; ++c) d[j][c] = 0.0f;
         }
       }
     }
-    __syncwarp();
-    if (lane == 0 && ok) mbar_arrive(&r.empty[r.s]);
-    r.next(p.stages);
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[j][c] *= inv[j][c & 1];
+}
+
+// The groups that KB blocks touch at most.
+constexpr int w4_groups(int kb, int gshift) { return ((2 * kb - 2) >> gshift) + 2; }
+
+// Copies this warp's share of a tile into a slot (asynchronously): codes from q
+// on, group records from s on.  Blocks past the last are left as they are (any
+// code times zero is zero), but every record that is read is a real one.
+template <int KB>
+__device__ __forceinline__ void w4_fetch(const W4Args& a, const W4Share& sh, uint32_t slot,
+                                         const uint8_t* q, const uint8_t* s) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 0; k < KB; ++k)
+    if (k < sh.myb) cp_async_16(slot + lane * 16 + k * kW4BlockBytes, q + k * kW4BlockBytes, 16);
+  const uint32_t dst = slot + KB * kW4BlockBytes + lane * a.m.rec;
+  const int groups = w4_groups(KB, a.m.gshift);
+  for (int i = lane >> 3; i < groups; i += 4) {  // four groups of eight records at a time
+    const int from = min(i, a.m.ng - 1 - sh.g0) - (lane >> 3), o = (i - (lane >> 3)) * 8 * a.m.rec;
+    if (a.m.rec == 8) cp_async_small<8>(dst + o, s + from * 64);
+    else cp_async_small<4>(dst + o, s + from * 32);
   }
 }
 
-template <int N>
-__device__ __forceinline__ void setmaxnreg_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void setmaxnreg_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-// Units [lo, hi) of the tile table on this CTA: warp 8 produces, warps 0..7
-// consume.
-template <bool SWIGLU, int KBT, bool FOLD>
-__device__ __forceinline__ void w4_units_loop(const W4Args& a, W4Ring r, float* part, int nt,
-                                              W4Pos lo, W4Pos hi) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// The units [lo, hi) of the tile table on this CTA, NT * 8 records to a chunk at
+// most.  Each group of ks warps takes every tl-th unit.
+template <bool SWIGLU, int KB, int NT, int SLOTS, int MODE>
+__device__ __forceinline__ void w4_units(const W4Args& a, uint8_t* smem, float* part, int nt,
+                                         const W4Pos& lo, const W4Pos& hi) {
   const W4Plan& p = a.p;
-  constexpr int kMaxNT = w4_max_nt<KBT>();
-  if (warp >= kW4Warps) {
-    setmaxnreg_dec<kW4ProducerRegs>();
-    if (warp != kW4Warps || lane != 0) return;
-    uint32_t issued = 0;
-    bool ok = true;
-    for (int e = lo.entry; ok && e <= hi.entry && e < nt; ++e) {
-      const int4 t = a.tiles[e];
-      const int units = w4_units(a, t);
-      const int u1 = e == hi.entry ? min(hi.unit, units) : units;
-      for (int u = e == lo.entry ? lo.unit : 0; u < u1; ++u) {
-        const int tile0 = u % p.groups * p.ts;
-        if (!w4_produce(a.m, p, r, t.x, tile0, min(p.ts, a.m.tiles - tile0), a.status)) {
-          ok = false;
-          break;
-        }
-        ++issued;
+  const W4Share sh = w4_share<KB>(a);
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int warp = sh.tl * p.ks + sh.ks;
+  const uint32_t base = smem_u32(smem) + warp * SLOTS * p.slot_bytes;
+  W4Walk<NT> f, c;  // the next run to fetch, the run to work on
+  c.start(a, nt, lo, sh.tl);
+  f = c;
+  const uint8_t* fq = nullptr;  // next tile to fetch
+  const uint8_t* fsrc = nullptr;
+  int left = f.run(a, nt, hi);
+  uint32_t fslot = base, slot = base;
+  const uint32_t end_slot = base + SLOTS * p.slot_bytes;
+  const int q_tile = a.m.nb * kW4BlockBytes, s_tile = a.m.ng * 8 * a.m.rec;
+  auto aim = [&]() {  // pointers of the run's first tile
+    const size_t et = static_cast<size_t>(f.t.x) * a.m.tiles + f.tile;
+    fq = a.m.q + et * q_tile + sh.kb0 * kW4BlockBytes + lane * 16;
+    fsrc = a.m.s + et * s_tile + (sh.g0 * 8 + lane) * a.m.rec;
+  };
+  if (left > 0) aim();
+  auto fetch = [&]() {
+    if (left > 0) {
+      w4_fetch<KB>(a, sh, fslot, fq, fsrc);
+      fq += static_cast<size_t>(q_tile) << p.tl_shift;
+      fsrc += static_cast<size_t>(s_tile) << p.tl_shift;
+      f.tile += p.tl;
+      if (--left == 0) {
+        left = f.run(a, nt, hi);
+        if (left > 0) aim();
       }
     }
-    if (*r.abort_flag) w4_drain(r.full, p.stages, issued);
-    return;
+    cp_async_commit();
+    fslot += p.slot_bytes;
+    if (fslot == end_slot) fslot = base;
+  };
+#pragma unroll
+  for (int i = 0; i < SLOTS - 1; ++i) fetch();
+  constexpr int kStride = NT * 128;
+  constexpr int kBuffer = kW4Warps * kStride;
+  int buffer = 0;
+  for (int count; (count = c.run(a, nt, hi)) > 0;) {
+    const int rec0 = c.t.y + c.chunk * (8 * NT), n = min(8 * NT, c.t.z - rec0);
+    auto pass = [&](auto nt_c) {
+      constexpr int N = decltype(nt_c)::value;
+      uint32_t b[KB][N][8];
+      float fold[KB][N][2], inv[N][2];
+      w4_load_records<KB, N, MODE>(a, sh, rec0, n, b, fold, inv);
+      // Value pairs u = 2j + c (records 8j + 2t + c) are stored by the warps u
+      // modulo ks: their rows (-1: none) and scales.
+      int orow[2 * N];
+      float scale[2 * N];
+#pragma unroll
+      for (int u = 0; u < 2 * N; ++u) {
+        const int rec = 8 * (u >> 1) + 2 * t + (u & 1);
+        orow[u] = -1;
+        scale[u] = 1.0f;
+        if ((u & (p.ks - 1)) == sh.ks && rec < n) {
+          orow[u] = rec0 + rec;
+          if (!SWIGLU && a.row_map != nullptr) orow[u] = __ldg(a.row_map + rec0 + rec);
+          if (orow[u] < 0 || orow[u] >= a.out_rows) {
+            record_status(a.status, kErrBadRow);
+            orow[u] = -1;
+          } else if (!SWIGLU && a.row_scale != nullptr) {
+            scale[u] = __ldg(a.row_scale + orow[u]);
+          }
+        }
+      }
+      __nv_bfloat16* out = a.out + c.tile * (SWIGLU ? 8 : 16) + g;
+      for (int i = 0; i < count; ++i) {
+        cp_async_wait_group<SLOTS - 2>();
+        __syncwarp();  // every lane's copies have landed, and the last tile's slot is free
+        fetch();
+        float acc[N][4];
+        w4_tile<KB, N, MODE>(a, sh, slot, b, fold, inv, acc);
+        slot += p.slot_bytes;
+        if (slot == end_slot) slot = base;
+        if (p.ks > 1) {
+          // The ks partials of the tile meet in shared memory: [buffer][warp][value]
+          // [lane], two buffers so that one barrier per tile suffices.
+          float* pw = part + buffer + warp * kStride + lane;
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) pw[(4 * j + v) * 32] = acc[j][v];
+          named_barrier(1 + sh.tl, p.ks * 32);
+        }
+#pragma unroll
+        for (int u = 0; u < 2 * N; ++u) {
+          if ((u & (p.ks - 1)) == sh.ks) {
+            float v0 = acc[u >> 1][u & 1], v1 = acc[u >> 1][(u & 1) + 2];
+            if (p.ks > 1) {
+              v0 = v1 = 0.0f;
+              const float* pr =
+                  part + buffer + sh.tl * p.ks * kStride + (4 * (u >> 1) + (u & 1)) * 32 + lane;
+              for (int w = 0; w < p.ks; w += 2) {
+                v0 += pr[0] + pr[kStride];
+                v1 += pr[64] + pr[kStride + 64];
+                pr += 2 * kStride;
+              }
+            }
+            if (orow[u] >= 0) {
+              __nv_bfloat16* dst = out + static_cast<size_t>(orow[u]) * a.out_ld;
+              if constexpr (SWIGLU) {
+                dst[0] = __float2bfloat16_rn(silu_f(v0) * v1);
+              } else {
+                dst[0] = __float2bfloat16_rn(v0 * scale[u]);
+                dst[8] = __float2bfloat16_rn(v1 * scale[u]);
+              }
+            }
+          }
+        }
+        out += p.tl * (SWIGLU ? 8 : 16);
+        buffer ^= kBuffer;
+      }
+    };
+    if (NT > 1 && n > 8) pass(std::integral_constant<int, NT>{});
+    else pass(std::integral_constant<int, 1>{});
+    c.tile += count * p.tl;
   }
-  setmaxnreg_inc<kW4ConsumerRegs>();
-  uint32_t round = 0;
-  bool ok = true;
-  for (int e = lo.entry; e <= hi.entry && e < nt; ++e) {
-    const int4 t = a.tiles[e];
-    const int units = w4_units(a, t);
-    const int u1 = e == hi.entry ? min(hi.unit, units) : units;
-    for (int u = e == lo.entry ? lo.unit : 0; u < u1;) {
-      const int chunk = u / p.groups;
-      const int g0 = u - chunk * p.groups;
-      const int g1 = min(p.groups, g0 + u1 - u);
-      const int rec0 = t.y + chunk * p.nr;
-      const int n = min(p.nr, t.z - rec0);
-      if (kMaxNT >= 4 && n > 16)
-        w4_consume<SWIGLU, KBT, kMaxNT >= 4 ? 4 : 1, FOLD>(a, r, part, round, rec0, n, g0, g1, ok);
-      else if (kMaxNT >= 2 && n > 8)
-        w4_consume<SWIGLU, KBT, kMaxNT >= 2 ? 2 : 1, FOLD>(a, r, part, round, rec0, n, g0, g1, ok);
-      else
-        w4_consume<SWIGLU, KBT, 1, FOLD>(a, r, part, round, rec0, n, g0, g1, ok);
-      u += g1 - g0;
-    }
-  }
+  cp_async_wait_all();  // nothing is in flight when the CTA exits
 }
 
-template <int KBT>
+template <int NT>
 constexpr int w4_part_bytes() {
-  return 2 * kW4Warps * w4_max_nt<KBT>() * 128 * 4;
+  return 2 * kW4Warps * NT * 128 * 4;
 }
-constexpr int kW4RingBytes = 184 * 1024;
-constexpr int kW4TailBytes = 2 * kW4MaxStages * 8 + 16;
+constexpr int kW4SmemBytes = 224 * 1024;
 
-template <bool SWIGLU, int KBT, bool FOLD>
+template <bool SWIGLU, int KB, int NT, int SLOTS, int MODE>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_stream(const W4Args a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  uint8_t* tail = smem_raw + kW4RingBytes + w4_part_bytes<KBT>();
-  W4Ring r;
-  r.base = smem_raw;
-  r.full = reinterpret_cast<uint64_t*>(tail);
-  r.empty = r.full + kW4MaxStages;
-  r.abort_flag = reinterpret_cast<volatile int*>(r.empty + kW4MaxStages);
-  r.s = 0;
-  r.ph = 0;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < a.p.stages; ++s) {
-      mbar_init(&r.full[s], 1);
-      mbar_init(&r.empty[s], kW4Warps);
-    }
-    *r.abort_flag = 0;
-    fence_barrier_init();
-  }
-  __syncthreads();
   pdl_wait();
   pdl_trigger();
   const int nt = max(0, min(*a.num_tiles, a.max_tiles));
   W4Pos lo, hi;
-  w4_range(a, nt, &lo, &hi);
-  w4_units_loop<SWIGLU, KBT, FOLD>(a, r, reinterpret_cast<float*>(smem_raw + kW4RingBytes), nt, lo,
-                                   hi);
+  w4_range<NT>(a, nt, &lo, &hi);
+  w4_units<SWIGLU, KB, NT, SLOTS, MODE>(a, smem_raw + w4_part_bytes<NT>(),
+                                         reinterpret_cast<float*>(smem_raw), nt, lo, hi);
 }
 
 // ------------------------------------------------------------------ launchers
@@ -584,42 +662,38 @@ static bool allow_smem(Kernel* fn, int bytes, std::atomic<uint64_t>& done) {
   return true;
 }
 
-// Cuts a projection over the warps: the fewest idle block slots, then the most
-// warps to a tile (a shorter pass over a tile balances better over the SMs).
-static W4Plan w4_plan(const W4Matrix& m) {
+// Cuts a projection over the warps, kb blocks to each.
+static W4Plan w4_plan(const W4Matrix& m, int kb) {
   W4Plan p{};
-  long long best = -1;
-  for (int ks = kW4Warps; ks >= 1; ks /= 2) {
-    const int kbn = (m.nb + ks - 1) / ks;
-    if (kbn > 16) break;
-    const long long waste = static_cast<long long>(kbn) * ks - m.nb;
-    if (best < 0 || waste * p.kbn * p.ks < best * kbn * ks) {
-      // fewer warps to a tile only while the records still fit (kbn <= 4)
-      if (best >= 0 && kbn > 4) break;
-      best = waste;
-      p.ks = ks;
-      p.kbn = kbn;
+  p.ks = 1;
+  while (p.ks * kb < m.nb) p.ks *= 2;
+  p.tl = kW4Warps / p.ks;
+  while ((1 << p.ks_shift) < p.ks) ++p.ks_shift;
+  while ((1 << p.tl_shift) < p.tl) ++p.tl_shift;
+  p.slot_bytes = kb * kW4BlockBytes + w4_groups(kb, m.gshift) * 8 * m.rec;
+  return p;
+}
+
+// Of the block counts the kernels are built for, the one that leaves the fewest
+// slots idle (then the largest: fewer warps share a tile and add their partials).
+static int w4_best_kb(int nb, std::initializer_list<int> kbs) {
+  int best = 0, best_slots = 0;
+  for (const int kb : kbs) {
+    int ks = 1;
+    while (ks * kb < nb) ks *= 2;
+    if (ks <= kW4Warps && (best == 0 || ks * kb <= best_slots)) {
+      best = kb;
+      best_slots = ks * kb;
     }
   }
-  if (best < 0) return p;
-  p.tl = kW4Warps / p.ks;
-  const int tile_bytes = m.nb * kW4BlockBytes + m.ng * (m.z != nullptr ? 48 : 32);
-  const int want = std::max(1, 12 * 1024 / (p.tl * tile_bytes));
-  p.ts = p.tl * want;
-  p.groups = (m.tiles + p.ts - 1) / p.ts;
-  p.nr = 8 * (p.kbn <= 4 ? 4 : p.kbn <= 8 ? 2 : 1);
-  p.s_off = p.ts * m.nb * kW4BlockBytes;
-  p.z_off = p.s_off + p.ts * m.ng * 32;
-  p.stage_bytes = (p.ts * tile_bytes + 127) / 128 * 128;
-  p.stages = std::min(kW4MaxStages, kW4RingBytes / p.stage_bytes);
-  return p;
+  return best;
 }
 
 static W4Matrix w4_matrix(const W4Bank& bank, bool down) {
   W4Matrix m{};
   m.q = static_cast<const uint8_t*>(down ? bank.w2_q : bank.w13_q);
   m.s = static_cast<const uint8_t*>(down ? bank.w2_s : bank.w13_s);
-  m.z = static_cast<const uint8_t*>(down ? bank.w2_z : bank.w13_z);
+  m.rec = bank.zeros ? 8 : 4;
   m.tiles = down ? bank.H / 16 : bank.I / 8;
   const int K = down ? bank.I : bank.H;
   m.nb = K / 64;
@@ -630,39 +704,56 @@ static W4Matrix w4_matrix(const W4Bank& bank, bool down) {
 
 int w4_check_bank(const W4Bank& b) {
   if (b.E <= 0 || b.H <= 0 || b.I <= 0 || b.w13_q == nullptr || b.w13_s == nullptr ||
-      b.w2_q == nullptr || b.w2_s == nullptr || (b.w13_z == nullptr) != (b.w2_z == nullptr))
+      b.w2_q == nullptr || b.w2_s == nullptr)
     return kRcBadArgument;
   if (b.group != 32 && b.group != 64 && b.group != 128) return kRcUnsupported;
   if (b.H % 64 != 0 || b.I % 64 != 0 || b.H % b.group != 0 || b.I % b.group != 0 ||
       b.H > kW4MaxK || b.I > kW4MaxK || b.E > 1024)
     return kRcUnsupported;
-  for (const void* p : {b.w13_q, b.w13_s, b.w13_z, b.w2_q, b.w2_s, b.w2_z})
+  for (const void* p : {b.w13_q, b.w13_s, b.w2_q, b.w2_s})
     if (!aligned16(p)) return kRcBadArgument;
   return kRcOk;
 }
 
-template <bool SWIGLU, int KBT, bool FOLD>
-static int w4_launch(const W4Args& a, cudaStream_t stream) {
-  constexpr int sh = kW4RingBytes + w4_part_bytes<KBT>() + kW4TailBytes;
+template <bool SWIGLU, int KB, int NT, int SLOTS, int MODE>
+static int w4_launch(W4Args& a, cudaStream_t stream) {
+  a.p = w4_plan(a.m, KB);
+  const int sh = w4_part_bytes<NT>() + kW4Warps * SLOTS * a.p.slot_bytes;
+  if (sh > kW4SmemBytes) return kRcUnsupported;
   static std::atomic<uint64_t> attr{0};
-  if (!allow_smem(w4_stream<SWIGLU, KBT, FOLD>, sh, attr)) return kRcCudaError;
-  const long long units = static_cast<long long>(a.max_tiles) * a.p.groups *
-                          ((kBM + a.p.nr - 1) / a.p.nr);
+  if (!allow_smem(w4_stream<SWIGLU, KB, NT, SLOTS, MODE>, kW4SmemBytes, attr)) return kRcCudaError;
+  const long long units = static_cast<long long>(a.max_tiles) * a.m.tiles;
   const int grid = static_cast<int>(std::min<long long>(units, device_sm_count()));
-  return note_cuda_error(launch_pdl(w4_stream<SWIGLU, KBT, FOLD>, dim3(grid), dim3(kW4Threads), sh,
-                                    stream, a)) == cudaSuccess
+  return note_cuda_error(launch_pdl(w4_stream<SWIGLU, KB, NT, SLOTS, MODE>, dim3(grid),
+                                    dim3(kW4Threads), sh, stream, a)) == cudaSuccess
              ? kRcOk
              : kRcCudaError;
 }
 
+template <bool SWIGLU, int MODE>
+static int w4_dispatch_mode(W4Args& a, cudaStream_t stream) {
+  // Up to about six records per expert a pass takes eight, so that a warp can
+  // hold twice the blocks and half as many warps add partials; beyond, sixteen.
+  const int wide = a.M > 6 * a.E ? w4_best_kb(a.m.nb, {2, 3, 4}) : 0;
+  constexpr int kSlots8 = MODE == kW4Half ? 2 : 3;
+  switch (wide) {
+    case 2: return w4_launch<SWIGLU, 2, 2, 8, MODE>(a, stream);
+    case 3: return w4_launch<SWIGLU, 3, 2, 5, MODE == kW4TwoBlocks ? kW4Block : MODE>(a, stream);
+    case 4: return w4_launch<SWIGLU, 4, 2, 4, MODE>(a, stream);
+  }
+  switch (w4_best_kb(a.m.nb, {4, 6, 8})) {
+    case 4: return w4_launch<SWIGLU, 4, 1, 4, MODE>(a, stream);
+    case 6: return w4_launch<SWIGLU, 6, 1, 3, MODE>(a, stream);
+    case 8: return w4_launch<SWIGLU, 8, 1, kSlots8, MODE>(a, stream);
+  }
+  return kRcUnsupported;
+}
+
 template <bool SWIGLU>
-static int w4_dispatch(const W4Args& a, cudaStream_t stream) {
-  const bool fold = a.m.z == nullptr && a.m.gshift > 0;
-  if (a.p.kbn <= 4)
-    return fold ? w4_launch<SWIGLU, 4, true>(a, stream) : w4_launch<SWIGLU, 4, false>(a, stream);
-  if (a.p.kbn <= 8)
-    return fold ? w4_launch<SWIGLU, 8, true>(a, stream) : w4_launch<SWIGLU, 8, false>(a, stream);
-  return fold ? w4_launch<SWIGLU, 16, true>(a, stream) : w4_launch<SWIGLU, 16, false>(a, stream);
+static int w4_dispatch(W4Args& a, cudaStream_t stream) {
+  if (a.m.rec == 8 || a.m.gshift == 0) return w4_dispatch_mode<SWIGLU, kW4Half>(a, stream);
+  if (a.m.gshift == 1) return w4_dispatch_mode<SWIGLU, kW4Block>(a, stream);
+  return w4_dispatch_mode<SWIGLU, kW4TwoBlocks>(a, stream);
 }
 
 int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* index,
@@ -676,8 +767,7 @@ int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* 
   if (src == nullptr || h_out == nullptr || !aligned16(src)) return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, false);
-  a.p = w4_plan(a.m);
-  a.act = static_cast<const uint4*>(src);
+  a.act = static_cast<const uint32_t*>(src);
   a.act_rows = src_rows;
   a.index = index;
   a.index_div = index_div;
@@ -703,8 +793,7 @@ int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, co
   if (h == nullptr || out == nullptr || !aligned16(h)) return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, true);
-  a.p = w4_plan(a.m);
-  a.act = static_cast<const uint4*>(h);
+  a.act = static_cast<const uint32_t*>(h);
   a.act_rows = M;
   a.index_div = 1;
   a.M = M;
@@ -723,16 +812,16 @@ int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, co
 
 int launch_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros0,
                    const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E, int N,
-                   int K, int group, void* q, void* s, void* z, int* status, cudaStream_t stream) {
+                   int K, int group, void* q, void* s, int* status, cudaStream_t stream) {
   if (codes0 == nullptr || scales0 == nullptr || q == nullptr || s == nullptr ||
-      (codes1 == nullptr) != (scales1 == nullptr) || (z == nullptr) != (zeros0 == nullptr) ||
+      (codes1 == nullptr) != (scales1 == nullptr) ||
       (codes1 != nullptr && (zeros0 == nullptr) != (zeros1 == nullptr)) ||
       (codes1 == nullptr && zeros1 != nullptr) || E <= 0 || N <= 0 || K <= 0)
     return kRcBadArgument;
   if ((group != 32 && group != 64 && group != 128) || K % 64 != 0 || K % group != 0 ||
       K > kW4MaxK || N % (codes1 != nullptr ? 8 : 16) != 0 || E > 1024)
     return kRcUnsupported;
-  if (!aligned16(q) || !aligned16(s) || !aligned16(z) || !aligned16(codes0) || !aligned16(codes1))
+  if (!aligned16(q) || !aligned16(s) || !aligned16(codes0) || !aligned16(codes1))
     return kRcBadArgument;
   W4PackArgs a{};
   a.codes[0] = codes0;
@@ -747,7 +836,6 @@ int launch_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* ze
   a.group = group;
   a.q = static_cast<uint8_t*>(q);
   a.s = static_cast<uint16_t*>(s);
-  a.z = static_cast<uint8_t*>(z);
   a.status = status;
   return note_cuda_error(launch_pdl(w4_pack, dim3(device_sm_count() * 8), dim3(256), 0, stream,
                                     a)) == cudaSuccess

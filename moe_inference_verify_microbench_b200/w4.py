@@ -75,18 +75,18 @@ class W4Experts:
     """Packed 4-bit expert weights (w_gate, w_up [E, I, H], w_down [E, H, I])."""
 
     def __init__(self, w13, w2, num_experts: int, hidden: int, intermediate: int,
-                 group_size: int) -> None:
-        """Use ``from_codes`` or ``quantize``; w13 and w2 are packed (q, s, z)."""
+                 group_size: int, has_zeros: bool) -> None:
+        """Use ``from_codes`` or ``quantize``; w13 and w2 are packed (q, s)."""
         self.w13, self.w2 = w13, w2
         self.num_experts, self.hidden, self.intermediate = num_experts, hidden, intermediate
-        self.group_size = group_size
+        self.group_size, self.has_zeros = group_size, has_zeros
         self.device = w13[0].device
-        ptr = [None if t is None else t.data_ptr() for t in (*w13, *w2)]
-        self._struct = _native.W4BankStruct(*ptr, num_experts, hidden, intermediate, group_size)
+        self._struct = _native.W4BankStruct(*(t.data_ptr() for t in (*w13, *w2)), num_experts,
+                                            hidden, intermediate, group_size, int(has_zeros))
         self.native = ctypes.addressof(self._struct)  # const moe_w4_bank*
 
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (*self.w13, *self.w2) if t is not None)
+        return sum(t.numel() * t.element_size() for t in (*self.w13, *self.w2))
 
     @classmethod
     @torch.no_grad()
@@ -135,7 +135,7 @@ class W4Experts:
         if code:
             raise ValueError(f"codes and zero points must be in 0..15 "
                              f"({_native.error_string(code)})")
-        return cls(w13, w2, E, H, I, group)
+        return cls(w13, w2, E, H, I, group, gz is not None)
 
     @classmethod
     @torch.no_grad()
@@ -159,11 +159,11 @@ def _pack(first, second, group: int, status: torch.Tensor):
     M = N if second is None else 2 * N
     dev = codes.device
     q = torch.empty(E * M * K // 2, dtype=torch.uint8, device=dev)
-    s = torch.empty(E * M * (K // group), dtype=torch.bfloat16, device=dev)
-    z = None if zeros is None else torch.empty(s.numel(), dtype=torch.uint8, device=dev)
+    s = torch.empty(E * M * (K // group) * (1 if zeros is None else 2), dtype=torch.bfloat16,
+                    device=dev)
     p = ops._p
     c1, s1, z1 = second if second is not None else (None, None, None)
     ops._rc(_native.load().moe_w4_pack(p(codes), p(scales), p(zeros), p(c1), p(s1), p(z1), E, N, K,
-                                       group, p(q), p(s), p(z), p(status), ops._stream(dev)),
+                                       group, p(q), p(s), p(status), ops._stream(dev)),
             "moe_w4_pack")
-    return q, s, z
+    return q, s

@@ -58,11 +58,10 @@ P = ctypes.c_void_p(4096)  # stand-in address, never dereferenced
 
 
 def bank(E=16, H=256, I=128, group=64, **ptr):
-    fields = dict(w13_q=4096, w13_s=4096, w13_z=None, w2_q=4096, w2_s=4096, w2_z=None)
+    fields = dict(w13_q=4096, w13_s=4096, w2_q=4096, w2_s=4096)
     fields.update(ptr)
-    return ctypes.byref(_native.W4BankStruct(*[fields[n] for n in ("w13_q", "w13_s", "w13_z",
-                                                                   "w2_q", "w2_s", "w2_z")],
-                                             E, H, I, group))
+    return ctypes.byref(_native.W4BankStruct(fields["w13_q"], fields["w13_s"], fields["w2_q"],
+                                             fields["w2_s"], E, H, I, group, 0))
 
 
 def layer(b, T=4, k=4, x=P, wr=P, ws=P, ws_bytes=1 << 40, y=P):
@@ -85,7 +84,6 @@ def test_calls_are_refused_on_the_host(call):
     assert call(bank(I=64, group=128)) == -2
     assert call(bank(H=8256)) == -2
     assert call(bank(w13_q=None)) == -1
-    assert call(bank(w13_z=4096)) == -1          # zero points for one projection only
     assert call(bank(w2_q=4100)) == -1           # misaligned
     assert call(bank(), x=None) == -1
     assert call(bank(), y=None) == -1
@@ -127,15 +125,13 @@ def test_grouped_calls_are_refused_on_the_host():
 def test_pack_is_refused_on_the_host():
     pack = _native.load().moe_w4_pack
 
-    def call(c0=P, s0=P, z0=None, c1=None, s1=None, z1=None, E=2, N=64, K=128, group=64, q=P, s=P,
-             z=None):
-        return pack(c0, s0, z0, c1, s1, z1, E, N, K, group, q, s, z, None, None)
+    def call(c0=P, s0=P, z0=None, c1=None, s1=None, z1=None, E=2, N=64, K=128, group=64, q=P, s=P):
+        return pack(c0, s0, z0, c1, s1, z1, E, N, K, group, q, s, None, None)
 
     assert call(c0=None) == -1
     assert call(c1=P) == -1
-    assert call(z0=P) == -1
-    assert call(z=P) == -1
-    assert call(c1=P, s1=P, z0=P, z=P) == -1
+    assert call(z1=P) == -1
+    assert call(c1=P, s1=P, z0=P) == -1
     assert call(E=0) == -1
     assert call(group=16) == -2
     assert call(K=96) == -2

@@ -33,18 +33,18 @@ def values(m):
 
 
 def operand_sums(m, x, e):
-    """sum_k s * 144 * |x_k| per (row of x, output): what the fp32 sums of
-    products with 128 + q are formed from, in absolute value."""
+    """sum_k s * 1040 * |x_k| per (row of x, output): what the fp32 sums of products
+    with 1024 + q are formed from, in absolute value."""
     codes, scales, _ = m
     g = codes.shape[-1] // scales.shape[-1]
-    wide = scales[e].double().abs().repeat_interleave(g, dim=1) * 144.0
+    wide = scales[e].double().abs().repeat_interleave(g, dim=1) * 1040.0
     return x.double().abs() @ wide.t()
 
 
-# A product is summed in a chain of at most a few dozen fp32 additions (four matrix
-# instructions per block, then the blocks and warps), each off by at most 2^-23
-# of the absolute sum where the tensor core truncates: 2^-18 of it covers them.
-ACC = 2.0 ** -18
+# A group is summed by eight matrix instructions at most, each adding 17 numbers that
+# are off by at most 2^-24 of the largest: 8 * 17 * 2^-24 < 2^-16 of the absolute sum,
+# which also covers the few fp32 additions of groups and warps.
+ACC = 2.0 ** -16
 
 
 def swiglu_rows(w_gate, w_up, vg, vu, x, e):
