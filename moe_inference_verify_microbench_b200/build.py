@@ -20,7 +20,7 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libmoe_b200.so")
 SOURCES = ["capi.cu", "gemm.cu", "sort_align.cu", "rows.cu", "sort_align_static.cu", "decode.cu",
-           "ep_plan.cu", "ep_peer.cu", "w4.cu"]
+           "ep_plan.cu", "ep_peer.cu", "w4.cu", "w4_gemm.cu"]
 HEADERS = ["ptx.cuh", "grouped_gemm.cuh", "grouped_gemm_pair.cuh", "internal.h", "sort_block.cuh",
            "router_splitk.cuh", "w4.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -134,13 +134,14 @@ bool w4_count_ok(int T, int k) {
 
 // The experts' products of sorted records and the weighted sum per token.
 int w4_products(const W4Bank& b, const W4Layout& l, const void* x, const int* ids, const float* w,
-                int T, int k, int e_begin, void* y, int* status, cudaStream_t stream) {
-  const int R = T * k;
-  int rc = launch_w4_w13(b, x, T, l.perm, k, R, l.tiles, l.num_tiles, l.max_tiles, l.h, status,
-                         stream);
+                int T, int k, int num_experts, int e_begin, void* y, int* status,
+                cudaStream_t stream) {
+  const int R = T * k, avg = R / num_experts;
+  int rc = launch_w4_w13(b, x, T, l.perm, k, R, l.tiles, l.num_tiles, l.max_tiles, l.h, avg,
+                         status, stream);
   if (rc != kRcOk) return rc;
-  rc = launch_w4_w2(b, l.h, R, l.tiles, l.num_tiles, l.max_tiles, l.perm, w, l.slots, R, status,
-                    stream);
+  rc = launch_w4_w2(b, l.h, R, l.tiles, l.num_tiles, l.max_tiles, l.perm, w, l.slots, R, avg,
+                    status, stream);
   if (rc != kRcOk) return rc;
   return launch_combine(l.slots, R, nullptr, nullptr, ids, e_begin, e_begin + b.E, T, k, b.H, y,
                         status, stream);
@@ -569,8 +570,8 @@ int moe_grouped_w13_swiglu_w4(const void* src, int src_rows, const int32_t* inde
                               cudaStream_t stream) {
   if (bank == nullptr) return kRcBadArgument;
   return launch_w4_w13(w4_bank(*bank), src, src_rows, index, index_div, M,
-                       reinterpret_cast<const int4*>(tiles), num_tiles, max_tiles, h, status,
-                       stream);
+                       reinterpret_cast<const int4*>(tiles), num_tiles, max_tiles, h,
+                       bank->E > 0 ? M / bank->E : 0, status, stream);
 }
 
 int moe_grouped_w2_w4(const void* h, int M, const int32_t* tiles, const int32_t* num_tiles,
@@ -579,7 +580,8 @@ int moe_grouped_w2_w4(const void* h, int M, const int32_t* tiles, const int32_t*
                       cudaStream_t stream) {
   if (bank == nullptr) return kRcBadArgument;
   return launch_w4_w2(w4_bank(*bank), h, M, reinterpret_cast<const int4*>(tiles), num_tiles,
-                      max_tiles, row_map, slot_scale, out, out_rows, status, stream);
+                      max_tiles, row_map, slot_scale, out, out_rows,
+                      bank->E > 0 ? M / bank->E : 0, status, stream);
 }
 
 size_t moe_w4_experts_workspace_bytes(int T, int top_k, const moe_w4_bank* bank) {
@@ -610,7 +612,7 @@ int moe_w4_experts_forward(const void* x, const int32_t* ids, const float* weigh
                          l.counts, l.offsets, nullptr, l.perm, nullptr, l.tiles, l.max_tiles,
                          l.num_tiles, status, stream);
   if (rc != kRcOk) return rc;
-  return w4_products(b, l, x, ids, weights, T, top_k, e_begin, y, status, stream);
+  return w4_products(b, l, x, ids, weights, T, top_k, num_experts, e_begin, y, status, stream);
 }
 
 size_t moe_w4_layer_workspace_bytes(int T, int top_k, const moe_w4_bank* bank) {
@@ -651,7 +653,7 @@ int moe_w4_layer_forward(const void* x, const void* router_weight, const float* 
                            status, stream);
     if (rc != kRcOk) return rc;
   }
-  return w4_products(b, l, x, l.ids, l.w, T, top_k, 0, y, status, stream);
+  return w4_products(b, l, x, l.ids, l.w, T, top_k, b.E, 0, y, status, stream);
 }
 
 }  // extern "C"

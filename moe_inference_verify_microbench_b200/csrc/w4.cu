@@ -20,8 +20,6 @@
 // group (or a warp's share of it) is summed on the tensor cores in fp32 and
 // then scaled in fp32, so no weight is ever rounded to bf16.
 #include <algorithm>
-#include <atomic>
-#include <cuda_fp16.h>
 #include <initializer_list>
 #include <type_traits>
 
@@ -113,35 +111,11 @@ __global__ void __launch_bounds__(256) w4_pack(const W4PackArgs a) {
 
 // ------------------------------------------------------------------ streaming
 
-struct W4Args {
-  W4Matrix m;
-  W4Plan p;
-  const uint32_t* act;  // A rows [act_rows][K], bf16 pairs
-  int act_rows;
-  const int* index;     // A row of record p = act[index[p] / index_div] (null = p)
-  int index_div;
-  int M;                // records
-  const int4* tiles;
-  const int* num_tiles;
-  int max_tiles;
-  int E;
-  __nv_bfloat16* out;
-  int out_ld;
-  int out_rows;
-  const int* row_map;
-  const float* row_scale;
-  int* status;
-};
-
 // Work of a tile-table entry: its records in chunks of 8 NT, each chunk one pass
 // over the expert's tiles (units).  A bad entry has none and is reported.
 template <int NT>
 __device__ __forceinline__ int w4_chunks(const W4Args& a, const int4& t) {
-  if (t.x < 0 || t.x >= a.E || t.y < 0 || t.z > a.M || t.z <= t.y) {
-    if (t.z != t.y || t.x < 0 || t.x >= a.E)
-      record_status(a.status, t.x < 0 || t.x >= a.E ? kErrBadExpert : kErrBadRow);
-    return 0;
-  }
+  if (!w4_entry_ok(a, t)) return 0;
   return static_cast<int>(static_cast<unsigned>(t.z - t.y + 8 * NT - 1) / (8u * NT));
 }
 
@@ -263,24 +237,6 @@ struct W4Walk {
     return end > tile ? (end - tile + a.p.tl - 1) >> a.p.tl_shift : 0;
   }
 };
-
-__device__ __forceinline__ void named_barrier(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr));
-  return v;
-}
-
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
 
 template <int BYTES>
 __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
@@ -647,21 +603,6 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_stream(const W4Args a) {
 
 // ------------------------------------------------------------------ launchers
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-template <class Kernel>
-static bool allow_smem(Kernel* fn, int bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const uint64_t bit = 1ull << (dev & 63);
-  if ((done.load(std::memory_order_acquire) & bit) != 0) return true;
-  if (note_cuda_error(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           bytes)) != cudaSuccess)
-    return false;
-  done.fetch_or(bit, std::memory_order_acq_rel);
-  return true;
-}
-
 // Cuts a projection over the warps, kb blocks to each.
 static W4Plan w4_plan(const W4Matrix& m, int kb) {
   W4Plan p{};
@@ -715,6 +656,8 @@ int w4_check_bank(const W4Bank& b) {
   return kRcOk;
 }
 
+#include <cstdlib>
+static int w4_tc_min() { const char* e = getenv("W4TC"); return e ? atoi(e) : 12; }
 template <bool SWIGLU, int KB, int NT, int SLOTS, int MODE>
 static int w4_launch(W4Args& a, cudaStream_t stream) {
   a.p = w4_plan(a.m, KB);
@@ -734,7 +677,7 @@ template <bool SWIGLU, int MODE>
 static int w4_dispatch_mode(W4Args& a, cudaStream_t stream) {
   // Up to about six records per expert a pass takes eight, so that a warp can
   // hold twice the blocks and half as many warps add partials; beyond, sixteen.
-  const int wide = a.M > 6 * a.E ? w4_best_kb(a.m.nb, {2, 3, 4}) : 0;
+  const int wide = a.avg > 6 ? w4_best_kb(a.m.nb, {2, 3, 4}) : 0;
   constexpr int kSlots8 = MODE == kW4Half ? 2 : 3;
   switch (wide) {
     case 2: return w4_launch<SWIGLU, 2, 2, 8, MODE>(a, stream);
@@ -751,6 +694,7 @@ static int w4_dispatch_mode(W4Args& a, cudaStream_t stream) {
 
 template <bool SWIGLU>
 static int w4_dispatch(W4Args& a, cudaStream_t stream) {
+  if (a.avg >= w4_tc_min()) return w4_gemm(a, SWIGLU, stream);
   if (a.m.rec == 8 || a.m.gshift == 0) return w4_dispatch_mode<SWIGLU, kW4Half>(a, stream);
   if (a.m.gshift == 1) return w4_dispatch_mode<SWIGLU, kW4Block>(a, stream);
   return w4_dispatch_mode<SWIGLU, kW4TwoBlocks>(a, stream);
@@ -758,13 +702,13 @@ static int w4_dispatch(W4Args& a, cudaStream_t stream) {
 
 int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* index,
                   int index_div, int M, const int4* tiles, const int* num_tiles, int max_tiles,
-                  void* h_out, int* status, cudaStream_t stream) {
+                  void* h_out, int avg, int* status, cudaStream_t stream) {
   if (const int rc = w4_check_bank(bank); rc != kRcOk) return rc;
   if (M < 0 || max_tiles < 0 || index_div <= 0 || src_rows < 0 || tiles == nullptr ||
       num_tiles == nullptr)
     return kRcBadArgument;
   if (M == 0 || max_tiles == 0) return kRcOk;
-  if (src == nullptr || h_out == nullptr || !aligned16(src)) return kRcBadArgument;
+  if (src == nullptr || h_out == nullptr || !aligned16(src) || !aligned16(h_out)) return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, false);
   a.act = static_cast<const uint32_t*>(src);
@@ -779,18 +723,19 @@ int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* 
   a.out = static_cast<__nv_bfloat16*>(h_out);
   a.out_ld = bank.I;
   a.out_rows = M;
+  a.avg = avg;
   a.status = status;
   return w4_dispatch<true>(a, stream);
 }
 
 int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
                  int max_tiles, const int* row_map, const float* row_scale, void* out,
-                 int out_rows, int* status, cudaStream_t stream) {
+                 int out_rows, int avg, int* status, cudaStream_t stream) {
   if (const int rc = w4_check_bank(bank); rc != kRcOk) return rc;
   if (M < 0 || max_tiles < 0 || out_rows < 0 || tiles == nullptr || num_tiles == nullptr)
     return kRcBadArgument;
   if (M == 0 || max_tiles == 0) return kRcOk;
-  if (h == nullptr || out == nullptr || !aligned16(h)) return kRcBadArgument;
+  if (h == nullptr || out == nullptr || !aligned16(h) || !aligned16(out)) return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, true);
   a.act = static_cast<const uint32_t*>(h);
@@ -806,6 +751,7 @@ int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, co
   a.out_rows = out_rows;
   a.row_map = row_map;
   a.row_scale = row_scale;
+  a.avg = avg;
   a.status = status;
   return w4_dispatch<false>(a, stream);
 }

@@ -17,6 +17,10 @@
 // one thread ends up with both and applies the SwiGLU without an exchange.
 #pragma once
 
+#include <atomic>
+#include <cuda_fp16.h>
+
+#include "internal.h"
 #include "ptx.cuh"
 
 namespace moe {
@@ -77,5 +81,72 @@ enum W4Mode : int { kW4TwoBlocks = 0, kW4Block = 1, kW4Half = 2 };
 
 constexpr int kW4Warps = 16;
 constexpr int kW4Threads = 32 * kW4Warps;
+
+// Operands of a grouped product with 4-bit weights.
+struct W4Args {
+  W4Matrix m;
+  W4Plan p;
+  const uint32_t* act;  // A rows [act_rows][K], bf16 pairs
+  int act_rows;
+  const int* index;     // A row of record p = act[index[p] / index_div] (null = p)
+  int index_div;
+  int M;                // records
+  const int4* tiles;
+  const int* num_tiles;
+  int max_tiles;
+  int E;
+  __nv_bfloat16* out;
+  int out_ld;
+  int out_rows;
+  const int* row_map;
+  const float* row_scale;
+  int avg;              // records per expert to expect (chooses the kernel)
+  int* status;
+};
+
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+// Whether a tile-table entry is an expert's row range of at most kBM rows; a bad one is
+// reported (an empty one is not) and skipped.
+__device__ __forceinline__ bool w4_entry_ok(const W4Args& a, const int4& t) {
+  if (t.x >= 0 && t.x < a.E && t.y >= 0 && t.y < t.z && t.z <= a.M && t.z - t.y <= 128) return true;
+  if (t.x < 0 || t.x >= a.E) record_status(a.status, kErrBadExpert);
+  else if (t.y != t.z) record_status(a.status, kErrBadRow);
+  return false;
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <class Kernel>
+bool allow_smem(Kernel* fn, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if ((done.load(std::memory_order_acquire) & bit) != 0) return true;
+  if (note_cuda_error(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           bytes)) != cudaSuccess)
+    return false;
+  done.fetch_or(bit, std::memory_order_acq_rel);
+  return true;
+}
+
+// The tensor-core form for experts with many records (w4_gemm.cu).
+int w4_gemm(const W4Args& a, bool swiglu, cudaStream_t stream);
 
 }  // namespace moe

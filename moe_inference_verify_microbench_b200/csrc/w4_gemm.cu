@@ -1,0 +1,581 @@
+// Grouped products with 4-bit expert weights on tcgen05, for experts with many
+// records (layout: w4.cuh; the form for few records: w4.cu).
+//
+// The weights are the 128-row operand and live in tensor memory: sixteen warps turn
+// codes into bf16 s * (q - z) in registers, in the fragment order that
+// tcgen05.st.16x128b writes, so the dequantised weights never touch shared
+// memory, whose bandwidth the operand reads of 128-row tiles would fill.  The
+// records are the N operand (16 to 128 columns of one tile-table entry) in
+// shared memory, and the accumulators hold D[weight row][record].  So a pass
+// over an expert's weights costs the same integer work for 16 records as for
+// 128: about 60 instructions per 16 x 64 block (28 to extract, 32 to subtract
+// and scale), which together with the stream of codes bounds small N; the
+// tensor pipe bounds N = 128.
+//
+// Work unit: (tile-table entry, 16 packed tiles), i.e. 256 weight rows as two
+// operands of 128 that share the records: for the gate/up product the gate rows
+// and the up rows of the same 128 outputs (the two accumulators then hold gate
+// and up in the same lane and column), for the down product two runs of 128 rows.
+//
+// CTA (896 threads, one per SM, persistent):
+//   warps 0..15   dequantise: warp w writes lane quarter w % 4; warps 0..7 take the
+//                 even 64-column blocks, 8..15 the odd ones
+//   warps 16..19  epilogue: tensor memory -> bf16 -> staging rows -> bulk stores
+//   warps 20..23  gather the records' rows (cp.async into the 128-byte swizzle)
+//   warp 24       bulk copies of codes and group records into a ring
+//   warp 25       issues tcgen05.mma: 2 operands x 4 steps of 16 columns per block
+//   warp 26       allocates tensor memory
+//   warp 27       publishes gathered stages to the async proxy
+//
+// A weight is rounded once, s * (q - z) to bf16: the operand's type.  That is
+// 2^-9 of it in the mean, like the rounding of the activations themselves; the
+// sums stay fp32.
+#include <algorithm>
+
+#include "grouped_gemm.cuh"
+#include "w4.cuh"
+
+namespace moe {
+
+namespace {
+
+constexpr int kTcStages = 4;      // operand stages (64 columns): tensor memory and records
+constexpr int kTcRing = 3;        // code stages (256 columns)
+constexpr int kTcTiles = 16;      // packed tiles per unit
+constexpr int kTcBlocks = 4;      // blocks per code stage
+constexpr int kTcRows = 128;      // records per unit at most
+constexpr int kTcDequantWarps = 16;
+constexpr int kTcEpiWarp = 16, kTcLoadWarp = 20, kTcCopyWarp = 24, kTcMmaWarp = 25,
+              kTcAllocWarp = 26, kTcForwardWarp = 27;
+constexpr int kTcThreads = 28 * 32;
+constexpr int kTcBBytes = kTcRows * 128;
+constexpr int kTcOutBytes = kTcRows * 256;  // staging: 128 records x 128 outputs
+constexpr int kTcCodeBytes = kTcTiles * kTcBlocks * kW4BlockBytes;
+constexpr uint32_t kTcOperandCol = 256;     // accumulators below, operand stages above
+
+struct TcArgs {
+  W4Args a;
+  int ring_bytes;  // code stage: codes, then records
+  int rec_stride;  // bytes of a tile's records in it
+};
+
+__device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]^T, bf16 inputs, fp32 accumulate.
+__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// The column pairs of a word as bf16 s * (q - z): 0x4300 is 128.0 and a code is
+// the last four bits of the mantissa; 128 + q - (128 + z) is exact, the product
+// is rounded once.
+__device__ __forceinline__ void w4_scaled_pairs(uint32_t w, uint32_t z, uint32_t s, uint32_t* r,
+                                                int stride) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;"
+        : "=r"(v)
+        : "r"(w >> (4 * i)), "n"(0x000f000f), "r"(0x43004300u));
+    asm("sub.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(v), "r"(z));
+    asm("mul.bf16x2 %0, %1, %2;" : "=r"(r[i * stride]) : "r"(v), "r"(s));
+  }
+}
+
+// Which accumulator columns a unit uses.  Up to 64 records: one of two halves of
+// 128 columns in turn, so that the epilogue of a unit overlaps the next unit's
+// products; more: all 256.
+struct TcAcc {
+  uint32_t used[2] = {0, 0}, filled[2] = {0, 0};
+  int next = 0;
+  int first, last;     // halves of the current unit
+  uint32_t d0, d1;     // its columns
+  __device__ __forceinline__ void take(int n) {
+    const bool small = n <= 64;
+    first = small ? next : 0;
+    last = small ? next : 1;
+    next = small ? next ^ 1 : 0;
+    d0 = first * 128;
+    d1 = d0 + (small ? 64 : 128);
+  }
+};
+
+// Units of the grid in turn: entry, 16-tile group, and whether there is work.
+struct TcUnit {
+  int4 t;
+  int m;
+  bool ok;
+};
+__device__ __forceinline__ TcUnit tc_unit(const W4Args& a, int w, int groups) {
+  TcUnit u;
+  const int e = w / groups;
+  u.m = w - e * groups;
+  u.t = a.tiles[e];
+  u.ok = w4_entry_ok(a, u.t);
+  return u;
+}
+
+template <bool SWIGLU>
+__global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const W4Args& a = args.a;
+  uint8_t* sB = smem;
+  uint8_t* sOut = sB + kTcStages * kTcBBytes;
+  uint8_t* sRing = sOut + kTcOutBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sRing + kTcRing * args.ring_bytes);
+  uint64_t* empty = full + kTcStages;
+  uint64_t* gat = empty + kTcStages;
+  uint64_t* qfull = gat + kTcStages;
+  uint64_t* qempty = qfull + kTcRing;
+  uint64_t* acc_full = qempty + kTcRing;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_row = reinterpret_cast<int*>(tmem_slot + 2);
+  float* s_scale = reinterpret_cast<float*>(s_row + kTcRows);
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kTcStages; ++s) {
+      mbar_init(&full[s], kTcDequantWarps / 2 + 1);  // half of the dequantising warps, forwarder
+      mbar_init(&empty[s], 1);
+      mbar_init(&gat[s], 128);
+    }
+    for (int s = 0; s < kTcRing; ++s) {
+      mbar_init(&qfull[s], 1);
+      mbar_init(&qempty[s], kTcDequantWarps);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == kTcAllocWarp) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  const int nt = max(0, min(*a.num_tiles, a.max_tiles));
+  const int groups = (a.m.tiles + kTcTiles - 1) / kTcTiles;
+  const long long units = static_cast<long long>(nt) * groups;
+  const int total = static_cast<int>(min(units, 0x7fffffffLL - static_cast<long long>(gridDim.x)));
+  const int nb = a.m.nb;
+  // columns of a code stage span 8 >> gshift groups
+  const int stage_groups = 8 >> a.m.gshift;
+
+  if (warp < kTcDequantWarps) {
+    // ------------------------------------------------------------ dequantise
+    const int quarter = warp & 3, half = (warp >> 2) & 1, set = warp >> 3;
+    const int g = lane >> 2;
+    // The pair of packed tiles this warp turns into operand rows, and where.
+    const int tile0 = SWIGLU ? 4 * quarter + 2 * half : 8 * half + 2 * quarter;
+    const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
+    uint32_t cnt = 0, rings = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+      const TcUnit u = tc_unit(a, w, groups);
+      if (!u.ok) continue;
+      const bool have = u.m * kTcTiles + tile0 < a.m.tiles;
+      for (int kb = 0; ok && kb < nb; ++kb, ++cnt) {
+        const uint32_t rs = rings % kTcRing;
+        const int bk = kb & (kTcBlocks - 1);
+        if (bk == 0) {  // every warp waits for every code stage, so none releases one early
+          ok = mbar_wait(&qfull[rs], (rings / kTcRing) & 1u, abort_flag, a.status,
+                         kErrTimeoutFull);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        if ((cnt & 1u) == static_cast<uint32_t>(set)) {
+          const uint32_t s = cnt % kTcStages;
+          ok = mbar_wait(&empty[s], ((cnt / kTcStages) & 1u) ^ 1u, abort_flag, a.status,
+                         kErrTimeoutEmpty);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (have) {
+            const uint32_t ring = smem_u32(sRing) + rs * args.ring_bytes;
+            const uint32_t q = ring + (tile0 * kTcBlocks + bk) * kW4BlockBytes + lane * 16;
+            const uint32_t rec =
+                ring + kTcCodeBytes + tile0 * args.rec_stride + g * a.m.rec;
+            const uint4 w0 = lds128(q), w1 = lds128(q + kTcBlocks * kW4BlockBytes);
+            const uint32_t dst = tmem + kTcOperandCol + s * 64 + lanes;
+            // [half block] of {tile 0, tile 1} x {row g, row g + 8}
+            uint32_t sc[2][2][2], zp[2][2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t grp = static_cast<uint32_t>(2 * bk + h) >> a.m.gshift;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t r = rec + i * args.rec_stride + grp * 8 * a.m.rec;
+                const uint32_t sv = lds32(r);
+                sc[h][i][0] = __byte_perm(sv, 0, 0x1010);
+                sc[h][i][1] = __byte_perm(sv, 0, 0x3232);
+                zp[h][i][0] = zp[h][i][1] = 0x43084308u;
+                if (a.m.rec == 8) {  // fp16 1024 + z -> bf16 128 + z
+                  const uint32_t zv = (lds32(r + 4) & 0x000f000fu) | 0x43004300u;
+                  zp[h][i][0] = __byte_perm(zv, 0, 0x1010);
+                  zp[h][i][1] = __byte_perm(zv, 0, 0x3232);
+                }
+              }
+            }
+            uint32_t r[16];
+            if constexpr (SWIGLU) {
+              // gate rows of both tiles, then their up rows, as 16 operand rows each
+              w4_scaled_pairs(w0.x, zp[0][0][0], sc[0][0][0], r, 2);
+              w4_scaled_pairs(w0.y, zp[1][0][0], sc[1][0][0], r + 8, 2);
+              w4_scaled_pairs(w1.x, zp[0][1][0], sc[0][1][0], r + 1, 2);
+              w4_scaled_pairs(w1.y, zp[1][1][0], sc[1][1][0], r + 9, 2);
+              tmem_st_16x128b_x8(dst + (static_cast<uint32_t>(16 * half) << 16), r);
+              w4_scaled_pairs(w0.z, zp[0][0][1], sc[0][0][1], r, 2);
+              w4_scaled_pairs(w0.w, zp[1][0][1], sc[1][0][1], r + 8, 2);
+              w4_scaled_pairs(w1.z, zp[0][1][1], sc[0][1][1], r + 1, 2);
+              w4_scaled_pairs(w1.w, zp[1][1][1], sc[1][1][1], r + 9, 2);
+              tmem_st_16x128b_x8(dst + 32 + (static_cast<uint32_t>(16 * half) << 16), r);
+            } else {
+              w4_scaled_pairs(w0.x, zp[0][0][0], sc[0][0][0], r, 2);
+              w4_scaled_pairs(w0.y, zp[1][0][0], sc[1][0][0], r + 8, 2);
+              w4_scaled_pairs(w0.z, zp[0][0][1], sc[0][0][1], r + 1, 2);
+              w4_scaled_pairs(w0.w, zp[1][0][1], sc[1][0][1], r + 9, 2);
+              tmem_st_16x128b_x8(dst + 32 * half, r);
+              w4_scaled_pairs(w1.x, zp[0][1][0], sc[0][1][0], r, 2);
+              w4_scaled_pairs(w1.y, zp[1][1][0], sc[1][1][0], r + 8, 2);
+              w4_scaled_pairs(w1.z, zp[0][1][1], sc[0][1][1], r + 1, 2);
+              w4_scaled_pairs(w1.w, zp[1][1][1], sc[1][1][1], r + 9, 2);
+              tmem_st_16x128b_x8(dst + 32 * half + (16u << 16), r);
+            }
+            tmem_wait_st();
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
+        }
+        if (bk == kTcBlocks - 1 || kb == nb - 1) {  // this warp is done with the code stage
+          if (lane == 0) mbar_arrive(&qempty[rs]);
+          ++rings;
+        }
+      }
+    }
+  } else if (warp >= kTcEpiWarp && warp < kTcLoadWarp) {
+    // -------------------------------------------------------------- epilogue
+    const int quarter = warp & 3;
+    const int r = threadIdx.x - kTcEpiWarp * 32;  // record this thread stores
+    const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
+    const uint32_t stage = smem_u32(sOut);
+    TcAcc acc;
+    bool ok = true;
+    for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+      const TcUnit u = tc_unit(a, w, groups);
+      if (!u.ok) continue;
+      const int n = u.t.z - u.t.y, cols = (n + 15) & ~15;
+      acc.take(cols);
+      int o = -1;
+      if (r < n) {
+        const int p = u.t.y + r;
+        o = a.row_map != nullptr ? a.row_map[p] : p;
+        if (o < 0 || o >= a.out_rows) {
+          record_status(a.status, kErrBadRow);
+          o = -1;
+        }
+      }
+      s_scale[r] = !SWIGLU && o >= 0 && a.row_scale != nullptr ? a.row_scale[o] : 1.0f;
+      ok = mbar_wait(&acc_full[acc.first], acc.filled[acc.first] & 1u, abort_flag, a.status,
+                     kErrTimeoutAccFull);
+      ok = __all_sync(0xffffffffu, ok);
+      ++acc.filled[acc.first];
+      tc_fence_after();
+      for (int part = 0; part < (SWIGLU ? 1 : 2); ++part) {
+        // outputs of this part: 128 from `first`, fewer at the end of the matrix
+        const int first = SWIGLU ? u.m * 128 : u.m * 256 + part * 128;
+        const int outs = min(128, (SWIGLU ? a.m.tiles * 8 : a.m.tiles * 16) - first);
+        bulk_wait_read();  // the staging rows this thread stored are free
+        named_barrier(1, 128);
+        if (ok && outs > 0) {
+          const uint32_t d = tmem + lanes + (part == 0 ? acc.d0 : acc.d1);
+          const uint32_t dst = stage + (32 * quarter + lane) * 2;
+          for (int c = 0; c < cols; c += 16) {
+            uint32_t v[16];
+            tmem_ld16(d + c, v);
+            if constexpr (SWIGLU) {
+              uint32_t up[16];
+              tmem_ld16(tmem + lanes + acc.d1 + c, up);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                v[i] = __float_as_uint(silu_f(__uint_as_float(v[i])) * __uint_as_float(up[i]));
+            } else {
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                v[i] = __float_as_uint(__uint_as_float(v[i]) * s_scale[c + i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const uint32_t pk = pack_bf16x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+              asm volatile("st.shared.b16 [%0], %1;" ::"r"(dst + (c + i) * 256),
+                           "h"(static_cast<unsigned short>(pk & 0xffffu))
+                           : "memory");
+              asm volatile("st.shared.b16 [%0], %1;" ::"r"(dst + (c + i + 1) * 256),
+                           "h"(static_cast<unsigned short>(pk >> 16))
+                           : "memory");
+            }
+          }
+        }
+        if (SWIGLU || part == 1) {  // the accumulators are read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            for (int b = acc.first; b <= acc.last; ++b) mbar_arrive(&acc_empty[b]);
+          }
+        }
+        fence_proxy_async_smem();
+        named_barrier(1, 128);
+        if (ok && outs > 0 && o >= 0)
+          bulk_store(a.out + static_cast<size_t>(o) * a.out_ld + first, stage + r * 256, outs * 2);
+        bulk_commit();
+      }
+    }
+    bulk_wait_all();
+  } else if (warp >= kTcLoadWarp && warp < kTcCopyWarp) {
+    // -------------------------------------------------------- records' rows
+    // Thread i copies 16-byte chunk i % 8 of records i / 8 + 16 j: eight lanes read
+    // one row's 128 contiguous bytes.
+    const int i = threadIdx.x - kTcLoadWarp * 32;
+    const uint32_t chunk = static_cast<uint32_t>(i & 7);
+    const int row0 = i >> 3;
+    uint32_t cnt = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+      const TcUnit u = tc_unit(a, w, groups);
+      if (!u.ok) continue;
+      const int n = u.t.z - u.t.y, steps = (n + 15) >> 4;
+      const uint8_t* src[8];
+      uint32_t present = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int p = u.t.y + row0 + 16 * j;
+        src[j] = reinterpret_cast<const uint8_t*>(a.act);
+        if (p < u.t.z) {
+          const int row = a.index != nullptr ? a.index[p] / a.index_div : p;
+          if (row >= 0 && row < a.act_rows) {
+            src[j] += static_cast<size_t>(row) * nb * 128 + chunk * 16;
+            present |= 1u << j;
+          } else {
+            record_status(a.status, kErrBadRow);
+          }
+        }
+      }
+      for (int kb = 0; kb < nb; ++kb, ++cnt) {
+        const uint32_t s = cnt % kTcStages;
+        ok = mbar_wait(&empty[s], ((cnt / kTcStages) & 1u) ^ 1u, abort_flag, a.status,
+                       kErrTimeoutEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t base = smem_u32(sB) + s * kTcBBytes;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j < steps) {
+            const uint32_t r = static_cast<uint32_t>(row0 + 16 * j);
+            const bool have = (present >> j) & 1u;
+            cp_async_16(base + r * 128u + ((chunk ^ (r & 7u)) << 4),
+                        have ? src[j] + static_cast<size_t>(kb) * 128 : src[j], have ? 16u : 0u);
+          }
+        }
+        cp_async_arrive_noinc(&gat[s]);
+      }
+    }
+    cp_async_wait_all();  // every copy lands before the CTA can exit
+  } else if (warp == kTcCopyWarp) {
+    // ------------------------------------------------ codes and group records
+    uint32_t rings = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+      const TcUnit u = tc_unit(a, w, groups);
+      if (!u.ok) continue;
+      const int tile0 = u.m * kTcTiles, tiles = min(kTcTiles, a.m.tiles - tile0);
+      const size_t et = static_cast<size_t>(u.t.x) * a.m.tiles + tile0 + lane;
+      for (int kb = 0; kb < nb; kb += kTcBlocks, ++rings) {
+        const uint32_t rs = rings % kTcRing;
+        ok = mbar_wait(&qempty[rs], ((rings / kTcRing) & 1u) ^ 1u, abort_flag, a.status,
+                       kErrTimeoutEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int blocks = min(kTcBlocks, nb - kb);
+        const int g0 = (2 * kb) >> a.m.gshift;
+        const int grps = min(stage_groups, a.m.ng - g0);
+        const uint32_t qb = blocks * kW4BlockBytes, sb = grps * 8 * a.m.rec;
+        if (lane == 0) mbar_arrive_expect_tx(&qfull[rs], tiles * (qb + sb));
+        __syncwarp();
+        if (lane < tiles) {
+          uint8_t* dst = sRing + rs * args.ring_bytes;
+          bulk_load(dst + lane * kTcBlocks * kW4BlockBytes, a.m.q + (et * nb + kb) * kW4BlockBytes,
+                    qb, &qfull[rs]);
+          bulk_load(dst + kTcCodeBytes + lane * args.rec_stride,
+                    a.m.s + (et * a.m.ng + g0) * 8 * a.m.rec, sb, &qfull[rs]);
+        }
+      }
+    }
+    if (*abort_flag && lane == 0) {
+      // Let every copy still in flight land before the CTA exits.
+      for (uint32_t i = rings > kTcRing ? rings - kTcRing : 0u; i < rings; ++i) {
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(&qfull[i % kTcRing], (i / kTcRing) & 1u)) {
+          if (globaltimer_ns() - t0 > kWaitLimitNs) break;
+        }
+      }
+    }
+  } else if (warp == kTcMmaWarp) {
+    if (lane == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      TcAcc acc;
+      uint32_t cnt = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+        const TcUnit u = tc_unit(a, w, groups);
+        if (!u.ok) continue;
+        const int cols = (u.t.z - u.t.y + 15) & ~15;
+        acc.take(cols);
+        for (int b = acc.first; ok && b <= acc.last; ++b) {
+          ok = mbar_wait(&acc_empty[b], (acc.used[b] & 1u) ^ 1u, abort_flag, a.status,
+                         kErrTimeoutAccEmpty);
+          ++acc.used[b];
+        }
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>(cols));
+        const bool second = SWIGLU || u.m * kTcTiles + 8 < a.m.tiles;
+        for (int kb = 0; kb < nb; ++kb, ++cnt) {
+          const uint32_t s = cnt % kTcStages;
+          if (!mbar_wait(&full[s], (cnt / kTcStages) & 1u, abort_flag, a.status,
+                         kErrTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t at = tmem + kTcOperandCol + s * 64;
+          const uint32_t b0 = smem_u32(sB) + s * kTcBBytes;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_bf16_ts(tmem + acc.d0, at + kk * 8, sw128_kmajor_desc(b0 + kk * 32), idesc,
+                           (kb | kk) != 0 ? 1u : 0u);
+          if (second) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_bf16_ts(tmem + acc.d1, at + 32 + kk * 8, sw128_kmajor_desc(b0 + kk * 32),
+                             idesc, (kb | kk) != 0 ? 1u : 0u);
+          }
+          tc_commit(&empty[s]);
+        }
+        if (ok) tc_commit(&acc_full[acc.first]);
+      }
+      // Every MMA issued by this thread has finished once `drain` completes.
+      tc_commit(drain);
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain, 0)) {
+        if (globaltimer_ns() - t0 > kWaitLimitNs) break;
+      }
+    }
+  } else if (warp == kTcForwardWarp) {
+    if (lane == 0) {
+      // ------------------------------------------------------------ forwarder
+      uint32_t cnt = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+        const TcUnit u = tc_unit(a, w, groups);
+        if (!u.ok) continue;
+        for (int kb = 0; kb < nb; ++kb, ++cnt) {
+          const uint32_t s = cnt % kTcStages;
+          if (!mbar_wait(&gat[s], (cnt / kTcStages) & 1u, abort_flag, a.status, kErrTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(&full[s]);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kTcAllocWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool SWIGLU>
+int tc_launch(const W4Args& a, cudaStream_t stream) {
+  TcArgs t{};
+  t.a = a;
+  t.rec_stride = (8 >> a.m.gshift) * 8 * a.m.rec;
+  t.ring_bytes = kTcCodeBytes + kTcTiles * t.rec_stride;
+  const int sh = 1024 + kTcStages * kTcBBytes + kTcOutBytes + kTcRing * t.ring_bytes + 256 +
+                 kTcRows * 8;
+  constexpr int kMost = 1024 + kTcStages * kTcBBytes + kTcOutBytes +
+                        kTcRing * (kTcCodeBytes + kTcTiles * 512) + 256 + kTcRows * 8;
+  static_assert(kMost <= 227 * 1024, "shared memory");
+  static std::atomic<uint64_t> attr{0};
+  if (!allow_smem(w4_tc<SWIGLU>, kMost, attr)) return kRcCudaError;
+  const long long units =
+      static_cast<long long>(a.max_tiles) * ((a.m.tiles + kTcTiles - 1) / kTcTiles);
+  const int grid = static_cast<int>(std::min<long long>(units, device_sm_count()));
+  return note_cuda_error(launch_pdl(w4_tc<SWIGLU>, dim3(grid), dim3(kTcThreads), sh, stream, t)) ==
+                 cudaSuccess
+             ? kRcOk
+             : kRcCudaError;
+}
+
+}  // namespace
+
+int w4_gemm(const W4Args& a, bool swiglu, cudaStream_t stream) {
+  return swiglu ? tc_launch<true>(a, stream) : tc_launch<false>(a, stream);
+}
+
+}  // namespace moe

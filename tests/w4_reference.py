@@ -47,12 +47,25 @@ def operand_sums(m, x, e):
 ACC = 2.0 ** -16
 
 
-def swiglu_rows(w_gate, w_up, vg, vu, x, e):
+def weight_rounding(values, x):
+    """sum_k BF16 * |w_k x_k|: what rounding every weight to bf16 can move a product by.
+    The tensor-memory form for many records per expert (records >= TC_RECORDS * experts)
+    does that; the streaming form keeps the weights exact."""
+    return BF16 * (x.double().abs() @ values.abs().t())
+
+
+import os
+TC_RECORDS = int(os.environ.get("W4TC", 12))
+
+
+def swiglu_rows(w_gate, w_up, vg, vu, x, e, rounded):
     """h = silu(x Wg^T) * (x Wu^T) of expert e in 64 bits, and a bound of a
-    kernel's error: the rounding of h and the fp32 sums."""
+    kernel's error: the rounding of h, the fp32 sums and, if so, of the weights."""
     xd = x.double()
     g, u = xd @ vg[e].t(), xd @ vu[e].t()
     dg, du = ACC * operand_sums(w_gate, x, e), ACC * operand_sums(w_up, x, e)
+    if rounded:
+        dg, du = dg + weight_rounding(vg[e], x), du + weight_rounding(vu[e], x)
     sg = torch.sigmoid(g)
     # |silu'| <= 1.1, |silu(g)| <= |g|; the fast exponential and division: 2^-20 relative
     h = g * sg * u
@@ -60,16 +73,18 @@ def swiglu_rows(w_gate, w_up, vg, vu, x, e):
     return h, bound * 1.01 + 1e-30
 
 
-def down_rows(w_down, vd, h, e):
-    """o = h Wd^T of expert e in 64 bits, and the bound of its fp32 sums."""
-    return h.double() @ vd[e].t(), ACC * operand_sums(w_down, h, e)
+def down_rows(w_down, vd, h, e, rounded):
+    """o = h Wd^T of expert e in 64 bits, and the bound of its sums."""
+    do = ACC * operand_sums(w_down, h, e)
+    return h.double() @ vd[e].t(), do + weight_rounding(vd[e], h) if rounded else do
 
 
-def experts(p, x, ids, weights, e_begin=0):
+def experts(p, x, ids, weights, e_begin=0, num_experts=None):
     """y = sum_j w_j MLP_{ids_j}(x) in 64 bits, and a bound of a kernel's error that
-    rounds h, each weighted row and y to bf16."""
+    rounds h, each weighted row and y to bf16, and the weights where the records are many."""
     vg, vu, vd = (values(m) for m in p)
     T, H = x.shape
+    rounded = ids.numel() // (num_experts or vg.shape[0]) >= TC_RECORDS
     y = torch.zeros((T, H), dtype=torch.float64, device=x.device)
     bound = torch.zeros_like(y)
     for e in range(vg.shape[0]):
@@ -77,12 +92,20 @@ def experts(p, x, ids, weights, e_begin=0):
         if not n.numel():
             continue
         w = weights[n, j].double().unsqueeze(1)
-        h, dh = swiglu_rows(p[0], p[1], vg, vu, x[n], e)
-        o, do = down_rows(p[2], vd, h, e)
-        do = do * 1.01 + dh @ vd[e].abs().t()
+        h, dh = swiglu_rows(p[0], p[1], vg, vu, x[n], e, rounded)
+        o, do = down_rows(p[2], vd, h, e, rounded)
+        do = do * 1.01 + dh @ vd[e].abs().t() * (1 + BF16)
         y.index_add_(0, n, w * o)
         bound.index_add_(0, n, w.abs() * (do + BF16 * (o.abs() + do)))
     return y, bound + BF16 * (y.abs() + bound) + 1e-30
+
+
+def roundings(parts, rounded):
+    """Independent roundings that the relative error of a result is made of: the given
+    ones, and of the weights of the gate and up products (through silu, whose slope
+    is at most 1.1) and of the down product."""
+    more = {"h": 2.5, "out": 1.0, "y": 3.5}[parts] if rounded else 0.0
+    return {"h": 1, "out": 1, "y": 3}[parts] + more
 
 
 def route(x, router, bias, k, norm):
