@@ -66,6 +66,29 @@ int map_3d(CUtensorMap* m, const void* base, int E, int rows, int cols, int box_
   return make_map(m, base, 3, dims, strides, box);
 }
 
+}  // namespace
+
+int map_rows(CUtensorMap* m, const void* base, int elem_bytes, long long inner, long long rows,
+             int box_inner, int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return kRcTensorMap;
+  const cuuint64_t pitch = static_cast<cuuint64_t>(inner) * elem_bytes;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (pitch & 15u) != 0) return kRcBadArgument;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {pitch};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner),
+                             static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r =
+      enc(m, elem_bytes == 8 ? CU_TENSOR_MAP_DATA_TYPE_INT64 : CU_TENSOR_MAP_DATA_TYPE_INT32, 2,
+          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? kRcOk : kRcTensorMap;
+}
+
+namespace {
+
 constexpr int kMaxDevices = 64;
 constexpr int kMaxSmemPerBlock = 232448;  // sm_100 opt-in dynamic shared memory per block
 

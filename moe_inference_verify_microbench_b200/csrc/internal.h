@@ -106,6 +106,11 @@ inline bool use_pair_gemm(long long R, int E, int H, int I) {
 
 int device_sm_count();
 
+// Tensor map of [rows][inner] elements of 4 or 8 bytes, unswizzled, box
+// [box_rows][box_inner]; elements outside read as zero.
+int map_rows(CUtensorMap* m, const void* base, int elem_bytes, long long inner, long long rows,
+             int box_inner, int box_rows);
+
 // The cudaError_t of the most recent failed CUDA call a launcher recorded on
 // this thread (0 = none), and the recorder: returns `e` unchanged.
 int last_cuda_error();

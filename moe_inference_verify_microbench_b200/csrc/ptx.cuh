@@ -118,6 +118,33 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// mbar_wait for a warp with little to do beside busy ones: the hardware suspends
+// it for up to 10 us at a time instead of letting it poll, which leaves the issue
+// slots to the others.
+__device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t parity,
+                                               volatile int* abort, int* status, int code) {
+  unsigned long long t0 = 0;
+  for (uint32_t it = 0;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(10000u)
+        : "memory");
+    if (ok != 0) return true;
+    if ((it & 15u) != 15u) continue;
+    if (*abort) return false;
+    if (t0 == 0) t0 = globaltimer_ns();
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      record_status(status, code);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- TMA
 
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {

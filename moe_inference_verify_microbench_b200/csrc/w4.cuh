@@ -104,7 +104,10 @@ struct W4Args {
   int* status;
 };
 
+// `threads` threads (whole warps) meet at barrier `id`.  bar.sync wants a converged
+// warp, and lanes may come from a branch.
 __device__ __forceinline__ void named_barrier(int id, int threads) {
+  __syncwarp();
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
@@ -146,7 +149,9 @@ bool allow_smem(Kernel* fn, int bytes, std::atomic<uint64_t>& done) {
   return true;
 }
 
-// The tensor-core form for experts with many records (w4_gemm.cu).
+// The tensor-memory form for experts with many records (w4_gemm.cu), from this
+// many records per expert on.
+constexpr int kW4TcRecords = 8;
 int w4_gemm(const W4Args& a, bool swiglu, cudaStream_t stream);
 
 }  // namespace moe

@@ -18,11 +18,11 @@
 // and up in the same lane and column), for the down product two runs of 128 rows.
 //
 // CTA (896 threads, one per SM, persistent):
-//   warps 0..15   dequantise: warp w writes lane quarter w % 4; warps 0..7 take the
-//                 even 64-column blocks, 8..15 the odd ones
+//   warps 0..15   dequantise: warp w writes lane quarter w % 4 of every fourth
+//                 64-column block
 //   warps 16..19  epilogue: tensor memory -> bf16 -> staging rows -> bulk stores
 //   warps 20..23  gather the records' rows (cp.async into the 128-byte swizzle)
-//   warp 24       bulk copies of codes and group records into a ring
+//   warp 24       tiled copies of codes and group records into a ring
 //   warp 25       issues tcgen05.mma: 2 operands x 4 steps of 16 columns per block
 //   warp 26       allocates tensor memory
 //   warp 27       publishes gathered stages to the async proxy
@@ -39,10 +39,11 @@ namespace moe {
 
 namespace {
 
-constexpr int kTcStages = 4;      // operand stages (64 columns): tensor memory and records
-constexpr int kTcRing = 3;        // code stages (256 columns)
+constexpr int kTcStages = 4;      // weight operand stages (64 columns) in tensor memory
+constexpr int kTcSlots = 6;       // record slots in shared memory (see tc_blocks)
+constexpr int kTcRing = 4;        // code stages (128 columns)
 constexpr int kTcTiles = 16;      // packed tiles per unit
-constexpr int kTcBlocks = 4;      // blocks per code stage
+constexpr int kTcBlocks = 2;      // blocks per code stage
 constexpr int kTcRows = 128;      // records per unit at most
 constexpr int kTcDequantWarps = 16;
 constexpr int kTcEpiWarp = 16, kTcLoadWarp = 20, kTcCopyWarp = 24, kTcMmaWarp = 25,
@@ -74,14 +75,26 @@ __device__ __forceinline__ void tmem_wait_st() {
 }
 
 // D[tmem] (+)= A[tmem] * B[smem]^T, bf16 inputs, fp32 accumulate.
-__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                               uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t desc_lo,
+                                               uint32_t desc_hi, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 bd;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 bd, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(desc_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t p;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p;
 }
 
 __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
@@ -139,6 +152,10 @@ struct TcUnit {
   int m;
   bool ok;
 };
+// A record slot is 128 rows of 64 columns; with fewer records it holds as many
+// 64-column blocks as fit, so that the same bytes are in flight.
+__device__ __forceinline__ int tc_blocks(int n) { return 8 / ((n + 15) >> 4); }
+
 __device__ __forceinline__ TcUnit tc_unit(const W4Args& a, int w, int groups) {
   TcUnit u;
   const int e = w / groups;
@@ -148,19 +165,25 @@ __device__ __forceinline__ TcUnit tc_unit(const W4Args& a, int w, int groups) {
   return u;
 }
 
-template <bool SWIGLU>
-__global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
+// HALVES: groups of 32, two to a block; ZEROS: zero points are kept.
+template <bool SWIGLU, bool HALVES, bool ZEROS>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    w4_tc(const __grid_constant__ CUtensorMap tm_codes,
+          const __grid_constant__ CUtensorMap tm_records, const TcArgs args) {
+  constexpr int kRec = ZEROS ? 8 : 4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   const W4Args& a = args.a;
   uint8_t* sB = smem;
-  uint8_t* sOut = sB + kTcStages * kTcBBytes;
+  uint8_t* sOut = sB + kTcSlots * kTcBBytes;
   uint8_t* sRing = sOut + kTcOutBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(sRing + kTcRing * args.ring_bytes);
   uint64_t* empty = full + kTcStages;
-  uint64_t* gat = empty + kTcStages;
-  uint64_t* qfull = gat + kTcStages;
+  uint64_t* gat = empty + kTcStages;  // a slot's copies have landed
+  uint64_t* bfull = gat + kTcSlots;
+  uint64_t* bempty = bfull + kTcSlots;
+  uint64_t* qfull = bempty + kTcSlots;
   uint64_t* qempty = qfull + kTcRing;
   uint64_t* acc_full = qempty + kTcRing;
   uint64_t* acc_empty = acc_full + 2;
@@ -174,13 +197,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kTcStages; ++s) {
-      mbar_init(&full[s], kTcDequantWarps / 2 + 1);  // half of the dequantising warps, forwarder
+      mbar_init(&full[s], 4);  // the warps of a set
       mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < kTcSlots; ++s) {
       mbar_init(&gat[s], 128);
+      mbar_init(&bfull[s], 1);
+      mbar_init(&bempty[s], 1);
     }
     for (int s = 0; s < kTcRing; ++s) {
       mbar_init(&qfull[s], 1);
-      mbar_init(&qempty[s], kTcDequantWarps);
+      mbar_init(&qempty[s], 4 * kTcBlocks);  // a set for each block
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -207,61 +234,75 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
   const long long units = static_cast<long long>(nt) * groups;
   const int total = static_cast<int>(min(units, 0x7fffffffLL - static_cast<long long>(gridDim.x)));
   const int nb = a.m.nb;
-  // columns of a code stage span 8 >> gshift groups
-  const int stage_groups = 8 >> a.m.gshift;
+  const uint32_t nbe = (nb + kTcBlocks - 1) / kTcBlocks * kTcBlocks;
+  static_assert(kTcStages == kTcDequantWarps / 4, "an operand stage for each set");
 
   if (warp < kTcDequantWarps) {
     // ------------------------------------------------------------ dequantise
-    const int quarter = warp & 3, half = (warp >> 2) & 1, set = warp >> 3;
-    const int g = lane >> 2;
-    // The pair of packed tiles this warp turns into operand rows, and where.
-    const int tile0 = SWIGLU ? 4 * quarter + 2 * half : 8 * half + 2 * quarter;
-    const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
-    uint32_t cnt = 0, rings = 0;
+    // Blocks are counted through all units, an odd number in a unit rounded up to
+    // whole code stages; set i of four warps, one per lane quarter, takes the blocks
+    // i modulo 4 and fills operand stage i with them.
+    const int quarter = warp & 3, set = warp >> 2;
+    const uint32_t codes = smem_u32(sRing) + lane * 16;
+    const uint32_t records = smem_u32(sRing) + kTcCodeBytes + (lane >> 2) * kRec;
+    const uint32_t dst = tmem + kTcOperandCol + set * 64 + (static_cast<uint32_t>(32 * quarter) << 16);
+    uint32_t base = 0;  // blocks before this unit
+    uint32_t uses = 0;  // of the operand stage
     bool ok = true;
     for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
       const TcUnit u = tc_unit(a, w, groups);
       if (!u.ok) continue;
-      const bool have = u.m * kTcTiles + tile0 < a.m.tiles;
-      for (int kb = 0; ok && kb < nb; ++kb, ++cnt) {
-        const uint32_t rs = rings % kTcRing;
-        const int bk = kb & (kTcBlocks - 1);
-        if (bk == 0) {  // every warp waits for every code stage, so none releases one early
-          ok = mbar_wait(&qfull[rs], (rings / kTcRing) & 1u, abort_flag, a.status,
-                         kErrTimeoutFull);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+      const int tiles = a.m.tiles - u.m * kTcTiles;  // packed tiles from here to the end
+      for (uint32_t kb = (set - base) & 3u; kb < nbe; kb += 4) {
+        const uint32_t cnt = base + kb, ring = cnt / kTcBlocks, rs = ring % kTcRing;
+        ok = mbar_wait_idle(&qfull[rs], (ring / kTcRing) & 1u, abort_flag, a.status,
+                            kErrTimeoutFull);
+        if (kb >= static_cast<uint32_t>(nb)) {  // the block that rounds the unit up
+          __syncwarp();
+          if (lane == 0 && ok) mbar_arrive(&qempty[rs]);
+          __syncwarp();
+          continue;
         }
-        if ((cnt & 1u) == static_cast<uint32_t>(set)) {
-          const uint32_t s = cnt % kTcStages;
-          ok = mbar_wait(&empty[s], ((cnt / kTcStages) & 1u) ^ 1u, abort_flag, a.status,
-                         kErrTimeoutEmpty);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          if (have) {
-            const uint32_t ring = smem_u32(sRing) + rs * args.ring_bytes;
-            const uint32_t q = ring + (tile0 * kTcBlocks + bk) * kW4BlockBytes + lane * 16;
-            const uint32_t rec =
-                ring + kTcCodeBytes + tile0 * args.rec_stride + g * a.m.rec;
-            const uint4 w0 = lds128(q), w1 = lds128(q + kTcBlocks * kW4BlockBytes);
-            const uint32_t dst = tmem + kTcOperandCol + s * 64 + lanes;
+        ok = ok && mbar_wait_idle(&empty[set], (uses & 1u) ^ 1u, abort_flag, a.status,
+                                  kErrTimeoutEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++uses;
+        tc_fence_after();
+        const uint32_t bk = kb & (kTcBlocks - 1);
+        const uint32_t q = codes + rs * args.ring_bytes + bk * kW4BlockBytes;
+        const uint32_t grp = HALVES ? 2 * bk : (2 * bk) >> a.m.gshift;
+        const uint32_t rec = records + rs * args.ring_bytes + grp * (8 * kRec);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // two packed tiles: 16 gate and 16 up rows, or 32 rows
+          const int tile0 = SWIGLU ? 4 * quarter + 2 * half : 8 * half + 2 * quarter;
+          if (tile0 < tiles) {
+            const uint4 w0 = lds128(q + tile0 * (kTcBlocks * kW4BlockBytes));
+            const uint4 w1 = lds128(q + (tile0 + 1) * (kTcBlocks * kW4BlockBytes));
             // [half block] of {tile 0, tile 1} x {row g, row g + 8}
             uint32_t sc[2][2][2], zp[2][2][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t grp = static_cast<uint32_t>(2 * bk + h) >> a.m.gshift;
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const uint32_t r = rec + i * args.rec_stride + grp * 8 * a.m.rec;
-                const uint32_t sv = lds32(r);
-                sc[h][i][0] = __byte_perm(sv, 0, 0x1010);
-                sc[h][i][1] = __byte_perm(sv, 0, 0x3232);
-                zp[h][i][0] = zp[h][i][1] = 0x43084308u;
-                if (a.m.rec == 8) {  // fp16 1024 + z -> bf16 128 + z
-                  const uint32_t zv = (lds32(r + 4) & 0x000f000fu) | 0x43004300u;
-                  zp[h][i][0] = __byte_perm(zv, 0, 0x1010);
-                  zp[h][i][1] = __byte_perm(zv, 0, 0x3232);
+                if (HALVES || h == 0) {
+                  const uint32_t r = rec + (tile0 + i) * args.rec_stride + h * (8 * kRec);
+                  const uint32_t sv = lds32(r);
+                  sc[h][i][0] = __byte_perm(sv, 0, 0x1010);
+                  sc[h][i][1] = __byte_perm(sv, 0, 0x3232);
+                  zp[h][i][0] = zp[h][i][1] = 0x43084308u;
+                  if (ZEROS) {  // fp16 1024 + z -> bf16 128 + z
+                    const uint32_t zv = (lds32(r + 4) & 0x000f000fu) | 0x43004300u;
+                    zp[h][i][0] = __byte_perm(zv, 0, 0x1010);
+                    zp[h][i][1] = __byte_perm(zv, 0, 0x3232);
+                  }
+                } else {
+#pragma unroll
+                  for (int k = 0; k < 2; ++k) {
+                    sc[1][i][k] = sc[0][i][k];
+                    zp[1][i][k] = zp[0][i][k];
+                  }
                 }
               }
             }
@@ -290,17 +331,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
               w4_scaled_pairs(w1.w, zp[1][1][1], sc[1][1][1], r + 9, 2);
               tmem_st_16x128b_x8(dst + 32 * half + (16u << 16), r);
             }
-            tmem_wait_st();
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[s]);
         }
-        if (bk == kTcBlocks - 1 || kb == nb - 1) {  // this warp is done with the code stage
-          if (lane == 0) mbar_arrive(&qempty[rs]);
-          ++rings;
+        // tcgen05.wait is .sync.aligned: no lane may branch off in front of it
+        if ((SWIGLU ? 4 * quarter : 2 * quarter) < tiles) tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&qempty[rs]);  // the codes have been read
+          mbar_arrive(&full[set]);
         }
+        __syncwarp();
       }
+      base += nbe;
     }
   } else if (warp >= kTcEpiWarp && warp < kTcLoadWarp) {
     // -------------------------------------------------------------- epilogue
@@ -325,7 +368,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
         }
       }
       s_scale[r] = !SWIGLU && o >= 0 && a.row_scale != nullptr ? a.row_scale[o] : 1.0f;
-      ok = mbar_wait(&acc_full[acc.first], acc.filled[acc.first] & 1u, abort_flag, a.status,
+      ok = mbar_wait_idle(&acc_full[acc.first], acc.filled[acc.first] & 1u, abort_flag, a.status,
                      kErrTimeoutAccFull);
       ok = __all_sync(0xffffffffu, ok);
       ++acc.filled[acc.first];
@@ -411,20 +454,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
           }
         }
       }
-      for (int kb = 0; kb < nb; ++kb, ++cnt) {
-        const uint32_t s = cnt % kTcStages;
-        ok = mbar_wait(&empty[s], ((cnt / kTcStages) & 1u) ^ 1u, abort_flag, a.status,
-                       kErrTimeoutEmpty);
+      const int per = tc_blocks(n);
+      for (int kb = 0; kb < nb; kb += per, ++cnt) {
+        const uint32_t s = cnt % kTcSlots;
+        ok = mbar_wait_idle(&bempty[s], ((cnt / kTcSlots) & 1u) ^ 1u, abort_flag, a.status,
+                            kErrTimeoutEmpty);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint32_t base = smem_u32(sB) + s * kTcBBytes;
+        uint32_t base = smem_u32(sB) + s * kTcBBytes;
+        const int last = min(kb + per, nb);
+        for (int k = kb; k < last; ++k, base += steps * 2048) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j < steps) {
-            const uint32_t r = static_cast<uint32_t>(row0 + 16 * j);
-            const bool have = (present >> j) & 1u;
-            cp_async_16(base + r * 128u + ((chunk ^ (r & 7u)) << 4),
-                        have ? src[j] + static_cast<size_t>(kb) * 128 : src[j], have ? 16u : 0u);
+          for (int j = 0; j < 8; ++j) {
+            if (j < steps) {
+              const uint32_t r = static_cast<uint32_t>(row0 + 16 * j);
+              const bool have = (present >> j) & 1u;
+              cp_async_16(base + r * 128u + ((chunk ^ (r & 7u)) << 4),
+                          have ? src[j] + static_cast<size_t>(k) * 128 : src[j], have ? 16u : 0u);
+            }
           }
         }
         cp_async_arrive_noinc(&gat[s]);
@@ -432,90 +479,114 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
     }
     cp_async_wait_all();  // every copy lands before the CTA can exit
   } else if (warp == kTcCopyWarp) {
-    // ------------------------------------------------ codes and group records
-    uint32_t rings = 0;
-    bool ok = true;
-    for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
-      const TcUnit u = tc_unit(a, w, groups);
-      if (!u.ok) continue;
-      const int tile0 = u.m * kTcTiles, tiles = min(kTcTiles, a.m.tiles - tile0);
-      const size_t et = static_cast<size_t>(u.t.x) * a.m.tiles + tile0 + lane;
-      for (int kb = 0; kb < nb; kb += kTcBlocks, ++rings) {
-        const uint32_t rs = rings % kTcRing;
-        ok = mbar_wait(&qempty[rs], ((rings / kTcRing) & 1u) ^ 1u, abort_flag, a.status,
-                       kErrTimeoutEmpty);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const int blocks = min(kTcBlocks, nb - kb);
-        const int g0 = (2 * kb) >> a.m.gshift;
-        const int grps = min(stage_groups, a.m.ng - g0);
-        const uint32_t qb = blocks * kW4BlockBytes, sb = grps * 8 * a.m.rec;
-        if (lane == 0) mbar_arrive_expect_tx(&qfull[rs], tiles * (qb + sb));
-        __syncwarp();
-        if (lane < tiles) {
-          uint8_t* dst = sRing + rs * args.ring_bytes;
-          bulk_load(dst + lane * kTcBlocks * kW4BlockBytes, a.m.q + (et * nb + kb) * kW4BlockBytes,
-                    qb, &qfull[rs]);
-          bulk_load(dst + kTcCodeBytes + lane * args.rec_stride,
-                    a.m.s + (et * a.m.ng + g0) * 8 * a.m.rec, sb, &qfull[rs]);
-        }
-      }
-    }
-    if (*abort_flag && lane == 0) {
-      // Let every copy still in flight land before the CTA exits.
-      for (uint32_t i = rings > kTcRing ? rings - kTcRing : 0u; i < rings; ++i) {
-        const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(&qfull[i % kTcRing], (i / kTcRing) & 1u)) {
-          if (globaltimer_ns() - t0 > kWaitLimitNs) break;
-        }
-      }
-    }
-  } else if (warp == kTcMmaWarp) {
     if (lane == 0) {
-      // ---------------------------------------------------------- MMA issuer
-      TcAcc acc;
-      uint32_t cnt = 0;
+      // ---------------------------------------------- codes and group records
+      // One tiled copy of sixteen packed tiles' codes and one of their records per
+      // stage; past the matrix they bring the next expert's rows or zeros, which
+      // no operand row uses.
+      uint32_t rings = 0;
       bool ok = true;
       for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
         const TcUnit u = tc_unit(a, w, groups);
         if (!u.ok) continue;
-        const int cols = (u.t.z - u.t.y + 15) & ~15;
-        acc.take(cols);
-        for (int b = acc.first; ok && b <= acc.last; ++b) {
-          ok = mbar_wait(&acc_empty[b], (acc.used[b] & 1u) ^ 1u, abort_flag, a.status,
-                         kErrTimeoutAccEmpty);
-          ++acc.used[b];
-        }
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>(cols));
-        const bool second = SWIGLU || u.m * kTcTiles + 8 < a.m.tiles;
-        for (int kb = 0; kb < nb; ++kb, ++cnt) {
-          const uint32_t s = cnt % kTcStages;
-          if (!mbar_wait(&full[s], (cnt / kTcStages) & 1u, abort_flag, a.status,
-                         kErrTimeoutFull)) {
+        const int row = u.t.x * a.m.tiles + u.m * kTcTiles;
+        for (int kb = 0; kb < nb; kb += kTcBlocks, ++rings) {
+          const uint32_t rs = rings % kTcRing;
+          if (!mbar_wait_idle(&qempty[rs], ((rings / kTcRing) & 1u) ^ 1u, abort_flag, a.status,
+                              kErrTimeoutEmpty)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint32_t at = tmem + kTcOperandCol + s * 64;
-          const uint32_t b0 = smem_u32(sB) + s * kTcBBytes;
+          mbar_arrive_expect_tx(&qfull[rs], args.ring_bytes);
+          uint8_t* dst = sRing + rs * args.ring_bytes;
+          tma_load_2d(dst, &tm_codes, &qfull[rs], kb * (kW4BlockBytes / 8), row);
+          tma_load_2d(dst + kTcCodeBytes, &tm_records, &qfull[rs],
+                      ((2 * kb) >> a.m.gshift) * (8 * kRec / 4), row);
+        }
+      }
+      if (*abort_flag) {
+        // Let every copy still in flight land before the CTA exits.
+        for (uint32_t i = rings > kTcRing ? rings - kTcRing : 0u; i < rings; ++i) {
+          const unsigned long long t0 = globaltimer_ns();
+          while (!mbar_try_wait(&qfull[i % kTcRing], (i / kTcRing) & 1u)) {
+            if (globaltimer_ns() - t0 > kWaitLimitNs) break;
+          }
+        }
+      }
+    }
+  } else if (warp == kTcMmaWarp) {
+    // ------------------------------------------------------------ MMA issuer
+    // The whole warp walks the stages, so that addresses and descriptors are
+    // uniform values, and one elected lane issues.  With 16 records a stage lasts
+    // a few hundred cycles: issued from a lane's own branch, the eight products
+    // of a stage took 1300.
+    TcAcc acc;
+    const uint32_t leader = elect_one();
+    // descriptor of a K-major 128-byte-swizzled tile, without its start address
+    constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    uint32_t s = 0, phases = 0, bs = 0, bph = 0;  // bit i of phases: parity of stage i
+    bool ok = true;
+    for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+      const TcUnit u = tc_unit(a, w, groups);
+      if (!u.ok) continue;
+      const int n = __shfl_sync(0xffffffffu, u.t.z - u.t.y, 0);
+      const int per = tc_blocks(n), cols = (n + 15) & ~15;
+      acc.take(cols);
+      for (int b = acc.first; ok && b <= acc.last; ++b) {
+        ok = mbar_wait_idle(&acc_empty[b], (acc.used[b] & 1u) ^ 1u, abort_flag, a.status,
+                            kErrTimeoutAccEmpty);
+        ++acc.used[b];
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>(cols));
+      const bool second = SWIGLU || u.m * kTcTiles + 8 < a.m.tiles;
+      const uint32_t d0 = tmem + acc.d0, d1 = tmem + acc.d1;
+      int in_slot = 0;
+      for (int kb = 0; kb < nb; ++kb) {
+        if (in_slot == 0)
+          ok = mbar_wait(&bfull[bs], bph, abort_flag, a.status, kErrTimeoutFull);
+        ok = mbar_wait(&full[s], (phases >> s) & 1u, abort_flag, a.status, kErrTimeoutFull) && ok;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t at = tmem + kTcOperandCol + s * 64;
+        const uint32_t lo =
+            (((smem_u32(sB) + bs * kTcBBytes + in_slot * cols * 128) >> 4) & 0x3fffu) | (1u << 16);
+        const bool end = ++in_slot == per || kb + 1 == nb;
+        if (leader) {
+          const uint32_t acc0 = kb != 0 ? 1u : 0u;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            tc_mma_bf16_ts(tmem + acc.d0, at + kk * 8, sw128_kmajor_desc(b0 + kk * 32), idesc,
-                           (kb | kk) != 0 ? 1u : 0u);
+            tc_mma_bf16_ts(d0, at + kk * 8, lo + 2 * kk, kDescHi, idesc, kk != 0 ? 1u : acc0);
           if (second) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              tc_mma_bf16_ts(tmem + acc.d1, at + 32 + kk * 8, sw128_kmajor_desc(b0 + kk * 32),
-                             idesc, (kb | kk) != 0 ? 1u : 0u);
+              tc_mma_bf16_ts(d1, at + 32 + kk * 8, lo + 2 * kk, kDescHi, idesc,
+                             kk != 0 ? 1u : acc0);
           }
           tc_commit(&empty[s]);
+          if (end) tc_commit(&bempty[bs]);
+          if (kb + 1 == nb) tc_commit(&acc_full[acc.first]);
         }
-        if (ok) tc_commit(&acc_full[acc.first]);
+        __syncwarp();
+        if (end) {
+          in_slot = 0;
+          if (++bs == kTcSlots) {
+            bs = 0;
+            bph ^= 1u;
+          }
+        }
+        phases ^= 1u << s;
+        s = (s + 1) % kTcStages;
       }
-      // Every MMA issued by this thread has finished once `drain` completes.
-      tc_commit(drain);
+      if (nb % kTcBlocks != 0) s = (s + 1) % kTcStages;
+    }
+    // The epilogue has waited for every unit's products; only after an abort some
+    // may still run, and have finished once `drain` completes.
+    if (!ok) {
+      if (leader) tc_commit(drain);
+      __syncwarp();
       const unsigned long long t0 = globaltimer_ns();
       while (!mbar_try_wait(drain, 0)) {
         if (globaltimer_ns() - t0 > kWaitLimitNs) break;
@@ -529,14 +600,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
       for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
         const TcUnit u = tc_unit(a, w, groups);
         if (!u.ok) continue;
-        for (int kb = 0; kb < nb; ++kb, ++cnt) {
-          const uint32_t s = cnt % kTcStages;
-          if (!mbar_wait(&gat[s], (cnt / kTcStages) & 1u, abort_flag, a.status, kErrTimeoutFull)) {
+        const int per = tc_blocks(u.t.z - u.t.y);
+        for (int kb = 0; kb < nb; kb += per, ++cnt) {
+          const uint32_t s = cnt % kTcSlots;
+          if (!mbar_wait_idle(&gat[s], (cnt / kTcSlots) & 1u, abort_flag, a.status,
+                              kErrTimeoutFull)) {
             ok = false;
             break;
           }
           fence_proxy_async_smem();
-          mbar_arrive(&full[s]);
+          mbar_arrive(&bfull[s]);
         }
       }
     }
@@ -550,32 +623,49 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc(const TcArgs args) {
   }
 }
 
-template <bool SWIGLU>
+template <bool SWIGLU, bool HALVES, bool ZEROS>
 int tc_launch(const W4Args& a, cudaStream_t stream) {
   TcArgs t{};
   t.a = a;
-  t.rec_stride = (8 >> a.m.gshift) * 8 * a.m.rec;
+  t.rec_stride = (4 >> a.m.gshift) * 8 * a.m.rec;
   t.ring_bytes = kTcCodeBytes + kTcTiles * t.rec_stride;
-  const int sh = 1024 + kTcStages * kTcBBytes + kTcOutBytes + kTcRing * t.ring_bytes + 256 +
-                 kTcRows * 8;
-  constexpr int kMost = 1024 + kTcStages * kTcBBytes + kTcOutBytes +
-                        kTcRing * (kTcCodeBytes + kTcTiles * 512) + 256 + kTcRows * 8;
+  const int sh =
+      1024 + kTcSlots * kTcBBytes + kTcOutBytes + kTcRing * t.ring_bytes + 512 + kTcRows * 8;
+  constexpr int kMost = 1024 + kTcSlots * kTcBBytes + kTcOutBytes +
+                        kTcRing * (kTcCodeBytes + kTcTiles * 256) + 512 + kTcRows * 8;
   static_assert(kMost <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> attr{0};
-  if (!allow_smem(w4_tc<SWIGLU>, kMost, attr)) return kRcCudaError;
+  if (!allow_smem(w4_tc<SWIGLU, HALVES, ZEROS>, kMost, attr)) return kRcCudaError;
+  // x of a copy is a multiple of 16 bytes: blocks of 512, records of 8 rows of 4 or 8
+  CUtensorMap codes, records;
+  const long long rows = static_cast<long long>(a.E) * a.m.tiles;
+  int rc = map_rows(&codes, a.m.q, 8, a.m.nb * (kW4BlockBytes / 8), rows,
+                    kTcBlocks * kW4BlockBytes / 8, kTcTiles);
+  if (rc == kRcOk)
+    rc = map_rows(&records, a.m.s, 4, a.m.ng * 8 * a.m.rec / 4, rows, t.rec_stride / 4, kTcTiles);
+  if (rc != kRcOk) return rc;
   const long long units =
       static_cast<long long>(a.max_tiles) * ((a.m.tiles + kTcTiles - 1) / kTcTiles);
   const int grid = static_cast<int>(std::min<long long>(units, device_sm_count()));
-  return note_cuda_error(launch_pdl(w4_tc<SWIGLU>, dim3(grid), dim3(kTcThreads), sh, stream, t)) ==
-                 cudaSuccess
+  return note_cuda_error(launch_pdl(w4_tc<SWIGLU, HALVES, ZEROS>, dim3(grid), dim3(kTcThreads), sh,
+                                    stream, codes, records, t)) == cudaSuccess
              ? kRcOk
              : kRcCudaError;
+}
+
+template <bool SWIGLU>
+int tc_dispatch(const W4Args& a, cudaStream_t stream) {
+  if (a.m.gshift == 0)
+    return a.m.rec == 8 ? tc_launch<SWIGLU, true, true>(a, stream)
+                        : tc_launch<SWIGLU, true, false>(a, stream);
+  return a.m.rec == 8 ? tc_launch<SWIGLU, false, true>(a, stream)
+                      : tc_launch<SWIGLU, false, false>(a, stream);
 }
 
 }  // namespace
 
 int w4_gemm(const W4Args& a, bool swiglu, cudaStream_t stream) {
-  return swiglu ? tc_launch<true>(a, stream) : tc_launch<false>(a, stream);
+  return swiglu ? tc_dispatch<true>(a, stream) : tc_dispatch<false>(a, stream);
 }
 
 }  // namespace moe

@@ -54,8 +54,7 @@ def weight_rounding(values, x):
     return BF16 * (x.double().abs() @ values.abs().t())
 
 
-import os
-TC_RECORDS = int(os.environ.get("W4TC", 12))
+TC_RECORDS = 8
 
 
 def swiglu_rows(w_gate, w_up, vg, vu, x, e, rounded):
