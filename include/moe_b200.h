@@ -440,6 +440,18 @@ MOE_API int moe_w4_experts_forward(const void* x, const int32_t* ids, const floa
                                    cudaStream_t stream);
 
 /*
+ * The 4-bit experts for rows that are sorted by expert already: rows
+ * offsets[e] .. offsets[e + 1] of sorted_x [M, H] (int64 offsets [E + 1], on the
+ * device) through expert e, unweighted, in sorted order; rows from offsets[E] on
+ * are zero (C9/python/solution.py:207-222).
+ */
+MOE_API size_t moe_w4_sorted_workspace_bytes(int M, const moe_w4_bank* bank);
+MOE_API int moe_w4_sorted_forward(const void* sorted_x, int M, const int64_t* offsets,
+                                  const moe_w4_bank* bank, void* workspace,
+                                  size_t workspace_bytes, void* y, int32_t* status,
+                                  cudaStream_t stream);
+
+/*
  * moe_layer_forward on a 4-bit bank that holds all E experts.  The router as
  * in moe_router_topk (E % 16 == 0, 16 <= E <= 256).
  */

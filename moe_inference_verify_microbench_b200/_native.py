@@ -107,6 +107,8 @@ SIGNATURES: dict[str, tuple] = {
     "moe_w4_experts_workspace_bytes": (_c_size, [_c_int, _c_int, _ptr]),
     "moe_w4_experts_forward": (_c_int, [_ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr,
                                         _ptr, _c_size, _ptr, _ptr, _ptr]),
+    "moe_w4_sorted_workspace_bytes": (_c_size, [_c_int, _ptr]),
+    "moe_w4_sorted_forward": (_c_int, [_ptr, _c_int, _ptr, _ptr, _ptr, _c_size, _ptr, _ptr, _ptr]),
     "moe_w4_layer_workspace_bytes": (_c_size, [_c_int, _c_int, _ptr]),
     "moe_w4_layer_forward": (_c_int, [_ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _ptr,
                                       _c_size, _ptr, _ptr, _ptr]),

@@ -128,6 +128,17 @@ W4Layout w4_layout(void* ws, int T, int k, const W4Bank& b, bool routed) {
   return l;
 }
 
+W4Layout w4_sorted_layout(void* ws, int M, const W4Bank& b) {
+  W4Layout l{};
+  Carver c(ws);
+  l.max_tiles = max_tiles_bound(M, b.E, MOE_BLOCK_M);
+  l.tiles = c.take<int4>(l.max_tiles);
+  l.num_tiles = c.take<int>(1);
+  l.h = c.take<__nv_bfloat16>(static_cast<size_t>(M) * b.I);
+  l.bytes = c.used;
+  return l;
+}
+
 bool w4_count_ok(int T, int k) {
   return static_cast<long long>(T) * k <= 0x7fffffffLL;
 }
@@ -613,6 +624,36 @@ int moe_w4_experts_forward(const void* x, const int32_t* ids, const float* weigh
                          l.num_tiles, status, stream);
   if (rc != kRcOk) return rc;
   return w4_products(b, l, x, ids, weights, T, top_k, num_experts, e_begin, y, status, stream);
+}
+
+size_t moe_w4_sorted_workspace_bytes(int M, const moe_w4_bank* bank) {
+  if (M < 0 || bank == nullptr || bank->E <= 0 || bank->H <= 0 || bank->I <= 0) return 0;
+  return w4_sorted_layout(nullptr, M, w4_bank(*bank)).bytes;
+}
+
+int moe_w4_sorted_forward(const void* sorted_x, int M, const int64_t* offsets,
+                          const moe_w4_bank* bank, void* workspace, size_t workspace_bytes,
+                          void* y, int32_t* status, cudaStream_t stream) {
+  if (bank == nullptr || M < 0 || offsets == nullptr) return kRcBadArgument;
+  const W4Bank b = w4_bank(*bank);
+  int rc = w4_check_bank(b);
+  if (rc != kRcOk) return rc;
+  if (M == 0) return kRcOk;
+  if (sorted_x == nullptr || y == nullptr || workspace == nullptr ||
+      (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+    return kRcBadArgument;
+  const W4Layout l = w4_sorted_layout(workspace, M, b);
+  if (workspace_bytes < l.bytes) return kRcWorkspace;
+  const long long* off = reinterpret_cast<const long long*>(offsets);
+  rc = launch_tiles_from_offsets(off, b.E, MOE_BLOCK_M, l.tiles, l.max_tiles, l.num_tiles, status,
+                                 stream);
+  if (rc != kRcOk) return rc;
+  const int avg = M / b.E;
+  rc = launch_w4_w13(b, sorted_x, M, nullptr, 1, M, l.tiles, l.num_tiles, l.max_tiles, l.h, avg,
+                     status, stream);
+  if (rc != kRcOk) return rc;
+  return launch_w4_w2(b, l.h, M, l.tiles, l.num_tiles, l.max_tiles, nullptr, nullptr, y, M, avg,
+                      status, stream, off + b.E);
 }
 
 size_t moe_w4_layer_workspace_bytes(int T, int top_k, const moe_w4_bank* bank) {

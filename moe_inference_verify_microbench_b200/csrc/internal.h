@@ -185,13 +185,14 @@ int launch_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* ze
                    const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E, int N,
                    int K, int group, void* q, void* s, int* status, cudaStream_t stream);
 // avg: records per expert to expect; it chooses the kernel and changes no result
-// beyond rounding.
+// beyond rounding.  tail (device, optional): output rows from *tail on are zeroed.
 int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* index,
                   int index_div, int M, const int4* tiles, const int* num_tiles, int max_tiles,
                   void* h_out, int avg, int* status, cudaStream_t stream);
 int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
                  int max_tiles, const int* row_map, const float* row_scale, void* out,
-                 int out_rows, int avg, int* status, cudaStream_t stream);
+                 int out_rows, int avg, int* status, cudaStream_t stream,
+                 const long long* tail = nullptr);
 
 // Norms around a block: n = RMSNorm(delta) * post, h = x + scale * act(gate) * n,
 // y = RMSNorm(h) * pre.  gate[t * gate_row + c * gate_col], bf16 or fp32, null: 1.

@@ -11,6 +11,9 @@
 // Both are HBM-bound copies with 16-byte vector accesses; the combine sums the
 // k contributions in fp32 in slot order (deterministic, unlike the atomic
 // index_add_ of the reference on CUDA).
+#include <algorithm>
+#include <atomic>
+
 #include "internal.h"
 
 namespace moe {
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(kRowsThreads) add_rmsnorm_rows(
 }
 
 // The norm after a block, its gate and residual scale, and the norm before the
-// next block, in one pass over the row:
+// next block, in one pass over the rows:
 //   n = delta * rsqrt(mean(delta^2) + eps) * post
 //   h = x + scale * act(gate) * n
 //   y = h * rsqrt(mean(h^2) + eps) * pre
@@ -261,10 +264,18 @@ __global__ void __launch_bounds__(kRowsThreads) add_rmsnorm_rows(
 // CTA per row keeps x, delta and then h in registers (VPT 16-byte vectors per
 // thread), so nothing is read twice; both sums of squares and h are fp32, and y
 // is the norm of the unrounded h.
+// The sigmoid and tanh by one exponential each: tanh x = sign(x) (1 - e) / (1 + e),
+// e = exp(-2 |x|), whose difference loses bits near zero, so below 2^-6 it is
+// x - x^3 / 3 (the next term is 2 x^4 / 15 < 2^-26 of it).
 template <int ACT>
 __device__ __forceinline__ float gate_act(float g) {
-  if (ACT == 1) return 1.0f / (1.0f + __expf(-g));
-  if (ACT == 2) return tanhf(g);
+  if (ACT == 1) return __fdividef(1.0f, 1.0f + __expf(-g));
+  if (ACT == 2) {
+    const float a = fabsf(g);
+    const float e = __expf(-2.0f * a);
+    const float t = copysignf(__fdividef(1.0f - e, 1.0f + e), g);
+    return a < 0.015625f ? fmaf(g * g * g, -1.0f / 3.0f, g) : t;
+  }
   return g;
 }
 
@@ -301,8 +312,17 @@ __device__ __forceinline__ float cta_sum(float v, float* sh) {
 
 constexpr int kBlockNormMaxH = 4 * 8 * 1024;
 
-template <int VPT, int ACT>
-__global__ void __launch_bounds__(1024) block_norm_rows(const BlockNormArgs a) {
+// Read once: past L1.
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+template <int VPT, int ACT, int MAX_THREADS>
+__global__ void __launch_bounds__(MAX_THREADS) block_norm_rows(const BlockNormArgs a) {
   __shared__ float sh[2][32];
   pdl_wait();
   pdl_trigger();
@@ -310,17 +330,26 @@ __global__ void __launch_bounds__(1024) block_norm_rows(const BlockNormArgs a) {
   const size_t n = blockIdx.x;
   const uint4* xr = static_cast<const uint4*>(a.x) + n * vec;
   const uint4* dr = static_cast<const uint4*>(a.delta) + n * vec;
-  uint4 xv[VPT], dv[VPT];
-  float ss = 0.0f;
+  const bool gated = a.gate != nullptr && a.gate_col != 0, gate_bf16 = gated && !a.gate_f32;
+  const __nv_bfloat16* gr = static_cast<const __nv_bfloat16*>(a.gate) + n * a.gate_row;
+  uint4 xv[VPT], dv[VPT], gv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    xv[i] = dv[i] = make_uint4(0, 0, 0, 0);
+    xv[i] = dv[i] = gv[i] = make_uint4(0, 0, 0, 0);
     if (v < vec) {
-      dv[i] = __ldg(dr + v);
-      xv[i] = __ldg(xr + v);
+      dv[i] = load_once(dr + v);
+      xv[i] = load_once(xr + v);
+      if (gate_bf16) gv[i] = load_once(reinterpret_cast<const uint4*>(gr) + v);
     }
   }
+  float token_gate = 1.0f;  // one gate for the row
+  if (a.gate != nullptr && a.gate_col == 0) {
+    const float g = a.gate_f32 ? static_cast<const float*>(a.gate)[n * a.gate_row]
+                               : __bfloat162float(gr[0]);
+    token_gate = gate_act<ACT>(g);
+  }
+  float ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     float d[8];
@@ -330,13 +359,6 @@ __global__ void __launch_bounds__(1024) block_norm_rows(const BlockNormArgs a) {
   }
   const float inv_h = 1.0f / static_cast<float>(a.H);
   const float r1 = rsqrtf(cta_sum(ss, sh[0]) * inv_h + a.eps) * a.scale;
-  float token_gate = 1.0f;  // one gate for the row
-  if (a.gate != nullptr && a.gate_col == 0) {
-    const float g = a.gate_f32 ? static_cast<const float*>(a.gate)[n * a.gate_row]
-                               : __bfloat162float(static_cast<const __nv_bfloat16*>(
-                                     a.gate)[n * a.gate_row]);
-    token_gate = gate_act<ACT>(g);
-  }
   float h[VPT][8];
   ss = 0.0f;
 #pragma unroll
@@ -351,11 +373,9 @@ __global__ void __launch_bounds__(1024) block_norm_rows(const BlockNormArgs a) {
       load8(a.post + 8 * v, w);
 #pragma unroll
       for (int q = 0; q < 8; ++q) gt[q] = token_gate;
-      if (a.gate != nullptr && a.gate_col != 0) {
-        const size_t o = n * a.gate_row + 8 * v;
-        if (a.gate_f32) load8(static_cast<const float*>(a.gate) + o, gt);
-        else unpack8(__ldg(reinterpret_cast<const uint4*>(
-                 static_cast<const __nv_bfloat16*>(a.gate) + o)), gt);
+      if (gated) {
+        if (gate_bf16) unpack8(gv[i], gt);
+        else load8(static_cast<const float*>(a.gate) + n * a.gate_row + 8 * v, gt);
 #pragma unroll
         for (int q = 0; q < 8; ++q) gt[q] = gate_act<ACT>(gt[q]);
       }
@@ -381,6 +401,179 @@ __global__ void __launch_bounds__(1024) block_norm_rows(const BlockNormArgs a) {
       for (int q = 0; q < 4; ++q)
         o[q] = pack_bf16x2(h[i][2 * q] * r2 * w[2 * q], h[i][2 * q + 1] * r2 * w[2 * q + 1]);
       static_cast<uint4*>(a.y)[n * vec + v] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+}
+
+// The same for many rows: persistent CTAs whose rows arrive through a ring of
+// shared-memory stages by bulk copies (x, delta and, where there is one for every
+// element, the gate), so that HBM reads never wait for a reduction.  A thread
+// keeps its columns' weights in registers for all rows; a gate for each channel is
+// multiplied into them once.
+constexpr int kNormThreads = 256;
+// CTAs per SM: a row is a chain of two reductions, so short rows want more of them.
+template <int VPT>
+constexpr int norm_ctas() {
+  return VPT == 1 ? 4 : 2;
+}
+template <int VPT>
+constexpr int norm_ring_bytes() {
+  return (VPT == 1 ? 50 : 100) * 1024;
+}
+constexpr int kNormMaxStages = 8;
+
+template <int VPT, int ACT>
+__global__ void __launch_bounds__(kNormThreads, norm_ctas<VPT>())
+    block_norm_stream(const BlockNormArgs a,
+                                                                     int stages) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float sh[2][8];
+  __shared__ __align__(8) uint64_t full[kNormMaxStages];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int vec = a.H / 8;
+  const uint32_t row_bytes = static_cast<uint32_t>(a.H) * 2;
+  const bool elem = a.gate != nullptr && a.gate_col != 0 && a.gate_row != 0;
+  const uint32_t gate_bytes = elem ? (a.gate_f32 ? 2 * row_bytes : row_bytes) : 0u;
+  const uint32_t stage_bytes = 2 * row_bytes + gate_bytes;
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  auto fetch = [&](int row, int s) {  // one thread
+    uint8_t* dst = ring + s * stage_bytes;
+    const size_t o = static_cast<size_t>(row);
+    mbar_arrive_expect_tx(&full[s], stage_bytes);
+    bulk_load(dst, static_cast<const uint8_t*>(a.x) + o * row_bytes, row_bytes, &full[s]);
+    bulk_load(dst + row_bytes, static_cast<const uint8_t*>(a.delta) + o * row_bytes, row_bytes,
+              &full[s]);
+    if (elem)
+      bulk_load(dst + 2 * row_bytes, static_cast<const uint8_t*>(a.gate) + o * gate_bytes,
+                gate_bytes, &full[s]);
+  };
+  const int grid = gridDim.x;
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) {
+      const long long row = blockIdx.x + static_cast<long long>(s) * grid;
+      if (row < a.T) fetch(static_cast<int>(row), s);
+    }
+  }
+  float post[VPT][8], pre[VPT][8];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = tid + i * kNormThreads;
+    if (v < vec) {
+      load8(a.post + 8 * v, post[i]);
+      load8(a.pre + 8 * v, pre[i]);
+      float g[8];
+      if (a.gate != nullptr && a.gate_col != 0 && !elem) {
+        if (a.gate_f32) load8(static_cast<const float*>(a.gate) + 8 * v, g);
+        else unpack8(__ldg(static_cast<const uint4*>(a.gate) + v), g);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) post[i][q] *= gate_act<ACT>(g[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) post[i][q] *= a.scale;
+    }
+  }
+  const float inv_h = 1.0f / static_cast<float>(a.H);
+  int s = 0;
+  uint32_t ph = 0;
+  long long refill = -1;  // row to fetch into the stage before s, once every thread left it
+  for (long long row = blockIdx.x; row < a.T; row += grid) {
+    float token_gate = 1.0f;
+    if (a.gate != nullptr && a.gate_col == 0)
+      token_gate = gate_act<ACT>(
+          a.gate_f32 ? static_cast<const float*>(a.gate)[row]
+                     : __bfloat162float(static_cast<const __nv_bfloat16*>(a.gate)[row]));
+    if (!mbar_try_wait(&full[s], ph)) {
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(&full[s], ph) && globaltimer_ns() - t0 < kWaitLimitNs) {
+      }
+    }
+    const uint4* sx = reinterpret_cast<const uint4*>(ring + s * stage_bytes);
+    const uint4* sd = sx + vec;
+    float h[VPT][8], d[VPT][8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * kNormThreads;
+      if (v < vec) {
+        unpack8(sd[v], d[i]);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) ss = fmaf(d[i][q], d[i][q], ss);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (lane == 0) sh[0][warp] = ss;
+    __syncthreads();  // also: every thread has left the previous row's stage
+    if (tid == 0 && refill >= 0) {
+      fence_proxy_async_smem();
+      fetch(static_cast<int>(refill), s == 0 ? stages - 1 : s - 1);
+    }
+    ss = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kNormThreads / 32; ++w) ss += sh[0][w];
+    const float r1 = rsqrtf(ss * inv_h + a.eps) * token_gate;
+    ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * kNormThreads;
+      if (v < vec) {
+        unpack8(sx[v], h[i]);
+        float g[8];
+        if (elem) {
+          const uint8_t* sg = reinterpret_cast<const uint8_t*>(sd + vec);
+          if (a.gate_f32) {
+            const float4 g0 = reinterpret_cast<const float4*>(sg)[2 * v];
+            const float4 g1 = reinterpret_cast<const float4*>(sg)[2 * v + 1];
+            g[0] = g0.x, g[1] = g0.y, g[2] = g0.z, g[3] = g0.w;
+            g[4] = g1.x, g[5] = g1.y, g[6] = g1.z, g[7] = g1.w;
+          } else {
+            unpack8(reinterpret_cast<const uint4*>(sg)[v], g);
+          }
+#pragma unroll
+          for (int q = 0; q < 8; ++q) d[i][q] *= gate_act<ACT>(g[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          h[i][q] = fmaf(d[i][q] * r1, post[i][q], h[i][q]);
+          ss = fmaf(h[i][q], h[i][q], ss);
+        }
+        static_cast<uint4*>(a.h)[static_cast<size_t>(row) * vec + v] =
+            make_uint4(pack_bf16x2(h[i][0], h[i][1]), pack_bf16x2(h[i][2], h[i][3]),
+                       pack_bf16x2(h[i][4], h[i][5]), pack_bf16x2(h[i][6], h[i][7]));
+      }
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (lane == 0) sh[1][warp] = ss;
+    __syncthreads();
+    ss = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kNormThreads / 32; ++w) ss += sh[1][w];
+    const float r2 = rsqrtf(ss * inv_h + a.eps);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * kNormThreads;
+      if (v < vec) {
+        uint32_t o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          o[q] = pack_bf16x2(h[i][2 * q] * r2 * pre[i][2 * q],
+                             h[i][2 * q + 1] * r2 * pre[i][2 * q + 1]);
+        static_cast<uint4*>(a.y)[static_cast<size_t>(row) * vec + v] =
+            make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+    refill = row + static_cast<long long>(stages) * grid;
+    if (refill >= a.T) refill = -1;
+    if (++s == stages) {
+      s = 0;
+      ph ^= 1u;
     }
   }
 }
@@ -444,14 +637,39 @@ int launch_add_rmsnorm(const void* x, const void* delta, const float* w, int T, 
   return e == cudaSuccess ? kRcOk : kRcCudaError;
 }
 
-template <int VPT>
+template <int VPT, int MAX_THREADS = 1024>
 static cudaError_t block_norm_launch(const BlockNormArgs& a, cudaStream_t stream) {
   const int vec = a.H / 8;
   const int threads = ((vec + VPT - 1) / VPT + 31) / 32 * 32;
-  auto kern = a.act == 1 ? block_norm_rows<VPT, 1>
-              : a.act == 2 ? block_norm_rows<VPT, 2>
-                           : block_norm_rows<VPT, 0>;
+  auto kern = a.act == 1   ? block_norm_rows<VPT, 1, MAX_THREADS>
+              : a.act == 2 ? block_norm_rows<VPT, 2, MAX_THREADS>
+                           : block_norm_rows<VPT, 0, MAX_THREADS>;
   return launch_pdl(kern, dim3(a.T), dim3(threads), 0, stream, a);
+}
+
+template <int VPT>
+static cudaError_t block_norm_stream_launch(const BlockNormArgs& a, int stage,
+                                            cudaStream_t stream) {
+  const int stages = std::min(kNormMaxStages, norm_ring_bytes<VPT>() / stage);
+  auto kern = a.act == 1   ? block_norm_stream<VPT, 1>
+              : a.act == 2 ? block_norm_stream<VPT, 2>
+                           : block_norm_stream<VPT, 0>;
+  static std::atomic<uint64_t> done{0};  // per device: the three kernels' limits are raised
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if ((done.load(std::memory_order_acquire) & bit) == 0) {
+    for (auto* k : {block_norm_stream<VPT, 0>, block_norm_stream<VPT, 1>, block_norm_stream<VPT, 2>}) {
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               norm_ring_bytes<VPT>());
+      if (e != cudaSuccess) return e;
+    }
+    done.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  const int grid = std::min(a.T, norm_ctas<VPT>() * device_sm_count());
+  return launch_pdl(kern, dim3(grid), dim3(kNormThreads), static_cast<size_t>(stage) * stages,
+                    stream, a, stages);
 }
 
 int launch_block_norm(const BlockNormArgs& a, cudaStream_t stream) {
@@ -470,8 +688,30 @@ int launch_block_norm(const BlockNormArgs& a, cudaStream_t stream) {
     return kRcBadArgument;
   if (a.T == 0) return kRcOk;
   const int vec = a.H / 8;
-  const cudaError_t e = vec <= 2 * 1024 ? block_norm_launch<2>(a, stream)
-                                        : block_norm_launch<4>(a, stream);
+  // Measured (ncu, L2 cold, B200).  Few rows are a latency: a thread for each vector
+  // (333 x 2048: 4.6 us, two vectors a thread 5.6).  From about a thousand on
+  // the rows in flight count: two vectors a thread (16384 x 2048: 49 us against 57),
+  // four where a row is long (1200 x 8192: 24 us against 33).  Streaming rows through
+  // shared memory wins once every CTA has many of them and its threads are busy
+  // (16384 x 2048: 46 us; 9001 x 5120: 57 us against 72; 4096 x 2048: 16.6 against 15.1).
+  const bool elem = a.gate != nullptr && a.gate_col != 0 && a.gate_row != 0;
+  const int stage = a.H * (elem ? (a.gate_f32 ? 8 : 6) : 4);
+  const int min_rows = vec <= kNormThreads ? 8192 : 2048;
+  cudaError_t e;
+  if (a.T >= min_rows && 2 * vec > kNormThreads && vec <= 4 * kNormThreads &&
+      3 * stage <= norm_ring_bytes<2>())
+    e = vec <= kNormThreads       ? block_norm_stream_launch<1>(a, stage, stream)
+        : vec <= 2 * kNormThreads ? block_norm_stream_launch<2>(a, stage, stream)
+        : vec <= 3 * kNormThreads ? block_norm_stream_launch<3>(a, stage, stream)
+                                  : block_norm_stream_launch<4>(a, stage, stream);
+  else if (a.T >= 1024 && vec > 512 && vec <= 1024)
+    e = block_norm_launch<4, 256>(a, stream);
+  else if (a.T >= 1024 && vec >= 128 && vec <= 512)
+    e = block_norm_launch<2, 256>(a, stream);
+  else
+    e = vec <= 1024   ? block_norm_launch<1>(a, stream)
+        : vec <= 2048 ? block_norm_launch<2>(a, stream)
+                      : block_norm_launch<4>(a, stream);
   return note_cuda_error(e) == cudaSuccess ? kRcOk : kRcCudaError;
 }
 

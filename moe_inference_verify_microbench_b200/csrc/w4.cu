@@ -597,6 +597,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_stream(const W4Args a) {
   const int nt = max(0, min(*a.num_tiles, a.max_tiles));
   W4Pos lo, hi;
   w4_range<NT>(a, nt, &lo, &hi);
+  if constexpr (!SWIGLU) w4_zero_tail(a, threadIdx.x, kW4Threads);
   w4_units<SWIGLU, KB, NT, SLOTS, MODE>(a, smem_raw + w4_part_bytes<NT>(),
                                          reinterpret_cast<float*>(smem_raw), nt, lo, hi);
 }
@@ -730,7 +731,8 @@ int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* 
 
 int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
                  int max_tiles, const int* row_map, const float* row_scale, void* out,
-                 int out_rows, int avg, int* status, cudaStream_t stream) {
+                 int out_rows, int avg, int* status, cudaStream_t stream,
+                 const long long* tail) {
   if (const int rc = w4_check_bank(bank); rc != kRcOk) return rc;
   if (M < 0 || max_tiles < 0 || out_rows < 0 || tiles == nullptr || num_tiles == nullptr)
     return kRcBadArgument;
@@ -751,6 +753,7 @@ int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, co
   a.out_rows = out_rows;
   a.row_map = row_map;
   a.row_scale = row_scale;
+  a.tail = tail;
   a.avg = avg;
   a.status = status;
   return w4_dispatch<false>(a, stream);

@@ -100,6 +100,7 @@ struct W4Args {
   int out_rows;
   const int* row_map;
   const float* row_scale;
+  const long long* tail;  // rows of out from *tail on are zeroed (null: none)
   int avg;              // records per expert to expect (chooses the kernel)
   int* status;
 };
@@ -132,6 +133,17 @@ __device__ __forceinline__ bool w4_entry_ok(const W4Args& a, const int4& t) {
   if (t.x < 0 || t.x >= a.E) record_status(a.status, kErrBadExpert);
   else if (t.y != t.z) record_status(a.status, kErrBadRow);
   return false;
+}
+
+// Zeroes the output rows from *a.tail on, with `count` threads of every CTA.
+__device__ __forceinline__ void w4_zero_tail(const W4Args& a, int thread, int count) {
+  if (a.tail == nullptr) return;
+  const long long first = max(0ll, min(*a.tail, static_cast<long long>(a.out_rows)));
+  const int vec = a.out_ld / 8;
+  for (long long r = first + blockIdx.x; r < a.out_rows; r += gridDim.x) {
+    uint4* row = reinterpret_cast<uint4*>(a.out + static_cast<size_t>(r) * a.out_ld);
+    for (int v = thread; v < vec; v += count) row[v] = make_uint4(0, 0, 0, 0);
+  }
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -38,14 +38,5 @@ def fused_moe_forward_w4(sorted_x: torch.Tensor, offsets: torch.Tensor, bank) ->
     """``fused_moe_forward`` on a 4-bit bank (``W4Experts``): rows
     ``offsets[e]:offsets[e+1]`` of ``sorted_x`` through expert e, unweighted, in
     sorted order; rows past ``offsets[E]`` are zero."""
-    M, H = sorted_x.shape
-    E = bank.num_experts
-    if offsets.numel() != E + 1:
-        raise ValueError(f"offsets must have E+1 = {E + 1} entries")
     off = offsets.to(device=sorted_x.device, dtype=torch.int64).contiguous()
-    with ops._on(sorted_x.device):
-        tiles, num_tiles, mt = ops.tiles_from_offsets(off, M)
-        h = ops.grouped_w13_swiglu_w4(sorted_x.contiguous(), tiles, num_tiles, mt, bank)
-        y = torch.zeros((M, H), dtype=sorted_x.dtype, device=sorted_x.device)
-        ops.grouped_w2_w4(h, tiles, num_tiles, mt, bank, out=y)
-    return y
+    return ops.sorted_experts_w4(sorted_x.contiguous(), off, bank)

@@ -94,15 +94,45 @@ _HERE = contextlib.nullcontext()
 def _on(device: torch.device):
     """Makes ``device`` the current one for a launch on its stream (nothing to do
     where it is already)."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index == torch.cuda.current_device():
         return _HERE
     return torch.cuda.device(device)
+
+
+def _is(t, dtype: torch.dtype, ndim: int, device: torch.device) -> bool:
+    """Whether ``t`` is a contiguous tensor of this type, rank and device: what the
+    calls of a few microseconds ask first, leaving the messages to ``_need``."""
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == ndim
+            and t.device == device and t.is_contiguous())
+
+
+def _at(t: torch.Tensor, name: str, dtype: torch.dtype, ndim: int, device: torch.device) -> int:
+    """Address of a tensor that has to be as ``_is`` says."""
+    if not _is(t, dtype, ndim, device):
+        _need(t, name, dtype, ndim)
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    return t.data_ptr()
 
 
 def _same_device(device: torch.device, **tensors: torch.Tensor | None) -> None:
     for name, t in tensors.items():
         if t is not None and t.device != device:
             raise ValueError(f"{name} must be on {device}, got {t.device}")
+
+
+# The library, once loaded, and the raw stream of a device without a Stream object.
+_lib: ctypes.CDLL | None = None
+
+
+def _native_lib() -> ctypes.CDLL:
+    global _lib
+    if _lib is None:
+        _lib = _native.load()
+    return _lib
+
+
+def _raw_stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 # --------------------------------------------------------------------------- router
@@ -410,17 +440,15 @@ def block_norm(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor,
     _need(delta, "delta", torch.bfloat16)
     if x.dim() == 0 or delta.shape != x.shape:
         raise ValueError("delta must have the shape of x, [..., H]")
-    if gate_act not in _GATE_ACTS:
+    act = _GATE_ACTS.get(gate_act)
+    if act is None:
         raise ValueError(f"gate_act must be one of {tuple(_GATE_ACTS)}, got {gate_act!r}")
     H = x.shape[-1]
     T = x.numel() // max(H, 1)
     dev = x.device
-    w = []
-    for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight)):
-        if t.device != dev or t.numel() != H:
-            raise ValueError(f"{name} must be [H] on the device of x")
-        w.append(t.detach().float().contiguous())
-    kind = 0
+    post, pre = (_norm_weight(t, name, H, dev) for name, t in (("post_weight", post_weight),
+                                                               ("pre_weight", pre_weight)))
+    kind, g_ptr, g_f32 = 0, None, 0
     if gate is not None:
         if gate.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError(f"gate must be bfloat16 or float32, got {gate.dtype}")
@@ -434,14 +462,27 @@ def block_norm(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor,
         else:
             raise ValueError(f"gate must be [H], [..., 1] or [..., H] for x {tuple(x.shape)}, got "
                              f"{tuple(gate.shape)}")
-    _same_device(dev, delta=delta, gate=gate)
+        _same_device(dev, gate=gate)
+        g_ptr, g_f32 = gate.data_ptr(), int(gate.dtype is torch.float32)
+    if delta.device != dev:
+        raise ValueError(f"delta must be on {dev}, got {delta.device}")
     h, y = torch.empty_like(x), torch.empty_like(x)
     with _on(dev):
-        _rc(_native.load().moe_block_norm(
-            _p(x), _p(delta), _p(w[0]), _p(w[1]), _p(gate), kind,
-            int(gate is not None and gate.dtype == torch.float32), _GATE_ACTS[gate_act],
-            float(residual_scale), T, H, float(eps), _p(h), _p(y), _stream(dev)), "moe_block_norm")
+        rc = _native_lib().moe_block_norm(x.data_ptr(), delta.data_ptr(), post.data_ptr(),
+                                          pre.data_ptr(), g_ptr, kind, g_f32, act, residual_scale,
+                                          T, H, eps, h.data_ptr(), y.data_ptr(), _raw_stream(dev))
+    if rc:
+        _rc(rc, "moe_block_norm")
     return h, y
+
+
+def _norm_weight(t: torch.Tensor, name: str, H: int, device: torch.device) -> torch.Tensor:
+    """A norm's weight as the contiguous fp32 [H] the kernel reads."""
+    if t.device != device or t.numel() != H:
+        raise ValueError(f"{name} must be [H] on the device of x")
+    if t.dtype is torch.float32 and t.is_contiguous():
+        return t
+    return t.detach().float().contiguous()
 
 
 # --------------------------------------------------------------------------- EP send plan
@@ -587,9 +628,11 @@ def layer_workspace_bytes(T: int, H: int, I: int, E: int, top_k: int,
 # --------------------------------------------------------------------------- 4-bit experts
 
 
+_W4Experts: type = type(None)  # the bank's class, set by the module that defines it
+
+
 def _bank_of(bank, device: torch.device, hidden: int | None = None):
-    from .w4 import W4Experts
-    if not isinstance(bank, W4Experts):
+    if bank is None or not isinstance(bank, _W4Experts):
         raise TypeError(f"bank must be a W4Experts, got {type(bank).__name__}")
     if bank.device != device:
         raise ValueError(f"the 4-bit bank is on {bank.device}, the activations on {device}")
@@ -696,11 +739,11 @@ def experts_w4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, bank,
     held); records of other experts add nothing, as in C6's local-expert filter
     (C6/python/solution.py:137-176).  ``ids`` int32 [T, k], ``weights`` fp32 [T, k], k <= 8."""
     _need(x, "x", torch.bfloat16, 2)
-    _need(ids, "ids", torch.int32, 2)
-    _need(weights, "weights", torch.float32, 2)
     dev = x.device
     T, H = x.shape
     _bank_of(bank, dev, H)
+    ids_p = _at(ids, "ids", torch.int32, 2, dev)
+    weights_p = _at(weights, "weights", torch.float32, 2, dev)
     k = ids.shape[1]
     if ids.shape[0] != T or weights.shape != ids.shape:
         raise ValueError(f"ids and weights must be [T, k] with T = {T}, got {tuple(ids.shape)} and "
@@ -710,15 +753,40 @@ def experts_w4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, bank,
     if e_begin < 0 or e_begin + bank.num_experts > num_experts:
         raise ValueError(f"experts [{e_begin}, {e_begin + bank.num_experts}) of the bank are not "
                          f"among {num_experts}")
-    _same_device(dev, ids=ids, weights=weights)
-    lib = _native.load()
+    lib = _native_lib()
     y = _output(out, (T, H), dev)
-    ws = _workspace(workspace, int(lib.moe_w4_experts_workspace_bytes(T, k, bank.native)), dev)
+    ws = _workspace(workspace, lib.moe_w4_experts_workspace_bytes(T, k, bank.native), dev)
     with _on(dev):
-        _rc(lib.moe_w4_experts_forward(_p(x), _p(ids), _p(weights), T, k, num_experts, e_begin,
-                                       bank.native, _p(ws), ws.numel() * ws.element_size(), _p(y),
-                                       _p(status_word(dev)), _stream(dev)),
-            "moe_w4_experts_forward")
+        rc = lib.moe_w4_experts_forward(x.data_ptr(), ids_p, weights_p, T, k, num_experts, e_begin,
+                                        bank.native, ws.data_ptr(), ws.nbytes, y.data_ptr(),
+                                        status_word(dev).data_ptr(), _raw_stream(dev))
+    if rc:
+        _rc(rc, "moe_w4_experts_forward")
+    return y
+
+
+def sorted_experts_w4(sorted_x: torch.Tensor, offsets: torch.Tensor, bank,
+                      out: torch.Tensor | None = None,
+                      workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """The 4-bit experts for rows sorted by expert (C9/python/solution.py:207-222):
+    rows ``offsets[e]:offsets[e+1]`` (int64 [E+1]) through expert e, unweighted, in
+    sorted order; rows past ``offsets[E]`` are zero.  One C-ABI call."""
+    _need(sorted_x, "sorted_x", torch.bfloat16, 2)
+    dev = sorted_x.device
+    M, H = sorted_x.shape
+    _bank_of(bank, dev, H)
+    offsets_p = _at(offsets, "offsets", torch.int64, 1, dev)
+    if offsets.numel() != bank.num_experts + 1:
+        raise ValueError(f"offsets must have E+1 = {bank.num_experts + 1} entries")
+    lib = _native_lib()
+    y = _output(out, (M, H), dev)
+    ws = _workspace(workspace, lib.moe_w4_sorted_workspace_bytes(M, bank.native), dev)
+    with _on(dev):
+        rc = lib.moe_w4_sorted_forward(sorted_x.data_ptr(), M, offsets_p, bank.native,
+                                       ws.data_ptr(), ws.nbytes, y.data_ptr(),
+                                       status_word(dev).data_ptr(), _raw_stream(dev))
+    if rc:
+        _rc(rc, "moe_w4_sorted_forward")
     return y
 
 
@@ -734,24 +802,25 @@ def moe_layer_w4(x: torch.Tensor, router_weight: torch.Tensor, bank, top_k: int,
     """``moe_layer`` on a 4-bit bank (``W4Experts``) that holds all experts: router,
     top-k, experts and the weighted sum in one C-ABI call."""
     _need(x, "x", torch.bfloat16, 2)
-    _need(router_weight, "router_weight", torch.bfloat16, 2)
     dev = x.device
     T, H = x.shape
     _bank_of(bank, dev, H)
-    if tuple(router_weight.shape) != (bank.num_experts, H):
+    router_p = _at(router_weight, "router_weight", torch.bfloat16, 2, dev)
+    if router_weight.shape != (bank.num_experts, H):
         raise ValueError(f"router_weight must be [E, H] = {(bank.num_experts, H)}, got "
                          f"{tuple(router_weight.shape)}")
+    bias_p = None
     if bias is not None:
-        _need(bias, "bias", torch.float32, 1)
+        bias_p = _at(bias, "bias", torch.float32, 1, dev)
         if bias.numel() != bank.num_experts:
             raise ValueError(f"bias must hold E = {bank.num_experts} entries")
-    _same_device(dev, router_weight=router_weight, bias=bias)
-    lib = _native.load()
+    lib = _native_lib()
     y = _output(out, (T, H), dev)
-    ws = _workspace(workspace, int(lib.moe_w4_layer_workspace_bytes(T, top_k, bank.native)), dev)
+    ws = _workspace(workspace, lib.moe_w4_layer_workspace_bytes(T, top_k, bank.native), dev)
     with _on(dev):
-        _rc(lib.moe_w4_layer_forward(_p(x), _p(router_weight), _p(bias), bank.native, T, top_k,
-                                     int(bool(norm_topk_prob)), _p(ws),
-                                     ws.numel() * ws.element_size(), _p(y), _p(status_word(dev)),
-                                     _stream(dev)), "moe_w4_layer_forward")
+        rc = lib.moe_w4_layer_forward(x.data_ptr(), router_p, bias_p, bank.native, T, top_k,
+                                      1 if norm_topk_prob else 0, ws.data_ptr(), ws.nbytes,
+                                      y.data_ptr(), status_word(dev).data_ptr(), _raw_stream(dev))
+    if rc:
+        _rc(rc, "moe_w4_layer_forward")
     return y

@@ -167,3 +167,6 @@ def _pack(first, second, group: int, status: torch.Tensor):
                                        group, p(q), p(s), p(status), ops._stream(dev)),
             "moe_w4_pack")
     return q, s
+
+
+ops._W4Experts = W4Experts

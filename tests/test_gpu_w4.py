@@ -357,7 +357,9 @@ def test_two_streams_at_once(cuda):
 # ------------------------------------------------------------------ block norm
 
 
-@pytest.mark.parametrize("T,H", [(1, 8), (1, 2048), (3, 264), (17, 2048), (5, 5120), (2, 16392),
+@pytest.mark.parametrize("T,H", [(1, 8), (1, 2048), (3, 264), (17, 2048), (5, 5120), (2, 16392), (1500, 264),
+                                 (2048, 5120), (2100, 8192), (8200, 1032), (1100, 4104),
+                                 (1030, 2056), (8192, 2048),
                                  (1, 32768), (1000, 1024)])
 @pytest.mark.parametrize("gate,act", [("absent", "none"), ("token", "sigmoid"), ("channel", "none"),
                                       ("element", "tanh"), ("channel", "sigmoid"), ("element", "none")])
