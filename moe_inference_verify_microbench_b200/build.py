@@ -20,9 +20,10 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libmoe_b200.so")
 SOURCES = ["capi.cu", "gemm.cu", "sort_align.cu", "rows.cu", "sort_align_static.cu", "decode.cu",
-           "ep_plan.cu", "ep_peer.cu", "w4.cu", "w4_gemm.cu"]
+           "ep_plan.cu", "ep_peer.cu", "w4.cu", "w4_gemm.cu", "w4_decode.cu"]
 HEADERS = ["ptx.cuh", "grouped_gemm.cuh", "grouped_gemm_pair.cuh", "internal.h", "sort_block.cuh",
-           "router_splitk.cuh", "w4.cuh"]
+           "router_splitk.cuh", "w4.cuh", "w4_stream.cuh",
+           "decode_route.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
     "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr",

@@ -2,6 +2,8 @@
 #include "../../include/moe_b200.h"
 #include "internal.h"
 
+#include <algorithm>
+
 using namespace moe;
 
 namespace {
@@ -102,7 +104,7 @@ struct W4Layout {
   int4* tiles;
   int max_tiles;
   int* num_tiles;
-  void *h, *slots;
+  void *h, *slots, *decode;
   size_t bytes;
 };
 
@@ -124,6 +126,7 @@ W4Layout w4_layout(void* ws, int T, int k, const W4Bank& b, bool routed) {
   l.num_tiles = c.take<int>(1);
   l.h = c.take<__nv_bfloat16>(R * b.I);
   l.slots = c.take<__nv_bfloat16>(R * b.H);
+  if (routed) l.decode = c.take<uint8_t>(w4_decode_scratch_bytes(b, std::min(T, 64)));
   l.bytes = c.used;
   return l;
 }
@@ -680,6 +683,9 @@ int moe_w4_layer_forward(const void* x, const void* router_weight, const float* 
     return kRcBadArgument;
   const W4Layout l = w4_layout(workspace, T, top_k, b, true);
   if (workspace_bytes < l.bytes) return kRcWorkspace;
+  if (w4_decode_ok(b, T, top_k))
+    return launch_w4_decode(b, x, router_weight, router_bias, T, top_k, norm_topk_prob, l.decode,
+                            l.h, y, status, stream);
   if (use_router_small(T, b.H, b.E, top_k)) {
     rc = launch_router_sort_small(x, router_weight, router_bias, T, b.H, b.E, top_k,
                                   norm_topk_prob, l.ids, l.w, nullptr, l.counts, l.offsets, l.perm,

@@ -194,6 +194,14 @@ int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, co
                  int out_rows, int avg, int* status, cudaStream_t stream,
                  const long long* tail = nullptr);
 
+// The whole layer for a few tokens (w4_decode.cu; T <= 16, T * k <= 64): `scratch`
+// holds w4_decode_scratch_bytes(b, T) bytes, h [T * k, I] bf16.
+bool w4_decode_ok(const W4Bank& b, int T, int k);
+size_t w4_decode_scratch_bytes(const W4Bank& b, int T);
+int launch_w4_decode(const W4Bank& b, const void* x, const void* wr, const float* bias, int T,
+                     int k, int norm_topk_prob, void* scratch, void* h, void* y, int* status,
+                     cudaStream_t stream);
+
 // Norms around a block: n = RMSNorm(delta) * post, h = x + scale * act(gate) * n,
 // y = RMSNorm(h) * pre.  gate[t * gate_row + c * gate_col], bf16 or fp32, null: 1.
 struct BlockNormArgs {
