@@ -100,8 +100,8 @@ __global__ void __launch_bounds__(256) w4_pack(const W4PackArgs a) {
     if (zp) {
       const uint8_t z0 = a.zeros[0][o0], z1 = a.zeros[pair ? 1 : 0][o1];
       bad |= z0 > 15 || z1 > 15;
-      rec[2] = 0x6400u | (z0 & 15u);  // fp16 1024 + z
-      rec[3] = 0x6400u | (z1 & 15u);
+      rec[2] = 0x4300u | (z0 & 15u);  // bf16 128 + z
+      rec[3] = 0x4300u | (z1 & 15u);
     }
   }
   if (bad) record_status(a.status, kErrBadCode);
@@ -109,17 +109,16 @@ __global__ void __launch_bounds__(256) w4_pack(const W4PackArgs a) {
 
 // ------------------------------------------------------------------ streaming
 
-template <bool SWIGLU, int KB, int NT, int SLOTS, int MODE>
+template <bool SWIGLU, int KB, int MODE>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_stream(const W4Args a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   pdl_wait();
   pdl_trigger();
   const int nt = max(0, min(*a.num_tiles, a.max_tiles));
-  W4Pos lo, hi;
-  w4_range<NT>(a, nt, &lo, &hi);
+  W4TableWalk walk;
+  walk.open_range(a, nt);
   if constexpr (!SWIGLU) w4_zero_tail(a, threadIdx.x, kW4Threads);
-  w4_units<SWIGLU, KB, NT, SLOTS, MODE>(a, smem_raw + w4_part_bytes<NT>(),
-                                         reinterpret_cast<float*>(smem_raw), nt, lo, hi);
+  w4_units<SWIGLU, KB, MODE>(a, smem_raw + kW4PartBytes, reinterpret_cast<float*>(smem_raw), walk);
 }
 
 // ------------------------------------------------------------------ launchers
@@ -137,36 +136,27 @@ int w4_check_bank(const W4Bank& b) {
   return kRcOk;
 }
 
-template <bool SWIGLU, int KB, int NT, int SLOTS, int MODE>
+template <bool SWIGLU, int KB, int MODE>
 static int w4_launch(W4Args& a, cudaStream_t stream) {
   a.p = w4_plan(a.m, KB);
-  const int sh = w4_part_bytes<NT>() + kW4Warps * SLOTS * a.p.slot_bytes;
+  const int sh = kW4PartBytes + kW4Warps * w4_slots<KB, MODE>() * a.p.slot_bytes;
   if (sh > kW4SmemBytes) return kRcUnsupported;
   static std::atomic<uint64_t> attr{0};
-  if (!allow_smem(w4_stream<SWIGLU, KB, NT, SLOTS, MODE>, kW4SmemBytes, attr)) return kRcCudaError;
+  if (!allow_smem(w4_stream<SWIGLU, KB, MODE>, kW4SmemBytes, attr)) return kRcCudaError;
   const long long units = static_cast<long long>(a.max_tiles) * a.m.tiles;
   const int grid = static_cast<int>(std::min<long long>(units, device_sm_count()));
-  return note_cuda_error(launch_pdl(w4_stream<SWIGLU, KB, NT, SLOTS, MODE>, dim3(grid),
-                                    dim3(kW4Threads), sh, stream, a)) == cudaSuccess
+  return note_cuda_error(launch_pdl(w4_stream<SWIGLU, KB, MODE>, dim3(grid), dim3(kW4Threads), sh,
+                                    stream, a)) == cudaSuccess
              ? kRcOk
              : kRcCudaError;
 }
 
 template <bool SWIGLU, int MODE>
 static int w4_dispatch_mode(W4Args& a, cudaStream_t stream) {
-  // Up to about six records per expert a pass takes eight, so that a warp can
-  // hold twice the blocks and half as many warps add partials; beyond, sixteen.
-  const int wide = a.avg > 6 ? w4_best_kb(a.m.nb, {2, 3, 4}) : 0;
-  constexpr int kSlots8 = MODE == kW4Half ? 2 : 3;
-  switch (wide) {
-    case 2: return w4_launch<SWIGLU, 2, 2, 8, MODE>(a, stream);
-    case 3: return w4_launch<SWIGLU, 3, 2, 5, MODE == kW4TwoBlocks ? kW4Block : MODE>(a, stream);
-    case 4: return w4_launch<SWIGLU, 4, 2, 4, MODE>(a, stream);
-  }
   switch (w4_best_kb(a.m.nb, {4, 6, 8})) {
-    case 4: return w4_launch<SWIGLU, 4, 1, 4, MODE>(a, stream);
-    case 6: return w4_launch<SWIGLU, 6, 1, 3, MODE>(a, stream);
-    case 8: return w4_launch<SWIGLU, 8, 1, kSlots8, MODE>(a, stream);
+    case 4: return w4_launch<SWIGLU, 4, MODE>(a, stream);
+    case 6: return w4_launch<SWIGLU, 6, MODE>(a, stream);
+    case 8: return w4_launch<SWIGLU, 8, MODE>(a, stream);
   }
   return kRcUnsupported;
 }

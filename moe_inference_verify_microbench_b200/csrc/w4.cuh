@@ -6,7 +6,7 @@
 // Packed layout, written once when the weights are loaded (w4_pack):
 //   q  [expert][tile][block][32 lanes][16 bytes]  tile: 16 rows, block: 64 columns
 //   s  [expert][tile][group][8] records of rows g and g + 8: two bf16 scales and,
-//      with zero points, two fp16 values 1024 + z
+//      with zero points, two bf16 values 128 + z
 // Lane 4g + t of a block holds rows g and g + 8 of the tile: {row g columns 0..31,
 // row g 32..63, row g+8 0..31, row g+8 32..63}, eight codes to a word.  Within a
 // word, nibble i holds column 8i + 2t and nibble i + 4 column 8i + 2t + 1 (i < 4)
@@ -18,7 +18,6 @@
 #pragma once
 
 #include <atomic>
-#include <cuda_fp16.h>
 
 #include "internal.h"
 #include "ptx.cuh"
@@ -38,29 +37,28 @@ struct W4Matrix {
   int gshift;        // log2(group / 32)
 };
 
-// The codes of one word's column pair i as an fp16 pair: 1024 + q for even i,
-// 64 + q for odd i.  The ten mantissa bits of 1024.0 (0x6400) end with the ones,
-// those of 64.0 (0x5400) have the ones at bits 4..7, so one shift serves two
-// pairs and the or is exact: five integer instructions for eight codes.
+// The column pairs of a word as bf16 pairs 128 + q: 0x4300 is 128.0 and a code is
+// the last four bits of the seven-bit mantissa, so the or is exact: seven integer
+// instructions for eight codes.
 __device__ __forceinline__ void w4_pairs(uint32_t w, uint32_t (&r)[4]) {
-  const uint32_t v = w >> 8;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r[0]) : "r"(w), "n"(0x000f000f), "r"(0x64006400u));
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r[1]) : "r"(w), "n"(0x00f000f0), "r"(0x54005400u));
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r[2]) : "r"(v), "n"(0x000f000f), "r"(0x64006400u));
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r[3]) : "r"(v), "n"(0x00f000f0), "r"(0x54005400u));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;"
+        : "=r"(r[i])
+        : "r"(w >> (4 * i)), "n"(0x000f000f), "r"(0x43004300u));
 }
 
-// fp16 pair a - b, exact for the small integers used here.
-__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+// bf16 pair a - b, exact for the small integers used here.
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
-// d += a * b, 16 x 8 x 16, fp16 operands, fp32 accumulate.
+// d += a * b, 16 x 8 x 16, bf16 operands, fp32 accumulate.
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                           uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -78,6 +76,7 @@ struct W4Plan {
 // How often a warp applies scales: after every two blocks, after every block, or
 // after every 32 columns.  The last also subtracts zero points from each operand.
 enum W4Mode : int { kW4TwoBlocks = 0, kW4Block = 1, kW4Half = 2 };
+constexpr int kW4Recs = 8;  // records that share one pass over the weights
 
 constexpr int kW4Warps = 16;
 constexpr int kW4Threads = 32 * kW4Warps;

@@ -69,7 +69,6 @@ __global__ void __launch_bounds__(32) w4_logits(const uint4* __restrict__ x,
 constexpr int kLayerSmemBytes = 223 * 1024;  // beside 3.4 KB of static shared memory
 constexpr int kLayerSlots = 2;   // of a warp in the down phase
 constexpr int kLayerMaxT = 16;   // as the small router's
-constexpr int kItemRecs = 8;
 constexpr int kDsumBytes = kFusedMaxRecs * 16 * 4;
 
 // Bytes between the staged rows of h: 16 more than a row, so that the eight rows
@@ -80,15 +79,16 @@ __host__ __device__ constexpr int h_pitch(int I) { return 2 * I + 16; }
 // records); the groups of ks warps take them in turn.
 template <int KB, int MODE>
 __device__ __forceinline__ void w4_down(const W4LayerArgs& d, const RouteSmem& rs, uint8_t* smem,
-                                        const int2* items, int nitems,
+                                        const int4* items, int nitems,
                                         volatile int* abort_flag) {
   const W4Args& a = d.down;
   const W4Plan& p = a.p;
   const W4Share sh = w4_share<KB>(a);
+  const W4Lane<KB, MODE> own(a, sh);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int warp = sh.tl * p.ks + sh.ks;
   float* part = reinterpret_cast<float*>(smem);
-  uint8_t* slots = smem + w4_part_bytes<1>();
+  uint8_t* slots = smem + kW4PartBytes;
   // the products of every record for a row tile, then the staged rows of h
   auto* dsum = reinterpret_cast<float(*)[16]>(slots + kW4Warps * kLayerSlots * p.slot_bytes);
   uint8_t* hs = reinterpret_cast<uint8_t*>(dsum + kFusedMaxRecs);
@@ -100,10 +100,10 @@ __device__ __forceinline__ void w4_down(const W4LayerArgs& d, const RouteSmem& r
   int f_tile = blockIdx.x, f_item = sh.tl, f_slot = 0;
   auto fetch = [&]() {
     if (f_tile < a.m.tiles && sh.tl < nitems) {
-      const size_t et = static_cast<size_t>(rs.tiles[items[f_item].x].x) * a.m.tiles + f_tile;
-      w4_fetch<KB>(a, sh, base + f_slot * p.slot_bytes,
-                   a.m.q + (et * a.m.nb + sh.kb0) * kW4BlockBytes + lane * 16,
-                   a.m.s + ((et * a.m.ng + sh.g0) * 8 + lane) * a.m.rec);
+      const size_t et = static_cast<size_t>(items[f_item].x) * a.m.tiles + f_tile;
+      own.fetch(a, sh, base + f_slot * p.slot_bytes,
+                a.m.q + (et * a.m.nb + sh.kb0) * kW4BlockBytes + lane * 16,
+                a.m.s + et * a.m.ng * 8 * a.m.rec);
       f_item += p.tl;
       if (f_item >= nitems) {
         f_item = sh.tl;
@@ -131,52 +131,34 @@ __device__ __forceinline__ void w4_down(const W4LayerArgs& d, const RouteSmem& r
   __syncthreads();
 
   int slot = 0, buffer = 0;
-  constexpr int kStride = 128, kBuffer = kW4Warps * kStride;
   for (int tile = blockIdx.x; tile < a.m.tiles; tile += grid) {
     for (int item = sh.tl; item < nitems; item += p.tl) {
-      const int rec0 = items[item].y, n = min(kItemRecs, rs.tiles[items[item].x].z - rec0);
-      uint32_t b[KB][1][8];
-      float fold[KB][1][2], inv[1][2], acc[1][4];
+      const int rec0 = items[item].y, n = items[item].z - rec0;
+      uint32_t b[KB][8];
+      float fold[KB][2], acc[4];
       const uint32_t src = smem_u32(hs) + (rec0 + min(g, n - 1)) * pitch + sh.kb0 * 128 + t * 4;
 #pragma unroll
       for (int k = 0; k < KB; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          b[k][0][i] = g < n && k < sh.myb ? lds32(src + k * 128 + i * 16) : 0u;
-      w4_prepare_records<KB, 1, MODE>(b, fold, inv);
+          b[k][i] = g < n && k < sh.myb ? lds32(src + k * 128 + i * 16) : 0u;
+      w4_fold<KB, MODE>(b, fold);
       cp_async_wait_group<1>();
       __syncwarp();  // every lane's copies of this tile have landed
-      w4_tile<KB, 1, MODE>(a, sh, base + slot * p.slot_bytes, b, fold, inv, acc);
+      w4_tile<KB, MODE>(a, base + slot * p.slot_bytes, b, fold, acc);
       slot ^= 1;
       __syncwarp();  // and every lane has read them
       fetch();
-      if (p.ks > 1) {
-        float* pw = part + buffer + warp * kStride + lane;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) pw[v * 32] = acc[0][v];
-        named_barrier(1 + sh.tl, p.ks * 32);
-      }
+      w4_meet(a, sh, acc, part, buffer);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        if ((u & (p.ks - 1)) == sh.ks) {
-          float v0 = acc[0][u], v1 = acc[0][u + 2];
-          if (p.ks > 1) {
-            v0 = v1 = 0.0f;
-            const float* pr = part + buffer + sh.tl * p.ks * kStride + u * 32 + lane;
-            for (int w = 0; w < p.ks; w += 2) {
-              v0 += pr[0] + pr[kStride];
-              v1 += pr[64] + pr[kStride + 64];
-              pr += 2 * kStride;
-            }
-          }
-          const int rec = 2 * t + u;
-          if (rec < n) {
-            dsum[rec0 + rec][g] = v0;
-            dsum[rec0 + rec][g + 8] = v1;
-          }
+        const int rec = 2 * t + u;
+        if ((u & (p.ks - 1)) == sh.ks && rec < n) {
+          dsum[rec0 + rec][g] = acc[u];
+          dsum[rec0 + rec][g + 8] = acc[u + 2];
         }
       }
-      buffer ^= kBuffer;
+      buffer ^= kW4Warps * 128;
     }
     __syncthreads();
     // y = sum over the token's slots, in slot order, rounded once
@@ -192,11 +174,38 @@ __device__ __forceinline__ void w4_down(const W4LayerArgs& d, const RouteSmem& r
   cp_async_wait_all();
 }
 
-template <int KB_UP, int KB_DOWN, int SLOTS, int MODE>
+// This CTA's share of the units (item, tile), split evenly over the grid, and a walk
+// through it as w4_units takes it.
+struct W4ItemWalk {
+  const int4* items;
+  int item, tile, hi_item, hi_tile;
+  __device__ __forceinline__ W4ItemWalk(const int4* its, int nitems, int tiles) : items(its) {
+    const uint32_t total = static_cast<uint32_t>(nitems) * tiles;
+    const uint32_t lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
+    item = lo / tiles;
+    tile = lo - item * tiles;
+    hi_item = hi / tiles;
+    hi_tile = hi - hi_item * tiles;
+  }
+  __device__ __forceinline__ int expert() const { return items[item].x; }
+  __device__ __forceinline__ int first() const { return items[item].y; }
+  __device__ __forceinline__ int count() const { return items[item].z - items[item].y; }
+  __device__ __forceinline__ int run(const W4Args& a) {
+    while (tile >= a.m.tiles) {
+      tile -= a.m.tiles;
+      ++item;
+    }
+    if (item > hi_item) return 0;
+    const int end = item == hi_item ? hi_tile : a.m.tiles;
+    return end > tile ? (end - tile + a.p.tl - 1) >> a.p.tl_shift : 0;
+  }
+};
+
+template <int KB_UP, int KB_DOWN, int MODE>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_layer(const W4LayerArgs d) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ RouteSmem rs;
-  __shared__ int2 items[kFusedMaxRecs];  // {expert tile, first record}
+  __shared__ int4 items[kFusedMaxRecs];  // {expert, first record, last + 1, 0}
   __shared__ int nitems, abort_word;
   volatile int* abort_flag = &abort_word;
   if (threadIdx.x == 0) abort_word = 0;
@@ -205,46 +214,46 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_layer(const W4LayerArgs d) {
   topk_and_sort(d.logits, d.T, d.E, d.k, d.norm_topk_prob, rs);
   const int R = d.T * d.k;
   {
-    // every eighth record of a tile opens an item
+    // every eighth record of an expert opens an item
     const int r = threadIdx.x;
-    bool opens = false;
-    int tile = 0, before = 0;
     if (r < R) {  // r-th record in expert order
-      for (int q = 0; q <= r; ++q) {
-        const int tq = rs.tile_of[rs.perm[q]];
-        const bool o = (q - rs.tiles[tq].y) % kItemRecs == 0;
-        if (q < r) before += o ? 1 : 0;
-        else opens = o, tile = tq;
+      int before = 0, last = 0;
+      bool opens = false;
+      for (int i = 0; i < rs.nt; ++i) {
+        const int4 t = rs.tiles[i];
+        if (r >= t.z) {
+          before += (t.z - t.y + kW4Recs - 1) / kW4Recs;
+        } else if (r >= t.y) {
+          opens = (r - t.y) % kW4Recs == 0;
+          before += (r - t.y) / kW4Recs;
+          last = min(t.z, r + kW4Recs);
+          if (opens) items[before] = make_int4(t.x, r, last, 0);
+        }
       }
-      if (opens) items[before] = make_int2(tile, r);
-      if (r == R - 1) nitems = before + (opens ? 1 : 0);
+      if (r == R - 1) nitems = before + 1;
     }
   }
   __syncthreads();
 
   W4Args a = d.up;
-  a.tiles = rs.tiles;
   a.index = rs.perm;
   a.index_div = d.k;
-  W4Pos lo, hi;
-  w4_range<1>(a, rs.nt, &lo, &hi);
-  w4_units<true, KB_UP, 1, SLOTS, MODE>(a, smem_raw + w4_part_bytes<1>(),
-                                        reinterpret_cast<float*>(smem_raw), rs.nt, lo, hi);
+  w4_units<true, KB_UP, MODE>(a, smem_raw + kW4PartBytes, reinterpret_cast<float*>(smem_raw),
+                              W4ItemWalk(items, nitems, a.m.tiles));
   __syncthreads();  // every warp has left its slots
   w4_down<KB_DOWN, MODE>(d, rs, smem_raw, items, nitems, abort_flag);
 }
 
 template <int KB_UP, int KB_DOWN, int MODE>
 int layer_launch(W4LayerArgs& d, cudaStream_t stream) {
-  constexpr int kSlots = KB_UP == 8 && MODE == kW4Half ? 2 : 3;
   d.up.p = w4_plan(d.up.m, KB_UP);
   d.down.p = w4_plan(d.down.m, KB_DOWN);
-  const int up = w4_part_bytes<1>() + kW4Warps * kSlots * d.up.p.slot_bytes;
-  const int down = w4_part_bytes<1>() + kW4Warps * kLayerSlots * d.down.p.slot_bytes +
+  const int up = kW4PartBytes + kW4Warps * w4_slots<KB_UP, MODE>() * d.up.p.slot_bytes;
+  const int down = kW4PartBytes + kW4Warps * kLayerSlots * d.down.p.slot_bytes +
                    kDsumBytes + d.T * d.k * h_pitch(64 * d.down.m.nb);
   const int sh = std::max(up, down);
   if (sh > kLayerSmemBytes) return kRcUnsupported;
-  auto* kernel = w4_layer<KB_UP, KB_DOWN, kSlots, MODE>;
+  auto* kernel = w4_layer<KB_UP, KB_DOWN, MODE>;
   static std::atomic<uint64_t> attr{0};
   if (!allow_smem(kernel, kLayerSmemBytes, attr)) return kRcCudaError;
   cudaLaunchConfig_t cfg = {};
@@ -276,7 +285,7 @@ bool w4_decode_ok(const W4Bank& b, int T, int k) {
   const W4Matrix m = w4_matrix(b, true);
   const int kb = w4_best_kb(m.nb, {6, 8});
   if (T < 1 || T > kLayerMaxT || T * k > kFusedMaxRecs || kb == 0) return false;
-  const int down = w4_part_bytes<1>() + kW4Warps * kLayerSlots * w4_plan(m, kb).slot_bytes +
+  const int down = kW4PartBytes + kW4Warps * kLayerSlots * w4_plan(m, kb).slot_bytes +
                    kDsumBytes + T * k * h_pitch(b.I);
   return router_small_ok(T, b.H, b.E, k) && w4_best_kb(b.H / 64, {6, 8}) > 0 &&
          down <= kLayerSmemBytes;

@@ -117,15 +117,11 @@ __device__ __forceinline__ void bulk_wait_all() {
 // is rounded once.
 __device__ __forceinline__ void w4_scaled_pairs(uint32_t w, uint32_t z, uint32_t s, uint32_t* r,
                                                 int stride) {
+  uint32_t v[4];
+  w4_pairs(w, v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t v;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;"
-        : "=r"(v)
-        : "r"(w >> (4 * i)), "n"(0x000f000f), "r"(0x43004300u));
-    asm("sub.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(v), "r"(z));
-    asm("mul.bf16x2 %0, %1, %2;" : "=r"(r[i * stride]) : "r"(v), "r"(s));
-  }
+  for (int i = 0; i < 4; ++i)
+    asm("mul.bf16x2 %0, %1, %2;" : "=r"(r[i * stride]) : "r"(sub_bf16x2(v[i], z)), "r"(s));
 }
 
 // Which accumulator columns a unit uses.  Up to 64 records: one of two halves of
@@ -292,8 +288,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                   sc[h][i][0] = __byte_perm(sv, 0, 0x1010);
                   sc[h][i][1] = __byte_perm(sv, 0, 0x3232);
                   zp[h][i][0] = zp[h][i][1] = 0x43084308u;
-                  if (ZEROS) {  // fp16 1024 + z -> bf16 128 + z
-                    const uint32_t zv = (lds32(r + 4) & 0x000f000fu) | 0x43004300u;
+                  if (ZEROS) {
+                    const uint32_t zv = lds32(r + 4);
                     zp[h][i][0] = __byte_perm(zv, 0, 0x1010);
                     zp[h][i][1] = __byte_perm(zv, 0, 0x3232);
                   }

@@ -64,8 +64,8 @@ def test_packed_layout(cuda, E, H, I, group, zeros):
     assert torch.equal(s13[..., 0].permute(0, 1, 3, 2).reshape(E, I, -1), p[0][1])
     assert torch.equal(s13[..., 1].permute(0, 1, 3, 2).reshape(E, I, -1), p[1][1])
     assert torch.equal(s2[..., :2].permute(0, 1, 4, 3, 2).reshape(E, H, -1), p[2][1])
-    if zeros:  # kept as fp16 1024 + z
-        z13, z2 = (t.view(torch.float16).float() - 1024 for t in (s13[..., 3], s2[..., 2:]))
+    if zeros:  # kept as 128 + z
+        z13, z2 = (t.float() - 128 for t in (s13[..., 3], s2[..., 2:]))
         assert torch.equal(z13.permute(0, 1, 3, 2).reshape(E, I, -1), p[1][2].float())
         assert torch.equal(z2.permute(0, 1, 4, 3, 2).reshape(E, H, -1), p[2][2].float())
 

@@ -33,11 +33,11 @@ def values(m):
 
 
 def operand_sums(m, x, e):
-    """sum_k s * 1040 * |x_k| per (row of x, output): what the fp32 sums of products
-    with 1024 + q are formed from, in absolute value."""
+    """sum_k s * 144 * |x_k| per (row of x, output): what the fp32 sums of products
+    with 128 + q are formed from, in absolute value."""
     codes, scales, _ = m
     g = codes.shape[-1] // scales.shape[-1]
-    wide = scales[e].double().abs().repeat_interleave(g, dim=1) * 1040.0
+    wide = scales[e].double().abs().repeat_interleave(g, dim=1) * 144.0
     return x.double().abs() @ wide.t()
 
 
