@@ -66,10 +66,10 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 
 // How a projection is cut over a CTA's sixteen warps (w4_plan): `ks` warps share
 // a tile, kb blocks of 64 columns each (a kernel parameter; blocks past the last
-// are multiplied with zeros), and tl = 16 / ks tiles are worked on at once.
+// are multiplied with zeros), and tl = 16 / ks such groups work side by side.
 struct W4Plan {
   int ks, tl;
-  int ks_shift, tl_shift;  // their logarithms
+  int ks_shift;            // log2(ks)
   int slot_bytes;          // one tile's share of a warp: codes, then records
 };
 

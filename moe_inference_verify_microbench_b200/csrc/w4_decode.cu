@@ -174,14 +174,16 @@ __device__ __forceinline__ void w4_down(const W4LayerArgs& d, const RouteSmem& r
   cp_async_wait_all();
 }
 
-// This CTA's share of the units (item, tile), split evenly over the grid, and a walk
-// through it as w4_units takes it.
+// This group's share of the units (item, tile), split evenly over all groups of
+// the grid, and a walk through it as w4_units takes it.
 struct W4ItemWalk {
   const int4* items;
   int item, tile, hi_item, hi_tile;
-  __device__ __forceinline__ W4ItemWalk(const int4* its, int nitems, int tiles) : items(its) {
-    const uint32_t total = static_cast<uint32_t>(nitems) * tiles;
-    const uint32_t lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
+  __device__ __forceinline__ W4ItemWalk(const W4Args& a, const int4* its, int nitems) : items(its) {
+    const uint32_t tiles = a.m.tiles, total = nitems * tiles;
+    const uint32_t parts = gridDim.x * a.p.tl;  // total * parts < 2^16 * 2^12
+    const uint32_t part = blockIdx.x * a.p.tl + (threadIdx.x >> 5 >> a.p.ks_shift);
+    const uint32_t lo = total * part / parts, hi = total * (part + 1) / parts;
     item = lo / tiles;
     tile = lo - item * tiles;
     hi_item = hi / tiles;
@@ -196,8 +198,7 @@ struct W4ItemWalk {
       ++item;
     }
     if (item > hi_item) return 0;
-    const int end = item == hi_item ? hi_tile : a.m.tiles;
-    return end > tile ? (end - tile + a.p.tl - 1) >> a.p.tl_shift : 0;
+    return max((item == hi_item ? hi_tile : a.m.tiles) - tile, 0);
   }
 };
 
@@ -212,25 +213,30 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_layer(const W4LayerArgs d) {
   pdl_wait();
   pdl_trigger();
   topk_and_sort(d.logits, d.T, d.E, d.k, d.norm_topk_prob, rs);
-  const int R = d.T * d.k;
-  {
-    // every eighth record of an expert opens an item
-    const int r = threadIdx.x;
-    if (r < R) {  // r-th record in expert order
-      int before = 0, last = 0;
-      bool opens = false;
-      for (int i = 0; i < rs.nt; ++i) {
-        const int4 t = rs.tiles[i];
-        if (r >= t.z) {
-          before += (t.z - t.y + kW4Recs - 1) / kW4Recs;
-        } else if (r >= t.y) {
-          opens = (r - t.y) % kW4Recs == 0;
-          before += (r - t.y) / kW4Recs;
-          last = min(t.z, r + kW4Recs);
-          if (opens) items[before] = make_int4(t.x, r, last, 0);
-        }
+  if (threadIdx.x < 32) {
+    // Items: every expert's records by eights (32 lanes, two tiles each; 64 at most).
+    const int lane = threadIdx.x;
+    int chunks[2], at = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int e = 2 * lane + i;
+      chunks[i] = e < rs.nt ? (rs.tiles[e].z - rs.tiles[e].y + kW4Recs - 1) / kW4Recs : 0;
+    }
+    at = chunks[0] + chunks[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += y;
+    }
+    if (lane == 31) nitems = at;
+    at -= chunks[0] + chunks[1];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      for (int c = 0; c < chunks[i]; ++c, ++at) {
+        const int4 t = rs.tiles[2 * lane + i];
+        const int first = t.y + c * kW4Recs;
+        items[at] = make_int4(t.x, first, min(t.z, first + kW4Recs), 0);
       }
-      if (r == R - 1) nitems = before + 1;
     }
   }
   __syncthreads();
@@ -239,7 +245,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_layer(const W4LayerArgs d) {
   a.index = rs.perm;
   a.index_div = d.k;
   w4_units<true, KB_UP, MODE>(a, smem_raw + kW4PartBytes, reinterpret_cast<float*>(smem_raw),
-                              W4ItemWalk(items, nitems, a.m.tiles));
+                              W4ItemWalk(a, items, nitems));
   __syncthreads();  // every warp has left its slots
   w4_down<KB_DOWN, MODE>(d, rs, smem_raw, items, nitems, abort_flag);
 }

@@ -16,9 +16,11 @@ __device__ __forceinline__ int w4_chunks(const W4Args& a, const int4& t) {
   return (t.z - t.y + kW4Recs - 1) / kW4Recs;
 }
 
-// A CTA's contiguous range of units, the units split evenly over the grid, and a
-// walk through it: every tl-th unit from a first one on, in runs of tiles that
-// share their expert and records.
+// The contiguous range of units of one group of ks warps, the units split evenly
+// over all groups of the grid, and a walk through it in runs of tiles that share
+// their expert and records.  (Groups with ranges of their own load their
+// records at different times: with the tiles of one range per CTA dealt out in turn,
+// every group of the SM waited for its records at once.)
 struct W4TableWalk {
   int entry, chunk, tile;  // next unit
   int chunks;              // of the entry
@@ -27,10 +29,10 @@ struct W4TableWalk {
 
   // Every thread of the CTA calls it.  The kernel serves tables of fewer than 8
   // records per expert on average, so 32 bits hold a table's units (2048 chunks x
-  // 1024 tiles at most) and their product with the grid.
+  // 1024 tiles at most).
   __device__ __forceinline__ void open_range(const W4Args& a, int n_entries) {
     __shared__ uint32_t sums[kW4Warps];
-    __shared__ int2 pos[2];
+    __shared__ int2 pos[kW4Warps + 1];
     nt = n_entries;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto units = [&](int i) -> uint32_t {
@@ -39,7 +41,7 @@ struct W4TableWalk {
     const uint32_t first = units(threadIdx.x);  // most tables fit the CTA
     uint32_t mine = first;
     for (int i = threadIdx.x + kW4Threads; i < nt; i += kW4Threads) mine += units(i);
-    if (threadIdx.x < 2) pos[threadIdx.x] = make_int2(0, 0);
+    if (threadIdx.x <= kW4Warps) pos[threadIdx.x] = make_int2(0, 0);
     uint32_t total = 0, carry = 0;
     for (int base = 0; base < nt; base += kW4Threads) {
       const uint32_t c = base == 0 ? first : units(base + static_cast<int>(threadIdx.x));
@@ -70,19 +72,22 @@ struct W4TableWalk {
         carry += s;
       }
       incl += before;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t want = total * (blockIdx.x + k) / gridDim.x;
+      // the boundaries of this CTA's groups that fall into this entry
+      const uint32_t parts = gridDim.x * a.p.tl;
+      for (int k = 0; k <= a.p.tl; ++k) {
+        const uint32_t want = static_cast<uint32_t>(
+            static_cast<unsigned long long>(total) * (blockIdx.x * a.p.tl + k) / parts);
         if (want > incl - c && want <= incl)
           pos[k] = make_int2(base + static_cast<int>(threadIdx.x), static_cast<int>(want - (incl - c)));
       }
     }
     __syncthreads();
-    entry = pos[0].x;
-    tile = pos[0].y;
+    const int tl = warp >> a.p.ks_shift;
+    entry = pos[tl].x;
+    tile = pos[tl].y;
     chunk = 0;
-    hi_entry = pos[1].x;
-    hi_unit = pos[1].y;
+    hi_entry = pos[tl + 1].x;
+    hi_unit = pos[tl + 1].y;
     open(a);
   }
   __device__ __forceinline__ void open(const W4Args& a) {
@@ -107,7 +112,7 @@ struct W4TableWalk {
     }
     if (entry >= nt || entry > hi_entry) return 0;
     const int end = entry == hi_entry ? min(a.m.tiles, hi_unit - chunk * a.m.tiles) : a.m.tiles;
-    return end > tile ? (end - tile + a.p.tl - 1) >> a.p.tl_shift : 0;
+    return max(end - tile, 0);
   }
 };
 
@@ -295,8 +300,8 @@ __device__ __forceinline__ void w4_meet(const W4Args& a, const W4Share& sh, floa
   }
 }
 
-// The units of a walk (copied for the fetches that run ahead of the products); each
-// group of ks warps takes every tl-th unit.
+// The units of a group's walk (copied for the fetches that run ahead of the
+// products).
 template <bool SWIGLU, int KB, int MODE, class Walk>
 __device__ __forceinline__ void w4_units(const W4Args& a, uint8_t* smem, float* part, Walk c) {
   constexpr int SLOTS = w4_slots<KB, MODE>();
@@ -305,7 +310,6 @@ __device__ __forceinline__ void w4_units(const W4Args& a, uint8_t* smem, float* 
   const W4Lane<KB, MODE> own(a, sh);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t base = smem_u32(smem) + (sh.tl * p.ks + sh.ks) * SLOTS * p.slot_bytes;
-  c.tile += sh.tl;
   Walk f = c;                   // the next run to fetch; c: the run to work on
   const uint8_t* fq = nullptr;  // next tile to fetch
   const uint8_t* fs = nullptr;
@@ -322,9 +326,9 @@ __device__ __forceinline__ void w4_units(const W4Args& a, uint8_t* smem, float* 
   auto fetch = [&]() {
     if (left > 0) {
       own.fetch(a, sh, fslot, fq, fs);
-      fq += static_cast<size_t>(q_tile) << p.tl_shift;
-      fs += static_cast<size_t>(s_tile) << p.tl_shift;
-      f.tile += p.tl;
+      fq += q_tile;
+      fs += s_tile;
+      ++f.tile;
       if (--left == 0) {
         left = f.run(a);
         if (left > 0) aim();
@@ -401,10 +405,10 @@ __device__ __forceinline__ void w4_units(const W4Args& a, uint8_t* smem, float* 
           }
         }
       }
-      out += p.tl * (SWIGLU ? 8 : 16);
+      out += SWIGLU ? 8 : 16;
       buffer ^= kW4Warps * 128;
     }
-    c.tile += count * p.tl;
+    c.tile += count;
   }
   cp_async_wait_all();  // nothing is in flight when the CTA exits
 }
@@ -416,7 +420,6 @@ inline W4Plan w4_plan(const W4Matrix& m, int kb) {
   while (p.ks * kb < m.nb) p.ks *= 2;
   p.tl = kW4Warps / p.ks;
   while ((1 << p.ks_shift) < p.ks) ++p.ks_shift;
-  while ((1 << p.tl_shift) < p.tl) ++p.tl_shift;
   const int groups = (2 * kb) >> m.gshift;  // kb is even: a share starts with a group
   p.slot_bytes = kb * kW4BlockBytes + groups * 8 * m.rec;
   return p;
