@@ -87,6 +87,10 @@ int map_rows(CUtensorMap* m, const void* base, int elem_bytes, long long inner, 
   return r == CUDA_SUCCESS ? kRcOk : kRcTensorMap;
 }
 
+int map_gather_rows(CUtensorMap* m, const void* base, long long rows, int cols) {
+  return map_2d(m, base, rows, cols, 1);
+}
+
 namespace {
 
 constexpr int kMaxDevices = 64;

@@ -110,6 +110,9 @@ int device_sm_count();
 // [box_rows][box_inner]; elements outside read as zero.
 int map_rows(CUtensorMap* m, const void* base, int elem_bytes, long long inner, long long rows,
              int box_inner, int box_rows);
+// Tensor map of bf16 rows [rows][cols] for row gathers: box of one row of 64 columns,
+// 128-byte swizzle.
+int map_gather_rows(CUtensorMap* m, const void* base, long long rows, int cols);
 
 // The cudaError_t of the most recent failed CUDA call a launcher recorded on
 // this thread (0 = none), and the recorder: returns `e` unchanged.

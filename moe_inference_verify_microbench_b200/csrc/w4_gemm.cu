@@ -17,15 +17,17 @@
 // and the up rows of the same 128 outputs (the two accumulators then hold gate
 // and up in the same lane and column), for the down product two runs of 128 rows.
 //
-// CTA (896 threads, one per SM, persistent):
+// CTA (864 threads, one per SM, persistent):
 //   warps 0..15   dequantise: warp w writes lane quarter w % 4 of every fourth
 //                 64-column block
 //   warps 16..19  epilogue: tensor memory -> bf16 -> staging rows -> bulk stores
-//   warps 20..23  gather the records' rows (cp.async into the 128-byte swizzle)
+//   warps 20..23  gather the records' rows (a lane copies four of them with one
+//                 tile::gather4, into the 128-byte swizzle; issued from one warp
+//                 the copies of 128 records take 80 cycles each: T = 8192 1578 us
+//                 instead of 863)
 //   warp 24       tiled copies of codes and group records into a ring
 //   warp 25       issues tcgen05.mma: 2 operands x 4 steps of 16 columns per block
 //   warp 26       allocates tensor memory
-//   warp 27       publishes gathered stages to the async proxy
 //
 // A weight is rounded once, s * (q - z) to bf16: the operand's type.  That is
 // 2^-9 of it in the mean, like the rounding of the activations themselves; the
@@ -47,8 +49,9 @@ constexpr int kTcBlocks = 2;      // blocks per code stage
 constexpr int kTcRows = 128;      // records per unit at most
 constexpr int kTcDequantWarps = 16;
 constexpr int kTcEpiWarp = 16, kTcLoadWarp = 20, kTcCopyWarp = 24, kTcMmaWarp = 25,
-              kTcAllocWarp = 26, kTcForwardWarp = 27;
-constexpr int kTcThreads = 28 * 32;
+              kTcAllocWarp = 26;
+constexpr int kTcLoadWarps = kTcCopyWarp - kTcLoadWarp;
+constexpr int kTcThreads = 27 * 32;
 constexpr int kTcBBytes = kTcRows * 128;
 constexpr int kTcOutBytes = kTcRows * 256;  // staging: 128 records x 128 outputs
 constexpr int kTcCodeBytes = kTcTiles * kTcBlocks * kW4BlockBytes;
@@ -95,6 +98,17 @@ __device__ __forceinline__ uint32_t elect_one() {
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(p));
   return p;
+}
+
+// Rows r0..r3, 64 columns from x on, of a tensor map whose box is one row.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* m, uint64_t* bar,
+                                            int x, int r0, int r1, int r2, int r3) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(r0), "r"(r1), "r"(r2),
+      "r"(r3)
+      : "memory");
 }
 
 __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
@@ -165,7 +179,8 @@ __device__ __forceinline__ TcUnit tc_unit(const W4Args& a, int w, int groups) {
 template <bool SWIGLU, bool HALVES, bool ZEROS>
 __global__ void __launch_bounds__(kTcThreads, 1)
     w4_tc(const __grid_constant__ CUtensorMap tm_codes,
-          const __grid_constant__ CUtensorMap tm_records, const TcArgs args) {
+          const __grid_constant__ CUtensorMap tm_records,
+          const __grid_constant__ CUtensorMap tm_rows, const TcArgs args) {
   constexpr int kRec = ZEROS ? 8 : 4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -176,8 +191,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t* sRing = sOut + kTcOutBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(sRing + kTcRing * args.ring_bytes);
   uint64_t* empty = full + kTcStages;
-  uint64_t* gat = empty + kTcStages;  // a slot's copies have landed
-  uint64_t* bfull = gat + kTcSlots;
+  uint64_t* bfull = empty + kTcStages;
   uint64_t* bempty = bfull + kTcSlots;
   uint64_t* qfull = bempty + kTcSlots;
   uint64_t* qempty = qfull + kTcRing;
@@ -197,8 +211,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kTcSlots; ++s) {
-      mbar_init(&gat[s], 128);
-      mbar_init(&bfull[s], 1);
+      mbar_init(&bfull[s], kTcLoadWarps);
       mbar_init(&bempty[s], 1);
     }
     for (int s = 0; s < kTcRing; ++s) {
@@ -231,6 +244,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int total = static_cast<int>(min(units, 0x7fffffffLL - static_cast<long long>(gridDim.x)));
   const int nb = a.m.nb;
   const uint32_t nbe = (nb + kTcBlocks - 1) / kTcBlocks * kTcBlocks;
+
   static_assert(kTcStages == kTcDequantWarps / 4, "an operand stage for each set");
 
   if (warp < kTcDequantWarps) {
@@ -239,9 +253,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // whole code stages; set i of four warps, one per lane quarter, takes the blocks
     // i modulo 4 and fills operand stage i with them.
     const int quarter = warp & 3, set = warp >> 2;
+    const uint32_t dst = tmem + kTcOperandCol + set * 64 + (static_cast<uint32_t>(32 * quarter) << 16);
     const uint32_t codes = smem_u32(sRing) + lane * 16;
     const uint32_t records = smem_u32(sRing) + kTcCodeBytes + (lane >> 2) * kRec;
-    const uint32_t dst = tmem + kTcOperandCol + set * 64 + (static_cast<uint32_t>(32 * quarter) << 16);
     uint32_t base = 0;  // blocks before this unit
     uint32_t uses = 0;  // of the operand stage
     bool ok = true;
@@ -261,9 +275,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         ok = ok && mbar_wait_idle(&empty[set], (uses & 1u) ^ 1u, abort_flag, a.status,
                                   kErrTimeoutEmpty);
+        ++uses;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        ++uses;
         tc_fence_after();
         const uint32_t bk = kb & (kTcBlocks - 1);
         const uint32_t q = codes + rs * args.ring_bytes + bk * kW4BlockBytes;
@@ -423,58 +437,57 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     bulk_wait_all();
   } else if (warp >= kTcLoadWarp && warp < kTcCopyWarp) {
-    // -------------------------------------------------------- records' rows
-    // Thread i copies 16-byte chunk i % 8 of records i / 8 + 16 j: eight lanes read
-    // one row's 128 contiguous bytes.
-    const int i = threadIdx.x - kTcLoadWarp * 32;
-    const uint32_t chunk = static_cast<uint32_t>(i & 7);
-    const int row0 = i >> 3;
-    uint32_t cnt = 0;
+    // A slot is 32 copies of four rows; these warps issue an equal share of them, a
+    // lane one.  Columns past the last record get the first record's row: no output
+    // is taken from them.
+    constexpr int kShare = 32 / kTcLoadWarps;
+    const int part = (warp - kTcLoadWarp) * kShare + lane;
+    uint32_t s = 0, ph = 0;
     bool ok = true;
     for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
       const TcUnit u = tc_unit(a, w, groups);
       if (!u.ok) continue;
-      const int n = u.t.z - u.t.y, steps = (n + 15) >> 4;
-      const uint8_t* src[8];
-      uint32_t present = 0;
+      const int n = u.t.z - u.t.y, quads = ((n + 15) & ~15) / 4;
+      const int k = part / quads, r0 = 4 * (part - k * quads);
+      int row[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int p = u.t.y + row0 + 16 * j;
-        src[j] = reinterpret_cast<const uint8_t*>(a.act);
-        if (p < u.t.z) {
-          const int row = a.index != nullptr ? a.index[p] / a.index_div : p;
-          if (row >= 0 && row < a.act_rows) {
-            src[j] += static_cast<size_t>(row) * nb * 128 + chunk * 16;
-            present |= 1u << j;
-          } else {
-            record_status(a.status, kErrBadRow);
-          }
+      for (int j = 0; j < 4; ++j) {
+        const int p = u.t.y + (r0 + j < n ? r0 + j : 0);
+        row[j] = a.index != nullptr ? a.index[p] / a.index_div : p;
+        if (row[j] < 0 || row[j] >= a.act_rows) {
+          record_status(a.status, kErrBadRow);
+          row[j] = 0;
         }
       }
       const int per = tc_blocks(n);
-      for (int kb = 0; kb < nb; kb += per, ++cnt) {
-        const uint32_t s = cnt % kTcSlots;
-        ok = mbar_wait_idle(&bempty[s], ((cnt / kTcSlots) & 1u) ^ 1u, abort_flag, a.status,
-                            kErrTimeoutEmpty);
+      for (int kb = 0; kb < nb; kb += per) {
+        ok = mbar_wait_idle(&bempty[s], ph ^ 1u, abort_flag, a.status, kErrTimeoutEmpty);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint32_t base = smem_u32(sB) + s * kTcBBytes;
-        const int last = min(kb + per, nb);
-        for (int k = kb; k < last; ++k, base += steps * 2048) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (j < steps) {
-              const uint32_t r = static_cast<uint32_t>(row0 + 16 * j);
-              const bool have = (present >> j) & 1u;
-              cp_async_16(base + r * 128u + ((chunk ^ (r & 7u)) << 4),
-                          have ? src[j] + static_cast<size_t>(k) * 128 : src[j], have ? 16u : 0u);
-            }
-          }
+        const bool mine = lane < kShare && k < per && kb + k < nb;
+        const int copies = __popc(__ballot_sync(0xffffffffu, mine));
+        if (lane == 0) mbar_arrive_expect_tx(&bfull[s], copies * 512);
+        __syncwarp();
+        if (mine)
+          tma_gather4(smem_u32(sB) + s * kTcBBytes + part * 512, &tm_rows, &bfull[s],
+                      (kb + k) * 64, row[0], row[1], row[2], row[3]);
+        if (++s == kTcSlots) {
+          s = 0;
+          ph ^= 1u;
         }
-        cp_async_arrive_noinc(&gat[s]);
       }
     }
-    cp_async_wait_all();  // every copy lands before the CTA can exit
+    if (*abort_flag && lane == 0) {
+      // Let every copy still in flight land before the CTA exits: the slots before s
+      // are in their current round, the others in the one before.
+      for (uint32_t i = 0; i < kTcSlots; ++i) {
+        if (i >= s && ph == 0) break;  // never filled
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(&bfull[i], i < s ? ph : ph ^ 1u)) {
+          if (globaltimer_ns() - t0 > kWaitLimitNs) break;
+        }
+      }
+    }
   } else if (warp == kTcCopyWarp) {
     if (lane == 0) {
       // ---------------------------------------------- codes and group records
@@ -542,8 +555,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int in_slot = 0;
       for (int kb = 0; kb < nb; ++kb) {
         if (in_slot == 0)
-          ok = mbar_wait(&bfull[bs], bph, abort_flag, a.status, kErrTimeoutFull);
-        ok = mbar_wait(&full[s], (phases >> s) & 1u, abort_flag, a.status, kErrTimeoutFull) && ok;
+          ok = mbar_wait_idle(&bfull[bs], bph, abort_flag, a.status, kErrTimeoutFull);
+        ok = mbar_wait_idle(&full[s], (phases >> s) & 1u, abort_flag, a.status, kErrTimeoutFull) &&
+             ok;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -589,27 +603,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (globaltimer_ns() - t0 > kWaitLimitNs) break;
       }
     }
-  } else if (warp == kTcForwardWarp) {
-    if (lane == 0) {
-      // ------------------------------------------------------------ forwarder
-      uint32_t cnt = 0;
-      bool ok = true;
-      for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
-        const TcUnit u = tc_unit(a, w, groups);
-        if (!u.ok) continue;
-        const int per = tc_blocks(u.t.z - u.t.y);
-        for (int kb = 0; kb < nb; kb += per, ++cnt) {
-          const uint32_t s = cnt % kTcSlots;
-          if (!mbar_wait_idle(&gat[s], (cnt / kTcSlots) & 1u, abort_flag, a.status,
-                              kErrTimeoutFull)) {
-            ok = false;
-            break;
-          }
-          fence_proxy_async_smem();
-          mbar_arrive(&bfull[s]);
-        }
-      }
-    }
   }
 
   tc_fence_before();
@@ -634,18 +627,19 @@ int tc_launch(const W4Args& a, cudaStream_t stream) {
   static std::atomic<uint64_t> attr{0};
   if (!allow_smem(w4_tc<SWIGLU, HALVES, ZEROS>, kMost, attr)) return kRcCudaError;
   // x of a copy is a multiple of 16 bytes: blocks of 512, records of 8 rows of 4 or 8
-  CUtensorMap codes, records;
+  CUtensorMap codes, records, act;
   const long long rows = static_cast<long long>(a.E) * a.m.tiles;
   int rc = map_rows(&codes, a.m.q, 8, a.m.nb * (kW4BlockBytes / 8), rows,
                     kTcBlocks * kW4BlockBytes / 8, kTcTiles);
   if (rc == kRcOk)
     rc = map_rows(&records, a.m.s, 4, a.m.ng * 8 * a.m.rec / 4, rows, t.rec_stride / 4, kTcTiles);
+  if (rc == kRcOk) rc = map_gather_rows(&act, a.act, a.act_rows, a.m.nb * 64);
   if (rc != kRcOk) return rc;
   const long long units =
       static_cast<long long>(a.max_tiles) * ((a.m.tiles + kTcTiles - 1) / kTcTiles);
   const int grid = static_cast<int>(std::min<long long>(units, device_sm_count()));
   return note_cuda_error(launch_pdl(w4_tc<SWIGLU, HALVES, ZEROS>, dim3(grid), dim3(kTcThreads), sh,
-                                    stream, codes, records, t)) == cudaSuccess
+                                    stream, codes, records, act, t)) == cudaSuccess
              ? kRcOk
              : kRcCudaError;
 }
