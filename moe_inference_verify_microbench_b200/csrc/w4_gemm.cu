@@ -197,8 +197,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* qempty = qfull + kTcRing;
   uint64_t* acc_full = qempty + kTcRing;
   uint64_t* acc_empty = acc_full + 2;
-  uint64_t* drain = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_row = reinterpret_cast<int*>(tmem_slot + 2);
   float* s_scale = reinterpret_cast<float*>(s_row + kTcRows);
@@ -222,7 +221,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 4);
     }
-    mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -527,44 +525,64 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else if (warp == kTcMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     // The whole warp walks the stages, so that addresses and descriptors are
-    // uniform values, and one elected lane issues.  With 16 records a stage lasts
-    // a few hundred cycles: issued from a lane's own branch, the eight products
-    // of a stage took 1300.
+    // uniform values, and one elected lane issues.  This loop is what the block
+    // rate hangs on: a wait for a barrier that is long complete costs 100 cycles, so
+    // the next block's barriers are tested while this block's products are issued;
+    // a vote costs 75, so none is taken inside a unit.  After an abort the waits
+    // return at once and the unit is finished on what the stages hold.
     TcAcc acc;
     const uint32_t leader = elect_one();
     // descriptor of a K-major 128-byte-swizzled tile, without its start address
     constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
     uint32_t s = 0, phases = 0, bs = 0, bph = 0;  // bit i of phases: parity of stage i
-    bool ok = true;
-    for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
-      const TcUnit u = tc_unit(a, w, groups);
+    int issued = -1;                              // half of the last unit
+    TcUnit next{};
+    if (static_cast<int>(blockIdx.x) < total) next = tc_unit(a, blockIdx.x, groups);
+    for (int w = blockIdx.x; w < total; w += gridDim.x) {
+      const TcUnit u = next;
+      if (w + static_cast<int>(gridDim.x) < total) next = tc_unit(a, w + gridDim.x, groups);
       if (!u.ok) continue;
       const int n = __shfl_sync(0xffffffffu, u.t.z - u.t.y, 0);
       const int per = tc_blocks(n), cols = (n + 15) & ~15;
       acc.take(cols);
+      bool ok = true;
       for (int b = acc.first; ok && b <= acc.last; ++b) {
-        ok = mbar_wait_idle(&acc_empty[b], (acc.used[b] & 1u) ^ 1u, abort_flag, a.status,
-                            kErrTimeoutAccEmpty);
+        ok = mbar_wait(&acc_empty[b], (acc.used[b] & 1u) ^ 1u, abort_flag, a.status,
+                       kErrTimeoutAccEmpty);
         ++acc.used[b];
       }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      if (!__all_sync(0xffffffffu, ok && *abort_flag == 0)) break;
+      issued = acc.first;
+      ++acc.filled[issued];
       const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>(cols));
       const bool second = SWIGLU || u.m * kTcTiles + 8 < a.m.tiles;
       const uint32_t d0 = tmem + acc.d0, d1 = tmem + acc.d1;
       int in_slot = 0;
+      bool ready = false, bready = false;
       for (int kb = 0; kb < nb; ++kb) {
-        if (in_slot == 0)
-          ok = mbar_wait_idle(&bfull[bs], bph, abort_flag, a.status, kErrTimeoutFull);
-        ok = mbar_wait_idle(&full[s], (phases >> s) & 1u, abort_flag, a.status, kErrTimeoutFull) &&
-             ok;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!bready) mbar_wait(&bfull[bs], bph, abort_flag, a.status, kErrTimeoutFull);
+        if (!ready)
+          mbar_wait(&full[s], (phases >> s) & 1u, abort_flag, a.status, kErrTimeoutFull);
+        __syncwarp();
         tc_fence_after();
-        const uint32_t at = tmem + kTcOperandCol + s * 64;
+        const uint32_t at = tmem + kTcOperandCol + s * 64, at_s = s, at_b = bs;
         const uint32_t lo =
             (((smem_u32(sB) + bs * kTcBBytes + in_slot * cols * 128) >> 4) & 0x3fffu) | (1u << 16);
         const bool end = ++in_slot == per || kb + 1 == nb;
+        phases ^= 1u << s;
+        s = (s + 1) % kTcStages;
+        if (end) {
+          in_slot = 0;
+          if (++bs == kTcSlots) {
+            bs = 0;
+            bph ^= 1u;
+          }
+        }
+        ready = bready = true;
+        if (kb + 1 < nb) {
+          ready = mbar_test(&full[s], (phases >> s) & 1u);
+          if (end) bready = mbar_test(&bfull[bs], bph);
+        }
         if (leader) {
           const uint32_t acc0 = kb != 0 ? 1u : 0u;
 #pragma unroll
@@ -576,30 +594,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tc_mma_bf16_ts(d1, at + 32 + kk * 8, lo + 2 * kk, kDescHi, idesc,
                              kk != 0 ? 1u : acc0);
           }
-          tc_commit(&empty[s]);
-          if (end) tc_commit(&bempty[bs]);
-          if (kb + 1 == nb) tc_commit(&acc_full[acc.first]);
+          tc_commit(&empty[at_s]);
+          if (end) tc_commit(&bempty[at_b]);
+          if (kb + 1 == nb) tc_commit(&acc_full[issued]);
         }
         __syncwarp();
-        if (end) {
-          in_slot = 0;
-          if (++bs == kTcSlots) {
-            bs = 0;
-            bph ^= 1u;
-          }
-        }
-        phases ^= 1u << s;
-        s = (s + 1) % kTcStages;
       }
       if (nb % kTcBlocks != 0) s = (s + 1) % kTcStages;
     }
-    // The epilogue has waited for every unit's products; only after an abort some
-    // may still run, and have finished once `drain` completes.
-    if (!ok) {
-      if (leader) tc_commit(drain);
-      __syncwarp();
+    // Tensor memory is released below: the last unit's products have to be done,
+    // which the epilogue may not have waited for after an abort.
+    if (issued >= 0) {
       const unsigned long long t0 = globaltimer_ns();
-      while (!mbar_try_wait(drain, 0)) {
+      while (!mbar_try_wait(&acc_full[issued], (acc.filled[issued] & 1u) ^ 1u)) {
         if (globaltimer_ns() - t0 > kWaitLimitNs) break;
       }
     }
