@@ -42,6 +42,7 @@ namespace moe {
 namespace {
 
 constexpr int kTcStages = 4;      // weight operand stages (64 columns) in tensor memory
+constexpr int kTcPairs = 2;       // of them that are handed over together
 constexpr int kTcSlots = 6;       // record slots in shared memory (see tc_blocks)
 constexpr int kTcRing = 4;        // code stages (128 columns)
 constexpr int kTcTiles = 16;      // packed tiles per unit
@@ -175,6 +176,24 @@ __device__ __forceinline__ TcUnit tc_unit(const W4Args& a, int w, int groups) {
   return u;
 }
 
+// Low word of the descriptor of a record block in shared memory.
+__device__ __forceinline__ uint32_t tc_desc(const uint8_t* base, uint32_t offset) {
+  return (((smem_u32(base) + offset) >> 4) & 0x3fffu) | (1u << 16);
+}
+
+// The products of a 64-column block: both operands, four steps of 16 columns.
+__device__ __forceinline__ void tc_block(uint32_t d0, uint32_t d1, uint32_t at, uint32_t lo,
+                                         uint32_t hi, uint32_t idesc, bool add, bool second) {
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk)
+    tc_mma_bf16_ts(d0, at + kk * 8, lo + 2 * kk, hi, idesc, kk != 0 || add ? 1u : 0u);
+  if (second) {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      tc_mma_bf16_ts(d1, at + 32 + kk * 8, lo + 2 * kk, hi, idesc, kk != 0 || add ? 1u : 0u);
+  }
+}
+
 // HALVES: groups of 32, two to a block; ZEROS: zero points are kept.
 template <bool SWIGLU, bool HALVES, bool ZEROS>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -190,8 +209,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t* sOut = sB + kTcSlots * kTcBBytes;
   uint8_t* sRing = sOut + kTcOutBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(sRing + kTcRing * args.ring_bytes);
-  uint64_t* empty = full + kTcStages;
-  uint64_t* bfull = empty + kTcStages;
+  uint64_t* empty = full + kTcPairs;
+  uint64_t* bfull = empty + kTcPairs;
   uint64_t* bempty = bfull + kTcSlots;
   uint64_t* qfull = bempty + kTcSlots;
   uint64_t* qempty = qfull + kTcRing;
@@ -205,8 +224,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kTcStages; ++s) {
-      mbar_init(&full[s], 4);  // the warps of a set
+    for (int s = 0; s < kTcPairs; ++s) {
+      mbar_init(&full[s], 4 * kTcBlocks);  // the warps of two sets
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kTcSlots; ++s) {
@@ -249,34 +268,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ------------------------------------------------------------ dequantise
     // Blocks are counted through all units, an odd number in a unit rounded up to
     // whole code stages; set i of four warps, one per lane quarter, takes the blocks
-    // i modulo 4 and fills operand stage i with them.
+    // i modulo 4 and fills operand stage i with them.  Two blocks, of sets 0 and 1 or
+    // of sets 2 and 3, are handed over together.
     const int quarter = warp & 3, set = warp >> 2;
     const uint32_t dst = tmem + kTcOperandCol + set * 64 + (static_cast<uint32_t>(32 * quarter) << 16);
     const uint32_t codes = smem_u32(sRing) + lane * 16;
     const uint32_t records = smem_u32(sRing) + kTcCodeBytes + (lane >> 2) * kRec;
     uint32_t base = 0;  // blocks before this unit
+    const int pair = set >> 1;
     uint32_t uses = 0;  // of the operand stage
     bool ok = true;
     for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
       const TcUnit u = tc_unit(a, w, groups);
       if (!u.ok) continue;
-      const int tiles = a.m.tiles - u.m * kTcTiles;  // packed tiles from here to the end
       for (uint32_t kb = (set - base) & 3u; kb < nbe; kb += 4) {
         const uint32_t cnt = base + kb, ring = cnt / kTcBlocks, rs = ring % kTcRing;
         ok = mbar_wait_idle(&qfull[rs], (ring / kTcRing) & 1u, abort_flag, a.status,
                             kErrTimeoutFull);
-        if (kb >= static_cast<uint32_t>(nb)) {  // the block that rounds the unit up
-          __syncwarp();
-          if (lane == 0 && ok) mbar_arrive(&qempty[rs]);
-          __syncwarp();
-          continue;
-        }
-        ok = ok && mbar_wait_idle(&empty[set], (uses & 1u) ^ 1u, abort_flag, a.status,
+        ok = ok && mbar_wait_idle(&empty[pair], (uses & 1u) ^ 1u, abort_flag, a.status,
                                   kErrTimeoutEmpty);
         ++uses;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
+        // packed tiles from here to the end; none for a block that rounds the unit up
+        const int tiles = kb < static_cast<uint32_t>(nb) ? a.m.tiles - u.m * kTcTiles : 0;
         const uint32_t bk = kb & (kTcBlocks - 1);
         const uint32_t q = codes + rs * args.ring_bytes + bk * kW4BlockBytes;
         const uint32_t grp = HALVES ? 2 * bk : (2 * bk) >> a.m.gshift;
@@ -347,7 +363,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&qempty[rs]);  // the codes have been read
-          mbar_arrive(&full[set]);
+          mbar_arrive(&full[pair]);
         }
         __syncwarp();
       }
@@ -534,8 +550,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t leader = elect_one();
     // descriptor of a K-major 128-byte-swizzled tile, without its start address
     constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    uint32_t s = 0, phases = 0, bs = 0, bph = 0;  // bit i of phases: parity of stage i
-    int issued = -1;                              // half of the last unit
+    uint32_t p = 0, phase = 0, bs = 0, bph = 0;
+    int issued = -1;  // half of the last unit
     TcUnit next{};
     if (static_cast<int>(blockIdx.x) < total) next = tc_unit(a, blockIdx.x, groups);
     for (int w = blockIdx.x; w < total; w += gridDim.x) {
@@ -557,20 +573,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>(cols));
       const bool second = SWIGLU || u.m * kTcTiles + 8 < a.m.tiles;
       const uint32_t d0 = tmem + acc.d0, d1 = tmem + acc.d1;
-      int in_slot = 0;
+      uint32_t in_slot = 0;
       bool ready = false, bready = false;
-      for (int kb = 0; kb < nb; ++kb) {
+      for (int kb = 0; kb < nb; kb += kTcBlocks) {
+        const bool two = kb + 1 < nb;
         if (!bready) mbar_wait(&bfull[bs], bph, abort_flag, a.status, kErrTimeoutFull);
-        if (!ready)
-          mbar_wait(&full[s], (phases >> s) & 1u, abort_flag, a.status, kErrTimeoutFull);
+        // more than 64 records: the second block has a slot of its own
+        const uint32_t bs0 = bs, in0 = in_slot;
+        if (per == 1 && two) {
+          if (++bs == kTcSlots) {
+            bs = 0;
+            bph ^= 1u;
+          }
+          mbar_wait(&bfull[bs], bph, abort_flag, a.status, kErrTimeoutFull);
+        }
+        if (!ready) mbar_wait(&full[p], phase, abort_flag, a.status, kErrTimeoutFull);
         __syncwarp();
         tc_fence_after();
-        const uint32_t at = tmem + kTcOperandCol + s * 64, at_s = s, at_b = bs;
-        const uint32_t lo =
-            (((smem_u32(sB) + bs * kTcBBytes + in_slot * cols * 128) >> 4) & 0x3fffu) | (1u << 16);
-        const bool end = ++in_slot == per || kb + 1 == nb;
-        phases ^= 1u << s;
-        s = (s + 1) % kTcStages;
+        const uint32_t at = tmem + kTcOperandCol + p * (kTcBlocks * 64);
+        const uint32_t lo0 = tc_desc(sB, bs0 * kTcBBytes + in0 * cols * 128);
+        const uint32_t lo1 = per == 1 ? tc_desc(sB, bs * kTcBBytes) : lo0 + cols * 8;
+        const uint32_t bs1 = bs, p0 = p;
+        const bool last = kb + kTcBlocks >= nb;
+        in_slot += kTcBlocks;
+        const bool end = in_slot >= static_cast<uint32_t>(per) || last;
         if (end) {
           in_slot = 0;
           if (++bs == kTcSlots) {
@@ -578,29 +604,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             bph ^= 1u;
           }
         }
+        if (++p == kTcPairs) {
+          p = 0;
+          phase ^= 1u;
+        }
         ready = bready = true;
-        if (kb + 1 < nb) {
-          ready = mbar_test(&full[s], (phases >> s) & 1u);
+        if (!last) {
+          ready = mbar_test(&full[p], phase);
           if (end) bready = mbar_test(&bfull[bs], bph);
         }
         if (leader) {
-          const uint32_t acc0 = kb != 0 ? 1u : 0u;
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_bf16_ts(d0, at + kk * 8, lo + 2 * kk, kDescHi, idesc, kk != 0 ? 1u : acc0);
-          if (second) {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc_mma_bf16_ts(d1, at + 32 + kk * 8, lo + 2 * kk, kDescHi, idesc,
-                             kk != 0 ? 1u : acc0);
+          tc_block(d0, d1, at, lo0, kDescHi, idesc, kb != 0, second);
+          if (two) {
+            if (per == 1) tc_commit(&bempty[bs0]);
+            tc_block(d0, d1, at + 64, lo1, kDescHi, idesc, true, second);
           }
-          tc_commit(&empty[at_s]);
-          if (end) tc_commit(&bempty[at_b]);
-          if (kb + 1 == nb) tc_commit(&acc_full[issued]);
+          tc_commit(&empty[p0]);
+          if (end) tc_commit(&bempty[bs1]);
+          if (last) tc_commit(&acc_full[issued]);
         }
         __syncwarp();
       }
-      if (nb % kTcBlocks != 0) s = (s + 1) % kTcStages;
     }
     // Tensor memory is released below: the last unit's products have to be done,
     // which the epilogue may not have waited for after an abort.
