@@ -451,19 +451,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     bulk_wait_all();
   } else if (warp >= kTcLoadWarp && warp < kTcCopyWarp) {
-    // A slot is 32 copies of four rows; these warps issue an equal share of them, a
-    // lane one.  Columns past the last record get the first record's row: no output
-    // is taken from them.
+    // A slot is up to 32 copies of four rows, dealt out to these warps.  A unit's row
+    // numbers are uniform values of the warp and one elected lane issues its copies:
+    // issued from eight lanes they took 80 cycles each.  Columns past the last record
+    // get the first record's row: no output is taken from them.
     constexpr int kShare = 32 / kTcLoadWarps;
-    const int part = (warp - kTcLoadWarp) * kShare + lane;
+    const int me = warp - kTcLoadWarp;
+    const uint32_t leader = elect_one();
     uint32_t s = 0, ph = 0;
     bool ok = true;
     for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
       const TcUnit u = tc_unit(a, w, groups);
       if (!u.ok) continue;
       const int n = u.t.z - u.t.y, quads = ((n + 15) & ~15) / 4;
-      const int k = part / quads, r0 = 4 * (part - k * quads);
-      int row[4];
+      // lane j has the rows of this warp's copy j
+      const int mine = lane % kShare * kTcLoadWarps + me, k = mine / quads;
+      const int r0 = 4 * (mine - k * quads);
+      int row[4], rows[kShare][4], block[kShare];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int p = u.t.y + (r0 + j < n ? r0 + j : 0);
@@ -473,18 +477,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           row[j] = 0;
         }
       }
+#pragma unroll
+      for (int c = 0; c < kShare; ++c) {
+        block[c] = __shfl_sync(0xffffffffu, k, c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rows[c][j] = __shfl_sync(0xffffffffu, row[j], c);
+      }
       const int per = tc_blocks(n);
       for (int kb = 0; kb < nb; kb += per) {
         ok = mbar_wait_idle(&bempty[s], ph ^ 1u, abort_flag, a.status, kErrTimeoutEmpty);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const bool mine = lane < kShare && k < per && kb + k < nb;
-        const int copies = __popc(__ballot_sync(0xffffffffu, mine));
-        if (lane == 0) mbar_arrive_expect_tx(&bfull[s], copies * 512);
+        const int blocks = min(per, nb - kb);
+        if (leader) {
+          // copies me, me + 4, ... of the blocks * quads of this slot
+          const int copies = (blocks * quads - me + kTcLoadWarps - 1) / kTcLoadWarps;
+          mbar_arrive_expect_tx(&bfull[s], copies * 512);
+          const uint32_t dst = smem_u32(sB) + s * kTcBBytes + me * 512;
+#pragma unroll
+          for (int c = 0; c < kShare; ++c) {
+            if (block[c] < blocks)
+              tma_gather4(dst + c * (kTcLoadWarps * 512), &tm_rows, &bfull[s],
+                          (kb + block[c]) * 64, rows[c][0], rows[c][1], rows[c][2], rows[c][3]);
+          }
+        }
         __syncwarp();
-        if (mine)
-          tma_gather4(smem_u32(sB) + s * kTcBBytes + part * 512, &tm_rows, &bfull[s],
-                      (kb + k) * 64, row[0], row[1], row[2], row[3]);
         if (++s == kTcSlots) {
           s = 0;
           ph ^= 1u;
