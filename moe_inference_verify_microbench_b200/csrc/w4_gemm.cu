@@ -54,7 +54,8 @@ constexpr int kTcEpiWarp = 16, kTcLoadWarp = 20, kTcCopyWarp = 24, kTcMmaWarp = 
 constexpr int kTcLoadWarps = kTcCopyWarp - kTcLoadWarp;
 constexpr int kTcThreads = 27 * 32;
 constexpr int kTcBBytes = kTcRows * 128;
-constexpr int kTcOutBytes = kTcRows * 256;  // staging: 128 records x 128 outputs
+constexpr int kTcOutRow = 272;  // staging: 128 records of 128 outputs, rows 16 bytes apart in banks
+constexpr int kTcOutBytes = kTcRows * kTcOutRow;
 constexpr int kTcCodeBytes = kTcTiles * kTcBlocks * kW4BlockBytes;
 constexpr uint32_t kTcOperandCol = 256;     // accumulators below, operand stages above
 
@@ -71,6 +72,24 @@ __device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t taddr, const uint32_
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
       "r"(r[15])
+      : "memory");
+}
+
+// 16 lanes, 16 columns from taddr on, in the order of product fragments: lane
+// 4 g + t has columns 2t, 2t + 1 of rows g and g + 8, then columns 8 + 2t, 9 + 2t.
+__device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr));
+}
+
+// Four 8 x 8 blocks of 16-bit values, transposed: lane i names row i % 8 of block i / 8.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile(
+      "stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
       : "memory");
 }
 
@@ -218,8 +237,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* s_row = reinterpret_cast<int*>(tmem_slot + 2);
-  float* s_scale = reinterpret_cast<float*>(s_row + kTcRows);
+  float* s_scale = reinterpret_cast<float*>(tmem_slot + 2);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
@@ -406,32 +424,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         named_barrier(1, 128);
         if (ok && outs > 0) {
           const uint32_t d = tmem + lanes + (part == 0 ? acc.d0 : acc.d1);
-          const uint32_t dst = stage + (32 * quarter + lane) * 2;
+          // records down the staging rows: the fragments go through transposing stores
+          const uint32_t dst = stage + ((lane >> 4) * 8 + (lane & 7)) * kTcOutRow +
+                               (32 * quarter + ((lane >> 3) & 1) * 8) * 2;
           for (int c = 0; c < cols; c += 16) {
-            uint32_t v[16];
-            tmem_ld16(d + c, v);
+            uint32_t v[2][8];
+            tmem_ld_16x256b_x2(d + c, v[0]);
+            tmem_ld_16x256b_x2(d + (16u << 16) + c, v[1]);
             if constexpr (SWIGLU) {
-              uint32_t up[16];
-              tmem_ld16(tmem + lanes + acc.d1 + c, up);
+              uint32_t up[2][8];
+              tmem_ld_16x256b_x2(tmem + lanes + acc.d1 + c, up[0]);
+              tmem_ld_16x256b_x2(tmem + lanes + (16u << 16) + acc.d1 + c, up[1]);
               tc_wait_ld();
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                v[i] = __float_as_uint(silu_f(__uint_as_float(v[i])) * __uint_as_float(up[i]));
+                v[i >> 3][i & 7] = __float_as_uint(silu_f(__uint_as_float(v[i >> 3][i & 7])) *
+                                                   __uint_as_float(up[i >> 3][i & 7]));
             } else {
+              const float* sc = s_scale + c + 2 * (lane & 3);
+              const float2 s0 = *reinterpret_cast<const float2*>(sc);
+              const float2 s1 = *reinterpret_cast<const float2*>(sc + 8);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                v[i] = __float_as_uint(__uint_as_float(v[i]) * s_scale[c + i]);
+              for (int i = 0; i < 16; ++i) {
+                const float2 sv = (i & 4) != 0 ? s1 : s0;
+                v[i >> 3][i & 7] = __float_as_uint(__uint_as_float(v[i >> 3][i & 7]) *
+                                                   ((i & 1) != 0 ? sv.y : sv.x));
+              }
             }
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const uint32_t pk = pack_bf16x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-              asm volatile("st.shared.b16 [%0], %1;" ::"r"(dst + (c + i) * 256),
-                           "h"(static_cast<unsigned short>(pk & 0xffffu))
-                           : "memory");
-              asm volatile("st.shared.b16 [%0], %1;" ::"r"(dst + (c + i + 1) * 256),
-                           "h"(static_cast<unsigned short>(pk >> 16))
-                           : "memory");
+            for (int h = 0; h < 2; ++h) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                pk[i] = pack_bf16x2(__uint_as_float(v[h][2 * i]), __uint_as_float(v[h][2 * i + 1]));
+              stmatrix_x4_trans(dst + c * kTcOutRow + h * 32, pk);
             }
           }
         }
@@ -445,7 +472,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         fence_proxy_async_smem();
         named_barrier(1, 128);
         if (ok && outs > 0 && o >= 0)
-          bulk_store(a.out + static_cast<size_t>(o) * a.out_ld + first, stage + r * 256, outs * 2);
+          bulk_store(a.out + static_cast<size_t>(o) * a.out_ld + first, stage + r * kTcOutRow, outs * 2);
         bulk_commit();
       }
     }
@@ -668,9 +695,9 @@ int tc_launch(const W4Args& a, cudaStream_t stream) {
   t.rec_stride = (4 >> a.m.gshift) * 8 * a.m.rec;
   t.ring_bytes = kTcCodeBytes + kTcTiles * t.rec_stride;
   const int sh =
-      1024 + kTcSlots * kTcBBytes + kTcOutBytes + kTcRing * t.ring_bytes + 512 + kTcRows * 8;
+      1024 + kTcSlots * kTcBBytes + kTcOutBytes + kTcRing * t.ring_bytes + 512 + kTcRows * 4;
   constexpr int kMost = 1024 + kTcSlots * kTcBBytes + kTcOutBytes +
-                        kTcRing * (kTcCodeBytes + kTcTiles * 256) + 512 + kTcRows * 8;
+                        kTcRing * (kTcCodeBytes + kTcTiles * 256) + 512 + kTcRows * 4;
   static_assert(kMost <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> attr{0};
   if (!allow_smem(w4_tc<SWIGLU, HALVES, ZEROS>, kMost, attr)) return kRcCudaError;
