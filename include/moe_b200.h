@@ -409,8 +409,8 @@ MOE_API int moe_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_
 
 /*
  * moe_grouped_w13_swiglu_gather and moe_grouped_w2 on a 4-bit bank: the same
- * tile tables (of either height), row index (NULL: row r itself), row map and
- * slot scale.  H % 64 == 0, I % 64 == 0, both <= 8192 and multiples of the
+ * tile tables (entries of at most 128 rows; longer ones are reported as bad
+ * rows), row index (NULL: row r itself), row map and slot scale.  H % 64 == 0, I % 64 == 0, both <= 8192 and multiples of the
  * group; E <= 1024.
  */
 MOE_API int moe_grouped_w13_swiglu_w4(const void* src, int src_rows, const int32_t* index,

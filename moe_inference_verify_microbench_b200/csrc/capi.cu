@@ -142,6 +142,8 @@ W4Layout w4_sorted_layout(void* ws, int M, const W4Bank& b) {
   return l;
 }
 
+bool w4_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
 bool w4_count_ok(int T, int k) {
   return static_cast<long long>(T) * k <= 0x7fffffffLL;
 }
@@ -617,8 +619,7 @@ int moe_w4_experts_forward(const void* x, const int32_t* ids, const float* weigh
   if (top_k > 8 || !w4_count_ok(T, top_k)) return kRcUnsupported;
   if (T == 0) return kRcOk;
   if (x == nullptr || ids == nullptr || weights == nullptr || y == nullptr ||
-      workspace == nullptr || (reinterpret_cast<uintptr_t>(y) & 15u) != 0 ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+      workspace == nullptr || !w4_aligned(x) || !w4_aligned(y) || !w4_aligned(workspace))
     return kRcBadArgument;
   const W4Layout l = w4_layout(workspace, T, top_k, b, false);
   if (workspace_bytes < l.bytes) return kRcWorkspace;
@@ -642,8 +643,8 @@ int moe_w4_sorted_forward(const void* sorted_x, int M, const int64_t* offsets,
   int rc = w4_check_bank(b);
   if (rc != kRcOk) return rc;
   if (M == 0) return kRcOk;
-  if (sorted_x == nullptr || y == nullptr || workspace == nullptr ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+  if (sorted_x == nullptr || y == nullptr || workspace == nullptr || !w4_aligned(sorted_x) ||
+      !w4_aligned(y) || !w4_aligned(workspace))
     return kRcBadArgument;
   const W4Layout l = w4_sorted_layout(workspace, M, b);
   if (workspace_bytes < l.bytes) return kRcWorkspace;
@@ -675,31 +676,25 @@ int moe_w4_layer_forward(const void* x, const void* router_weight, const float* 
   int rc = w4_check_bank(b);
   if (rc != kRcOk) return rc;
   if (top_k > b.E) return kRcBadArgument;
-  if (top_k > 8 || !w4_count_ok(T, top_k)) return kRcUnsupported;
+  if (top_k > 8 || b.E % 16 != 0 || b.E > 256 || !w4_count_ok(T, top_k)) return kRcUnsupported;
   if (T == 0) return kRcOk;
-  if (x == nullptr || y == nullptr || workspace == nullptr ||
-      (reinterpret_cast<uintptr_t>(y) & 15u) != 0 ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+  if (x == nullptr || y == nullptr || workspace == nullptr || !w4_aligned(x) ||
+      !w4_aligned(router_weight) || !w4_aligned(y) || !w4_aligned(workspace))
     return kRcBadArgument;
   const W4Layout l = w4_layout(workspace, T, top_k, b, true);
   if (workspace_bytes < l.bytes) return kRcWorkspace;
   if (w4_decode_ok(b, T, top_k))
     return launch_w4_decode(b, x, router_weight, router_bias, T, top_k, norm_topk_prob, l.decode,
                             l.h, y, status, stream);
-  if (use_router_small(T, b.H, b.E, top_k)) {
-    rc = launch_router_sort_small(x, router_weight, router_bias, T, b.H, b.E, top_k,
-                                  norm_topk_prob, l.ids, l.w, nullptr, l.counts, l.offsets, l.perm,
-                                  l.tiles, l.max_tiles, l.num_tiles, status, stream);
-    if (rc != kRcOk) return rc;
-  } else {
-    rc = launch_router(x, router_weight, router_bias, T, b.H, b.E, top_k, norm_topk_prob, l.ids,
-                       l.w, nullptr, status, stream);
-    if (rc != kRcOk) return rc;
+  // Past the one-kernel layer, the tiled router and the sort take 11 us at 12 and 16
+  // tokens of 128 experts, the one-cluster router that also sorts 22 us.
+  rc = launch_router_tiled(x, router_weight, router_bias, T, b.H, b.E, top_k, norm_topk_prob,
+                           l.ids, l.w, nullptr, status, stream);
+  if (rc == kRcOk)
     rc = launch_sort_align(l.ids, T * top_k, b.E, 0, b.E, MOE_BLOCK_M, l.sort_ws, l.counts,
                            l.offsets, nullptr, l.perm, nullptr, l.tiles, l.max_tiles, l.num_tiles,
                            status, stream);
-    if (rc != kRcOk) return rc;
-  }
+  if (rc != kRcOk) return rc;
   return w4_products(b, l, x, l.ids, l.w, T, top_k, b.E, 0, y, status, stream);
 }
 

@@ -225,21 +225,38 @@ cudaError_t note_cuda_error(cudaError_t e) {
   return e;
 }
 
-int launch_router(const void* x, const void* wr, const float* bias, int T, int H, int E, int k,
-                  int norm_topk_prob, int* ids_out, float* w_out, void* logits_out, int* status,
-                  cudaStream_t stream) {
+namespace {
+int router_args(const void* x, const void* wr, int T, int H, int E, int k, const int* ids_out,
+                const float* w_out) {
   if ((T > 0 && (x == nullptr || ids_out == nullptr || w_out == nullptr)) || wr == nullptr ||
       T < 0 || H <= 0)
     return kRcBadArgument;
   if ((H % kBK) != 0 || (E % 16) != 0 || E < 16 || E > 256 || k < 1 || k > kRouterMaxK || k > E)
     return kRcUnsupported;
-  if (T == 0) return kRcOk;
+  return kRcOk;
+}
+}  // namespace
+
+int launch_router(const void* x, const void* wr, const float* bias, int T, int H, int E, int k,
+                  int norm_topk_prob, int* ids_out, float* w_out, void* logits_out, int* status,
+                  cudaStream_t stream) {
+  const int rc = router_args(x, wr, T, H, E, k, ids_out, w_out);
+  if (rc != kRcOk || T == 0) return rc;
   if (use_router_small(T, H, E, k))
     return launch_router_sort_small(x, wr, bias, T, H, E, k, norm_topk_prob, ids_out, w_out,
                                     logits_out, nullptr, nullptr, nullptr, nullptr, 0, nullptr,
                                     status, stream);
+  return launch_router_tiled(x, wr, bias, T, H, E, k, norm_topk_prob, ids_out, w_out, logits_out,
+                             status, stream);
+}
+
+int launch_router_tiled(const void* x, const void* wr, const float* bias, int T, int H, int E,
+                        int k, int norm_topk_prob, int* ids_out, float* w_out, void* logits_out,
+                        int* status, cudaStream_t stream) {
+  int rc = router_args(x, wr, T, H, E, k, ids_out, w_out);
+  if (rc != kRcOk || T == 0) return rc;
   CUtensorMap ma, mb;
-  int rc = map_2d(&ma, x, T, H, kBM);
+  rc = map_2d(&ma, x, T, H, kBM);
   if (rc == kRcOk) rc = map_3d(&mb, wr, 1, E, H, E);
   if (rc != kRcOk) return rc;
   // At most 8 tiles of 128 tokens (T <= 1024): split K over a cluster of 2,

@@ -70,6 +70,10 @@ int launch_combine(const void* rows, int n_rows, const int* slot_src, const floa
 int launch_router(const void* x, const void* wr, const float* bias, int T, int H, int E, int k,
                   int norm_topk_prob, int* ids_out, float* w_out, void* logits_out, int* status,
                   cudaStream_t stream);
+// Its form for any T: 128-row tiles on the tensor cores.
+int launch_router_tiled(const void* x, const void* wr, const float* bias, int T, int H, int E,
+                        int k, int norm_topk_prob, int* ids_out, float* w_out, void* logits_out,
+                        int* status, cudaStream_t stream);
 // max_sms (grouped GEMMs and GEMVs): at most this many SMs (<= 0: all), the
 // others left to concurrent work on other streams.
 // tile_rows: the height of the tile table's row blocks, 128 (MOE_BLOCK_M) or

@@ -179,7 +179,8 @@ int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* 
       num_tiles == nullptr)
     return kRcBadArgument;
   if (M == 0 || max_tiles == 0) return kRcOk;
-  if (src == nullptr || h_out == nullptr || !aligned16(src) || !aligned16(h_out)) return kRcBadArgument;
+  if (src == nullptr || src_rows == 0 || h_out == nullptr || !aligned16(src) || !aligned16(h_out))
+    return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, false);
   a.act = static_cast<const uint32_t*>(src);
