@@ -10,7 +10,9 @@ row-parallel output projection closed by an all_reduce on the TP group
 (C1/python/solution.py:142).  They are not part of the optimised path.
 ``HybridBlock.forward`` runs the two RMSNorms and the first residual add in
 one row kernel (``ops.add_rmsnorm``); the ``RMSNorm`` module keeps the
-harness's PyTorch definition of the math.
+harness's PyTorch definition of the math.  With ``post_norm=True`` each branch's
+output is normed too, gated and scaled before it is added, and the add, both
+norms and the gate are one row kernel (``ops.block_norm``).
 """
 
 from __future__ import annotations
@@ -125,10 +127,30 @@ class HybridBlock(nn.Module):
                  head_dim: int, num_experts: int, top_k: int, tp_size: int, tp_rank: int,
                  tp_group: dist.ProcessGroup | None, ep_size: int, ep_rank: int,
                  ep_group: dist.ProcessGroup | None, norm_topk_prob: bool = True,
-                 rope_base: float = 10000.0, rms_eps: float = 1e-6, **moe_options) -> None:
+                 rope_base: float = 10000.0, rms_eps: float = 1e-6, *, post_norm: bool = False,
+                 gate_act: str | None = None, residual_scale: float = 1.0,
+                 **moe_options) -> None:
         """``moe_options``: keyword extras of ``HybridMoE`` (transport,
-        max_tokens_per_rank, check_errors, overlap, exchange_sms)."""
+        max_tokens_per_rank, check_errors, overlap, exchange_sms).
+
+        ``post_norm``: ``h = x + residual_scale * act(gate) * norm(attn(norm(x)))`` and the
+        same around the experts, with norms of their own (``attn_post_norm``,
+        ``moe_post_norm``).  ``gate_act`` ("none", "sigmoid" or "tanh") adds a learned
+        gate per channel to each branch (``attn_gate``, ``moe_gate``); None: no gate."""
         super().__init__()
+        if not post_norm and (gate_act is not None or residual_scale != 1.0):
+            raise ValueError("gate_act and residual_scale need post_norm=True")
+        if gate_act is not None:
+            ops.check_gate_act(gate_act)
+        self.post_norm = post_norm
+        self.gate_act = gate_act
+        self.residual_scale = residual_scale
+        if post_norm:
+            self.attn_post_norm = RMSNorm(hidden, eps=rms_eps)
+            self.moe_post_norm = RMSNorm(hidden, eps=rms_eps)
+            if gate_act is not None:
+                self.attn_gate = nn.Parameter(torch.ones(hidden))
+                self.moe_gate = nn.Parameter(torch.ones(hidden))
         self.attn_norm = RMSNorm(hidden, eps=rms_eps)
         self.attn = TPGQA(hidden, n_heads, n_kv_heads, head_dim, rope_base=rope_base,
                           tp_size=tp_size, tp_rank=tp_rank, group=tp_group)
@@ -139,7 +161,8 @@ class HybridBlock(nn.Module):
     @torch.no_grad()
     def weight_loader(self, attn_norm_weight, q_weight, k_weight, v_weight, o_weight,
                       moe_norm_weight, gate_weight, expert_gate_weights, expert_up_weights,
-                      expert_down_weights) -> None:
+                      expert_down_weights, *, attn_post_norm_weight=None,
+                      moe_post_norm_weight=None, attn_gate=None, moe_gate=None) -> None:
         self.attn_norm.weight.data.copy_(attn_norm_weight)
         self.attn.qkv_proj.weight_loader(q_weight, "q")
         self.attn.qkv_proj.weight_loader(k_weight, "k")
@@ -148,11 +171,49 @@ class HybridBlock(nn.Module):
         self.moe_norm.weight.data.copy_(moe_norm_weight)
         self.moe.weight_loader(gate_weight, expert_gate_weights, expert_up_weights,
                                expert_down_weights)
+        for have, name, given in (
+                (self.post_norm, "attn_post_norm", attn_post_norm_weight),
+                (self.post_norm, "moe_post_norm", moe_post_norm_weight),
+                (self.gate_act is not None, "attn_gate", attn_gate),
+                (self.gate_act is not None, "moe_gate", moe_gate)):
+            if given is None:
+                continue
+            if not have:
+                raise ValueError(f"this block has no {name}")
+            own = getattr(self, name)
+            (own.weight if isinstance(own, RMSNorm) else own).data.copy_(given)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def _join(self, x, branch, post: RMSNorm, gate, pre: RMSNorm):
+        """(x + scale * act(gate) * post(branch), its pre norm), one row kernel."""
+        return ops.block_norm(x, branch.contiguous(), post.weight, pre.weight, pre.eps, gate=gate,
+                              gate_act=self.gate_act or "none",
+                              residual_scale=self.residual_scale)
+
+    def forward(self, x: torch.Tensor, normed: torch.Tensor | None = None,
+                next_norm: RMSNorm | None = None):
+        """The block's output; with ``next_norm`` (the ``attn_norm`` of the block that
+        follows) also that norm of it, taken in the kernel that makes the output, to be
+        passed to that block as ``normed``."""
         # h = x + attn(norm(x)); y = h + moe(norm(h)) (C8:318-325).  Both norms
         # and the first residual add run in the fused row kernel.
         x = x.contiguous()
-        a = self.attn(ops.add_rmsnorm(x, self.attn_norm.weight, self.attn_norm.eps))
-        h, n2 = ops.add_rmsnorm(x, self.moe_norm.weight, self.moe_norm.eps, delta=a.contiguous())
-        return h + self.moe(n2)
+        if next_norm is not None and next_norm.eps != self.attn_norm.eps:
+            raise ValueError(f"next_norm has eps {next_norm.eps}, this block {self.attn_norm.eps}")
+        if normed is None:
+            normed = ops.add_rmsnorm(x, self.attn_norm.weight, self.attn_norm.eps)
+        elif normed.shape != x.shape:
+            raise ValueError(f"normed must have the shape of x, got {tuple(normed.shape)}")
+        a = self.attn(normed)
+        if not self.post_norm:
+            h, n2 = ops.add_rmsnorm(x, self.moe_norm.weight, self.moe_norm.eps,
+                                    delta=a.contiguous())
+            m = self.moe(n2)
+            if next_norm is None:
+                return h + m
+            return ops.add_rmsnorm(h, next_norm.weight, next_norm.eps, delta=m.contiguous())
+        gated = self.gate_act is not None
+        h, n2 = self._join(x, a, self.attn_post_norm, self.attn_gate if gated else None,
+                           self.moe_norm)
+        y, n = self._join(h, self.moe(n2), self.moe_post_norm, self.moe_gate if gated else None,
+                          self.attn_norm if next_norm is None else next_norm)
+        return y if next_norm is None else (y, n)

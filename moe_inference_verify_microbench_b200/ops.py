@@ -425,6 +425,14 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float,
 _GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}  # MOE_GATE_ACT_*
 
 
+def check_gate_act(gate_act: str) -> int:
+    """The code of a gate's activation; refuses what ``block_norm`` does not have."""
+    act = _GATE_ACTS.get(gate_act)
+    if act is None:
+        raise ValueError(f"gate_act must be one of {tuple(_GATE_ACTS)}, got {gate_act!r}")
+    return act
+
+
 def block_norm(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor,
                pre_weight: torch.Tensor, eps: float, gate: torch.Tensor | None = None,
                gate_act: str = "none", residual_scale: float = 1.0):
@@ -440,9 +448,7 @@ def block_norm(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor,
     _need(delta, "delta", torch.bfloat16)
     if x.dim() == 0 or delta.shape != x.shape:
         raise ValueError("delta must have the shape of x, [..., H]")
-    act = _GATE_ACTS.get(gate_act)
-    if act is None:
-        raise ValueError(f"gate_act must be one of {tuple(_GATE_ACTS)}, got {gate_act!r}")
+    act = check_gate_act(gate_act)
     H = x.shape[-1]
     T = x.numel() // max(H, 1)
     dev = x.device

@@ -16,7 +16,12 @@ recorded there (``ops.check_status`` reads it).  With the keyword extra
 ``decode_weights=True`` the module also keeps the down weights transposed
 (one more copy of ``w_down``; ``down_weights_transposed(refresh=True)``
 rebuilds it after the per-expert weights were written) and runs batches of
-up to 4 tokens on the one-pass decode layer.
+up to 4 tokens on the one-pass decode layer.  With the keyword extra
+``expert_weights="w4"`` the forward runs on a 4-bit copy of the expert weights
+(``ops.moe_layer_w4``; groups of ``group_size`` columns, with zero points unless
+``symmetric``), rounded on first use and again when a stacked weight is re-bound
+or written in place; ``experts_4bit(refresh=True)`` rebuilds it after the
+per-expert weights were written.
 
 The module must be bf16 on a CUDA device: there is no CPU path.
 """
@@ -28,6 +33,7 @@ from torch import nn
 
 from . import ops
 from .experts import ExpertBank, SwiGLU_MLP, router_bias_of
+from .w4 import GROUPS, W4Experts
 
 __all__ = ["PermutedSparseMoE", "SwiGLU_MLP"]
 
@@ -37,9 +43,25 @@ class PermutedSparseMoE(nn.Module):
 
     def __init__(self, hidden: int, intermediate: int, num_experts: int, top_k: int,
                  norm_topk_prob: bool = True, *, index_add: str = "deterministic",
-                 check_errors: bool = False, decode_weights: bool = False) -> None:
+                 check_errors: bool = False, decode_weights: bool = False,
+                 expert_weights: str = "bf16", group_size: int = 128,
+                 symmetric: bool = True) -> None:
         super().__init__()
         ops._combine_mode(index_add)  # validate
+        if expert_weights not in ("bf16", "w4"):
+            raise ValueError(f'expert_weights must be "bf16" or "w4", got {expert_weights!r}')
+        if expert_weights == "w4":
+            if index_add != "deterministic" or decode_weights:
+                raise ValueError('expert_weights="w4" has the deterministic combine and a decode '
+                                 "layer of its own: no index_add, no decode_weights")
+            if group_size not in GROUPS or hidden % group_size or intermediate % group_size:
+                raise ValueError(f"group_size must be one of {GROUPS} and divide hidden and "
+                                 f"intermediate, got {group_size}")
+        self.expert_weights = expert_weights
+        self.group_size = group_size
+        self.symmetric = symmetric
+        self._w4 = None
+        self._w4_key = None
         self.index_add = index_add
         self.check_errors = check_errors
         self.decode_weights = decode_weights
@@ -57,6 +79,7 @@ class PermutedSparseMoE(nn.Module):
     def _apply(self, fn, *args, **kwargs):
         self._bank.invalidate()
         self._w_down_t = None
+        self._w4 = None
         return super()._apply(fn, *args, **kwargs)
 
     def pack(self):
@@ -77,18 +100,32 @@ class PermutedSparseMoE(nn.Module):
             self._w_down_t_key = key
         return self._w_down_t
 
+    def experts_4bit(self, refresh: bool = False) -> W4Experts:
+        """The 4-bit bank of ``expert_weights="w4"``, rebuilt under the same rules as
+        ``down_weights_transposed``, for all three projections."""
+        weights = self.pack()
+        key = tuple((w.data_ptr(), w._version) for w in weights)
+        if refresh or self._w4 is None or self._w4_key != key:
+            self._w4 = W4Experts.quantize(*weights, self.group_size, self.symmetric)
+            self._w4_key = key
+        return self._w4
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape
         x_flat = x.reshape(-1, shape[-1])
         if not x_flat.is_contiguous():
             x_flat = x_flat.contiguous()
-        wg, wu, wd = self.pack()
-        w_down_t = None
-        if self.decode_weights and 0 < x_flat.shape[0] <= 4:
-            w_down_t = self.down_weights_transposed()
-        y = ops.moe_layer(x_flat, self.gate.weight, wg, wu, wd, self.top_k, self.norm_topk_prob,
-                          bias=router_bias_of(self.gate), index_add=self.index_add,
-                          w_down_t=w_down_t)
+        if self.expert_weights == "w4":
+            y = ops.moe_layer_w4(x_flat, self.gate.weight, self.experts_4bit(), self.top_k,
+                                 self.norm_topk_prob, bias=router_bias_of(self.gate))
+        else:
+            wg, wu, wd = self.pack()
+            w_down_t = None
+            if self.decode_weights and 0 < x_flat.shape[0] <= 4:
+                w_down_t = self.down_weights_transposed()
+            y = ops.moe_layer(x_flat, self.gate.weight, wg, wu, wd, self.top_k,
+                              self.norm_topk_prob, bias=router_bias_of(self.gate),
+                              index_add=self.index_add, w_down_t=w_down_t)
         if self.check_errors:
             ops.check_status(y.device)
         return y.reshape(shape)

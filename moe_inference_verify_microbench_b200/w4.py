@@ -52,6 +52,8 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True):
         lo, hi = g.amin(-1).clamp_max(0.0), g.amax(-1).clamp_min(0.0)
         scales = ((hi - lo) / 15.0).bfloat16()
     s = scales.float()
+    if not bool(torch.isfinite(s).all()):
+        raise ValueError("a group's range exceeds the scales' type (bfloat16)")
     s = torch.where(s > 0, s, torch.ones_like(s)).unsqueeze(-1)  # a group of zeros: any scale
     if symmetric:
         codes = (g / s).round_().add_(8.0)
