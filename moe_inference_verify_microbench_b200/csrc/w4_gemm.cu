@@ -26,8 +26,8 @@
 //                 the copies of 128 records take 80 cycles each: T = 8192 1578 us
 //                 instead of 863)
 //   warp 24       tiled copies of codes and group records into a ring
-//   warp 25       issues tcgen05.mma: 2 operands x 4 steps of 16 columns per block
-//   warp 26       allocates tensor memory
+//   warps 25, 26  issue tcgen05.mma, one operand each: 4 steps of 16 columns per
+//                 block; warp 25 allocates tensor memory
 //
 // A weight is rounded once, s * (q - z) to bf16: the operand's type.  That is
 // 2^-9 of it in the mean, like the rounding of the activations themselves; the
@@ -49,8 +49,7 @@ constexpr int kTcTiles = 16;      // packed tiles per unit
 constexpr int kTcBlocks = 2;      // blocks per code stage
 constexpr int kTcRows = 128;      // records per unit at most
 constexpr int kTcDequantWarps = 16;
-constexpr int kTcEpiWarp = 16, kTcLoadWarp = 20, kTcCopyWarp = 24, kTcMmaWarp = 25,
-              kTcAllocWarp = 26;
+constexpr int kTcEpiWarp = 16, kTcLoadWarp = 20, kTcCopyWarp = 24, kTcMmaWarp = 25;
 constexpr int kTcLoadWarps = kTcCopyWarp - kTcLoadWarp;
 constexpr int kTcThreads = 27 * 32;
 constexpr int kTcBBytes = kTcRows * 128;
@@ -200,17 +199,12 @@ __device__ __forceinline__ uint32_t tc_desc(const uint8_t* base, uint32_t offset
   return (((smem_u32(base) + offset) >> 4) & 0x3fffu) | (1u << 16);
 }
 
-// The products of a 64-column block: both operands, four steps of 16 columns.
-__device__ __forceinline__ void tc_block(uint32_t d0, uint32_t d1, uint32_t at, uint32_t lo,
-                                         uint32_t hi, uint32_t idesc, bool add, bool second) {
+// The products of a 64-column block with one operand: four steps of 16 columns.
+__device__ __forceinline__ void tc_block(uint32_t d, uint32_t at, uint32_t lo, uint32_t hi,
+                                         uint32_t idesc, bool add) {
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk)
-    tc_mma_bf16_ts(d0, at + kk * 8, lo + 2 * kk, hi, idesc, kk != 0 || add ? 1u : 0u);
-  if (second) {
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
-      tc_mma_bf16_ts(d1, at + 32 + kk * 8, lo + 2 * kk, hi, idesc, kk != 0 || add ? 1u : 0u);
-  }
+    tc_mma_bf16_ts(d, at + kk * 8, lo + 2 * kk, hi, idesc, kk != 0 || add ? 1u : 0u);
 }
 
 // HALVES: groups of 32, two to a block; ZEROS: zero points are kept.
@@ -244,25 +238,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kTcPairs; ++s) {
       mbar_init(&full[s], 4 * kTcBlocks);  // the warps of two sets
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);  // both issuers'
     }
     for (int s = 0; s < kTcSlots; ++s) {
       mbar_init(&bfull[s], kTcLoadWarps);
-      mbar_init(&bempty[s], 1);
+      mbar_init(&bempty[s], 2);
     }
     for (int s = 0; s < kTcRing; ++s) {
       mbar_init(&qfull[s], 1);
       mbar_init(&qempty[s], 4 * kTcBlocks);  // a set for each block
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_full[b], 2);
       mbar_init(&acc_empty[b], 4);
     }
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  if (warp == kTcAllocWarp) {
+  if (warp == kTcMmaWarp) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -582,15 +576,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
     }
-  } else if (warp == kTcMmaWarp) {
+  } else {
     // ------------------------------------------------------------ MMA issuer
-    // The whole warp walks the stages, so that addresses and descriptors are
+    // Each of the two warps issues the products of one operand, into an accumulator of
+    // its own: with one warp for both, the 16 products of two blocks took 375 of 1250
+    // cycles.  The whole warp walks the stages, so that addresses and descriptors are
     // uniform values, and one elected lane issues.  This loop is what the block
     // rate hangs on: a wait for a barrier that is long complete costs 100 cycles, so
     // the next block's barriers are tested while this block's products are issued;
     // a vote costs 75, so none is taken inside a unit.  After an abort the waits
     // return at once and the unit is finished on what the stages hold.
     TcAcc acc;
+    const int op = warp - kTcMmaWarp;
     const uint32_t leader = elect_one();
     // descriptor of a K-major 128-byte-swizzled tile, without its start address
     constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -615,8 +612,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       issued = acc.first;
       ++acc.filled[issued];
       const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>(cols));
-      const bool second = SWIGLU || u.m * kTcTiles + 8 < a.m.tiles;
-      const uint32_t d0 = tmem + acc.d0, d1 = tmem + acc.d1;
+      const bool rows = op == 0 || SWIGLU || u.m * kTcTiles + 8 < a.m.tiles;  // of this operand
+      const uint32_t d = tmem + (op == 0 ? acc.d0 : acc.d1);
       uint32_t in_slot = 0;
       bool ready = false, bready = false;
       for (int kb = 0; kb < nb; kb += kTcBlocks) {
@@ -634,7 +631,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!ready) mbar_wait(&full[p], phase, abort_flag, a.status, kErrTimeoutFull);
         __syncwarp();
         tc_fence_after();
-        const uint32_t at = tmem + kTcOperandCol + p * (kTcBlocks * 64);
+        const uint32_t at = tmem + kTcOperandCol + p * (kTcBlocks * 64) + op * 32;
         const uint32_t lo0 = tc_desc(sB, bs0 * kTcBBytes + in0 * cols * 128);
         const uint32_t lo1 = per == 1 ? tc_desc(sB, bs * kTcBBytes) : lo0 + cols * 8;
         const uint32_t bs1 = bs, p0 = p;
@@ -657,15 +654,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           ready = mbar_test(&full[p], phase);
           if (end) bready = mbar_test(&bfull[bs], bph);
         }
-        if (leader) {
-          tc_block(d0, d1, at, lo0, kDescHi, idesc, kb != 0, second);
+        if (leader && rows) {
+          tc_block(d, at, lo0, kDescHi, idesc, kb != 0);
           if (two) {
             if (per == 1) tc_commit(&bempty[bs0]);
-            tc_block(d0, d1, at + 64, lo1, kDescHi, idesc, true, second);
+            tc_block(d, at + 64, lo1, kDescHi, idesc, true);
           }
           tc_commit(&empty[p0]);
           if (end) tc_commit(&bempty[bs1]);
           if (last) tc_commit(&acc_full[issued]);
+        } else if (leader) {  // nothing of this operand to wait for
+          if (two && per == 1) mbar_arrive(&bempty[bs0]);
+          mbar_arrive(&empty[p0]);
+          if (end) mbar_arrive(&bempty[bs1]);
+          if (last) mbar_arrive(&acc_full[issued]);
         }
         __syncwarp();
       }
@@ -682,7 +684,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kTcAllocWarp) {
+  if (warp == kTcMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
