@@ -67,6 +67,10 @@ int launch_combine(const void* rows, int n_rows, const int* slot_src, const floa
                    const int* ids, int e_begin, int e_end, int T, int k, int H, void* y,
                    int* status, cudaStream_t stream);
 
+// y[n] = sum of the fp32 rows [T * k][H] of token n's slots whose expert is in range.
+int launch_combine_f32(const float* rows, const int* ids, int e_begin, int e_end, int T, int k,
+                       int H, void* y, cudaStream_t stream);
+
 int launch_router(const void* x, const void* wr, const float* bias, int T, int H, int E, int k,
                   int norm_topk_prob, int* ids_out, float* w_out, void* logits_out, int* status,
                   cudaStream_t stream);
@@ -174,6 +178,9 @@ int launch_decode_split(const void* x, const void* wr, const float* bias, int T,
                         const void* w_down_t, void* scratch, void* y, int* status,
                         cudaStream_t stream);
 
+// Records per expert, on average, from which the 4-bit products take the tensor-memory form.
+constexpr int kW4TcRecords = 8;
+
 // Down GEMM with the atomic combine: out_f32[row_map[p] / red_div] +=
 // row_scale[row_map[p]] * (h[p] @ w_down[e]^T) in fp32 (row_map[p] < n_slots).
 int launch_w2_atomic(const void* h, int M, const int4* tiles, const int* num_tiles,
@@ -199,7 +206,7 @@ int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* 
 int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
                  int max_tiles, const int* row_map, const float* row_scale, void* out,
                  int out_rows, int avg, int* status, cudaStream_t stream,
-                 const long long* tail = nullptr);
+                 const long long* tail = nullptr, float* out_f32 = nullptr);
 
 // The whole layer for a few tokens (w4_decode.cu; T <= 16, T * k <= 64): `scratch`
 // holds w4_decode_scratch_bytes(b, T) bytes, h [T * k, I] bf16.

@@ -110,6 +110,37 @@ __global__ void __launch_bounds__(kRowsThreads) combine_rows(
   }
 }
 
+// The same over fp32 rows, row s of slot s, four columns a thread: the experts of a few
+// tokens (a few MB at most, which stay in L2) need not be rounded before they are summed.
+__global__ void __launch_bounds__(kRowsThreads) combine_rows_f32(
+    const float4* __restrict__ rows, const int* __restrict__ ids, int e_begin, int e_end, int T,
+    int k, int vec_per_row, uint2* __restrict__ y) {
+  pdl_wait();
+  pdl_trigger();
+  const int total = T * vec_per_row;
+  for (int g = blockIdx.x * blockDim.x + threadIdx.x; g < total; g += gridDim.x * blockDim.x) {
+    const int n = g / vec_per_row, v = g - n * vec_per_row;
+    float4 val[kCombineMaxK];
+#pragma unroll
+    for (int j = 0; j < kCombineMaxK; ++j) {
+      val[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j < k) {
+        const int s = n * k + j, e = __ldg(ids + s);
+        if (e >= e_begin && e < e_end) val[j] = __ldg(rows + static_cast<size_t>(s) * vec_per_row + v);
+      }
+    }
+    float4 acc = val[0];
+#pragma unroll
+    for (int j = 1; j < kCombineMaxK; ++j) {
+      acc.x += val[j].x;
+      acc.y += val[j].y;
+      acc.z += val[j].z;
+      acc.w += val[j].w;
+    }
+    y[g] = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+  }
+}
+
 // Large batches: one warp per token, each lane sums 16-byte vectors of the k
 // rows.  All loads of COLS column vectors are issued before any is used
 // (KMAX x COLS = 16 loads in flight per lane), so a small k (the per-owner
@@ -617,6 +648,20 @@ int launch_combine(const void* rows, int n_rows, const int* slot_src, const floa
   const cudaError_t e = launch_pdl(combine_rows, dim3(grid), dim3(kRowsThreads), 0, stream,
                                    static_cast<const uint4*>(rows), n_rows, slot_src, slot_w, ids,
                                    e_begin, e_end, T, k, H / 8, static_cast<uint4*>(y), status);
+  return e == cudaSuccess ? kRcOk : kRcCudaError;
+}
+
+int launch_combine_f32(const float* rows, const int* ids, int e_begin, int e_end, int T, int k,
+                       int H, void* y, cudaStream_t stream) {
+  if (T < 0 || k <= 0 || k > kCombineMaxK || H <= 0 || (H % 4) != 0 ||
+      static_cast<long long>(T) * H > 0x7fffffffLL)
+    return kRcBadArgument;
+  if (T == 0) return kRcOk;
+  const int blocks = (T * (H / 4) + kRowsThreads - 1) / kRowsThreads;
+  const cudaError_t e =
+      launch_pdl(combine_rows_f32, dim3(blocks), dim3(kRowsThreads), 0, stream,
+                 reinterpret_cast<const float4*>(rows), ids, e_begin, e_end, T, k, H / 4,
+                 static_cast<uint2*>(y));
   return e == cudaSuccess ? kRcOk : kRcCudaError;
 }
 

@@ -10,11 +10,16 @@
 // sixteen warps per SM.  Every warp copies the part of a 16-row tile that it will
 // use itself (contiguous, in the order its lanes consume) into shared memory
 // with cp.async, several tiles ahead, so the stream needs no barrier; it turns
-// codes into fp16 operands in registers (20 integer instructions per 1024
-// weights, no conversion) and multiplies them on the tensor cores as the 16-row
-// operand of mma.m16n8k16, with up to 16 records as its columns.  The records'
-// rows stay in registers for all tiles of an expert.  The warps that share a
-// tile along K add their fp32 partials through shared memory.
+// codes into bf16 operands 128 + q in registers (seven integer instructions for
+// eight weights, no conversion) and multiplies them on the tensor cores as the
+// 16-row operand of mma.m16n8k16, with up to 8 records as its columns (more records
+// of an expert: another pass).  The records' rows stay in registers for all tiles
+// of an expert.  The warps that share a tile along K add their fp32 partials
+// through shared memory.
+//
+// Measured back to back, 128 experts of 2048 x 768, top 8, group 128: gate/up 3.5
+// TB/s at 12 tokens (30 us), 3.9 at 64 (52 us); down 2.6 and 3.2 TB/s.  The issue
+// slots are the next bound (66 instructions per 16 x 64 block of codes).
 //
 // Numerics: products of activations with (q - z) are exact in fp32; each
 // group (or a warp's share of it) is summed on the tensor cores in fp32 and
@@ -163,8 +168,9 @@ static int w4_dispatch_mode(W4Args& a, cudaStream_t stream) {
 
 template <bool SWIGLU>
 static int w4_dispatch(W4Args& a, cudaStream_t stream) {
-  // Whole layers, 128 experts of 2048 x 768, group 128: at 4 records per expert the
-  // stream takes 110 us and the tensor-memory form 140, at 8 they take 152 and 146.
+  // Experts of 2048 x 768, group 128, 128 of them, the whole call: at 4 records per expert
+  // the stream takes 95 us and the tensor-memory form 115, at 8 they take 120 and 117,
+  // at 10 140 and 120 (the stream passes over the weights once for 8 records).
   if (a.avg >= kW4TcRecords) return w4_gemm(a, SWIGLU, stream);
   if (a.m.rec == 8 || a.m.gshift == 0) return w4_dispatch_mode<SWIGLU, kW4Half>(a, stream);
   if (a.m.gshift == 1) return w4_dispatch_mode<SWIGLU, kW4Block>(a, stream);
@@ -203,12 +209,14 @@ int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* 
 int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
                  int max_tiles, const int* row_map, const float* row_scale, void* out,
                  int out_rows, int avg, int* status, cudaStream_t stream,
-                 const long long* tail) {
+                 const long long* tail, float* out_f32) {
   if (const int rc = w4_check_bank(bank); rc != kRcOk) return rc;
   if (M < 0 || max_tiles < 0 || out_rows < 0 || tiles == nullptr || num_tiles == nullptr)
     return kRcBadArgument;
   if (M == 0 || max_tiles == 0) return kRcOk;
-  if (h == nullptr || out == nullptr || !aligned16(h) || !aligned16(out)) return kRcBadArgument;
+  if (h == nullptr || (out == nullptr) == (out_f32 == nullptr) || !aligned16(h) || !aligned16(out) ||
+      (out_f32 != nullptr && (tail != nullptr || avg >= kW4TcRecords)))
+    return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, true);
   a.act = static_cast<const uint32_t*>(h);
@@ -220,6 +228,7 @@ int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, co
   a.max_tiles = max_tiles;
   a.E = bank.E;
   a.out = static_cast<__nv_bfloat16*>(out);
+  a.out_f32 = out_f32;
   a.out_ld = bank.H;
   a.out_rows = out_rows;
   a.row_map = row_map;

@@ -95,6 +95,7 @@ struct W4Args {
   int max_tiles;
   int E;
   __nv_bfloat16* out;
+  float* out_f32;       // where the rows go instead, unrounded (the stream's down product only)
   int out_ld;
   int out_rows;
   const int* row_map;
@@ -160,9 +161,8 @@ bool allow_smem(Kernel* fn, int bytes, std::atomic<uint64_t>& done) {
   return true;
 }
 
-// The tensor-memory form for experts with many records (w4_gemm.cu), from this
-// many records per expert on.
-constexpr int kW4TcRecords = 8;
+// The tensor-memory form for experts with many records (w4_gemm.cu), from
+// kW4TcRecords records per expert on.
 int w4_gemm(const W4Args& a, bool swiglu, cudaStream_t stream);
 
 }  // namespace moe

@@ -29,9 +29,19 @@
 //   warps 25, 26  issue tcgen05.mma, one operand each: 4 steps of 16 columns per
 //                 block; warp 25 allocates tensor memory
 //
-// A weight is rounded once, s * (q - z) to bf16: the operand's type.  That is
-// 2^-9 of it in the mean, like the rounding of the activations themselves; the
-// sums stay fp32.
+// A weight is rounded once, s * (q - z) to bf16: the operand's type, and what a bf16
+// checkpoint of the same weights would hold.  That is 2^-9 of it at most, like
+// the rounding of the activations themselves; the sums stay fp32.  (Exact operands
+// q - z would need the scale on every group's sums: a pass over the accumulators per
+// 128 columns, 256 fp32 sums a thread at 128 records.)
+//
+// Measured back to back, 128 experts of 2048 x 768, group 128, gate/up and down:
+// 16 records per expert 69 and 39 us (3.0 and 2.7 TB/s of codes), 64 records 93 and
+// 58 us, 512 records 420 and 260 us (0.98 and 0.79 PFLOP/s).  At 16 records the issue
+// slots are 70 % used (106 instructions per 16 x 64 block of codes, 66 of them the
+// dequantisation) and a set of warps waits for its own products before it refills
+// its stage; a third pair of stages was worth 3 %.  At 512 the tiles of 128 records and
+// 256 weight rows move 6.4 TB/s from L2.
 #include <algorithm>
 
 #include "grouped_gemm.cuh"

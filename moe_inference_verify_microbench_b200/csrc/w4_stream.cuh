@@ -383,7 +383,7 @@ __device__ __forceinline__ void w4_units(const W4Args& a, uint8_t* smem, float* 
     }
     float fold[KB][2];
     w4_fold<KB, MODE>(b, fold);
-    __nv_bfloat16* out = a.out + c.tile * (SWIGLU ? 8 : 16) + g;
+    int col = c.tile * (SWIGLU ? 8 : 16) + g;
     for (int i = 0; i < count; ++i) {
       cp_async_wait_group<SLOTS - 2>();
       __syncwarp();  // every lane's copies have landed, and the last tile's slot is free
@@ -396,16 +396,19 @@ __device__ __forceinline__ void w4_units(const W4Args& a, uint8_t* smem, float* 
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if (orow[u] >= 0) {
-          __nv_bfloat16* dst = out + static_cast<size_t>(orow[u]) * a.out_ld;
+          const size_t at = static_cast<size_t>(orow[u]) * a.out_ld + col;
           if constexpr (SWIGLU) {
-            dst[0] = __float2bfloat16_rn(silu_f(acc[u]) * acc[u + 2]);
+            a.out[at] = __float2bfloat16_rn(silu_f(acc[u]) * acc[u + 2]);
+          } else if (a.out_f32 != nullptr) {
+            a.out_f32[at] = acc[u] * scale[u];
+            a.out_f32[at + 8] = acc[u + 2] * scale[u];
           } else {
-            dst[0] = __float2bfloat16_rn(acc[u] * scale[u]);
-            dst[8] = __float2bfloat16_rn(acc[u + 2] * scale[u]);
+            a.out[at] = __float2bfloat16_rn(acc[u] * scale[u]);
+            a.out[at + 8] = __float2bfloat16_rn(acc[u + 2] * scale[u]);
           }
         }
       }
-      out += SWIGLU ? 8 : 16;
+      col += SWIGLU ? 8 : 16;
       buffer ^= kW4Warps * 128;
     }
     c.tile += count;
