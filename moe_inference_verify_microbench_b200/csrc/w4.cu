@@ -185,7 +185,8 @@ int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* 
       num_tiles == nullptr)
     return kRcBadArgument;
   if (M == 0 || max_tiles == 0) return kRcOk;
-  if (src == nullptr || src_rows == 0 || h_out == nullptr || !aligned16(src) || !aligned16(h_out))
+  if (src == nullptr || src_rows == 0 || h_out == nullptr || !aligned16(src) ||
+      !aligned16(h_out) || !aligned16(tiles))
     return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, false);
@@ -214,7 +215,8 @@ int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, co
   if (M < 0 || max_tiles < 0 || out_rows < 0 || tiles == nullptr || num_tiles == nullptr)
     return kRcBadArgument;
   if (M == 0 || max_tiles == 0) return kRcOk;
-  if (h == nullptr || (out == nullptr) == (out_f32 == nullptr) || !aligned16(h) || !aligned16(out) ||
+  if (h == nullptr || (out == nullptr) == (out_f32 == nullptr) || !aligned16(h) ||
+      !aligned16(out) || !aligned16(tiles) ||
       (out_f32 != nullptr && (tail != nullptr || avg >= kW4TcRecords)))
     return kRcBadArgument;
   W4Args a{};

@@ -37,29 +37,24 @@ __global__ void __launch_bounds__(32) w4_logits(const uint4* __restrict__ x,
                                                 const uint4* __restrict__ wr,
                                                 const float* __restrict__ bias, int vec, int E,
                                                 float* __restrict__ logits, unsigned int* bar) {
-  constexpr int kEarly = 8;  // vectors of the weight row read before the activations exist
+  constexpr int kEarly = 8;  // vectors of both rows asked for at once
   const int e = blockIdx.x % E, t = blockIdx.x / E, lane = threadIdx.x;
   const uint4* row = wr + static_cast<size_t>(e) * vec;
-  uint4 early[kEarly];
-#pragma unroll
-  for (int j = 0; j < kEarly; ++j) {
-    const int v = lane + 32 * j;
-    early[j] = v < vec ? __ldg(row + v) : make_uint4(0, 0, 0, 0);
-  }
-  pdl_wait();
+  pdl_wait();  // the weights too may have been written by the kernel before
   pdl_trigger();
   if (blockIdx.x == 0 && lane == 0) *bar = 0;
   const uint4* xr = x + static_cast<size_t>(t) * vec;
   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // the order of router_sort_small
-  uint4 xv[kEarly];
+  uint4 wv[kEarly], xv[kEarly];
 #pragma unroll
   for (int j = 0; j < kEarly; ++j) {
     const int v = lane + 32 * j;
+    wv[j] = v < vec ? __ldg(row + v) : make_uint4(0, 0, 0, 0);
     xv[j] = v < vec ? __ldg(xr + v) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int j = 0; j < kEarly; ++j)
-    if (lane + 32 * j < vec) dot8_acc(early[j], xv[j], acc);
+    if (lane + 32 * j < vec) dot8_acc(wv[j], xv[j], acc);
 #pragma unroll 4
   for (int v = lane + 32 * kEarly; v < vec; v += 32) dot8_acc(__ldg(row + v), __ldg(xr + v), acc);
   const float sum = warp_sum(acc_sum(acc));

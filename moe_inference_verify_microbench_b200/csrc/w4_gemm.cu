@@ -241,7 +241,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* s_scale = reinterpret_cast<float*>(tmem_slot + 2);
+  volatile int* store_stop = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  float* s_scale = reinterpret_cast<float*>(tmem_slot + 4);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
@@ -263,6 +264,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&acc_empty[b], 4);
     }
     *abort_flag = 0;
+    *store_stop = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
   }
@@ -425,7 +427,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int first = SWIGLU ? u.m * 128 : u.m * 256 + part * 128;
         const int outs = min(128, (SWIGLU ? a.m.tiles * 8 : a.m.tiles * 16) - first);
         bulk_wait_read();  // the staging rows this thread stored are free
+        if (!ok) *store_stop = 1;
         named_barrier(1, 128);
+        ok = *store_stop == 0;  // the four warps leave together: they meet at this barrier
         if (ok && outs > 0) {
           const uint32_t d = tmem + lanes + (part == 0 ? acc.d0 : acc.d1);
           // records down the staging rows: the fragments go through transposing stores

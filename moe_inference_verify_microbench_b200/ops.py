@@ -451,6 +451,8 @@ def block_norm(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor,
     act = check_gate_act(gate_act)
     H = x.shape[-1]
     T = x.numel() // max(H, 1)
+    if T > 0x7FFFFFFF:
+        raise ValueError(f"x has {T} rows; at most 2^31 - 1")
     dev = x.device
     post, pre = (_norm_weight(t, name, H, dev) for name, t in (("post_weight", post_weight),
                                                                ("pre_weight", pre_weight)))

@@ -102,7 +102,8 @@ class PermutedSparseMoE(nn.Module):
 
     def experts_4bit(self, refresh: bool = False) -> W4Experts:
         """The 4-bit bank of ``expert_weights="w4"``, rebuilt under the same rules as
-        ``down_weights_transposed``, for all three projections."""
+        ``down_weights_transposed``, for all three projections.  Building it
+        synchronises, so call this (or the module) once before a graph capture."""
         weights = self.pack()
         key = tuple((w.data_ptr(), w._version) for w in weights)
         if refresh or self._w4 is None or self._w4_key != key:

@@ -106,5 +106,14 @@ def test_layer_takes_the_routers_numbers_of_experts():
             assert lib.moe_w4_layer_forward(P, P, None, b, T, 2, 1, P, 0, P, None, None) == want
 
 
+def test_tile_tables_are_read_by_sixteen_bytes():
+    lib = _native.load()
+    b = ctypes.byref(_native.W4BankStruct(4096, 4096, 4096, 4096, 16, 256, 128, 64, 0))
+    odd = ctypes.c_void_p(4100)
+    assert lib.moe_grouped_w13_swiglu_w4(P, 5, None, 1, 5, odd, P, 3, b, P, None, None) == -1
+    assert lib.moe_grouped_w2_w4(P, 5, odd, P, 3, b, None, None, P, 5, None, None) == -1
+    assert lib.moe_grouped_w13_swiglu_w4(P, 0, P, 1, 5, P, P, 3, b, P, None, None) == -1  # no rows
+
+
 def test_gate_activations():
     assert [ops.check_gate_act(a) for a in ("none", "sigmoid", "tanh")] == [0, 1, 2]
