@@ -205,8 +205,42 @@ __device__ __forceinline__ TcUnit tc_unit(const W4Args& a, int w, int groups) {
 }
 
 // Low word of the descriptor of a record block in shared memory.
-__device__ __forceinline__ uint32_t tc_desc(const uint8_t* base, uint32_t offset) {
-  return (((smem_u32(base) + offset) >> 4) & 0x3fffu) | (1u << 16);
+__device__ __forceinline__ uint32_t tc_desc(uint32_t addr) {
+  return ((addr >> 4) & 0x3fffu) | (1u << 16);
+}
+
+// The issuers' barrier calls by shared-memory address; their loop counts instructions.
+__device__ __forceinline__ bool tc_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ void tc_spin(uint32_t bar, uint32_t parity, volatile int* abort,
+                                     int* status) {
+  const unsigned long long t0 = globaltimer_ns();
+  for (uint32_t it = 1; !tc_try(bar, parity); ++it) {
+    if ((it & 63u) != 0) continue;
+    if (*abort) return;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      record_status(status, kErrTimeoutFull);
+      *abort = 1;
+      return;
+    }
+  }
+}
+__device__ __forceinline__ void tc_commit32(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tc_arrive32(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // The products of a 64-column block with one operand: four steps of 16 columns.
@@ -596,16 +630,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // its own: with one warp for both, the 16 products of two blocks took 375 of 1250
     // cycles.  The whole warp walks the stages, so that addresses and descriptors are
     // uniform values, and one elected lane issues.  This loop is what the block
-    // rate hangs on: a wait for a barrier that is long complete costs 100 cycles, so
-    // the next block's barriers are tested while this block's products are issued;
-    // a vote costs 75, so none is taken inside a unit.  After an abort the waits
-    // return at once and the unit is finished on what the stages hold.
+    // rate hangs on, and among busy warps every instruction of it costs ten cycles:
+    // with votes, tests ahead and 64-bit addresses it took 1150 cycles for two blocks.
+    // After an abort the waits return at once and the unit is finished on what the
+    // stages hold.
     TcAcc acc;
     const int op = warp - kTcMmaWarp;
     const uint32_t leader = elect_one();
     // descriptor of a K-major 128-byte-swizzled tile, without its start address
     constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
     uint32_t p = 0, phase = 0, bs = 0, bph = 0;
+    const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), bfull0 = smem_u32(bfull),
+                   bempty0 = smem_u32(bempty), acc_full0 = smem_u32(acc_full);
+    const uint32_t sb = smem_u32(sB), at0 = tmem + kTcOperandCol + op * 32;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (!tc_try(bar, parity)) tc_spin(bar, parity, abort_flag, a.status);
+    };
+    auto next_slot = [&]() {
+      if (++bs == kTcSlots) {
+        bs = 0;
+        bph ^= 1u;
+      }
+    };
     int issued = -1;  // half of the last unit
     TcUnit next{};
     if (static_cast<int>(blockIdx.x) < total) next = tc_unit(a, blockIdx.x, groups);
@@ -628,62 +674,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>(cols));
       const bool rows = op == 0 || SWIGLU || u.m * kTcTiles + 8 < a.m.tiles;  // of this operand
       const uint32_t d = tmem + (op == 0 ? acc.d0 : acc.d1);
-      uint32_t in_slot = 0;
-      bool ready = false, bready = false;
-      for (int kb = 0; kb < nb; kb += kTcBlocks) {
-        const bool two = kb + 1 < nb;
-        if (!bready) mbar_wait(&bfull[bs], bph, abort_flag, a.status, kErrTimeoutFull);
-        // more than 64 records: the second block has a slot of its own
-        const uint32_t bs0 = bs, in0 = in_slot;
-        if (per == 1 && two) {
-          if (++bs == kTcSlots) {
-            bs = 0;
-            bph ^= 1u;
+      const uint32_t acc_bar = acc_full0 + issued * 8;
+      bool add = false;
+      for (int left = nb; left > 0;) {
+        // a slot: the blocks of several pairs, or with more than 64 records one block
+        wait(bfull0 + bs * 8, bph);
+        uint32_t lo = tc_desc(sb + bs * kTcBBytes);
+        for (int here = min(per, left); here > 0; here -= kTcBlocks) {
+          uint32_t bar = bempty0 + bs * 8, first_bar = 0, lo1 = lo + cols * 8;
+          if (per == 1 && left > 1) {  // the second block's slot
+            first_bar = bar;
+            next_slot();
+            bar = bempty0 + bs * 8;
+            lo1 = tc_desc(sb + bs * kTcBBytes);
+            wait(bfull0 + bs * 8, bph);
           }
-          mbar_wait(&bfull[bs], bph, abort_flag, a.status, kErrTimeoutFull);
-        }
-        if (!ready) mbar_wait(&full[p], phase, abort_flag, a.status, kErrTimeoutFull);
-        __syncwarp();
-        tc_fence_after();
-        const uint32_t at = tmem + kTcOperandCol + p * (kTcBlocks * 64) + op * 32;
-        const uint32_t lo0 = tc_desc(sB, bs0 * kTcBBytes + in0 * cols * 128);
-        const uint32_t lo1 = per == 1 ? tc_desc(sB, bs * kTcBBytes) : lo0 + cols * 8;
-        const uint32_t bs1 = bs, p0 = p;
-        const bool last = kb + kTcBlocks >= nb;
-        in_slot += kTcBlocks;
-        const bool end = in_slot >= static_cast<uint32_t>(per) || last;
-        if (end) {
-          in_slot = 0;
-          if (++bs == kTcSlots) {
-            bs = 0;
-            bph ^= 1u;
+          wait(full0 + p * 8, phase);
+          __syncwarp();  // no lane may fall a phase behind
+          tc_fence_after();
+          const uint32_t at = at0 + p * (kTcBlocks * 64);
+          if (leader) {
+            if (rows) {
+              tc_block(d, at, lo, kDescHi, idesc, add);
+              if (first_bar != 0) tc_commit32(first_bar);
+              if (left > 1) tc_block(d, at + 64, lo1, kDescHi, idesc, true);
+              tc_commit32(empty0 + p * 8);
+              if (here <= kTcBlocks) tc_commit32(bar);
+              if (left <= kTcBlocks) tc_commit32(acc_bar);
+            } else {  // nothing of this operand to wait for
+              if (first_bar != 0) tc_arrive32(first_bar);
+              tc_arrive32(empty0 + p * 8);
+              if (here <= kTcBlocks) tc_arrive32(bar);
+              if (left <= kTcBlocks) tc_arrive32(acc_bar);
+            }
           }
+          add = true;
+          lo += 2 * cols * 8;
+          left -= kTcBlocks;
+          p ^= 1u;
+          phase ^= p ^ 1u;
         }
-        if (++p == kTcPairs) {
-          p = 0;
-          phase ^= 1u;
-        }
-        ready = bready = true;
-        if (!last) {
-          ready = mbar_test(&full[p], phase);
-          if (end) bready = mbar_test(&bfull[bs], bph);
-        }
-        if (leader && rows) {
-          tc_block(d, at, lo0, kDescHi, idesc, kb != 0);
-          if (two) {
-            if (per == 1) tc_commit(&bempty[bs0]);
-            tc_block(d, at + 64, lo1, kDescHi, idesc, true);
-          }
-          tc_commit(&empty[p0]);
-          if (end) tc_commit(&bempty[bs1]);
-          if (last) tc_commit(&acc_full[issued]);
-        } else if (leader) {  // nothing of this operand to wait for
-          if (two && per == 1) mbar_arrive(&bempty[bs0]);
-          mbar_arrive(&empty[p0]);
-          if (end) mbar_arrive(&bempty[bs1]);
-          if (last) mbar_arrive(&acc_full[issued]);
-        }
-        __syncwarp();
+        next_slot();
       }
     }
     // Tensor memory is released below: the last unit's products have to be done,
