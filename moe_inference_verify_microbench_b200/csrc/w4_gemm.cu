@@ -36,11 +36,13 @@
 // 128 columns, 256 fp32 sums a thread at 128 records.)
 //
 // Measured back to back, 128 experts of 2048 x 768, group 128, gate/up and down:
-// 16 records per expert 69 and 39 us (3.0 and 2.7 TB/s of codes), 64 records 93 and
-// 58 us, 512 records 420 and 260 us (0.98 and 0.79 PFLOP/s).  At 16 records the issue
-// slots are 70 % used (106 instructions per 16 x 64 block of codes, 66 of them the
-// dequantisation) and a set of warps waits for its own products before it refills
-// its stage; a third pair of stages was worth 3 %.  At 512 the tiles of 128 records and
+// 16 records per expert 63 and 39 us (3.3 and 2.6 TB/s of codes), 64 records 93 and
+// 58 us, 512 records 413 and 268 us (1.0 and 0.77 PFLOP/s).  At 16 records the issue
+// slots are three quarters used (66 instructions per 16 x 64 block of codes for the
+// dequantisation, about 30 for all else) and a set of warps waits for its own products
+// before it refills its stage; a third pair of stages was worth 3 %.  Halves of units
+// in a last round that is not half full cost as much as whole ones (shard of 32
+// experts 78 -> 84 us).  At 512 the tiles of 128 records and
 // 256 weight rows move 6.4 TB/s from L2.
 #include <algorithm>
 
@@ -209,7 +211,8 @@ __device__ __forceinline__ uint32_t tc_desc(uint32_t addr) {
   return ((addr >> 4) & 0x3fffu) | (1u << 16);
 }
 
-// The issuers' barrier calls by shared-memory address; their loop counts instructions.
+// Barrier calls by shared-memory address, for the loops that count instructions.
+// (Suspending a waiting warp for up to 10 us at a time measured 1 to 2 % slower here.)
 __device__ __forceinline__ bool tc_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -222,17 +225,21 @@ __device__ __forceinline__ bool tc_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 __device__ __noinline__ void tc_spin(uint32_t bar, uint32_t parity, volatile int* abort,
-                                     int* status) {
+                                     int* status, int code) {
   const unsigned long long t0 = globaltimer_ns();
   for (uint32_t it = 1; !tc_try(bar, parity); ++it) {
     if ((it & 63u) != 0) continue;
     if (*abort) return;
     if (globaltimer_ns() - t0 > kWaitLimitNs) {
-      record_status(status, kErrTimeoutFull);
+      record_status(status, code);
       *abort = 1;
       return;
     }
   }
+}
+__device__ __forceinline__ void tc_wait(uint32_t bar, uint32_t parity, volatile int* abort,
+                                        int* status, int code) {
+  if (!tc_try(bar, parity)) tc_spin(bar, parity, abort, status, code);
 }
 __device__ __forceinline__ void tc_commit32(uint32_t bar) {
   asm volatile(
@@ -327,34 +334,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // Blocks are counted through all units, an odd number in a unit rounded up to
     // whole code stages; set i of four warps, one per lane quarter, takes the blocks
     // i modulo 4 and fills operand stage i with them.  Two blocks, of sets 0 and 1 or
-    // of sets 2 and 3, are handed over together.
-    const int quarter = warp & 3, set = warp >> 2;
+    // of sets 2 and 3, are handed over together.  So a set's j-th block comes through
+    // code stage (set / 2) + 2 (j mod 2).  After an abort the waits return at once and the
+    // unit is finished on what the stages hold.
+    static_assert(kTcRing == 2 * kTcPairs && kTcBlocks == 2, "the order of a set's stages");
+    const int quarter = warp & 3, set = warp >> 2, bk = set & 1;
     const uint32_t dst = tmem + kTcOperandCol + set * 64 + (static_cast<uint32_t>(32 * quarter) << 16);
-    const uint32_t codes = smem_u32(sRing) + lane * 16;
-    const uint32_t records = smem_u32(sRing) + kTcCodeBytes + (lane >> 2) * kRec;
+    const uint32_t stage = smem_u32(sRing) + (set >> 1) * args.ring_bytes;
+    const uint32_t q0 = stage + bk * kW4BlockBytes + lane * 16;
+    const uint32_t rec0 = stage + kTcCodeBytes + (lane >> 2) * kRec +
+                          (HALVES ? 2 * bk : (2 * bk) >> a.m.gshift) * (8 * kRec);
+    const uint32_t hand = (set >> 1) * 8;
+    const uint32_t qfull0 = smem_u32(qfull) + hand, qempty0 = smem_u32(qempty) + hand,
+                   full0 = smem_u32(full) + hand, empty0 = smem_u32(empty) + hand;
     uint32_t base = 0;  // blocks before this unit
-    const int pair = set >> 1;
-    uint32_t uses = 0;  // of the operand stage
-    bool ok = true;
-    for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+    uint32_t j = 0;     // of this set
+    for (int w = blockIdx.x; w < total; w += gridDim.x) {
       const TcUnit u = tc_unit(a, w, groups);
       if (!u.ok) continue;
-      for (uint32_t kb = (set - base) & 3u; kb < nbe; kb += 4) {
-        const uint32_t cnt = base + kb, ring = cnt / kTcBlocks, rs = ring % kTcRing;
-        ok = mbar_wait_idle(&qfull[rs], (ring / kTcRing) & 1u, abort_flag, a.status,
-                            kErrTimeoutFull);
-        ok = ok && mbar_wait_idle(&empty[pair], (uses & 1u) ^ 1u, abort_flag, a.status,
-                                  kErrTimeoutEmpty);
-        ++uses;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+      if (!__all_sync(0xffffffffu, *abort_flag == 0)) break;
+      const int left = a.m.tiles - u.m * kTcTiles;  // packed tiles from here to the end
+      for (uint32_t kb = (set - base) & 3u; kb < nbe; kb += 4, ++j) {
+        const uint32_t odd = j & 1u;
+        tc_wait(qfull0 + 16 * odd, (j >> 1) & 1u, abort_flag, a.status, kErrTimeoutFull);
+        tc_wait(empty0, odd ^ 1u, abort_flag, a.status, kErrTimeoutEmpty);
+        __syncwarp();
         tc_fence_after();
-        // packed tiles from here to the end; none for a block that rounds the unit up
-        const int tiles = kb < static_cast<uint32_t>(nb) ? a.m.tiles - u.m * kTcTiles : 0;
-        const uint32_t bk = kb & (kTcBlocks - 1);
-        const uint32_t q = codes + rs * args.ring_bytes + bk * kW4BlockBytes;
-        const uint32_t grp = HALVES ? 2 * bk : (2 * bk) >> a.m.gshift;
-        const uint32_t rec = records + rs * args.ring_bytes + grp * (8 * kRec);
+        // none for a block that rounds the unit up
+        const int tiles = kb < static_cast<uint32_t>(nb) ? left : 0;
+        const uint32_t q = q0 + odd * (2 * args.ring_bytes), rec = rec0 + odd * (2 * args.ring_bytes);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           // two packed tiles: 16 gate and 16 up rows, or 32 rows
@@ -420,10 +428,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&qempty[rs]);  // the codes have been read
-          mbar_arrive(&full[pair]);
+          tc_arrive32(qempty0 + 16 * odd);  // the codes have been read
+          tc_arrive32(full0);
         }
-        __syncwarp();
       }
       base += nbe;
     }
@@ -644,7 +651,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                    bempty0 = smem_u32(bempty), acc_full0 = smem_u32(acc_full);
     const uint32_t sb = smem_u32(sB), at0 = tmem + kTcOperandCol + op * 32;
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      if (!tc_try(bar, parity)) tc_spin(bar, parity, abort_flag, a.status);
+      tc_wait(bar, parity, abort_flag, a.status, kErrTimeoutFull);
     };
     auto next_slot = [&]() {
       if (++bs == kTcSlots) {
