@@ -20,7 +20,7 @@
 // CTA (864 threads, one per SM, persistent):
 //   warps 0..15   dequantise: warp w writes lane quarter w % 4 of every fourth
 //                 64-column block
-//   warps 16..19  epilogue: tensor memory -> bf16 -> staging rows -> bulk stores
+//   warps 16..19  epilogue: tensor memory -> bf16 -> staging rows -> output rows
 //   warps 20..23  gather the records' rows (a lane copies four of them with one
 //                 tile::gather4, into the 128-byte swizzle; issued from one warp
 //                 the copies of 128 records take 80 cycles each: T = 8192 1578 us
@@ -140,21 +140,6 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* m, 
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(r0), "r"(r1), "r"(r2),
       "r"(r3)
       : "memory");
-}
-
-__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src),
-               "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void bulk_commit() {
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-__device__ __forceinline__ void bulk_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
-__device__ __forceinline__ void bulk_wait_all() {
-  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // The column pairs of a word as bf16 s * (q - z): 0x4300 is 128.0 and a code is
@@ -284,6 +269,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* store_stop = reinterpret_cast<volatile int*>(tmem_slot + 2);
   float* s_scale = reinterpret_cast<float*>(tmem_slot + 4);
+  int* s_row = reinterpret_cast<int*>(s_scale + kTcRows);  // of this unit and of the last one
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
@@ -440,6 +426,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int r = threadIdx.x - kTcEpiWarp * 32;  // record this thread stores
     const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
     const uint32_t stage = smem_u32(sOut);
+    int* rows = s_row;
     if constexpr (!SWIGLU) w4_zero_tail(a, r, 128);
     TcAcc acc;
     bool ok = true;
@@ -457,6 +444,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           o = -1;
         }
       }
+      rows[r] = o;
       s_scale[r] = !SWIGLU && o >= 0 && a.row_scale != nullptr ? a.row_scale[o] : 1.0f;
       ok = mbar_wait_idle(&acc_full[acc.first], acc.filled[acc.first] & 1u, abort_flag, a.status,
                      kErrTimeoutAccFull);
@@ -467,7 +455,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // outputs of this part: 128 from `first`, fewer at the end of the matrix
         const int first = SWIGLU ? u.m * 128 : u.m * 256 + part * 128;
         const int outs = min(128, (SWIGLU ? a.m.tiles * 8 : a.m.tiles * 16) - first);
-        bulk_wait_read();  // the staging rows this thread stored are free
         if (!ok) *store_stop = 1;
         named_barrier(1, 128);
         ok = *store_stop == 0;  // the four warps leave together: they meet at this barrier
@@ -518,14 +505,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int b = acc.first; b <= acc.last; ++b) mbar_arrive(&acc_empty[b]);
           }
         }
-        fence_proxy_async_smem();
         named_barrier(1, 128);
-        if (ok && outs > 0 && o >= 0)
-          bulk_store(a.out + static_cast<size_t>(o) * a.out_ld + first, stage + r * kTcOutRow, outs * 2);
-        bulk_commit();
+        // Sixteen threads store a row.  (Bulk copies of whole rows, one from every
+        // thread, took 2700 cycles to issue.)
+        if (ok && (r & 15) * 8 < outs) {
+          const uint32_t src = stage + (r & 15) * 16;
+          __nv_bfloat16* dst = a.out + first + (r & 15) * 8;
+          for (int c = r >> 4; c < n; c += 32) {  // four rows in flight; -1 past the last
+            uint4 v[4];
+            int at[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              at[i] = c + 8 * i < kTcRows ? rows[c + 8 * i] : -1;
+              v[i] = lds128(src + min(c + 8 * i, kTcRows - 1) * kTcOutRow);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (at[i] >= 0)
+                *reinterpret_cast<uint4*>(dst + static_cast<size_t>(at[i]) * a.out_ld) = v[i];
+          }
+        }
       }
+      rows = rows == s_row ? s_row + kTcRows : s_row;
     }
-    bulk_wait_all();
   } else if (warp >= kTcLoadWarp && warp < kTcCopyWarp) {
     // A slot is up to 32 copies of four rows, dealt out to these warps.  A unit's row
     // numbers are uniform values of the warp and one elected lane issues its copies:
@@ -749,9 +751,9 @@ int tc_launch(const W4Args& a, cudaStream_t stream) {
   t.rec_stride = (4 >> a.m.gshift) * 8 * a.m.rec;
   t.ring_bytes = kTcCodeBytes + kTcTiles * t.rec_stride;
   const int sh =
-      1024 + kTcSlots * kTcBBytes + kTcOutBytes + kTcRing * t.ring_bytes + 512 + kTcRows * 4;
+      1024 + kTcSlots * kTcBBytes + kTcOutBytes + kTcRing * t.ring_bytes + 512 + kTcRows * 12;
   constexpr int kMost = 1024 + kTcSlots * kTcBBytes + kTcOutBytes +
-                        kTcRing * (kTcCodeBytes + kTcTiles * 256) + 512 + kTcRows * 4;
+                        kTcRing * (kTcCodeBytes + kTcTiles * 256) + 512 + kTcRows * 12;
   static_assert(kMost <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> attr{0};
   if (!allow_smem(w4_tc<SWIGLU, HALVES, ZEROS>, kMost, attr)) return kRcCudaError;
