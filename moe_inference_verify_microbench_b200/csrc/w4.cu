@@ -169,8 +169,9 @@ static int w4_dispatch_mode(W4Args& a, cudaStream_t stream) {
 template <bool SWIGLU>
 static int w4_dispatch(W4Args& a, cudaStream_t stream) {
   // Experts of 2048 x 768, group 128, 128 of them, the whole call: at 4 records per expert
-  // the stream takes 95 us and the tensor-memory form 115, at 8 they take 120 and 117,
-  // at 10 140 and 120 (the stream passes over the weights once for 8 records).
+  // the stream takes 94 us and the tensor-memory form 104, at 6 both take 105, at 8 they
+  // take 121 and 108 (the stream passes over the weights once for 8 records).  Between
+  // the two the stream's unrounded weights decide.
   if (a.avg >= kW4TcRecords) return w4_gemm(a, SWIGLU, stream);
   if (a.m.rec == 8 || a.m.gshift == 0) return w4_dispatch_mode<SWIGLU, kW4Half>(a, stream);
   if (a.m.gshift == 1) return w4_dispatch_mode<SWIGLU, kW4Block>(a, stream);

@@ -24,7 +24,7 @@
 //   warps 20..23  gather the records' rows (a lane copies four of them with one
 //                 tile::gather4, into the 128-byte swizzle; issued from one warp
 //                 the copies of 128 records take 80 cycles each: T = 8192 1578 us
-//                 instead of 863)
+//                 instead of 863 then)
 //   warp 24       tiled copies of codes and group records into a ring
 //   warps 25, 26  issue tcgen05.mma, one operand each: 4 steps of 16 columns per
 //                 block; warp 25 allocates tensor memory
@@ -36,8 +36,8 @@
 // 128 columns, 256 fp32 sums a thread at 128 records.)
 //
 // Measured back to back, 128 experts of 2048 x 768, group 128, gate/up and down:
-// 16 records per expert 63 and 39 us (3.3 and 2.6 TB/s of codes), 64 records 93 and
-// 58 us, 512 records 413 and 268 us (1.0 and 0.77 PFLOP/s).  At 16 records the issue
+// 16 records per expert 63 and 36 us (3.3 and 2.9 TB/s of codes), 64 records 90 and
+// 55 us, 512 records 430 and 263 us (0.96 and 0.78 PFLOP/s).  At 16 records the issue
 // slots are three quarters used (66 instructions per 16 x 64 block of codes for the
 // dequantisation, about 30 for all else) and a set of warps waits for its own products
 // before it refills its stage; a third pair of stages was worth 3 %.  Halves of units
@@ -55,7 +55,9 @@ namespace {
 
 constexpr int kTcStages = 4;      // weight operand stages (64 columns) in tensor memory
 constexpr int kTcPairs = 2;       // of them that are handed over together
-constexpr int kTcSlots = 6;       // record slots in shared memory (see tc_blocks)
+// Record slots in shared memory (see tc_blocks).
+template <bool SWIGLU>
+constexpr int kTcSlots = SWIGLU ? 6 : 4;
 constexpr int kTcRing = 4;        // code stages (128 columns)
 constexpr int kTcTiles = 16;      // packed tiles per unit
 constexpr int kTcBlocks = 2;      // blocks per code stage
@@ -65,8 +67,10 @@ constexpr int kTcEpiWarp = 16, kTcLoadWarp = 20, kTcCopyWarp = 24, kTcMmaWarp = 
 constexpr int kTcLoadWarps = kTcCopyWarp - kTcLoadWarp;
 constexpr int kTcThreads = 27 * 32;
 constexpr int kTcBBytes = kTcRows * 128;
-constexpr int kTcOutRow = 272;  // staging: 128 records of 128 outputs, rows 16 bytes apart in banks
-constexpr int kTcOutBytes = kTcRows * kTcOutRow;
+// Staging: the outputs of a unit for 128 records, rows 16 bytes apart in banks.  The down
+// product has 256 of them, so that its accumulators are free before anything is stored.
+template <bool SWIGLU>
+constexpr int kTcOutRow = (SWIGLU ? 256 : 512) + 16;
 constexpr int kTcCodeBytes = kTcTiles * kTcBlocks * kW4BlockBytes;
 constexpr uint32_t kTcOperandCol = 256;     // accumulators below, operand stages above
 
@@ -255,13 +259,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                              ~static_cast<uintptr_t>(1023));
   const W4Args& a = args.a;
   uint8_t* sB = smem;
-  uint8_t* sOut = sB + kTcSlots * kTcBBytes;
-  uint8_t* sRing = sOut + kTcOutBytes;
+  constexpr int kSlots = kTcSlots<SWIGLU>, kOutRow = kTcOutRow<SWIGLU>;
+  uint8_t* sOut = sB + kSlots * kTcBBytes;
+  uint8_t* sRing = sOut + kTcRows * kOutRow;
   uint64_t* full = reinterpret_cast<uint64_t*>(sRing + kTcRing * args.ring_bytes);
   uint64_t* empty = full + kTcPairs;
   uint64_t* bfull = empty + kTcPairs;
-  uint64_t* bempty = bfull + kTcSlots;
-  uint64_t* qfull = bempty + kTcSlots;
+  uint64_t* bempty = bfull + kSlots;
+  uint64_t* qfull = bempty + kSlots;
   uint64_t* qempty = qfull + kTcRing;
   uint64_t* acc_full = qempty + kTcRing;
   uint64_t* acc_empty = acc_full + 2;
@@ -278,7 +283,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&full[s], 4 * kTcBlocks);  // the warps of two sets
       mbar_init(&empty[s], 2);  // both issuers'
     }
-    for (int s = 0; s < kTcSlots; ++s) {
+    for (int s = 0; s < kSlots; ++s) {
       mbar_init(&bfull[s], kTcLoadWarps);
       mbar_init(&bempty[s], 2);
     }
@@ -451,18 +456,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       ++acc.filled[acc.first];
       tc_fence_after();
-      for (int part = 0; part < (SWIGLU ? 1 : 2); ++part) {
-        // outputs of this part: 128 from `first`, fewer at the end of the matrix
-        const int first = SWIGLU ? u.m * 128 : u.m * 256 + part * 128;
-        const int outs = min(128, (SWIGLU ? a.m.tiles * 8 : a.m.tiles * 16) - first);
-        if (!ok) *store_stop = 1;
-        named_barrier(1, 128);
-        ok = *store_stop == 0;  // the four warps leave together: they meet at this barrier
-        if (ok && outs > 0) {
+      // outputs of this unit from `first`, fewer at the end of the matrix
+      constexpr int kOuts = SWIGLU ? 128 : 256;
+      const int first = u.m * kOuts;
+      const int outs = min(kOuts, a.m.tiles * (SWIGLU ? 8 : 16) - first);
+      if (!ok) *store_stop = 1;
+      named_barrier(1, 128);
+      ok = *store_stop == 0;  // the four warps leave together: they meet at this barrier
+#pragma unroll
+      for (int part = 0; part < kOuts / 128; ++part) {
+        if (ok && part * 128 < outs) {
           const uint32_t d = tmem + lanes + (part == 0 ? acc.d0 : acc.d1);
           // records down the staging rows: the fragments go through transposing stores
-          const uint32_t dst = stage + ((lane >> 4) * 8 + (lane & 7)) * kTcOutRow +
-                               (32 * quarter + ((lane >> 3) & 1) * 8) * 2;
+          const uint32_t dst = stage + ((lane >> 4) * 8 + (lane & 7)) * kOutRow +
+                               (128 * part + 32 * quarter + ((lane >> 3) & 1) * 8) * 2;
           for (int c = 0; c < cols; c += 16) {
             uint32_t v[2][8];
             tmem_ld_16x256b_x2(d + c, v[0]);
@@ -494,36 +501,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 pk[i] = pack_bf16x2(__uint_as_float(v[h][2 * i]), __uint_as_float(v[h][2 * i + 1]));
-              stmatrix_x4_trans(dst + c * kTcOutRow + h * 32, pk);
+              stmatrix_x4_trans(dst + c * kOutRow + h * 32, pk);
             }
           }
         }
-        if (SWIGLU || part == 1) {  // the accumulators are read
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            for (int b = acc.first; b <= acc.last; ++b) mbar_arrive(&acc_empty[b]);
-          }
-        }
-        named_barrier(1, 128);
-        // Sixteen threads store a row.  (Bulk copies of whole rows, one from every
-        // thread, took 2700 cycles to issue.)
-        if (ok && (r & 15) * 8 < outs) {
-          const uint32_t src = stage + (r & 15) * 16;
-          __nv_bfloat16* dst = a.out + first + (r & 15) * 8;
-          for (int c = r >> 4; c < n; c += 32) {  // four rows in flight; -1 past the last
-            uint4 v[4];
-            int at[4];
+      }
+      tc_fence_before();  // the accumulators are read
+      __syncwarp();
+      if (lane == 0) {
+        for (int b = acc.first; b <= acc.last; ++b) mbar_arrive(&acc_empty[b]);
+      }
+      named_barrier(1, 128);
+      // Sixteen threads store 128 outputs of a row.  (Bulk copies of whole rows, one from
+      // every thread, took 2700 cycles to issue: 16 records per expert 39 us for the down
+      // product instead of 36; 512 records 269 instead of 263, but 421 instead of 430 for
+      // gate/up, where nobody waits for the stores.)
+      constexpr int kPer = kOuts / 8;
+      const int v = r % kPer;
+      if (ok && v * 8 < outs) {
+        const uint32_t src = stage + v * 16;
+        __nv_bfloat16* dst = a.out + first + v * 8;
+        for (int c = r / kPer; c < n; c += 4 * (128 / kPer)) {  // four rows in flight
+          uint4 val[4];
+          int at[4];  // -1 past the last
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              at[i] = c + 8 * i < kTcRows ? rows[c + 8 * i] : -1;
-              v[i] = lds128(src + min(c + 8 * i, kTcRows - 1) * kTcOutRow);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (at[i] >= 0)
-                *reinterpret_cast<uint4*>(dst + static_cast<size_t>(at[i]) * a.out_ld) = v[i];
+          for (int i = 0; i < 4; ++i) {
+            const int row = min(c + i * (128 / kPer), kTcRows - 1);
+            at[i] = c + i * (128 / kPer) < n ? rows[row] : -1;
+            val[i] = lds128(src + row * kOutRow);
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (at[i] >= 0)
+              *reinterpret_cast<uint4*>(dst + static_cast<size_t>(at[i]) * a.out_ld) = val[i];
         }
       }
       rows = rows == s_row ? s_row + kTcRows : s_row;
@@ -580,7 +590,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
         __syncwarp();
-        if (++s == kTcSlots) {
+        if (++s == kSlots) {
           s = 0;
           ph ^= 1u;
         }
@@ -589,7 +599,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (*abort_flag && lane == 0) {
       // Let every copy still in flight land before the CTA exits: the slots before s
       // are in their current round, the others in the one before.
-      for (uint32_t i = 0; i < kTcSlots; ++i) {
+      for (uint32_t i = 0; i < kSlots; ++i) {
         if (i >= s && ph == 0) break;  // never filled
         const unsigned long long t0 = globaltimer_ns();
         while (!mbar_try_wait(&bfull[i], i < s ? ph : ph ^ 1u)) {
@@ -656,7 +666,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_wait(bar, parity, abort_flag, a.status, kErrTimeoutFull);
     };
     auto next_slot = [&]() {
-      if (++bs == kTcSlots) {
+      if (++bs == kSlots) {
         bs = 0;
         bph ^= 1u;
       }
@@ -751,8 +761,8 @@ int tc_launch(const W4Args& a, cudaStream_t stream) {
   t.rec_stride = (4 >> a.m.gshift) * 8 * a.m.rec;
   t.ring_bytes = kTcCodeBytes + kTcTiles * t.rec_stride;
   const int sh =
-      1024 + kTcSlots * kTcBBytes + kTcOutBytes + kTcRing * t.ring_bytes + 512 + kTcRows * 12;
-  constexpr int kMost = 1024 + kTcSlots * kTcBBytes + kTcOutBytes +
+      1024 + kTcSlots<SWIGLU> * kTcBBytes + kTcRows * kTcOutRow<SWIGLU> + kTcRing * t.ring_bytes + 512 + kTcRows * 12;
+  constexpr int kMost = 1024 + kTcSlots<SWIGLU> * kTcBBytes + kTcRows * kTcOutRow<SWIGLU> +
                         kTcRing * (kTcCodeBytes + kTcTiles * 256) + 512 + kTcRows * 12;
   static_assert(kMost <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> attr{0};
