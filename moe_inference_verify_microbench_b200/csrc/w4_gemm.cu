@@ -369,15 +369,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               for (int i = 0; i < 2; ++i) {
                 if (HALVES || h == 0) {
                   const uint32_t r = rec + (tile0 + i) * args.rec_stride + h * (8 * kRec);
-                  const uint32_t sv = lds32(r);
+                  uint32_t sv, zv = 0;  // scales of rows g, g + 8, and 128 + z
+                  if (ZEROS) lds64(r, sv, zv);
+                  else sv = lds32(r);
                   sc[h][i][0] = __byte_perm(sv, 0, 0x1010);
                   sc[h][i][1] = __byte_perm(sv, 0, 0x3232);
-                  zp[h][i][0] = zp[h][i][1] = 0x43084308u;
-                  if (ZEROS) {
-                    const uint32_t zv = lds32(r + 4);
-                    zp[h][i][0] = __byte_perm(zv, 0, 0x1010);
-                    zp[h][i][1] = __byte_perm(zv, 0, 0x3232);
-                  }
+                  zp[h][i][0] = ZEROS ? __byte_perm(zv, 0, 0x1010) : 0x43084308u;
+                  zp[h][i][1] = ZEROS ? __byte_perm(zv, 0, 0x3232) : 0x43084308u;
                 } else {
 #pragma unroll
                   for (int k = 0; k < 2; ++k) {

@@ -9,6 +9,10 @@ bank holds the three projections in the layout the kernels stream
 tiles of 64-column blocks.  It takes 0.5 byte and the group's share of a scale
 per weight (``3 * H * I * (1/2 + 2/group)`` bytes per expert without zero points).
 
+The kernels multiply activations by 128 + code (or by the rounded weight) and sum in
+fp32, so K * 144 * |x| has to stay below 3.4e38; an infinity or a NaN in a row makes the
+outputs of that row NaN or infinite and no other's.
+
 Build it once when the weights are loaded, from codes (``from_codes``) or from
 bf16 weights (``quantize``); the ops that take it are ``ops.moe_layer_w4``,
 ``ops.experts_w4``, ``ops.grouped_w13_swiglu_w4``, ``ops.grouped_w2_w4`` and
