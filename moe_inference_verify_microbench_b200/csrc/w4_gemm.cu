@@ -9,8 +9,7 @@
 // shared memory, and the accumulators hold D[weight row][record].  So a pass
 // over an expert's weights costs the same integer work for 16 records as for
 // 128: about 60 instructions per 16 x 64 block (28 to extract, 32 to subtract
-// and scale), which together with the stream of codes bounds small N; the
-// tensor pipe bounds N = 128.
+// and scale), which bounds small N.
 //
 // Work unit: (tile-table entry, 16 packed tiles), i.e. 256 weight rows as two
 // operands of 128 that share the records: for the gate/up product the gate rows
@@ -21,16 +20,15 @@
 //   warps 0..15   dequantise: warp w writes lane quarter w % 4 of every fourth
 //                 64-column block
 //   warps 16..19  epilogue: tensor memory -> bf16 -> staging rows -> output rows
-//   warps 20..23  gather the records' rows (a lane copies four of them with one
-//                 tile::gather4, into the 128-byte swizzle; issued from one warp
-//                 the copies of 128 records take 80 cycles each: T = 8192 1578 us
-//                 instead of 863 then)
+//   warps 20..23  gather the records' rows (tile::gather4: four rows a copy, into the
+//                 128-byte swizzle; one warp for all copies of 128 records was the
+//                 bound: 8192 tokens 1578 us instead of 863 then)
 //   warp 24       tiled copies of codes and group records into a ring
 //   warps 25, 26  issue tcgen05.mma, one operand each: 4 steps of 16 columns per
 //                 block; warp 25 allocates tensor memory
 //
 // A weight is rounded once, s * (q - z) to bf16: the operand's type, and what a bf16
-// checkpoint of the same weights would hold.  That is 2^-9 of it at most, like
+// checkpoint of the same weights would hold.  That is 2^-8 of it at most, like
 // the rounding of the activations themselves; the sums stay fp32.  (Exact operands
 // q - z would need the scale on every group's sums: a pass over the accumulators per
 // 128 columns, 256 fp32 sums a thread at 128 records.)
@@ -42,8 +40,9 @@
 // dequantisation, about 30 for all else) and a set of warps waits for its own products
 // before it refills its stage; a third pair of stages was worth 3 %.  Halves of units
 // in a last round that is not half full cost as much as whole ones (shard of 32
-// experts 78 -> 84 us).  At 512 the tiles of 128 records and
-// 256 weight rows move 6.4 TB/s from L2.
+// experts 78 -> 84 us).  At 512 the tiles of 128 records and 256 weight rows move 6.3
+// TB/s from L2, and their products wait for the epilogue before them (5000 of 34000
+// cycles for gate/up), because tensor memory holds 128 records' sums once.
 #include <algorithm>
 
 #include "grouped_gemm.cuh"
