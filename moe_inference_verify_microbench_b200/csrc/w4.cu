@@ -18,8 +18,10 @@
 // through shared memory.
 //
 // Measured back to back, 128 experts of 2048 x 768, top 8, group 128: gate/up 3.5
-// TB/s at 12 tokens (30 us), 3.9 at 64 (52 us); down 2.6 and 3.2 TB/s.  The issue
-// slots are the next bound (66 instructions per 16 x 64 block of codes).
+// TB/s at 12 tokens (30 us), 3.9 at 64 (52 us); down 2.6 and 3.2 TB/s.  The integer
+// pipe is the next bound: it takes the extraction at half rate and is half busy (48 % of
+// the issue slots, 66 instructions per 16 x 64 block); a shift of the seven done by
+// mul.hi instead costs 3 us of 42.
 //
 // Numerics: products of activations with (q - z) are exact in fp32; each
 // group (or a warp's share of it) is summed on the tensor cores in fp32 and
