@@ -14,19 +14,23 @@ accumulation per token, fused into the down GEMM).  With the keyword extra
 word; by default the forward never synchronises and a failure is only
 recorded there (``ops.check_status`` reads it).  With the keyword extra
 ``decode_weights=True`` the module also keeps the down weights transposed
-(one more copy of ``w_down``; ``down_weights_transposed(refresh=True)``
-rebuilds it after the per-expert weights were written) and runs batches of
-up to 4 tokens on the one-pass decode layer.  With the keyword extra
+(one more copy of ``w_down``) and runs batches of up to 4 tokens on the
+one-pass decode layer.  With the keyword extra
 ``expert_weights="w4"`` the forward runs on a 4-bit copy of the expert weights
 (``ops.moe_layer_w4``; groups of ``group_size`` columns, with zero points unless
-``symmetric``), rounded on first use and again when a stacked weight is re-bound
-or written in place; ``experts_4bit(refresh=True)`` rebuilds it after the
-per-expert weights were written.
+``symmetric``), rounded on first use.  Both copies are made again by the next
+forward after the weights were written: through the stacked tensors, through an
+expert's parameters (``load_state_dict``, an optimizer's step) or by re-binding.
+Only writes that autograd's version counters do not see (through ``.data``, or
+by a kernel on the raw pointer) need ``down_weights_transposed(refresh=True)``
+or ``experts_4bit(refresh=True)``.
 
 The module must be bf16 on a CUDA device: there is no CPU path.
 """
 
 from __future__ import annotations
+
+import operator
 
 import torch
 from torch import nn
@@ -36,6 +40,28 @@ from .experts import ExpertBank, SwiGLU_MLP, router_bias_of
 from .w4 import GROUPS, W4Experts
 
 __all__ = ["PermutedSparseMoE", "SwiGLU_MLP"]
+
+_version_of = operator.attrgetter("_version")
+
+
+class _Source:
+    """The weights that a copy in another form was made from, as they were then: the
+    stacked tensors themselves (held, so that no later stack lies in their place and
+    passes for them) and how often these and the experts' parameters had been written.
+    The parameters are views of the stacks with version counters of their own, which
+    only grow, so the sum stays the same only if none was written.  Reading the 384
+    counters of 128 experts takes the host 22 us."""
+
+    def __init__(self, stacks, params) -> None:
+        self.stacks = tuple(stacks)
+        self._written = self.stacks + tuple(params)
+        self._writes = self._count()
+
+    def _count(self) -> int:
+        return sum(map(_version_of, self._written))
+
+    def unchanged(self, stacks) -> bool:
+        return all(map(operator.is_, self.stacks, stacks)) and self._count() == self._writes
 
 
 class PermutedSparseMoE(nn.Module):
@@ -61,12 +87,12 @@ class PermutedSparseMoE(nn.Module):
         self.group_size = group_size
         self.symmetric = symmetric
         self._w4 = None
-        self._w4_key = None
+        self._w4_source = None
         self.index_add = index_add
         self.check_errors = check_errors
         self.decode_weights = decode_weights
         self._w_down_t = None
-        self._w_down_t_key = None
+        self._w_down_t_source = None
         self.hidden = hidden
         self.intermediate = intermediate
         self.num_experts = num_experts
@@ -78,8 +104,8 @@ class PermutedSparseMoE(nn.Module):
 
     def _apply(self, fn, *args, **kwargs):
         self._bank.invalidate()
-        self._w_down_t = None
-        self._w4 = None
+        self._w_down_t = self._w_down_t_source = None
+        self._w4 = self._w4_source = None
         return super()._apply(fn, *args, **kwargs)
 
     def pack(self):
@@ -89,15 +115,15 @@ class PermutedSparseMoE(nn.Module):
 
     def down_weights_transposed(self, refresh: bool = False) -> torch.Tensor:
         """w_down as [E, I, H] for the one-pass decode layer: built on first
-        use and rebuilt when the stacked down weights are re-bound or written
-        in place through the stacked tensor.  Writes through the per-expert
-        parameters (``experts[e].down_proj.weight``) do not reach the stacked
-        tensor's version counter: call with ``refresh=True`` after those."""
+        use and rebuilt when the down weights are re-bound or written in place,
+        through the stacked tensor or an expert's parameter.  Writes through
+        ``experts[e].down_proj.weight.data`` leave no trace: call with
+        ``refresh=True`` after those."""
         wd = self.pack()[2]
-        key = (wd.data_ptr(), wd._version)
-        if refresh or self._w_down_t is None or self._w_down_t_key != key:
+        if refresh or self._w_down_t is None or not self._w_down_t_source.unchanged((wd,)):
+            source = _Source((wd,), (ex.down_proj.weight for ex in self.experts))
             self._w_down_t = ops.transpose_down_weights(wd)
-            self._w_down_t_key = key
+            self._w_down_t_source = source
         return self._w_down_t
 
     def experts_4bit(self, refresh: bool = False) -> W4Experts:
@@ -105,10 +131,10 @@ class PermutedSparseMoE(nn.Module):
         ``down_weights_transposed``, for all three projections.  Building it
         synchronises, so call this (or the module) once before a graph capture."""
         weights = self.pack()
-        key = tuple((w.data_ptr(), w._version) for w in weights)
-        if refresh or self._w4 is None or self._w4_key != key:
+        if refresh or self._w4 is None or not self._w4_source.unchanged(weights):
+            source = _Source(weights, self.experts.parameters())
             self._w4 = W4Experts.quantize(*weights, self.group_size, self.symmetric)
-            self._w4_key = key
+            self._w4_source = source
         return self._w4
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
