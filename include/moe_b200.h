@@ -442,8 +442,10 @@ MOE_API int moe_w4_experts_forward(const void* x, const int32_t* ids, const floa
 /*
  * The 4-bit experts for rows that are sorted by expert already: rows
  * offsets[e] .. offsets[e + 1] of sorted_x [M, H] (int64 offsets [E + 1], on the
- * device) through expert e, unweighted, in sorted order; rows from offsets[E] on
- * are zero (C9/python/solution.py:207-222).
+ * device) through expert e, unweighted, in sorted order; rows before offsets[0]
+ * and from offsets[E] on are zero (C9/python/solution.py:207-222).  Offsets that
+ * do not ascend, or leave 0 .. M, are reported (MOE_ERR_BAD_ROW), and all of y is
+ * zero then.
  */
 MOE_API size_t moe_w4_sorted_workspace_bytes(int M, const moe_w4_bank* bank);
 MOE_API int moe_w4_sorted_forward(const void* sorted_x, int M, const int64_t* offsets,

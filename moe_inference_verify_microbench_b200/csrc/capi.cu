@@ -166,7 +166,7 @@ int w4_products(const W4Bank& b, const W4Layout& l, const void* x, const int* id
   if (avg < kW4TcRecords && R < kW4WideRecords) {
     float* slots = static_cast<float*>(l.slots);
     rc = launch_w4_w2(b, l.h, R, l.tiles, l.num_tiles, l.max_tiles, l.perm, w, nullptr, R, avg,
-                      status, stream, nullptr, slots);
+                      status, stream, false, slots);
     if (rc != kRcOk) return rc;
     return launch_combine_f32(slots, ids, e_begin, e_begin + b.E, T, k, b.H, y, stream);
   }
@@ -664,14 +664,14 @@ int moe_w4_sorted_forward(const void* sorted_x, int M, const int64_t* offsets,
   if (workspace_bytes < l.bytes) return kRcWorkspace;
   const long long* off = reinterpret_cast<const long long*>(offsets);
   rc = launch_tiles_from_offsets(off, b.E, MOE_BLOCK_M, l.tiles, l.max_tiles, l.num_tiles, status,
-                                 stream);
+                                 stream, M);
   if (rc != kRcOk) return rc;
   const int avg = M / b.E;
   rc = launch_w4_w13(b, sorted_x, M, nullptr, 1, M, l.tiles, l.num_tiles, l.max_tiles, l.h, avg,
                      status, stream);
   if (rc != kRcOk) return rc;
   return launch_w4_w2(b, l.h, M, l.tiles, l.num_tiles, l.max_tiles, nullptr, nullptr, y, M, avg,
-                      status, stream, off + b.E);
+                      status, stream, true);
 }
 
 size_t moe_w4_layer_workspace_bytes(int T, int top_k, const moe_w4_bank* bank) {

@@ -58,8 +58,11 @@ int launch_sort_align(const int* ids, int R, int E, int e_begin, int E_local, in
                       void* workspace, int* counts, int* offsets, long long* offsets64, int* perm,
                       int* inv, int4* tiles, int max_tiles, int* num_tiles, int* status,
                       cudaStream_t stream);
+// row_limit >= 0: offsets that do not ascend from 0 on to at most row_limit leave the table
+// empty (and are reported); < 0: an expert whose two offsets are bad is left out.
 int launch_tiles_from_offsets(const long long* offsets, int E, int block_m, int4* tiles,
-                              int max_tiles, int* num_tiles, int* status, cudaStream_t stream);
+                              int max_tiles, int* num_tiles, int* status, cudaStream_t stream,
+                              long long row_limit = -1);
 
 int launch_gather_rows(const void* src, int src_rows, const int* idx, int R, const int* count,
                        int idx_div, int H, void* dst, int* status, cudaStream_t stream);
@@ -199,14 +202,15 @@ int launch_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* ze
                    const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E, int N,
                    int K, int group, void* q, void* s, int* status, cudaStream_t stream);
 // avg: records per expert to expect; it chooses the kernel and changes no result
-// beyond rounding.  tail (device, optional): output rows from *tail on are zeroed.
+// beyond rounding.  zero_rest: output rows of no tile are zeroed; the table's row ranges
+// follow one another then.
 int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* index,
                   int index_div, int M, const int4* tiles, const int* num_tiles, int max_tiles,
                   void* h_out, int avg, int* status, cudaStream_t stream);
 int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
                  int max_tiles, const int* row_map, const float* row_scale, void* out,
                  int out_rows, int avg, int* status, cudaStream_t stream,
-                 const long long* tail = nullptr, float* out_f32 = nullptr);
+                 bool zero_rest = false, float* out_f32 = nullptr);
 
 // The whole layer for a few tokens (w4_decode.cu; T <= 16, T * k <= 64): `scratch`
 // holds w4_decode_scratch_bytes(b, T) bytes, h [T * k, I] bf16.

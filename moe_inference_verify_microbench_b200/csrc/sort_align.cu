@@ -261,22 +261,25 @@ __global__ void __launch_bounds__(1024) tiles_from_offsets(const long long* __re
                                                            int E, int block_m,
                                                            int4* __restrict__ tiles, int max_tiles,
                                                            int* __restrict__ num_tiles,
-                                                           int* status) {
+                                                           long long row_limit, int* status) {
   pdl_wait();
   pdl_trigger();
   __shared__ int warp_sums[32];
   __shared__ int total;
   const int e = threadIdx.x;
   int count = 0, off = 0;
+  bool bad = false;
   if (e < E) {
     const long long a = offsets[e], b = offsets[e + 1];
-    if (a < 0 || b < a || b > 0x7fffffffLL) {
+    bad = a < 0 || b < a || b > (row_limit >= 0 ? row_limit : 0x7fffffffLL);
+    if (bad) {
       record_status(status, kErrBadRow);
     } else {
       off = static_cast<int>(a);
       count = static_cast<int>(b - a);
     }
   }
+  if (row_limit >= 0 && __syncthreads_or(bad)) count = 0;
   write_tiles(e, E, count, off, block_m, tiles, max_tiles, num_tiles, warp_sums, &total);
 }
 
@@ -329,11 +332,12 @@ int launch_sort_align(const int* ids, int R, int E, int e_begin, int E_local, in
 }
 
 int launch_tiles_from_offsets(const long long* offsets, int E, int block_m, int4* tiles,
-                              int max_tiles, int* num_tiles, int* status, cudaStream_t stream) {
+                              int max_tiles, int* num_tiles, int* status, cudaStream_t stream,
+                              long long row_limit) {
   if (E <= 0 || E > 1024 || block_m <= 0) return kRcBadArgument;
   const int threads = ((E + 31) / 32) * 32;
   const cudaError_t e = launch_pdl(tiles_from_offsets, dim3(1), dim3(threads), 0, stream, offsets,
-                                   E, block_m, tiles, max_tiles, num_tiles, status);
+                                   E, block_m, tiles, max_tiles, num_tiles, row_limit, status);
   return e == cudaSuccess ? kRcOk : kRcCudaError;
 }
 

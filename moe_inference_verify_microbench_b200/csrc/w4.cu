@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_stream(const W4Args a) {
   const int nt = max(0, min(*a.num_tiles, a.max_tiles));
   W4TableWalk walk;
   walk.open_range(a, nt);
-  if constexpr (!SWIGLU) w4_zero_tail(a, threadIdx.x, kW4Threads);
+  if constexpr (!SWIGLU) w4_zero_rest(a, nt, threadIdx.x, kW4Threads);
   w4_units<SWIGLU, KB, MODE>(a, smem_raw + kW4PartBytes, reinterpret_cast<float*>(smem_raw), walk);
 }
 
@@ -213,14 +213,14 @@ int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* 
 int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
                  int max_tiles, const int* row_map, const float* row_scale, void* out,
                  int out_rows, int avg, int* status, cudaStream_t stream,
-                 const long long* tail, float* out_f32) {
+                 bool zero_rest, float* out_f32) {
   if (const int rc = w4_check_bank(bank); rc != kRcOk) return rc;
   if (M < 0 || max_tiles < 0 || out_rows < 0 || tiles == nullptr || num_tiles == nullptr)
     return kRcBadArgument;
   if (M == 0 || max_tiles == 0) return kRcOk;
   if (h == nullptr || (out == nullptr) == (out_f32 == nullptr) || !aligned16(h) ||
       !aligned16(out) || !aligned16(tiles) ||
-      (out_f32 != nullptr && (tail != nullptr || avg >= kW4TcRecords)))
+      (out_f32 != nullptr && (zero_rest || avg >= kW4TcRecords)))
     return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, true);
@@ -238,7 +238,7 @@ int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, co
   a.out_rows = out_rows;
   a.row_map = row_map;
   a.row_scale = row_scale;
-  a.tail = tail;
+  a.zero_rest = zero_rest;
   a.avg = avg;
   a.status = status;
   return w4_dispatch<false>(a, stream);

@@ -100,7 +100,7 @@ struct W4Args {
   int out_rows;
   const int* row_map;
   const float* row_scale;
-  const long long* tail;  // rows of out from *tail on are zeroed (null: none)
+  bool zero_rest;       // rows of out before the first entry and after the last are zeroed
   int avg;              // records per expert to expect (chooses the kernel)
   int* status;
 };
@@ -139,12 +139,16 @@ __device__ __forceinline__ bool w4_entry_ok(const W4Args& a, const int4& t) {
   return false;
 }
 
-// Zeroes the output rows from *a.tail on, with `count` threads of every CTA.
-__device__ __forceinline__ void w4_zero_tail(const W4Args& a, int thread, int count) {
-  if (a.tail == nullptr) return;
-  const long long first = max(0ll, min(*a.tail, static_cast<long long>(a.out_rows)));
+// Zeroes the output rows before the first of nt entries and after the last (all rows,
+// where there are none), with `count` threads of every CTA.
+__device__ __forceinline__ void w4_zero_rest(const W4Args& a, int nt, int thread, int count) {
+  if (!a.zero_rest) return;
+  const int first = nt > 0 ? max(0, min(a.tiles[0].y, a.out_rows)) : a.out_rows;
+  const int last = nt > 0 ? max(first, a.tiles[nt - 1].z) : a.out_rows;
   const int vec = a.out_ld / 8;
-  for (long long r = first + blockIdx.x; r < a.out_rows; r += gridDim.x) {
+  for (long long i = blockIdx.x;; i += gridDim.x) {
+    const long long r = i < first ? i : last + (i - first);
+    if (r >= a.out_rows) break;
     uint4* row = reinterpret_cast<uint4*>(a.out + static_cast<size_t>(r) * a.out_ld);
     for (int v = thread; v < vec; v += count) row[v] = make_uint4(0, 0, 0, 0);
   }

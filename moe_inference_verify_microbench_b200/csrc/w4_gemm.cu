@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
     const uint32_t stage = smem_u32(sOut);
     int* rows = s_row;
-    if constexpr (!SWIGLU) w4_zero_tail(a, r, 128);
+    if constexpr (!SWIGLU) w4_zero_rest(a, nt, r, 128);
     TcAcc acc;
     bool ok = true;
     for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {

@@ -37,6 +37,6 @@ def fused_moe_forward(sorted_x: torch.Tensor, offsets: torch.Tensor, W_gate: tor
 def fused_moe_forward_w4(sorted_x: torch.Tensor, offsets: torch.Tensor, bank) -> torch.Tensor:
     """``fused_moe_forward`` on a 4-bit bank (``W4Experts``): rows
     ``offsets[e]:offsets[e+1]`` of ``sorted_x`` through expert e, unweighted, in
-    sorted order; rows past ``offsets[E]`` are zero."""
+    sorted order; rows before ``offsets[0]`` and from ``offsets[E]`` on are zero."""
     off = offsets.to(device=sorted_x.device, dtype=torch.int64).contiguous()
     return ops.sorted_experts_w4(sorted_x.contiguous(), off, bank)

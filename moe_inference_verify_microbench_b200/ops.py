@@ -778,7 +778,9 @@ def sorted_experts_w4(sorted_x: torch.Tensor, offsets: torch.Tensor, bank,
                       workspace: torch.Tensor | None = None) -> torch.Tensor:
     """The 4-bit experts for rows sorted by expert (C9/python/solution.py:207-222):
     rows ``offsets[e]:offsets[e+1]`` (int64 [E+1]) through expert e, unweighted, in
-    sorted order; rows past ``offsets[E]`` are zero.  One C-ABI call."""
+    sorted order; rows before ``offsets[0]`` and from ``offsets[E]`` on are zero.  Offsets
+    that do not ascend, or leave ``0..M``, are reported in the status word, and the whole
+    output is zero then.  One C-ABI call."""
     _need(sorted_x, "sorted_x", torch.bfloat16, 2)
     dev = sorted_x.device
     M, H = sorted_x.shape

@@ -6,8 +6,8 @@ import pytest
 import torch
 
 import w4_reference as ref
-from moe_inference_verify_microbench_b200 import PermutedSparseMoE, ops, quantize_w4
-from test_gpu_w4 import close, rms_close, rows
+from moe_inference_verify_microbench_b200 import PermutedSparseMoE, fused_moe_forward_w4, ops, quantize_w4
+from test_gpu_w4 import bank_of, close, rms_close, rows
 from test_gpu_w4_layers import module
 
 pytestmark = pytest.mark.gpu
@@ -49,3 +49,42 @@ def test_decode_weights_after_load_state_dict(cuda):
         mod.load_state_dict(other.state_dict())
         assert torch.equal(mod(x), other(x))
     ops.check_status(cuda)
+
+
+# ------------------------------------------------------------------ rows of no expert
+
+
+@pytest.mark.parametrize("counts", [[0, 3, 1, 9], [128, 0, 60, 129], [0, 0, 0, 0]])
+@pytest.mark.parametrize("lead,extra", [(1, 0), (5, 2), (300, 0), (130, 170)])
+def test_rows_before_the_first_expert(cuda, counts, lead, extra):
+    """Offsets that start above 0: the rows before them are zero, as those past the last
+    are, whatever stood in the output (both forms of the product)."""
+    E, H, I = 4, 256, 192
+    p = ref.parts(E, H, I, 64, True, device=cuda)
+    bank = bank_of(p)
+    off = (torch.tensor([0] + counts).cumsum(0) + lead).to(cuda)
+    M = int(off[-1]) + extra
+    x = rows(M, H, 3, cuda)
+    out = torch.full((M, H), 7.0, dtype=torch.bfloat16, device=cuda)
+    y = ops.sorted_experts_w4(x, off, bank, out=out)
+    ops.check_status(cuda)
+    assert not bool(y[:lead].any()) and not bool(y[int(off[-1]):].any())
+    owner = torch.full((M, 1), -1, device=cuda)
+    owner[lead:int(off[-1]), 0] = torch.repeat_interleave(torch.arange(E, device=cuda), off.diff())
+    want, bound = ref.experts(p, x, owner, torch.ones((M, 1), device=cuda))
+    close(y, want, bound)
+    assert torch.equal(y, fused_moe_forward_w4(x, off, bank))
+
+
+@pytest.mark.parametrize("M", [12, 400])
+@pytest.mark.parametrize("offsets", [[0, 5, 3, 9, 10], [-2, 0, 3, 6, 10], [0, 3, 6, 8, "M+1"],
+                                     [4, 3, 2, 1, 0], [0, 5, 5, 1 << 40, 1 << 41]])
+def test_bad_offsets_are_reported_and_give_zeros(cuda, M, offsets):
+    E, H, I = 4, 256, 192
+    bank = bank_of(ref.parts(E, H, I, 64, False, device=cuda))
+    off = torch.tensor([M + 1 if o == "M+1" else o for o in offsets], device=cuda)
+    out = torch.full((M, H), 7.0, dtype=torch.bfloat16, device=cuda)
+    ops.sorted_experts_w4(rows(M, H, 3, cuda), off, bank, out=out)
+    with pytest.raises(ops.MoEKernelError, match="row index"):
+        ops.check_status(cuda)
+    assert not bool(out.any())
