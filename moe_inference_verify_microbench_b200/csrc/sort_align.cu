@@ -271,7 +271,10 @@ __global__ void __launch_bounds__(1024) tiles_from_offsets(const long long* __re
   bool bad = false;
   if (e < E) {
     const long long a = offsets[e], b = offsets[e + 1];
-    bad = a < 0 || b < a || b > (row_limit >= 0 ? row_limit : 0x7fffffffLL);
+    // an expert of more rows than the table holds is none either: its tiles would
+    // overrun 32-bit positions
+    bad = a < 0 || b < a || b > (row_limit >= 0 ? row_limit : 0x7fffffffLL) ||
+          b - a > static_cast<long long>(max_tiles) * block_m;
     if (bad) {
       record_status(status, kErrBadRow);
     } else {

@@ -53,18 +53,18 @@ __device__ __forceinline__ int block_exclusive_scan(int v, int* warp_sums, int* 
 // Tile table from per-expert counts held by threads e < E (E <= blockDim.x).
 __device__ __forceinline__ void write_tiles(int e, int E, int count, int offset, int block_m, int4* tiles,
                             int max_tiles, int* num_tiles, int* warp_sums, int* total) {
-  const int nt = (e < E) ? (count + block_m - 1) / block_m : 0;
+  const int nt = e < E && count > 0 ? (count - 1) / block_m + 1 : 0;
   const int first = block_exclusive_scan(nt, warp_sums, total);
   if (e < E) {
     for (int t = 0; t < nt; ++t) {
       const int slot = first + t;
-      if (slot < max_tiles) {
+      if (static_cast<unsigned>(slot) < static_cast<unsigned>(max_tiles)) {
         const int r0 = offset + t * block_m;
         tiles[slot] = make_int4(e, r0, min(offset + count, r0 + block_m), 0);
       }
     }
   }
-  if (threadIdx.x == 0) *num_tiles = min(*total, max_tiles);
+  if (threadIdx.x == 0) *num_tiles = max(0, min(*total, max_tiles));
 }
 
 // One-CTA sort for R <= kSortChunk and E_local <= kSortThreads (decode

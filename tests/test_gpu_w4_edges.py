@@ -88,3 +88,29 @@ def test_bad_offsets_are_reported_and_give_zeros(cuda, M, offsets):
     with pytest.raises(ops.MoEKernelError, match="row index"):
         ops.check_status(cuda)
     assert not bool(out.any())
+
+
+@pytest.mark.parametrize("M,offsets,want", [
+    (200, [0, 2 ** 31 - 1, 0, 100], [[2, 0, 100]]),
+    (200, [0, 100, 2 ** 31 - 1, 50, 179], [[0, 0, 100], [3, 50, 178], [3, 178, 179]]),
+    (0, [0, 7, 7, 7], [[0, 0, 7]]),
+    (100, [0, 2 ** 31 - 1] + [0, 2 ** 31 - 1] * 300, [])])
+def test_tile_table_of_experts_with_too_many_rows(cuda, M, offsets, want):
+    """An expert with more rows than the table has room for is left out and reported; the
+    entries of the others stand at their places in the table, and nothing around it changes."""
+    E = len(offsets) - 1
+    lib = ops._native.load()
+    mt = int(lib.moe_max_tiles(M, E))
+    mem = torch.full((mt + 64, 4), -7, dtype=torch.int32, device=cuda)
+    num = torch.full((1,), -7, dtype=torch.int32, device=cuda)
+    off = torch.tensor(offsets, device=cuda)
+    tiles = mem[32:]
+    rc = lib.moe_tiles_from_offsets(ops._p(off), E, ops._p(tiles), mt, ops._p(num),
+                                    ops._p(ops.status_word(cuda)), ops._stream(cuda))
+    assert rc == 0
+    if len(want) < E and M:
+        with pytest.raises(ops.MoEKernelError, match="row index"):
+            ops.check_status(cuda)
+    n = int(num)
+    assert tiles[:n, :3].tolist() == want
+    assert bool((mem[:32] == -7).all()) and bool((tiles[n:] == -7).all())
