@@ -343,12 +343,14 @@ __device__ __forceinline__ float cta_sum(float v, float* sh) {
 
 constexpr int kBlockNormMaxH = 4 * 8 * 1024;
 
-// Read once: past L1.
+// Read once: past L1, and coherent, because h may be written over x and y over delta
+// (a .nc load may only read what nothing writes while the kernel runs).
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+               : "l"(p)
+               : "memory");
   return v;
 }
 

@@ -114,3 +114,42 @@ def test_tile_table_of_experts_with_too_many_rows(cuda, M, offsets, want):
     n = int(num)
     assert tiles[:n, :3].tolist() == want
     assert bool((mem[:32] == -7).all()) and bool((tiles[n:] == -7).all())
+
+
+# ------------------------------------------------------------------ block norm
+
+
+def norm_call(x, delta, post, pre, gate, kind, h, y, scale=0.7, act=2):
+    """The C entry point with outputs of the caller's choice."""
+    p = ops._p
+    T, H = x.shape
+    rc = ops._native.load().moe_block_norm(
+        p(x), p(delta), p(post), p(pre), p(gate), kind, int(gate.dtype is torch.float32), act,
+        scale, T, H, 1e-6, p(h), p(y), ops._stream(x.device))
+    assert rc == 0
+
+
+# rows whose ends share cache lines (264, 1032) and whole ones; a CTA for a row with 1, 2 and
+# 4 vectors a thread, and rows streamed through shared memory with every number of them
+@pytest.mark.parametrize("T,H", [(3, 264), (700, 264), (1500, 2056), (1100, 8192), (5, 16392),
+                                 (8200, 1032), (2100, 4104), (2100, 5120), (2100, 8192)])
+@pytest.mark.parametrize("kind", [2, 3])
+def test_block_norm_in_place(cuda, T, H, kind):
+    """h written over x and y over delta, either or both: the same as into memory of their
+    own, in every form of the kernel."""
+    gen = torch.Generator().manual_seed(T + H)
+    x = (torch.randn((T, H), generator=gen) * 2).bfloat16().to(cuda)
+    d = (torch.randn((T, H), generator=gen) * 0.5).bfloat16().to(cuda)
+    post, pre = ((torch.randn(H, generator=gen) * 0.2 + 1).to(cuda) for _ in range(2))
+    g = torch.randn((T, H) if kind == 3 else (H,), generator=gen).bfloat16().to(cuda)
+    h, y = torch.empty_like(x), torch.empty_like(x)
+    norm_call(x, d, post, pre, g, kind, h, y)
+    wh, wy, bh, by = ref.block_norm(x, d, post, pre, 1e-6, g, "tanh", 0.7)
+    close(h, wh, bh, "h")
+    close(y, wy, by, "y")
+    for over_x, over_d in ((True, False), (False, True), (True, True)):
+        a, b = x.clone(), d.clone()
+        h2 = a if over_x else torch.empty_like(x)
+        y2 = b if over_d else torch.empty_like(x)
+        norm_call(a, b, post, pre, g, kind, h2, y2)
+        assert torch.equal(h2, h) and torch.equal(y2, y), (over_x, over_d)
