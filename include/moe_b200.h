@@ -56,6 +56,7 @@ extern "C" {
 #define MOE_ERR_TIMEOUT_ACC_EMPTY 0x104
 #define MOE_ERR_PEER_TIMEOUT 0x105
 #define MOE_ERR_TIMEOUT_GRID 0x106
+#define MOE_ERR_TIMEOUT_ROWS 0x107
 #define MOE_ERR_BAD_EXPERT 0x201
 #define MOE_ERR_BAD_ROW 0x202
 #define MOE_ERR_BAD_CODE 0x203
@@ -374,6 +375,13 @@ MOE_API int moe_block_norm(const void* x, const void* delta, const float* post_w
                            const float* pre_weight, const void* gate, int gate_kind, int gate_f32,
                            int gate_act, float residual_scale, int T, int H, float eps,
                            void* h_out, void* y, cudaStream_t stream);
+/* The same with a status word (may be NULL): a bounded wait for rows that ran out records
+ * MOE_ERR_TIMEOUT_ROWS, and no row is written from what had not arrived. */
+MOE_API int moe_block_norm_ex(const void* x, const void* delta, const float* post_weight,
+                              const float* pre_weight, const void* gate, int gate_kind,
+                              int gate_f32, int gate_act, float residual_scale, int T, int H,
+                              float eps, void* h_out, void* y, int32_t* status,
+                              cudaStream_t stream);
 
 /*
  * Expert weights in 4 bits.  Every row of a projection is cut into groups of

@@ -98,6 +98,9 @@ SIGNATURES: dict[str, tuple] = {
     "moe_block_norm": (_c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int,
                                 ctypes.c_float, _c_int, _c_int, ctypes.c_float, _ptr, _ptr,
                                 _ptr]),
+    "moe_block_norm_ex": (_c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int,
+                                   ctypes.c_float, _c_int, _c_int, ctypes.c_float, _ptr, _ptr,
+                                   _ptr, _ptr]),
     "moe_w4_pack": (_c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int,
                              _ptr, _ptr, _ptr, _ptr]),
     "moe_grouped_w13_swiglu_w4": (_c_int, [_ptr, _c_int, _ptr, _c_int, _c_int, _ptr, _ptr, _c_int,

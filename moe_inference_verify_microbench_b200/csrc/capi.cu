@@ -197,6 +197,7 @@ const char* moe_error_string(int code) {
     case kErrTimeoutAccEmpty: return "device: MMA warp timed out waiting for the epilogue";
     case kErrPeerTimeout: return "device: timed out waiting for a peer rank of the expert-parallel group";
     case kErrTimeoutGrid: return "device: timed out in a grid-wide barrier of the single-launch decode layer";
+    case kErrTimeoutRows: return "device: timed out waiting for rows of the block norm";
     case kErrBadExpert: return "device: expert id out of range";
     case kErrBadRow: return "device: row index out of range";
     case kErrBadCode: return "device: 4-bit weight code or zero point above 15";
@@ -401,10 +402,10 @@ int moe_add_rmsnorm(const void* x, const void* delta, const float* weight, int T
   return launch_add_rmsnorm(x, delta, weight, T, H, eps, h_out, y, stream);
 }
 
-int moe_block_norm(const void* x, const void* delta, const float* post_weight,
-                   const float* pre_weight, const void* gate, int gate_kind, int gate_f32,
-                   int gate_act, float residual_scale, int T, int H, float eps, void* h_out,
-                   void* y, cudaStream_t stream) {
+int moe_block_norm_ex(const void* x, const void* delta, const float* post_weight,
+                      const float* pre_weight, const void* gate, int gate_kind, int gate_f32,
+                      int gate_act, float residual_scale, int T, int H, float eps, void* h_out,
+                      void* y, int32_t* status, cudaStream_t stream) {
   if (gate_kind < MOE_GATE_NONE || gate_kind > MOE_GATE_ELEMENT ||
       (gate_kind != MOE_GATE_NONE && T > 0 && gate == nullptr))
     return kRcBadArgument;
@@ -424,7 +425,16 @@ int moe_block_norm(const void* x, const void* delta, const float* post_weight,
   a.scale = residual_scale;
   a.h = h_out;
   a.y = y;
+  a.status = status;
   return launch_block_norm(a, stream);
+}
+
+int moe_block_norm(const void* x, const void* delta, const float* post_weight,
+                   const float* pre_weight, const void* gate, int gate_kind, int gate_f32,
+                   int gate_act, float residual_scale, int T, int H, float eps, void* h_out,
+                   void* y, cudaStream_t stream) {
+  return moe_block_norm_ex(x, delta, post_weight, pre_weight, gate, gate_kind, gate_f32, gate_act,
+                           residual_scale, T, H, eps, h_out, y, nullptr, stream);
 }
 
 int moe_cast_f32_to_bf16(const float* src, long long n, void* y, cudaStream_t stream) {

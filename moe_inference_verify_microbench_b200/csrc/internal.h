@@ -230,6 +230,7 @@ struct BlockNormArgs {
   int T, H;
   float eps, scale;
   void *h, *y;
+  int* status;  // may be null
 };
 int launch_block_norm(const BlockNormArgs& a, cudaStream_t stream);
 // Block glue: h = delta ? bf16(x + delta) : x; y = bf16(h * rsqrt(mean(h^2) + eps) * w).

@@ -23,6 +23,7 @@ enum StatusCode : int {
   kErrTimeoutAccEmpty = 0x104, // MMA warp: accumulator never drained
   kErrPeerTimeout = 0x105,     // expert-parallel exchange: a peer rank never signalled
   kErrTimeoutGrid = 0x106,     // a grid-wide barrier of a single-launch layer never completed
+  kErrTimeoutRows = 0x107,     // rows that a streaming row kernel asked for never arrived
   kErrBadExpert = 0x201,       // an expert id outside [0, E)
   kErrBadRow = 0x202,          // a tile row range outside the A operand
   kErrBadCode = 0x203,         // a 4-bit weight code or zero point above 15

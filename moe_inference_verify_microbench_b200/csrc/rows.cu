@@ -455,6 +455,15 @@ constexpr int norm_ring_bytes() {
 }
 constexpr int kNormMaxStages = 8;
 
+// Whether a stage's copies have landed, within the limit of every wait.
+__device__ __forceinline__ bool norm_rows_wait(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > kWaitLimitNs) return false;
+  return true;
+}
+
 template <int VPT, int ACT>
 __global__ void __launch_bounds__(kNormThreads, norm_ctas<VPT>())
     block_norm_stream(const BlockNormArgs a,
@@ -521,11 +530,7 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<VPT>())
       token_gate = gate_act<ACT>(
           a.gate_f32 ? static_cast<const float*>(a.gate)[row]
                      : __bfloat162float(static_cast<const __nv_bfloat16*>(a.gate)[row]));
-    if (!mbar_try_wait(&full[s], ph)) {
-      const unsigned long long t0 = globaltimer_ns();
-      while (!mbar_try_wait(&full[s], ph) && globaltimer_ns() - t0 < kWaitLimitNs) {
-      }
-    }
+    const bool late = !norm_rows_wait(&full[s], ph);
     const uint4* sx = reinterpret_cast<const uint4*>(ring + s * stage_bytes);
     const uint4* sd = sx + vec;
     float h[VPT][8], d[VPT][8];
@@ -542,7 +547,19 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<VPT>())
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (lane == 0) sh[0][warp] = ss;
-    __syncthreads();  // also: every thread has left the previous row's stage
+    // also: every thread has left the previous row's stage
+    if (__syncthreads_or(late)) {
+      // Nothing more is stored or asked for; what is on its way lands before the CTA
+      // exits: the stages from s on, without the one before s, which waits for its refill.
+      if (tid == 0) {
+        record_status(a.status, kErrTimeoutRows);
+        for (int j = 0; j < (row == blockIdx.x ? stages : stages - 1); ++j) {
+          if (row + static_cast<long long>(j) * grid >= a.T) break;
+          norm_rows_wait(&full[(s + j) % stages], s + j < stages ? ph : ph ^ 1u);
+        }
+      }
+      return;
+    }
     if (tid == 0 && refill >= 0) {
       fence_proxy_async_smem();
       fetch(static_cast<int>(refill), s == 0 ? stages - 1 : s - 1);

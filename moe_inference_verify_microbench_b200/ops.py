@@ -476,9 +476,10 @@ def block_norm(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor,
         raise ValueError(f"delta must be on {dev}, got {delta.device}")
     h, y = torch.empty_like(x), torch.empty_like(x)
     with _on(dev):
-        rc = _native_lib().moe_block_norm(x.data_ptr(), delta.data_ptr(), post.data_ptr(),
-                                          pre.data_ptr(), g_ptr, kind, g_f32, act, residual_scale,
-                                          T, H, eps, h.data_ptr(), y.data_ptr(), _raw_stream(dev))
+        rc = _native_lib().moe_block_norm_ex(
+            x.data_ptr(), delta.data_ptr(), post.data_ptr(), pre.data_ptr(), g_ptr, kind, g_f32,
+            act, residual_scale, T, H, eps, h.data_ptr(), y.data_ptr(),
+            status_word(dev).data_ptr(), _raw_stream(dev))
     if rc:
         _rc(rc, "moe_block_norm")
     return h, y

@@ -153,3 +153,24 @@ def test_block_norm_in_place(cuda, T, H, kind):
         y2 = b if over_d else torch.empty_like(x)
         norm_call(a, b, post, pre, g, kind, h2, y2)
         assert torch.equal(h2, h) and torch.equal(y2, y), (over_x, over_d)
+
+
+@pytest.mark.parametrize("T", [1, 8192])
+def test_block_norm_is_given_the_status_word(cuda, T, monkeypatch):
+    """A wait that runs out in it is reported where ``check_status`` reads it."""
+    seen = []
+    lib = ops._native_lib()
+
+    class Spy:
+        def __getattr__(self, name):
+            def call(*args):
+                seen.append((name, args))
+                return getattr(lib, name)(*args)
+            return call
+
+    monkeypatch.setattr(ops, "_lib", Spy())
+    x, one = rows(T, 2048, 1, cuda), torch.ones(2048, device=cuda)
+    ops.block_norm(x, x, one, one, 1e-6)
+    (name, args), = seen
+    assert name == "moe_block_norm_ex" and args[-2] == ops.status_word(cuda).data_ptr()
+    assert "rows of the block norm" in ops._native.error_string(0x107)
