@@ -53,11 +53,16 @@ class ExpertBank:
                 return False
         return True
 
-    @torch.no_grad()
     def bind(self, experts: nn.ModuleList):
         """Return (w_gate [E,I,H], w_up [E,I,H], w_down [E,H,I]), packing on first use."""
-        if self._bound(experts):
+        with torch.no_grad():
+            if not self._bound(experts):
+                # not under inference mode, whose tensors do not count the writes to them
+                with torch.inference_mode(False), torch.no_grad():
+                    self._pack(experts)
             return self.w_gate, self.w_up, self.w_down
+
+    def _pack(self, experts: nn.ModuleList) -> None:
         E = len(experts)
         g0 = experts[0].gate_proj.weight
         I, H = g0.shape
@@ -73,7 +78,6 @@ class ExpertBank:
             ex.up_proj.weight.data = wu[e]
             ex.down_proj.weight.data = wd[e]
         self.w_gate, self.w_up, self.w_down = wg, wu, wd
-        return wg, wu, wd
 
 
 def router_bias_of(gate: nn.Linear) -> torch.Tensor | None:

@@ -108,6 +108,22 @@ class PermutedSparseMoE(nn.Module):
         self._w4 = self._w4_source = None
         return super()._apply(fn, *args, **kwargs)
 
+    def _parameters_of(self, **stacks):
+        """The experts' parameters that are views of these stacked tensors, by projection.
+        One that was made under inference mode has no version counter, so a parameter
+        that has takes its place, on the same memory."""
+        params = []
+        with torch.inference_mode(False), torch.no_grad():
+            for name, stack in stacks.items():
+                for e, ex in enumerate(self.experts):
+                    proj = getattr(ex, name)
+                    try:
+                        proj.weight._version
+                    except RuntimeError:
+                        proj.weight = nn.Parameter(stack[e], proj.weight.requires_grad)
+                    params.append(proj.weight)
+        return params
+
     def pack(self):
         """Stacked expert weights (w_gate, w_up, w_down), binding the per-expert
         parameters to views of them on first use."""
@@ -121,7 +137,7 @@ class PermutedSparseMoE(nn.Module):
         ``refresh=True`` after those."""
         wd = self.pack()[2]
         if refresh or self._w_down_t is None or not self._w_down_t_source.unchanged((wd,)):
-            source = _Source((wd,), (ex.down_proj.weight for ex in self.experts))
+            source = _Source((wd,), self._parameters_of(down_proj=wd))
             self._w_down_t = ops.transpose_down_weights(wd)
             self._w_down_t_source = source
         return self._w_down_t
@@ -132,7 +148,9 @@ class PermutedSparseMoE(nn.Module):
         synchronises, so call this (or the module) once before a graph capture."""
         weights = self.pack()
         if refresh or self._w4 is None or not self._w4_source.unchanged(weights):
-            source = _Source(weights, self.experts.parameters())
+            gate, up, down = weights
+            source = _Source(weights, self._parameters_of(gate_proj=gate, up_proj=up,
+                                                          down_proj=down))
             self._w4 = W4Experts.quantize(*weights, self.group_size, self.symmetric)
             self._w4_source = source
         return self._w4

@@ -51,6 +51,25 @@ def test_decode_weights_after_load_state_dict(cuda):
     ops.check_status(cuda)
 
 
+@pytest.mark.parametrize("options", [{"expert_weights": "w4", "group_size": 64},
+                                     {"decode_weights": True}, {}])
+def test_module_under_inference_mode(cuda, options):
+    """First run, writes and further runs under inference mode."""
+    H = 256
+    torch.manual_seed(5)
+    make = lambda: PermutedSparseMoE(H, 128, 16, 4, **options).to(device=cuda, dtype=torch.bfloat16)
+    mod, other = make(), make()
+    x = rows(3, H, 3, cuda)
+    with torch.inference_mode():
+        mod(x)
+        mod.load_state_dict(other.state_dict())
+        assert torch.equal(mod(x), other(x))
+        mod.experts[2].down_proj.weight.zero_()
+        other.pack()[2][2].zero_()
+        assert torch.equal(mod(x), other(x))
+    ops.check_status(cuda)
+
+
 # ------------------------------------------------------------------ rows of no expert
 
 

@@ -97,3 +97,26 @@ def test_another_stack_in_the_same_place(module):
         assert [t.data_ptr() for t in module.pack()] == [t.data_ptr() for t in old]
         assert [t._version for t in module.pack()] == [t._version for t in old]
         assert module.experts_4bit() is not bank
+
+
+def test_writes_under_inference_mode(module):
+    with torch.inference_mode():
+        assert is_current(module)
+        module.experts[1].up_proj.weight.mul_(2.0)
+        assert is_current(module)
+        module.load_state_dict(other_state(module))
+        assert is_current(module)
+
+
+def test_module_made_and_bound_under_inference_mode(module):
+    """The stacks and the parameters that are bound to them count their writes, whatever
+    mode the module was made and first run in."""
+    with torch.inference_mode():
+        made = PermutedSparseMoE(64, 64, 4, 2, expert_weights="w4", group_size=64)
+        assert is_current(made)
+        made.experts[2].gate_proj.weight.add_(1.0)
+        assert is_current(made)
+    with torch.no_grad():
+        made.experts[0].down_proj.weight.add_(1.0)
+    assert is_current(made)
+    assert not any(t.is_inference() for t in (*made.pack(), *made.experts.parameters()))
