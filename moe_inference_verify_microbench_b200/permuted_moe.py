@@ -102,6 +102,11 @@ class PermutedSparseMoE(nn.Module):
         self.experts = nn.ModuleList(SwiGLU_MLP(hidden, intermediate) for _ in range(num_experts))
         self._bank = ExpertBank()
 
+    def __getstate__(self):
+        """A copy of the module makes its own forms of its weights, on first use."""
+        return {**self.__dict__, "_w4": None, "_w4_source": None, "_w_down_t": None,
+                "_w_down_t_source": None}
+
     def _apply(self, fn, *args, **kwargs):
         self._bank.invalidate()
         self._w_down_t = self._w_down_t_source = None

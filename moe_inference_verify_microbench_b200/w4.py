@@ -91,6 +91,14 @@ class W4Experts:
                                             hidden, intermediate, group_size, int(has_zeros))
         self.native = ctypes.addressof(self._struct)  # const moe_w4_bank*
 
+    def __getstate__(self):
+        """What a copy or a file holds of a bank: not the addresses of its tensors."""
+        return (self.w13, self.w2, self.num_experts, self.hidden, self.intermediate,
+                self.group_size, self.has_zeros)
+
+    def __setstate__(self, state) -> None:
+        self.__init__(*state)
+
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (*self.w13, *self.w2))
 

@@ -2,6 +2,8 @@
 written after a forward, rows that no expert owns, tensors in place, rows and forms
 beside one another."""
 
+import copy
+
 import pytest
 import torch
 
@@ -67,6 +69,22 @@ def test_module_under_inference_mode(cuda, options):
         mod.experts[2].down_proj.weight.zero_()
         other.pack()[2][2].zero_()
         assert torch.equal(mod(x), other(x))
+    ops.check_status(cuda)
+
+
+def test_copied_module_and_bank(cuda):
+    mod = module(cuda, group_size=64)
+    x = rows(3, 256, 3, cuda)
+    with torch.no_grad():
+        y = mod(x)
+        bank = copy.deepcopy(mod.experts_4bit())
+        assert torch.equal(ops.moe_layer_w4(x, mod.gate.weight, bank, 4), y)
+        twin = copy.deepcopy(mod)
+        assert torch.equal(twin(x), y)
+        twin.experts[0].up_proj.weight.zero_()
+        twin.gate.weight.zero_()  # experts 0..3 of every token
+        mod.gate.weight.zero_()
+        assert not torch.equal(twin(x), mod(x))
     ops.check_status(cuda)
 
 
