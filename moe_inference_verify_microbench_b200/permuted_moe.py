@@ -23,7 +23,8 @@ forward after the weights were written: through the stacked tensors, through an
 expert's parameters (``load_state_dict``, an optimizer's step) or by re-binding.
 Only writes that autograd's version counters do not see (through ``.data``, or
 by a kernel on the raw pointer) need ``down_weights_transposed(refresh=True)``
-or ``experts_4bit(refresh=True)``.
+or ``experts_4bit(refresh=True)``.  A copy is made again in its place in memory,
+for graphs that captured a forward; a replay itself does not look for writes.
 
 The module must be bf16 on a CUDA device: there is no CPU path.
 """
@@ -62,6 +63,11 @@ class _Source:
 
     def unchanged(self, stacks) -> bool:
         return all(map(operator.is_, self.stacks, stacks)) and self._count() == self._writes
+
+    def unlike(self, stacks) -> bool:
+        """Whether a copy of these would not fit where the one of those lies."""
+        return any((a.shape, a.dtype, a.device) != (b.shape, b.dtype, b.device)
+                   for a, b in zip(self.stacks, stacks))
 
 
 class PermutedSparseMoE(nn.Module):
@@ -139,11 +145,17 @@ class PermutedSparseMoE(nn.Module):
         use and rebuilt when the down weights are re-bound or written in place,
         through the stacked tensor or an expert's parameter.  Writes through
         ``experts[e].down_proj.weight.data`` leave no trace: call with
-        ``refresh=True`` after those."""
+        ``refresh=True`` after those.  It is rebuilt in its place, so a graph that
+        captured a forward reads the new weights once this (or the module) was
+        called; until the module is moved or cast, which ends such a graph."""
         wd = self.pack()[2]
         if refresh or self._w_down_t is None or not self._w_down_t_source.unchanged((wd,)):
             source = _Source((wd,), self._parameters_of(down_proj=wd))
-            self._w_down_t = ops.transpose_down_weights(wd)
+            with torch.inference_mode(False), torch.no_grad():
+                if self._w_down_t is None or self._w_down_t_source.unlike((wd,)):
+                    self._w_down_t = ops.transpose_down_weights(wd)
+                else:
+                    self._w_down_t.copy_(wd.transpose(1, 2))
             self._w_down_t_source = source
         return self._w_down_t
 
@@ -156,7 +168,8 @@ class PermutedSparseMoE(nn.Module):
             gate, up, down = weights
             source = _Source(weights, self._parameters_of(gate_proj=gate, up_proj=up,
                                                           down_proj=down))
-            self._w4 = W4Experts.quantize(*weights, self.group_size, self.symmetric)
+            self._w4 = W4Experts.quantize(*weights, self.group_size, self.symmetric,
+                                          into=self._w4)
             self._w4_source = source
         return self._w4
 

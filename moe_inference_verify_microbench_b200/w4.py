@@ -104,11 +104,13 @@ class W4Experts:
 
     @classmethod
     @torch.no_grad()
-    def from_codes(cls, w_gate, w_up, w_down) -> "W4Experts":
+    def from_codes(cls, w_gate, w_up, w_down, *, into: "W4Experts | None" = None) -> "W4Experts":
         """Each argument is ``(codes, scales, zeros)``: uint8 codes [E, N, K] with one
         code (0..15) per byte, bf16 scales [E, N, K / group], and uint8 zero points
         of the scales' shape or None (for all three projections or for none).
-        Synchronises once, to refuse codes or zero points above 15."""
+        Synchronises once, to refuse codes or zero points above 15.  ``into``: a bank of
+        the same sizes, form and device, whose memory the new one takes over (its values
+        change in place, so captured graphs that read it follow); another is not touched."""
         parts = []
         for name, part in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
             codes, scales, zeros = part
@@ -143,8 +145,11 @@ class W4Experts:
             raise ValueError("codes, scales and zero points must be on one device")
         with torch.cuda.device(dev):
             status = torch.zeros(1, dtype=torch.int32, device=dev)
-            w13 = _pack((gc, gs, gz), (uc, us, uz), group, status)
-            w2 = _pack((dc, ds, dz), None, group, status)
+            same = into is not None and (E, H, I, group, gz is not None, dev) == (
+                into.num_experts, into.hidden, into.intermediate, into.group_size,
+                into.has_zeros, into.device)
+            w13 = _pack((gc, gs, gz), (uc, us, uz), group, status, into.w13 if same else None)
+            w2 = _pack((dc, ds, dz), None, group, status, into.w2 if same else None)
             code = int(status.item())
         if code:
             raise ValueError(f"codes and zero points must be in 0..15 "
@@ -154,9 +159,11 @@ class W4Experts:
     @classmethod
     @torch.no_grad()
     def quantize(cls, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
-                 group_size: int = 128, symmetric: bool = True) -> "W4Experts":
+                 group_size: int = 128, symmetric: bool = True, *,
+                 into: "W4Experts | None" = None) -> "W4Experts":
         """Round stacked bf16 weights (w_gate, w_up [E, I, H], w_down [E, H, I]) to
-        4 bits (``quantize_w4``) and pack them, expert by expert."""
+        4 bits (``quantize_w4``) and pack them, expert by expert.  ``into``: as for
+        ``from_codes``."""
         packed = []
         for name, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
             if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dim() != 3:
@@ -164,17 +171,18 @@ class W4Experts:
             rows = [quantize_w4(w[e], group_size, symmetric) for e in range(w.shape[0])]
             codes, scales = (torch.stack([r[i] for r in rows]) for i in (0, 1))
             packed.append((codes, scales, None if symmetric else torch.stack([r[2] for r in rows])))
-        return cls.from_codes(*packed)
+        return cls.from_codes(*packed, into=into)
 
 
-def _pack(first, second, group: int, status: torch.Tensor):
+def _pack(first, second, group: int, status: torch.Tensor, into=None):
     codes, scales, zeros = first
     E, N, K = codes.shape
     M = N if second is None else 2 * N
     dev = codes.device
-    q = torch.empty(E * M * K // 2, dtype=torch.uint8, device=dev)
-    s = torch.empty(E * M * (K // group) * (1 if zeros is None else 2), dtype=torch.bfloat16,
-                    device=dev)
+    q, s = into if into is not None else (
+        torch.empty(E * M * K // 2, dtype=torch.uint8, device=dev),
+        torch.empty(E * M * (K // group) * (1 if zeros is None else 2), dtype=torch.bfloat16,
+                    device=dev))
     p = ops._p
     c1, s1, z1 = second if second is not None else (None, None, None)
     ops._rc(_native.load().moe_w4_pack(p(codes), p(scales), p(zeros), p(c1), p(s1), p(z1), E, N, K,

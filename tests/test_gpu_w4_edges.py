@@ -88,6 +88,47 @@ def test_copied_module_and_bank(cuda):
     ops.check_status(cuda)
 
 
+@pytest.mark.parametrize("options", [{"expert_weights": "w4", "group_size": 64},
+                                     {"expert_weights": "w4", "group_size": 32, "symmetric": False},
+                                     {"decode_weights": True}])
+def test_captured_forward_follows_the_weights(cuda, options):
+    """A copy that is made again takes the place of the old one in memory, so a captured
+    forward reads the new weights, not memory that was freed."""
+    H = 256
+    torch.manual_seed(5)
+    mod = PermutedSparseMoE(H, 128, 16, 4, **options).to(device=cuda, dtype=torch.bfloat16)
+    x = rows(3, H, 3, cuda)
+
+    def places():
+        if "decode_weights" in options:
+            return [mod.down_weights_transposed().data_ptr()]
+        bank = mod.experts_4bit()
+        return [t.data_ptr() for t in (*bank.w13, *bank.w2)]
+
+    with torch.no_grad():
+        mod(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mod(x)
+        was = places()
+        for _ in range(2):
+            state = {n: torch.randn_like(t) * 0.05 for n, t in mod.state_dict().items()}
+            mod.load_state_dict(state)
+            want = mod(x).clone()
+            assert places() == was  # before the replay: it must not read anything else
+            torch.cuda.empty_cache()
+            graph.replay()
+            assert torch.equal(out, want)
+        with torch.inference_mode():
+            mod.experts[0].down_proj.weight.mul_(3.0)
+            want = mod(x).clone()
+        mod.experts[0].down_proj.weight.mul_(1.0)
+        assert places() == was
+        graph.replay()
+        assert torch.equal(out, want)
+    ops.check_status(cuda)
+
+
 # ------------------------------------------------------------------ rows of no expert
 
 

@@ -15,16 +15,17 @@ class Copied:
 
 @pytest.fixture
 def module(monkeypatch):
-    made = []
+    made, made_into = [], []
 
-    def quantize(cls, w_gate, w_up, w_down, group_size=128, symmetric=True, **kwargs):
+    def quantize(cls, w_gate, w_up, w_down, group_size=128, symmetric=True, into=None):
         made.append(Copied((w_gate, w_up, w_down)))
+        made_into.append(into)
         return made[-1]
 
     monkeypatch.setattr(W4Experts, "quantize", classmethod(quantize))
     monkeypatch.setattr(ops, "transpose_down_weights", lambda w: w.transpose(1, 2).contiguous())
     mod = PermutedSparseMoE(64, 64, 4, 2, expert_weights="w4", group_size=64)
-    mod.made = made
+    mod.made, mod.made_into = made, made_into
     return mod
 
 
@@ -120,3 +121,21 @@ def test_module_made_and_bound_under_inference_mode(module):
         made.experts[0].down_proj.weight.add_(1.0)
     assert is_current(made)
     assert not any(t.is_inference() for t in (*made.pack(), *made.experts.parameters()))
+
+
+def test_a_copy_is_made_again_in_its_place(module):
+    """What a captured forward reads stays where it is."""
+    assert is_current(module)
+    down = module.down_weights_transposed()
+    bank = module.experts_4bit()
+    module.load_state_dict(other_state(module))
+    with torch.inference_mode():
+        assert is_current(module)
+    assert module.down_weights_transposed().data_ptr() == down.data_ptr()
+    assert module.made_into[-1] is bank and module.made_into[0] is None
+    module.load_state_dict(other_state(module))
+    assert is_current(module)
+    module.double()  # moved or cast: in memory of its own
+    assert module.down_weights_transposed().dtype is torch.float64
+    module.experts_4bit()
+    assert module.made_into[-1] is None
