@@ -150,6 +150,8 @@ class PermutedSparseMoE(nn.Module):
         called; until the module is moved or cast, which ends such a graph."""
         wd = self.pack()[2]
         if refresh or self._w_down_t is None or not self._w_down_t_source.unchanged((wd,)):
+            if wd.is_cuda and torch.cuda.is_current_stream_capturing():
+                return ops.transpose_down_weights(wd)  # recorded, not done: not kept
             source = _Source((wd,), self._parameters_of(down_proj=wd))
             with torch.inference_mode(False), torch.no_grad():
                 if self._w_down_t is None or self._w_down_t_source.unlike((wd,)):

@@ -129,6 +129,30 @@ def test_captured_forward_follows_the_weights(cuda, options):
     ops.check_status(cuda)
 
 
+@pytest.mark.parametrize("run_before", [True, False])
+def test_transposed_weights_of_a_capture_are_not_kept(cuda, run_before):
+    """Weights written before a capture: what the capture only records, an eager forward does
+    not take for done."""
+    H = 256
+    torch.manual_seed(5)
+    make = lambda: PermutedSparseMoE(H, 128, 16, 4, decode_weights=True).to(device=cuda, dtype=torch.bfloat16)
+    mod, other = make(), make()
+    x = rows(2, H, 3, cuda)
+    with torch.no_grad():
+        want = other(x)
+        mod.pack()
+        if run_before:
+            mod(x)
+        mod.load_state_dict(other.state_dict())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mod(x)
+        assert torch.equal(mod(x), want)
+        graph.replay()
+        assert torch.equal(out, want)
+    ops.check_status(cuda)
+
+
 # ------------------------------------------------------------------ rows of no expert
 
 
