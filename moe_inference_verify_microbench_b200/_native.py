@@ -147,13 +147,21 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
                 f"{path} is missing; build it with `python -m moe_inference_verify_microbench_b200.build` "
                 "(the CUDA path has no CPU fallback)")
         lib = ctypes.CDLL(path)
+        # Version 5 has grown by entry points, so a library of that version may lack some.
+        missing = [n for n in SIGNATURES if not hasattr(lib, n)]
+        if "moe_abi_version" not in missing:
+            version = lib.moe_abi_version()
+            if version != ABI_VERSION:
+                raise NativeLibraryError(f"ABI version mismatch: library {version}, "
+                                         f"bindings {ABI_VERSION}")
+        if missing:
+            raise NativeLibraryError(
+                f"{path} lacks {', '.join(missing)}: it was built from other sources; rebuild it "
+                "with `python -m moe_inference_verify_microbench_b200.build`")
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
-        if lib.moe_abi_version() != ABI_VERSION:
-            raise NativeLibraryError(f"ABI version mismatch: library {lib.moe_abi_version()}, "
-                                     f"bindings {ABI_VERSION}")
         _lib = lib
         return lib
 
