@@ -38,7 +38,7 @@ from torch import nn
 
 from . import ops
 from .experts import ExpertBank, SwiGLU_MLP, router_bias_of
-from .w4 import GROUPS, W4Experts
+from .w4 import BLOCK, GROUPS, MAX_COLUMNS, W4Experts
 
 __all__ = ["PermutedSparseMoE", "SwiGLU_MLP"]
 
@@ -89,6 +89,10 @@ class PermutedSparseMoE(nn.Module):
             if group_size not in GROUPS or hidden % group_size or intermediate % group_size:
                 raise ValueError(f"group_size must be one of {GROUPS} and divide hidden and "
                                  f"intermediate, got {group_size}")
+            for name, n in (("hidden", hidden), ("intermediate", intermediate)):
+                if n % BLOCK or n > MAX_COLUMNS:
+                    raise ValueError(f"4-bit experts need {name} to be a multiple of {BLOCK}, at "
+                                     f"most {MAX_COLUMNS}, got {n}")
         self.expert_weights = expert_weights
         self.group_size = group_size
         self.symmetric = symmetric

@@ -28,6 +28,8 @@ import torch
 from . import _native, ops
 
 GROUPS = (32, 64, 128)
+BLOCK = 64          # columns of a packed block
+MAX_COLUMNS = 8192  # of a projection
 
 
 @torch.no_grad()
