@@ -163,14 +163,7 @@ class HybridBlock(nn.Module):
                       moe_norm_weight, gate_weight, expert_gate_weights, expert_up_weights,
                       expert_down_weights, *, attn_post_norm_weight=None,
                       moe_post_norm_weight=None, attn_gate=None, moe_gate=None) -> None:
-        self.attn_norm.weight.data.copy_(attn_norm_weight)
-        self.attn.qkv_proj.weight_loader(q_weight, "q")
-        self.attn.qkv_proj.weight_loader(k_weight, "k")
-        self.attn.qkv_proj.weight_loader(v_weight, "v")
-        self.attn.o_proj.weight_loader(o_weight)
-        self.moe_norm.weight.data.copy_(moe_norm_weight)
-        self.moe.weight_loader(gate_weight, expert_gate_weights, expert_up_weights,
-                               expert_down_weights)
+        extras = []
         for have, name, given in (
                 (self.post_norm, "attn_post_norm", attn_post_norm_weight),
                 (self.post_norm, "moe_post_norm", moe_post_norm_weight),
@@ -181,7 +174,17 @@ class HybridBlock(nn.Module):
             if not have:
                 raise ValueError(f"this block has no {name}")
             own = getattr(self, name)
-            (own.weight if isinstance(own, RMSNorm) else own).data.copy_(given)
+            extras.append((own.weight if isinstance(own, RMSNorm) else own, given))
+        self.attn_norm.weight.data.copy_(attn_norm_weight)
+        self.attn.qkv_proj.weight_loader(q_weight, "q")
+        self.attn.qkv_proj.weight_loader(k_weight, "k")
+        self.attn.qkv_proj.weight_loader(v_weight, "v")
+        self.attn.o_proj.weight_loader(o_weight)
+        self.moe_norm.weight.data.copy_(moe_norm_weight)
+        self.moe.weight_loader(gate_weight, expert_gate_weights, expert_up_weights,
+                               expert_down_weights)
+        for own, given in extras:
+            own.data.copy_(given)
 
     def _join(self, x, branch, post: RMSNorm, gate, pre: RMSNorm):
         """(x + scale * act(gate) * post(branch), its pre norm), one row kernel."""
