@@ -7,6 +7,7 @@ import copy
 import pytest
 import torch
 
+import test_gpu_w4 as w4
 import w4_reference as ref
 from moe_inference_verify_microbench_b200 import PermutedSparseMoE, fused_moe_forward_w4, ops, quantize_w4
 from test_gpu_w4 import bank_of, close, rms_close, rows
@@ -276,3 +277,86 @@ def test_block_norm_is_given_the_status_word(cuda, T, monkeypatch):
     (name, args), = seen
     assert name == "moe_block_norm_ex" and args[-2] == ops.status_word(cuda).data_ptr()
     assert "rows of the block norm" in ops._native.error_string(0x107)
+
+
+# ------------------------------------------------------------------ the forms of the products
+
+
+# groups of 128 with zero points: one to four shares of a warp, odd numbers of groups, more
+# row tiles than a unit of the tensor-memory form holds
+@pytest.mark.parametrize("E,H,I", [(3, 128, 128), (4, 384, 256), (6, 2048, 768), (3, 1280, 384),
+                                   (2, 8192, 128), (2, 256, 4096)])
+@pytest.mark.parametrize("shift", [1, 6, 10, 100, 104, 106])
+def test_group_128_with_zero_points(cuda, E, H, I, shift):
+    w4.test_grouped_products(cuda, E, H, I, 128, True, shift)
+
+
+@pytest.mark.parametrize("E,H,I,k,T,bias,norm", [
+    (16, 128, 128, 4, 1, False, True), (16, 2048, 768, 8, 8, True, False),
+    (128, 2048, 768, 8, 1, False, True), (32, 1280, 384, 4, 16, False, False),
+    (16, 4096, 128, 2, 3, False, True), (16, 256, 1408, 4, 5, True, True),
+    (16, 512, 256, 4, 33, False, True), (16, 256, 128, 2, 500, True, True)])
+def test_layer_of_group_128_with_zero_points(cuda, E, H, I, k, T, bias, norm):
+    w4.test_layer(cuda, E, H, I, 128, True, k, T, bias, norm)
+
+
+@pytest.mark.parametrize("E,H,I,group,zeros,k,T", [
+    (16, 256, 128, 64, False, 4, 16), (32, 4096, 128, 128, True, 2, 2), (48, 512, 384, 32, True, 8, 8),
+    (128, 2048, 768, 128, False, 8, 7), (16, 2560, 64, 64, True, 4, 13)])
+def test_tokens_alone_and_in_a_batch(cuda, E, H, I, group, zeros, k, T):
+    """The one-kernel layer gives a token the same row whatever comes with it."""
+    p = ref.parts(E, H, I, group, zeros, seed=T, device=cuda)
+    bank = bank_of(p)
+    x = rows(T, H, 3, cuda)
+    router = (torch.randn((E, H), generator=torch.Generator().manual_seed(T)) * 1.8
+              * H ** -0.5).bfloat16().to(cuda)
+    y = ops.moe_layer_w4(x, router, bank, k)
+    for i in range(T):
+        assert torch.equal(ops.moe_layer_w4(x[i:i + 1].contiguous(), router, bank, k), y[i:i + 1])
+    ops.check_status(cuda)
+
+
+@pytest.mark.parametrize("group,zeros", [(64, False), (32, True), (128, True)])
+@pytest.mark.parametrize("T", [40, 301])
+def test_non_finite_rows_in_the_tensor_memory_form(cuda, group, zeros, T):
+    """Infinities and NaN stay in their token also where they stand in the first row of an
+    expert's tile, which fills the columns past the last record."""
+    E, H, I, k = 4, 256, 128, 2
+    assert T * k // E >= ref.TC_RECORDS
+    p = ref.parts(E, H, I, group, zeros, device=cuda)
+    bank = bank_of(p)
+    gen = torch.Generator().manual_seed(1)
+    ids = torch.rand((T, E), generator=gen).argsort(1)[:, :k].int().contiguous().to(cuda)
+    w = torch.rand((T, k), generator=gen).to(cuda)
+    x = rows(T, H, 2, cuda)
+    clean = ops.experts_w4(x, ids, w, bank)
+    bad = {0: float("nan"), 1: float("inf"), 5: float("-inf"), T - 1: float("nan")}
+    for n, v in bad.items():
+        x[n, (17 * n) % H] = v
+    y = ops.experts_w4(x, ids, w, bank)
+    ops.check_status(cuda)
+    keep = torch.ones(T, dtype=torch.bool, device=cuda)
+    keep[list(bad)] = False
+    assert bool(torch.isfinite(clean.float()).all()) and torch.equal(y[keep], clean[keep])
+    assert not bool(torch.isfinite(y[~keep].float()).any())
+
+
+@pytest.mark.parametrize("T", [40, 301])
+def test_bad_expert_ids_in_the_tensor_memory_form(cuda, T):
+    E, H, I, k = 4, 256, 128, 2
+    p = ref.parts(E, H, I, 64, True, device=cuda)
+    bank = bank_of(p)
+    gen = torch.Generator().manual_seed(T)
+    ids = torch.rand((T, E), generator=gen).argsort(1)[:, :k].int().contiguous().to(cuda)
+    w = torch.rand((T, k), generator=gen).to(cuda)
+    x = rows(T, H, 2, cuda)
+    good = torch.ones_like(ids, dtype=torch.bool)
+    good[0, 0] = good[7, 1] = good[T - 1, 0] = good[T - 1, 1] = False
+    wrong = ids.clone()
+    wrong[0, 0], wrong[7, 1], wrong[T - 1, 0], wrong[T - 1, 1] = 9, -1, 4, 2 ** 31 - 1
+    y = ops.experts_w4(x, wrong, w, bank)
+    with pytest.raises(ops.MoEKernelError, match="expert id"):
+        ops.check_status(cuda)
+    close(y, *ref.experts(p, x, ids, w * good))  # the good records are computed
+    assert not bool(y[T - 1].any())
+    ops.check_status(cuda)
