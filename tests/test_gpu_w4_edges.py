@@ -360,3 +360,19 @@ def test_bad_expert_ids_in_the_tensor_memory_form(cuda, T):
     close(y, *ref.experts(p, x, ids, w * good))  # the good records are computed
     assert not bool(y[T - 1].any())
     ops.check_status(cuda)
+
+
+@pytest.mark.parametrize("T", [3, 16, 40, 300])
+def test_non_finite_rows_in_the_layer(cuda, T):
+    """A token whose router logits are not numbers is routed somewhere; the others keep
+    their rows, bit for bit, in every form of the layer."""
+    E, H, I, k = 16, 256, 128, 4
+    bank = bank_of(ref.parts(E, H, I, 128, True, seed=T, device=cuda))
+    x = rows(T, H, 3, cuda)
+    router = (torch.randn((E, H), generator=torch.Generator().manual_seed(T)) * 0.1).bfloat16().to(cuda)
+    clean = ops.moe_layer_w4(x, router, bank, k)
+    x[0, 3], x[T - 1, 9] = float("nan"), float("inf")
+    y = ops.moe_layer_w4(x, router, bank, k)
+    ops.check_status(cuda)
+    assert torch.equal(y[1:T - 1], clean[1:T - 1])
+    assert not bool(torch.isfinite(y[[0, T - 1]].float()).any())
