@@ -43,24 +43,27 @@ class ExpertBank:
         self.w_gate = self.w_up = self.w_down = None
 
     def _bound(self, experts: nn.ModuleList) -> bool:
-        if self.w_gate is None or len(experts) == 0:
+        if self.w_gate is None or self.w_gate.shape[0] != len(experts):
             return False
-        for e in (0, len(experts) - 1):
+        last = len(experts) - 1
+        # bytes from the first expert's matrix to the last's, the same in all three stacks
+        far = last * self.w_gate.stride(0) * self.w_gate.element_size()
+        gate, up, down = self.w_gate.data_ptr(), self.w_up.data_ptr(), self.w_down.data_ptr()
+        for e, at in ((0, 0), (last, far)):
             ex = experts[e]
-            if (ex.gate_proj.weight.data_ptr() != self.w_gate[e].data_ptr()
-                    or ex.up_proj.weight.data_ptr() != self.w_up[e].data_ptr()
-                    or ex.down_proj.weight.data_ptr() != self.w_down[e].data_ptr()):
+            if (ex.gate_proj.weight.data_ptr() != gate + at
+                    or ex.up_proj.weight.data_ptr() != up + at
+                    or ex.down_proj.weight.data_ptr() != down + at):
                 return False
         return True
 
     def bind(self, experts: nn.ModuleList):
         """Return (w_gate [E,I,H], w_up [E,I,H], w_down [E,H,I]), packing on first use."""
-        with torch.no_grad():
-            if not self._bound(experts):
-                # not under inference mode, whose tensors do not count the writes to them
-                with torch.inference_mode(False), torch.no_grad():
-                    self._pack(experts)
-            return self.w_gate, self.w_up, self.w_down
+        if not self._bound(experts):
+            # not under inference mode, whose tensors do not count the writes to them
+            with torch.inference_mode(False), torch.no_grad():
+                self._pack(experts)
+        return self.w_gate, self.w_up, self.w_down
 
     def _pack(self, experts: nn.ModuleList) -> None:
         E = len(experts)

@@ -51,7 +51,7 @@ class _Source:
     passes for them) and how often these and the experts' parameters had been written.
     The parameters are views of the stacks with version counters of their own, which
     only grow, so the sum stays the same only if none was written.  Reading the 384
-    counters of 128 experts takes the host 22 us."""
+    counters of 128 experts takes the host about 15 us."""
 
     def __init__(self, stacks, params) -> None:
         self.stacks = tuple(stacks)
