@@ -122,6 +122,10 @@ class _EPBase(nn.Module):
             wu[local_e].copy_(expert_up_weights[global_e])
             wd[local_e].copy_(expert_down_weights[global_e])
 
+    def _stacks(self):
+        """``pack()`` as each forward takes it."""
+        return self._bank.bind(self.experts, every=False)
+
     def _route(self, x_flat):
         return self._kernels.router_topk(x_flat, self.gate.weight, self.top_k, self.norm_topk_prob,
                                          bias=router_bias_of(self.gate))[:2]
@@ -147,7 +151,7 @@ class EPSparseMoELean(_EPBase):
                            self.intermediate)                          # expected local records
         s = K.sort_align(ids, self.num_experts, self.expert_start,     # local filter + stable sort
                          self.experts_per_rank, tile_rows=rows)        # (C6:141-160)
-        wg, wu, wd = self.pack()
+        wg, wu, wd = self._stacks()
         slots = K.expert_compute(x_flat, s.perm, k, s, wg, wu, wd,     # gather (C6:156) fused;
                                  row_map=s.perm, slot_scale=w.reshape(-1),  # weighted, to slot
                                  out_rows=N * k)                       # rows (C6:163-170)
@@ -194,7 +198,7 @@ def dispatch_combine(mod: _EPBase, local_x: torch.Tensor, group) -> torch.Tensor
     recv_e = recv_m[:, :k].contiguous()
     recv_w = recv_m[:, k:].contiguous().view(torch.float32)
     n_recv = recv_x.shape[0]
-    wg, wu, wd = mod.pack()
+    wg, wu, wd = mod._stacks()
     if n_recv > 0:
         rows = K.tile_rows(n_recv * k // ep, epr, mod.hidden, mod.intermediate)
         s2 = K.sort_align(recv_e, epr + 1, 0, epr, want_inv=True,    # local re-sort (C7:224-226);
@@ -223,7 +227,7 @@ def dispatch_combine_peer(mod: _EPBase, local_x: torch.Tensor, px: PeerExchange)
     rows = K.tile_rows(px.cap_rows * k // ep, epr, mod.hidden, mod.intermediate)
     s2 = K.sort_align(px.recv_ids, epr + 1, 0, epr, want_inv=True,  # local re-sort (C7:224-226)
                       tile_rows=rows)
-    wg, wu, wd = mod.pack()
+    wg, wu, wd = mod._stacks()
     out = K.expert_compute(px.recv_rows, s2.perm, k, s2, wg, wu, wd)
     px.give_back(out, s2.inv)                                          # weighted row sums (C7:258-261)
     return K.combine(px.ret_rows, N, ep, slot_src=plan.inv)           # sum over owner ranks
@@ -296,7 +300,7 @@ def dispatch_combine_peer_pipelined(mod: _EPBase, local_x: torch.Tensor, pxs, st
     ids, w = mod._route(local_x)                                       # local router (C7:141-146)
     plans = [K.sort_align(K.ep_keys(ids[a:b], epr, ep), ep + 1, 0, ep, want_inv=True)
              for a, b in bounds]
-    wg, wu, wd = mod.pack()
+    wg, wu, wd = mod._stacks()
     budget = 0
     if st.cuda and exchange_sms > 0:
         budget = max(2, ops.device_sm_count() - int(exchange_sms))

@@ -42,24 +42,26 @@ class ExpertBank:
     def invalidate(self) -> None:
         self.w_gate = self.w_up = self.w_down = None
 
-    def _bound(self, experts: nn.ModuleList) -> bool:
+    def _bound(self, experts: nn.ModuleList, every: bool) -> bool:
         if self.w_gate is None or self.w_gate.shape[0] != len(experts):
             return False
         last = len(experts) - 1
-        # bytes from the first expert's matrix to the last's, the same in all three stacks
-        far = last * self.w_gate.stride(0) * self.w_gate.element_size()
+        # bytes from one expert's matrix to the next, the same in all three stacks
+        step = self.w_gate.stride(0) * self.w_gate.element_size()
         gate, up, down = self.w_gate.data_ptr(), self.w_up.data_ptr(), self.w_down.data_ptr()
-        for e, at in ((0, 0), (last, far)):
-            ex = experts[e]
+        for e in range(last + 1) if every else (0, last):
+            ex, at = experts[e], e * step
             if (ex.gate_proj.weight.data_ptr() != gate + at
                     or ex.up_proj.weight.data_ptr() != up + at
                     or ex.down_proj.weight.data_ptr() != down + at):
                 return False
         return True
 
-    def bind(self, experts: nn.ModuleList):
-        """Return (w_gate [E,I,H], w_up [E,I,H], w_down [E,H,I]), packing on first use."""
-        if not self._bound(experts):
+    def bind(self, experts: nn.ModuleList, every: bool = True):
+        """Return (w_gate [E,I,H], w_up [E,I,H], w_down [E,H,I]), packing on first use
+        and after an expert's ``Parameter`` was replaced.  ``every=False``, for each
+        forward: only the first and the last expert are looked at."""
+        if not self._bound(experts, every):
             # not under inference mode, whose tensors do not count the writes to them
             with torch.inference_mode(False), torch.no_grad():
                 self._pack(experts)

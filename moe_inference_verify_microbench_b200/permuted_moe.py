@@ -141,7 +141,7 @@ class PermutedSparseMoE(nn.Module):
 
     def pack(self):
         """Stacked expert weights (w_gate, w_up, w_down), binding the per-expert
-        parameters to views of them on first use."""
+        parameters to views of them on first use, and anew after one was replaced."""
         return self._bank.bind(self.experts)
 
     def down_weights_transposed(self, refresh: bool = False) -> torch.Tensor:
@@ -152,7 +152,7 @@ class PermutedSparseMoE(nn.Module):
         ``refresh=True`` after those.  It is rebuilt in its place, so a graph that
         captured a forward reads the new weights once this (or the module) was
         called; until the module is moved or cast, which ends such a graph."""
-        wd = self.pack()[2]
+        wd = self._bank.bind(self.experts, every=refresh)[2]
         if refresh or self._w_down_t is None or not self._w_down_t_source.unchanged((wd,)):
             if wd.is_cuda and torch.cuda.is_current_stream_capturing():
                 return ops.transpose_down_weights(wd)  # recorded, not done: not kept
@@ -169,7 +169,7 @@ class PermutedSparseMoE(nn.Module):
         """The 4-bit bank of ``expert_weights="w4"``, rebuilt under the same rules as
         ``down_weights_transposed``, for all three projections.  Building it
         synchronises, so call this (or the module) once before a graph capture."""
-        weights = self.pack()
+        weights = self._bank.bind(self.experts, every=refresh)
         if refresh or self._w4 is None or not self._w4_source.unchanged(weights):
             gate, up, down = weights
             source = _Source(weights, self._parameters_of(gate_proj=gate, up_proj=up,
@@ -188,7 +188,7 @@ class PermutedSparseMoE(nn.Module):
             y = ops.moe_layer_w4(x_flat, self.gate.weight, self.experts_4bit(), self.top_k,
                                  self.norm_topk_prob, bias=router_bias_of(self.gate))
         else:
-            wg, wu, wd = self.pack()
+            wg, wu, wd = self._bank.bind(self.experts, every=False)
             w_down_t = None
             if self.decode_weights and 0 < x_flat.shape[0] <= 4:
                 w_down_t = self.down_weights_transposed()

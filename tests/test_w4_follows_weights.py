@@ -139,3 +139,19 @@ def test_a_copy_is_made_again_in_its_place(module):
     assert module.down_weights_transposed().dtype is torch.float64
     module.experts_4bit()
     assert module.made_into[-1] is None
+
+
+@pytest.mark.parametrize("expert", [0, 2, 3])
+def test_pack_after_a_parameter_was_replaced(module, expert):
+    """``pack()`` (or a refresh) binds any expert's new ``Parameter`` object."""
+    assert is_current(module)
+    new = torch.randn(64, 64)
+    module.experts[expert].up_proj.weight = torch.nn.Parameter(new.clone())
+    assert torch.equal(module.pack()[1][expert], new)
+    assert is_current(module)
+    module.experts[expert].load_state_dict(other_state(module.experts[expert]), assign=True)
+    module.experts_4bit(refresh=True)
+    assert is_current(module)
+    with torch.no_grad():
+        module.experts[expert].up_proj.weight.zero_()
+    assert is_current(module) and not bool(module.pack()[1][expert].any())
