@@ -400,26 +400,45 @@ MOE_API int moe_block_norm_ex(const void* x, const void* delta, const float* pos
  * K % group == 0, K <= 8192; N % 16 == 0 (N % 8 for two matrices); all
  * pointers to codes and packed data 16-byte aligned.
  *
+ * moe_w4_pack_fine lays the same scales and zero points out for products of many
+ * records per expert (8 on average), which multiply fp16 s * (q - z), 2^-12 of a
+ * weight from it: f takes the bytes that s takes, r E*M + E floats, both 16-byte
+ * aligned; the same sizes and limits.
+ *
  * moe_w4_bank: a layer's packed projections (host struct, read during the
- * call): w13 gate and up [E, I, H], w2 down [E, H, I].
+ * call): w13 gate and up [E, I, H], w2 down [E, H, I].  has_zeros: 0 or 1, plus
+ * MOE_W4_FINE where the fields after it are set (they are not read otherwise, and
+ * products of many records then pass over the weights once for eight of them).
  */
+#define MOE_W4_FINE 2
 typedef struct moe_w4_bank {
   const void* w13_q;
   const void* w13_s;
   const void* w2_q;
   const void* w2_s;
   int32_t E, H, I, group, has_zeros;
+  const void* w13_f;
+  const float* w13_r;
+  const void* w2_f;
+  const float* w2_r;
 } moe_w4_bank;
 MOE_API int moe_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros0,
                         const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E,
                         int N, int K, int group, void* q, void* s, int32_t* status,
                         cudaStream_t stream);
 
+MOE_API int moe_w4_pack_fine(const void* scales0, const uint8_t* zeros0, const void* scales1,
+                             const uint8_t* zeros1, int E, int N, int K, int group, void* f,
+                             float* r, cudaStream_t stream);
+
 /*
  * moe_grouped_w13_swiglu_gather and moe_grouped_w2 on a 4-bit bank: the same
  * tile tables (entries of at most 128 rows; longer ones are reported as bad
- * rows), row index (NULL: row r itself), row map and slot scale.  H % 64 == 0, I % 64 == 0, both <= 8192 and multiples of the
- * group; E <= 1024.
+ * rows), row index (NULL: row r itself), row map and slot scale.  H % 64 == 0,
+ * I % 64 == 0, both <= 8192 and multiples of the group; E <= 1024.  The _ex forms
+ * take a workspace for the A operand in fp16 (moe_w4_grouped_workspace_bytes of
+ * src_rows and H, or of M and I), which products of many records per expert need;
+ * without one (NULL) they pass over the weights once for eight records.
  */
 MOE_API int moe_grouped_w13_swiglu_w4(const void* src, int src_rows, const int32_t* index,
                                       int index_div, int M, const int32_t* tiles,
@@ -430,6 +449,18 @@ MOE_API int moe_grouped_w2_w4(const void* h, int M, const int32_t* tiles,
                               const int32_t* num_tiles, int max_tiles, const moe_w4_bank* bank,
                               const int32_t* row_map, const float* slot_scale, void* out,
                               int out_rows, int32_t* status, cudaStream_t stream);
+MOE_API size_t moe_w4_grouped_workspace_bytes(int rows, int columns);
+MOE_API int moe_grouped_w13_swiglu_w4_ex(const void* src, int src_rows, const int32_t* index,
+                                         int index_div, int M, const int32_t* tiles,
+                                         const int32_t* num_tiles, int max_tiles,
+                                         const moe_w4_bank* bank, void* h, void* workspace,
+                                         size_t workspace_bytes, int32_t* status,
+                                         cudaStream_t stream);
+MOE_API int moe_grouped_w2_w4_ex(const void* h, int M, const int32_t* tiles,
+                                 const int32_t* num_tiles, int max_tiles, const moe_w4_bank* bank,
+                                 const int32_t* row_map, const float* slot_scale, void* out,
+                                 int out_rows, void* workspace, size_t workspace_bytes,
+                                 int32_t* status, cudaStream_t stream);
 
 /*
  * The 4-bit experts for routed tokens: y[n] = sum_j weights[n, j] *

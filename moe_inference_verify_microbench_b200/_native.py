@@ -107,6 +107,13 @@ SIGNATURES: dict[str, tuple] = {
                                            _ptr, _ptr, _ptr, _ptr]),
     "moe_grouped_w2_w4": (_c_int, [_ptr, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr, _ptr, _ptr,
                                    _c_int, _ptr, _ptr]),
+    "moe_w4_pack_fine": (_c_int, [_ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr,
+                                  _ptr, _ptr]),
+    "moe_w4_grouped_workspace_bytes": (_c_size, [_c_int, _c_int]),
+    "moe_grouped_w13_swiglu_w4_ex": (_c_int, [_ptr, _c_int, _ptr, _c_int, _c_int, _ptr, _ptr,
+                                              _c_int, _ptr, _ptr, _ptr, _c_size, _ptr, _ptr]),
+    "moe_grouped_w2_w4_ex": (_c_int, [_ptr, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr, _ptr, _ptr,
+                                      _c_int, _ptr, _c_size, _ptr, _ptr]),
     "moe_w4_experts_workspace_bytes": (_c_size, [_c_int, _c_int, _ptr]),
     "moe_w4_experts_forward": (_c_int, [_ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr,
                                         _ptr, _c_size, _ptr, _ptr, _ptr]),
@@ -123,7 +130,11 @@ class W4BankStruct(ctypes.Structure):
 
     _fields_ = [("w13_q", _ptr), ("w13_s", _ptr), ("w2_q", _ptr), ("w2_s", _ptr),
                 ("E", ctypes.c_int32), ("H", ctypes.c_int32), ("I", ctypes.c_int32),
-                ("group", ctypes.c_int32), ("has_zeros", ctypes.c_int32)]
+                ("group", ctypes.c_int32), ("has_zeros", ctypes.c_int32),
+                ("w13_f", _ptr), ("w13_r", _ptr), ("w2_f", _ptr), ("w2_r", _ptr)]
+
+
+W4_FINE = 2  # MOE_W4_FINE
 
 
 ABI_VERSION = 5

@@ -90,7 +90,14 @@ size_t layer_layout(int T, int H, int I, int E, int k, int mode, void* ws, Body&
 }
 
 W4Bank w4_bank(const moe_w4_bank& b) {
-  return {b.w13_q, b.w13_s, b.w2_q, b.w2_s, b.E, b.H, b.I, b.group, b.has_zeros};
+  W4Bank w{b.w13_q, b.w13_s, b.w2_q, b.w2_s, b.E, b.H, b.I, b.group, b.has_zeros & 1};
+  if ((b.has_zeros & MOE_W4_FINE) != 0) {
+    w.w13_f = b.w13_f;
+    w.w13_r = b.w13_r;
+    w.w2_f = b.w2_f;
+    w.w2_r = b.w2_r;
+  }
+  return w;
 }
 
 // Buffers of one pass over the 4-bit experts; with `routed`, also the router's
@@ -105,8 +112,22 @@ struct W4Layout {
   int max_tiles;
   int* num_tiles;
   void *h, *slots, *decode;
+  W4Rows x16;        // many records: the activations in fp16
+  float* h_factor;   // and the powers of two of h, which is fp32 first, then fp16 in its place
   size_t bytes;
 };
+
+// Takes h and what the tensor-memory form reads, where the sizes can lead to it.
+void w4_take_rows(Carver& c, W4Layout& l, const W4Bank& b, long long R, long long src_rows) {
+  if (!w4_many(b, static_cast<int>(R / b.E))) {  // R / num_experts is no larger
+    l.h = c.take<__nv_bfloat16>(R * b.I);
+    return;
+  }
+  l.h = c.take<float>(R * b.I);
+  l.x16.f16 = c.take<__nv_bfloat16>(src_rows * b.H);
+  l.x16.factor = c.take<float>(src_rows);
+  l.h_factor = c.take<float>(R);
+}
 
 // Slot rows of fewer records than this are kept in fp32 where the streaming form makes
 // them: one rounding less for a few MB more that stay in L2 (24 tokens of 128 experts:
@@ -129,7 +150,7 @@ W4Layout w4_layout(void* ws, int T, int k, const W4Bank& b, bool routed) {
   l.max_tiles = max_tiles_bound(R, b.E, MOE_BLOCK_M);
   l.tiles = c.take<int4>(l.max_tiles);
   l.num_tiles = c.take<int>(1);
-  l.h = c.take<__nv_bfloat16>(R * b.I);
+  w4_take_rows(c, l, b, R, T);
   // slot rows: fp32 for few records, see w4_products
   l.slots = R < kW4WideRecords ? static_cast<void*>(c.take<float>(R * b.H))
                                : static_cast<void*>(c.take<__nv_bfloat16>(R * b.H));
@@ -144,12 +165,29 @@ W4Layout w4_sorted_layout(void* ws, int M, const W4Bank& b) {
   l.max_tiles = max_tiles_bound(M, b.E, MOE_BLOCK_M);
   l.tiles = c.take<int4>(l.max_tiles);
   l.num_tiles = c.take<int>(1);
-  l.h = c.take<__nv_bfloat16>(static_cast<size_t>(M) * b.I);
+  w4_take_rows(c, l, b, M, M);
   l.bytes = c.used;
   return l;
 }
 
+size_t w4_rows(void* ws, long long rows, long long columns, W4Rows& r) {
+  Carver c(ws);
+  r.f16 = c.take<__nv_bfloat16>(rows * columns);
+  r.factor = c.take<float>(rows);
+  return c.used;
+}
+
 bool w4_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// The room that a grouped product has in its workspace; none leaves it to the stream.
+int w4_grouped_rows(const W4Bank& b, int M, int src_rows, int columns, void* workspace,
+                    size_t workspace_bytes, W4Rows& rows) {
+  if (workspace == nullptr || M <= 0 || src_rows <= 0 || b.E <= 0 || columns <= 0) return kRcOk;
+  if (!w4_aligned(workspace)) return kRcBadArgument;
+  if (workspace_bytes < w4_rows(workspace, src_rows, columns, rows)) return kRcWorkspace;
+  rows.count = nullptr;
+  return kRcOk;
+}
 
 bool w4_count_ok(int T, int k) {
   return static_cast<long long>(T) * k <= 0x7fffffffLL;
@@ -160,18 +198,21 @@ int w4_products(const W4Bank& b, const W4Layout& l, const void* x, const int* id
                 int T, int k, int num_experts, int e_begin, void* y, int* status,
                 cudaStream_t stream) {
   const int R = T * k, avg = R / num_experts;
-  int rc = launch_w4_w13(b, x, T, l.perm, k, R, l.tiles, l.num_tiles, l.max_tiles, l.h, avg,
-                         status, stream);
+  const bool many = w4_many(b, avg);
+  int rc = launch_w4_w13(b, x, T, l.perm, k, R, l.tiles, l.num_tiles, l.max_tiles,
+                         many ? nullptr : l.h, avg, status, stream, l.x16,
+                         many ? static_cast<float*>(l.h) : nullptr);
   if (rc != kRcOk) return rc;
-  if (avg < kW4TcRecords && R < kW4WideRecords) {
+  const W4Rows h{nullptr, l.h_factor, l.offsets + b.E};
+  if (!many && R < kW4WideRecords) {
     float* slots = static_cast<float*>(l.slots);
     rc = launch_w4_w2(b, l.h, R, l.tiles, l.num_tiles, l.max_tiles, l.perm, w, nullptr, R, avg,
-                      status, stream, false, slots);
+                      status, stream, h, false, slots);
     if (rc != kRcOk) return rc;
     return launch_combine_f32(slots, ids, e_begin, e_begin + b.E, T, k, b.H, y, stream);
   }
   rc = launch_w4_w2(b, l.h, R, l.tiles, l.num_tiles, l.max_tiles, l.perm, w, l.slots, R, avg,
-                    status, stream);
+                    status, stream, h, false, nullptr, many);
   if (rc != kRcOk) return rc;
   return launch_combine(l.slots, R, nullptr, nullptr, ids, e_begin, e_begin + b.E, T, k, b.H, y,
                         status, stream);
@@ -604,24 +645,59 @@ int moe_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros
                         status, stream);
 }
 
+int moe_w4_pack_fine(const void* scales0, const uint8_t* zeros0, const void* scales1,
+                     const uint8_t* zeros1, int E, int N, int K, int group, void* f, float* r,
+                     cudaStream_t stream) {
+  return launch_w4_pack_fine(scales0, zeros0, scales1, zeros1, E, N, K, group, f, r, stream);
+}
+
+size_t moe_w4_grouped_workspace_bytes(int rows, int columns) {
+  if (rows < 0 || columns <= 0 || columns % 8 != 0) return 0;
+  W4Rows r;
+  return w4_rows(nullptr, rows, columns, r);
+}
+
+int moe_grouped_w13_swiglu_w4_ex(const void* src, int src_rows, const int32_t* index,
+                                 int index_div, int M, const int32_t* tiles,
+                                 const int32_t* num_tiles, int max_tiles, const moe_w4_bank* bank,
+                                 void* h, void* workspace, size_t workspace_bytes,
+                                 int32_t* status, cudaStream_t stream) {
+  if (bank == nullptr) return kRcBadArgument;
+  const W4Bank b = w4_bank(*bank);
+  W4Rows rows{};
+  const int rc = w4_grouped_rows(b, M, src_rows, b.H, workspace, workspace_bytes, rows);
+  if (rc != kRcOk) return rc;
+  return launch_w4_w13(b, src, src_rows, index, index_div, M, reinterpret_cast<const int4*>(tiles),
+                       num_tiles, max_tiles, h, b.E > 0 ? M / b.E : 0, status, stream, rows);
+}
+
 int moe_grouped_w13_swiglu_w4(const void* src, int src_rows, const int32_t* index, int index_div,
                               int M, const int32_t* tiles, const int32_t* num_tiles,
                               int max_tiles, const moe_w4_bank* bank, void* h, int32_t* status,
                               cudaStream_t stream) {
+  return moe_grouped_w13_swiglu_w4_ex(src, src_rows, index, index_div, M, tiles, num_tiles,
+                                      max_tiles, bank, h, nullptr, 0, status, stream);
+}
+
+int moe_grouped_w2_w4_ex(const void* h, int M, const int32_t* tiles, const int32_t* num_tiles,
+                         int max_tiles, const moe_w4_bank* bank, const int32_t* row_map,
+                         const float* slot_scale, void* out, int out_rows, void* workspace,
+                         size_t workspace_bytes, int32_t* status, cudaStream_t stream) {
   if (bank == nullptr) return kRcBadArgument;
-  return launch_w4_w13(w4_bank(*bank), src, src_rows, index, index_div, M,
-                       reinterpret_cast<const int4*>(tiles), num_tiles, max_tiles, h,
-                       bank->E > 0 ? M / bank->E : 0, status, stream);
+  const W4Bank b = w4_bank(*bank);
+  W4Rows rows{};
+  const int rc = w4_grouped_rows(b, M, M, b.I, workspace, workspace_bytes, rows);
+  if (rc != kRcOk) return rc;
+  return launch_w4_w2(b, h, M, reinterpret_cast<const int4*>(tiles), num_tiles, max_tiles, row_map,
+                      slot_scale, out, out_rows, b.E > 0 ? M / b.E : 0, status, stream, rows);
 }
 
 int moe_grouped_w2_w4(const void* h, int M, const int32_t* tiles, const int32_t* num_tiles,
                       int max_tiles, const moe_w4_bank* bank, const int32_t* row_map,
                       const float* slot_scale, void* out, int out_rows, int32_t* status,
                       cudaStream_t stream) {
-  if (bank == nullptr) return kRcBadArgument;
-  return launch_w4_w2(w4_bank(*bank), h, M, reinterpret_cast<const int4*>(tiles), num_tiles,
-                      max_tiles, row_map, slot_scale, out, out_rows,
-                      bank->E > 0 ? M / bank->E : 0, status, stream);
+  return moe_grouped_w2_w4_ex(h, M, tiles, num_tiles, max_tiles, bank, row_map, slot_scale, out,
+                              out_rows, nullptr, 0, status, stream);
 }
 
 size_t moe_w4_experts_workspace_bytes(int T, int top_k, const moe_w4_bank* bank) {
@@ -677,11 +753,13 @@ int moe_w4_sorted_forward(const void* sorted_x, int M, const int64_t* offsets,
                                  stream, M);
   if (rc != kRcOk) return rc;
   const int avg = M / b.E;
-  rc = launch_w4_w13(b, sorted_x, M, nullptr, 1, M, l.tiles, l.num_tiles, l.max_tiles, l.h, avg,
-                     status, stream);
+  const bool many = w4_many(b, avg);
+  rc = launch_w4_w13(b, sorted_x, M, nullptr, 1, M, l.tiles, l.num_tiles, l.max_tiles,
+                     many ? nullptr : l.h, avg, status, stream, l.x16,
+                     many ? static_cast<float*>(l.h) : nullptr);
   if (rc != kRcOk) return rc;
   return launch_w4_w2(b, l.h, M, l.tiles, l.num_tiles, l.max_tiles, nullptr, nullptr, y, M, avg,
-                      status, stream, true);
+                      status, stream, W4Rows{nullptr, l.h_factor, nullptr}, true, nullptr, many);
 }
 
 size_t moe_w4_layer_workspace_bytes(int T, int top_k, const moe_w4_bank* bank) {

@@ -87,8 +87,12 @@ int map_rows(CUtensorMap* m, const void* base, int elem_bytes, long long inner, 
   return r == CUDA_SUCCESS ? kRcOk : kRcTensorMap;
 }
 
-int map_gather_rows(CUtensorMap* m, const void* base, long long rows, int cols) {
-  return map_2d(m, base, rows, cols, 1);
+int map_gather_rows(CUtensorMap* m, const void* base, long long rows, int cols,
+                    long long pitch_bytes) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch_bytes)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(kBK), 1u};
+  return make_map(m, base, 2, dims, strides, box);
 }
 
 namespace {

@@ -121,9 +121,10 @@ int device_sm_count();
 // [box_rows][box_inner]; elements outside read as zero.
 int map_rows(CUtensorMap* m, const void* base, int elem_bytes, long long inner, long long rows,
              int box_inner, int box_rows);
-// Tensor map of bf16 rows [rows][cols] for row gathers: box of one row of 64 columns,
-// 128-byte swizzle.
-int map_gather_rows(CUtensorMap* m, const void* base, long long rows, int cols);
+// Tensor map of rows [rows][cols] of 16-bit values for row gathers: box of one row of 64
+// columns, 128-byte swizzle.
+int map_gather_rows(CUtensorMap* m, const void* base, long long rows, int cols,
+                    long long pitch_bytes);
 
 // The cudaError_t of the most recent failed CUDA call a launcher recorded on
 // this thread (0 = none), and the recorder: returns `e` unchanged.
@@ -182,6 +183,9 @@ int launch_decode_split(const void* x, const void* wr, const float* bias, int T,
                         cudaStream_t stream);
 
 // Records per expert, on average, from which the 4-bit products take the tensor-memory form.
+// Experts of 2048 x 768, group 128, 128 of them, the whole call: at 6 records per expert the
+// stream takes 103 us and the tensor-memory form 114, at 7 113 and 116, at 8 123 and 117, at
+// 16 189 and 128 (the stream passes over the weights once for 8 records).
 constexpr int kW4TcRecords = 8;
 
 // Down GEMM with the atomic combine: out_f32[row_map[p] / red_div] +=
@@ -195,22 +199,43 @@ struct W4Bank {
   const void *w13_q, *w13_s;  // gate and up rows interleaved by eights
   const void *w2_q, *w2_s;    // down
   int E, H, I, group, zeros;
+  // The same scales for the tensor-memory form (w4_gemm.cu), null where a bank has none:
+  // records in fp16 and the powers of two that they are multiples of.
+  const void *w13_f, *w2_f;
+  const float *w13_r, *w2_r;
 };
 constexpr int kW4MaxK = 8192;
+// Room for activations in fp16 with a power of two for each row, which the tensor-memory
+// form reads: rows * columns halves and rows floats.  Null: the product streams.
+struct W4Rows {
+  void* f16;
+  float* factor;
+  const int* count;  // rows in use, on the device (null: all)
+};
 int w4_check_bank(const W4Bank& bank);
 int launch_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* zeros0,
                    const uint8_t* codes1, const void* scales1, const uint8_t* zeros1, int E, int N,
                    int K, int group, void* q, void* s, int* status, cudaStream_t stream);
 // avg: records per expert to expect; it chooses the kernel and changes no result
 // beyond rounding.  zero_rest: output rows of no tile are zeroed; the table's row ranges
-// follow one another then.
+// follow one another then.  h_f32 (tensor-memory form only): h in fp32, which the down
+// product takes and overwrites.
 int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* index,
                   int index_div, int M, const int4* tiles, const int* num_tiles, int max_tiles,
-                  void* h_out, int avg, int* status, cudaStream_t stream);
+                  void* h_out, int avg, int* status, cudaStream_t stream, const W4Rows& rows,
+                  float* h_f32 = nullptr);
+// Whether products of `avg` records per expert take the tensor-memory form.
+inline bool w4_many(const W4Bank& bank, int avg) {
+  return avg >= kW4TcRecords && bank.w13_f != nullptr;
+}
+int launch_w4_pack_fine(const void* scales0, const uint8_t* zeros0, const void* scales1,
+                        const uint8_t* zeros1, int E, int N, int K, int group, void* f, float* r,
+                        cudaStream_t stream);
 int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
                  int max_tiles, const int* row_map, const float* row_scale, void* out,
                  int out_rows, int avg, int* status, cudaStream_t stream,
-                 bool zero_rest = false, float* out_f32 = nullptr);
+                 const W4Rows& rows, bool zero_rest = false, float* out_f32 = nullptr,
+                 bool h_f32 = false);
 
 // The whole layer for a few tokens (w4_decode.cu; T <= 16, T * k <= 64): `scratch`
 // holds w4_decode_scratch_bytes(b, T) bytes, h [T * k, I] bf16.

@@ -26,6 +26,8 @@
 // Numerics: products of activations with (q - z) are exact in fp32; each
 // group (or a warp's share of it) is summed on the tensor cores in fp32 and
 // then scaled in fp32, so no weight is ever rounded to bf16.
+#include <cuda_fp16.h>
+
 #include <algorithm>
 
 #include "grouped_gemm.cuh"
@@ -114,6 +116,60 @@ __global__ void __launch_bounds__(256) w4_pack(const W4PackArgs a) {
   if (bad) record_status(a.status, kErrBadCode);
 }
 
+// The records of the tensor-memory form, of the same shape: scales as fp16 multiples of a
+// power of two, zero points as 1024 + z.  The power is the expert's, and puts its largest
+// scale into [2^10, 2^11), so that fifteen times it is in fp16's range.  A bf16 scale has
+// eight bits and stays exact down to 2^-17 (2^-27 of the largest); a row all of whose
+// scales are below 2^-16 of the largest has a power of its own.  r[expert][tile][16] holds
+// 1, or what such a row's power is of the expert's, and behind it, r[E * M + expert], the
+// experts'.  A row with an infinity or a NaN keeps its scales.  blockIdx.x is the expert;
+// its CTAs find its largest scale each for itself and share its rows.
+__global__ void __launch_bounds__(256) w4_pack_fine(const W4PackArgs a, float* r) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ int most;
+  const int ng = a.K / a.group, e = blockIdx.x;
+  const bool pair = a.scales[1] != nullptr;
+  const int tiles = a.N / (pair ? 8 : 16);
+  const bool zp = a.zeros[0] != nullptr;
+  const size_t row0 = static_cast<size_t>(e) * a.N;
+  if (threadIdx.x == 0) most = 0;
+  __syncthreads();
+  int top = 0;
+  for (int m = 0; m < (pair ? 2 : 1); ++m)
+#pragma unroll 8
+    for (int i = threadIdx.x; i < a.N * ng; i += blockDim.x) {
+      const int v = a.scales[m][row0 * ng + i] & 0x7fff;
+      if (v < 0x7f80) top = max(top, v);
+    }
+  atomicMax(&most, top);
+  __syncthreads();
+  auto shift_of = [](int bits) {
+    return bits == 0 ? 0 : 10 - ilogbf(__uint_as_float(static_cast<uint32_t>(bits) << 16));
+  };
+  const int base = shift_of(most);
+  if (threadIdx.x == 0 && blockIdx.y == 0) r[static_cast<size_t>(a.E) * tiles * 16 + e] = ldexpf(1.0f, -base);
+  for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < tiles * 16; i += gridDim.y * blockDim.x) {
+    const int tile = i >> 4, g = i & 7, half = (i >> 3) & 1;  // packed row g, or g + 8
+    const int m = pair ? half : 0;
+    const size_t row = row0 + (pair ? 8 * tile : 16 * tile + 8 * half) + g;
+    const uint16_t* s = a.scales[m] + row * ng;
+    top = 0;
+    for (int k = 0; k < ng; ++k) top = max(top, s[k] & 0x7fff);
+    int shift = base;
+    if (top >= 0x7f80) shift = 0;
+    else if (top > 0 && shift_of(top) - base > 16) shift = shift_of(top);
+    const size_t et = static_cast<size_t>(e) * tiles + tile;
+    r[et * 16 + (i & 15)] = top < 0x7f80 ? ldexpf(1.0f, base - shift) : 1.0f;
+    uint16_t* out = a.s + (et * ng * 8 + g) * (zp ? 4 : 2) + half;
+    for (int k = 0; k < ng; ++k, out += 8 * (zp ? 4 : 2)) {
+      const float v = __uint_as_float(static_cast<uint32_t>(s[k]) << 16);
+      out[0] = __half_as_ushort(__float2half_rn(ldexpf(v, shift)));
+      if (zp) out[2] = 0x6400u | (a.zeros[m][row * ng + k] & 15u);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ streaming
 
 template <bool SWIGLU, int KB, int MODE>
@@ -138,8 +194,12 @@ int w4_check_bank(const W4Bank& b) {
   if (b.H % 64 != 0 || b.I % 64 != 0 || b.H % b.group != 0 || b.I % b.group != 0 ||
       b.H > kW4MaxK || b.I > kW4MaxK || b.E > 1024)
     return kRcUnsupported;
-  for (const void* p : {b.w13_q, b.w13_s, b.w2_q, b.w2_s})
+  for (const void* p : {b.w13_q, b.w13_s, b.w2_q, b.w2_s, b.w13_f, b.w2_f,
+                        static_cast<const void*>(b.w13_r), static_cast<const void*>(b.w2_r)})
     if (!aligned16(p)) return kRcBadArgument;
+  const bool fine = b.w13_f != nullptr;
+  if ((b.w2_f != nullptr) != fine || (b.w13_r != nullptr) != fine || (b.w2_r != nullptr) != fine)
+    return kRcBadArgument;
   return kRcOk;
 }
 
@@ -151,6 +211,9 @@ static int w4_launch(W4Args& a, cudaStream_t stream) {
   static std::atomic<uint64_t> attr{0};
   if (!allow_smem(w4_stream<SWIGLU, KB, MODE>, kW4SmemBytes, attr)) return kRcCudaError;
   const long long units = static_cast<long long>(a.max_tiles) * a.m.tiles;
+  // a table of ranges that do not overlap has at most M / 8 chunks and one more an entry
+  if (units + static_cast<long long>(a.M / kW4Recs) * a.m.tiles > 0xffffffffLL)
+    return kRcUnsupported;  // the walk counts in 32 bits
   const int grid = static_cast<int>(std::min<long long>(units, device_sm_count()));
   return note_cuda_error(launch_pdl(w4_stream<SWIGLU, KB, MODE>, dim3(grid), dim3(kW4Threads), sh,
                                     stream, a)) == cudaSuccess
@@ -170,11 +233,6 @@ static int w4_dispatch_mode(W4Args& a, cudaStream_t stream) {
 
 template <bool SWIGLU>
 static int w4_dispatch(W4Args& a, cudaStream_t stream) {
-  // Experts of 2048 x 768, group 128, 128 of them, the whole call: at 4 records per expert
-  // the stream takes 94 us and the tensor-memory form 104, at 6 both take 105, at 8 they
-  // take 121 and 108 (the stream passes over the weights once for 8 records).  Between
-  // the two the stream's unrounded weights decide.
-  if (a.avg >= kW4TcRecords) return w4_gemm(a, SWIGLU, stream);
   if (a.m.rec == 8 || a.m.gshift == 0) return w4_dispatch_mode<SWIGLU, kW4Half>(a, stream);
   if (a.m.gshift == 1) return w4_dispatch_mode<SWIGLU, kW4Block>(a, stream);
   return w4_dispatch_mode<SWIGLU, kW4TwoBlocks>(a, stream);
@@ -182,14 +240,17 @@ static int w4_dispatch(W4Args& a, cudaStream_t stream) {
 
 int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* index,
                   int index_div, int M, const int4* tiles, const int* num_tiles, int max_tiles,
-                  void* h_out, int avg, int* status, cudaStream_t stream) {
+                  void* h_out, int avg, int* status, cudaStream_t stream, const W4Rows& rows,
+                  float* h_f32) {
   if (const int rc = w4_check_bank(bank); rc != kRcOk) return rc;
+  const bool many = w4_many(bank, avg) && rows.f16 != nullptr;
   if (M < 0 || max_tiles < 0 || index_div <= 0 || src_rows < 0 || tiles == nullptr ||
       num_tiles == nullptr)
     return kRcBadArgument;
   if (M == 0 || max_tiles == 0) return kRcOk;
-  if (src == nullptr || src_rows == 0 || h_out == nullptr || !aligned16(src) ||
-      !aligned16(h_out) || !aligned16(tiles))
+  if (src == nullptr || src_rows == 0 || (h_out == nullptr) == (h_f32 == nullptr) ||
+      !aligned16(src) || !aligned16(h_out) || !aligned16(h_f32) || !aligned16(tiles) ||
+      (h_f32 != nullptr && !many))
     return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, false);
@@ -203,24 +264,30 @@ int launch_w4_w13(const W4Bank& bank, const void* src, int src_rows, const int* 
   a.max_tiles = max_tiles;
   a.E = bank.E;
   a.out = static_cast<__nv_bfloat16*>(h_out);
+  a.out_f32 = h_f32;
   a.out_ld = bank.I;
   a.out_rows = M;
-  a.avg = avg;
   a.status = status;
+  if (many) {
+    a.m.s = static_cast<const uint8_t*>(bank.w13_f);
+    a.row_factor = bank.w13_r;
+    return w4_gemm(a, true, rows, false, stream);
+  }
   return w4_dispatch<true>(a, stream);
 }
 
 int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, const int* num_tiles,
                  int max_tiles, const int* row_map, const float* row_scale, void* out,
-                 int out_rows, int avg, int* status, cudaStream_t stream,
-                 bool zero_rest, float* out_f32) {
+                 int out_rows, int avg, int* status, cudaStream_t stream, const W4Rows& rows,
+                 bool zero_rest, float* out_f32, bool h_f32) {
   if (const int rc = w4_check_bank(bank); rc != kRcOk) return rc;
+  const bool many = w4_many(bank, avg) && (rows.f16 != nullptr || h_f32);
   if (M < 0 || max_tiles < 0 || out_rows < 0 || tiles == nullptr || num_tiles == nullptr)
     return kRcBadArgument;
   if (M == 0 || max_tiles == 0) return kRcOk;
   if (h == nullptr || (out == nullptr) == (out_f32 == nullptr) || !aligned16(h) ||
-      !aligned16(out) || !aligned16(tiles) ||
-      (out_f32 != nullptr && (zero_rest || avg >= kW4TcRecords)))
+      !aligned16(out) || !aligned16(tiles) || (out_f32 != nullptr && (zero_rest || many)) ||
+      (h_f32 && !many))
     return kRcBadArgument;
   W4Args a{};
   a.m = w4_matrix(bank, true);
@@ -239,8 +306,12 @@ int launch_w4_w2(const W4Bank& bank, const void* h, int M, const int4* tiles, co
   a.row_map = row_map;
   a.row_scale = row_scale;
   a.zero_rest = zero_rest;
-  a.avg = avg;
   a.status = status;
+  if (many) {
+    a.m.s = static_cast<const uint8_t*>(bank.w2_f);
+    a.row_factor = bank.w2_r;
+    return w4_gemm(a, false, rows, h_f32, stream);
+  }
   return w4_dispatch<false>(a, stream);
 }
 
@@ -273,6 +344,32 @@ int launch_w4_pack(const uint8_t* codes0, const void* scales0, const uint8_t* ze
   a.status = status;
   return note_cuda_error(launch_pdl(w4_pack, dim3(device_sm_count() * 8), dim3(256), 0, stream,
                                     a)) == cudaSuccess
+             ? kRcOk
+             : kRcCudaError;
+}
+
+int launch_w4_pack_fine(const void* scales0, const uint8_t* zeros0, const void* scales1,
+                        const uint8_t* zeros1, int E, int N, int K, int group, void* f, float* r,
+                        cudaStream_t stream) {
+  if (scales0 == nullptr || f == nullptr || r == nullptr || E <= 0 || N <= 0 || K <= 0 ||
+      (scales1 != nullptr && (zeros0 == nullptr) != (zeros1 == nullptr)) ||
+      (scales1 == nullptr && zeros1 != nullptr) || !aligned16(f) || !aligned16(r))
+    return kRcBadArgument;
+  if ((group != 32 && group != 64 && group != 128) || K % 64 != 0 || K % group != 0 ||
+      K > kW4MaxK || N % (scales1 != nullptr ? 8 : 16) != 0 || E > 1024)
+    return kRcUnsupported;
+  W4PackArgs a{};
+  a.scales[0] = static_cast<const uint16_t*>(scales0);
+  a.scales[1] = static_cast<const uint16_t*>(scales1);
+  a.zeros[0] = zeros0;
+  a.zeros[1] = zeros1;
+  a.E = E;
+  a.N = N;
+  a.K = K;
+  a.group = group;
+  a.s = static_cast<uint16_t*>(f);
+  return note_cuda_error(launch_pdl(w4_pack_fine, dim3(E, std::max(1, 4 * device_sm_count() / E)),
+                                    dim3(256), 0, stream, a, r)) == cudaSuccess
              ? kRcOk
              : kRcCudaError;
 }

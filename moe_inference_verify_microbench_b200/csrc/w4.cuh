@@ -40,12 +40,13 @@ struct W4Matrix {
 // The column pairs of a word as bf16 pairs 128 + q: 0x4300 is 128.0 and a code is
 // the last four bits of the seven-bit mantissa, so the or is exact: seven integer
 // instructions for eight codes.
+template <uint32_t BASE = 0x43004300u>
 __device__ __forceinline__ void w4_pairs(uint32_t w, uint32_t (&r)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     asm("lop3.b32 %0, %1, %2, %3, 0xea;"
         : "=r"(r[i])
-        : "r"(w >> (4 * i)), "n"(0x000f000f), "r"(0x43004300u));
+        : "r"(w >> (4 * i)), "n"(0x000f000f), "r"(BASE));
 }
 
 // bf16 pair a - b, exact for the small integers used here.
@@ -95,13 +96,16 @@ struct W4Args {
   int max_tiles;
   int E;
   __nv_bfloat16* out;
-  float* out_f32;       // where the rows go instead, unrounded (the stream's down product only)
+  float* out_f32;       // where the rows go instead, unrounded (the stream's down product and
+                        // the tensor-memory form's gate/up product)
+  const float* row_factor;  // tensor-memory form: of the weight rows [expert][tile][16], of
+                            // the experts behind them
+  const float* act_factor;  // and of the A rows
   int out_ld;
   int out_rows;
   const int* row_map;
   const float* row_scale;
   bool zero_rest;       // rows of out before the first entry and after the last are zeroed
-  int avg;              // records per expert to expect (chooses the kernel)
   int* status;
 };
 
@@ -170,7 +174,7 @@ bool allow_smem(Kernel* fn, int bytes, std::atomic<uint64_t>& done) {
 }
 
 // The tensor-memory form for experts with many records (w4_gemm.cu), from
-// kW4TcRecords records per expert on.
-int w4_gemm(const W4Args& a, bool swiglu, cudaStream_t stream);
+// kW4TcRecords records per expert on.  f32: a.act holds fp32 rows, which it overwrites.
+int w4_gemm(W4Args a, bool swiglu, const W4Rows& rows, bool f32, cudaStream_t stream);
 
 }  // namespace moe

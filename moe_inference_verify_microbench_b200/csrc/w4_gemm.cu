@@ -2,7 +2,7 @@
 // records (layout: w4.cuh; the form for few records: w4.cu).
 //
 // The weights are the 128-row operand and live in tensor memory: sixteen warps turn
-// codes into bf16 s * (q - z) in registers, in the fragment order that
+// codes into fp16 s * (q - z) in registers, in the fragment order that
 // tcgen05.st.16x128b writes, so the dequantised weights never touch shared
 // memory, whose bandwidth the operand reads of 128-row tiles would fill.  The
 // records are the N operand (16 to 128 columns of one tile-table entry) in
@@ -19,7 +19,8 @@
 // CTA (864 threads, one per SM, persistent):
 //   warps 0..15   dequantise: warp w writes lane quarter w % 4 of every fourth
 //                 64-column block
-//   warps 16..19  epilogue: tensor memory -> bf16 -> staging rows -> output rows
+//   warps 16..19  epilogue: tensor memory -> bf16 -> staging rows -> output rows (h that the
+//                 down product reads next: fp32, from the registers to its rows)
 //   warps 20..23  gather the records' rows (tile::gather4: four rows a copy, into the
 //                 128-byte swizzle; one warp for all copies of 128 records was the
 //                 bound: 8192 tokens 1578 us instead of 863 then)
@@ -27,20 +28,23 @@
 //   warps 25, 26  issue tcgen05.mma, one operand each: 4 steps of 16 columns per
 //                 block; warp 25 allocates tensor memory
 //
-// A weight is rounded once, s * (q - z) to bf16: the operand's type, and what a bf16
-// checkpoint of the same weights would hold.  That is 2^-8 of it at most, like
-// the rounding of the activations themselves; the sums stay fp32.  (Exact operands
-// q - z would need the scale on every group's sums: a pass over the accumulators per
-// 128 columns, 256 fp32 sums a thread at 128 records.)
+// Numerics: a weight s * (q - z) has twelve bits, eight of the bf16 scale and four; fp16
+// operands round it to eleven, 2^-12 of it at most (bf16 would leave eight: three such
+// roundings made the error of the whole call 3.8e-3 of 64 bits, where y and the slot rows
+// alone make 2.4e-3).  fp16's range is met by powers of two: an expert's scales are
+// multiples of one (w4_pack_fine; much smaller rows of their own), a row of activations of
+// another (w4_rows_f16, which also rounds h, fp32 from the gate/up product, to fp16:
+// 2^-12).  They come off the fp32 sums in the epilogue, exactly.
 //
-// Measured back to back, 128 experts of 2048 x 768, group 128, gate/up and down:
-// 16 records per expert 63 and 36 us (3.3 and 2.9 TB/s of codes), 64 records 90 and
-// 55 us, 512 records 430 and 263 us (0.96 and 0.78 PFLOP/s).  At 16 records the issue
-// slots are three quarters used (66 instructions per 16 x 64 block of codes for the
-// dequantisation, about 30 for all else) and a set of warps waits for its own products
-// before it refills its stage; a third pair of stages was worth 3 %.  Halves of units
-// in a last round that is not half full cost as much as whole ones (shard of 32
-// experts 78 -> 84 us).  At 512 the tiles of 128 records and 256 weight rows move 6.3
+// Measured, 128 experts of 2048 x 768, group 128, one launch with L2 cold, gate/up and
+// down: 16 records per expert 70 and 38 us (3.0 and 2.7 TB/s of codes), 512 records 498
+// and 289 us (0.83 and 0.71 PFLOP/s); with bf16 operands and h they took 67, 38, 470 and 286.
+// Activations to fp16: 8192 x 2048 bf16 10 us, 65536 x 768 fp32 41 us (HBM), small ones 4.
+// At 16 records the issue slots are three quarters used (66 instructions per 16 x 64
+// block of codes for the dequantisation, about 30 for all else) and a set of warps waits
+// for its own products before it refills its stage; a third pair of stages was worth 3 %.
+// Halves of units in a last round that is not half full cost as much as whole ones (shard
+// of 32 experts 78 -> 84 us).  At 512 the tiles of 128 records and 256 weight rows move 6
 // TB/s from L2, and their products wait for the epilogue before them (5000 of 34000
 // cycles for gate/up), because tensor memory holds 128 records' sums once.
 #include <algorithm>
@@ -89,6 +93,17 @@ __device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t taddr, const uint32_
       : "memory");
 }
 
+// 32 lanes, 16 columns from taddr on, a row to a lane.
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
+
 // 16 lanes, 16 columns from taddr on, in the order of product fragments: lane
 // 4 g + t has columns 2t, 2t + 1 of rows g and g + 8, then columns 8 + 2t, 9 + 2t.
 __device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)[8]) {
@@ -111,8 +126,8 @@ __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// D[tmem] (+)= A[tmem] * B[smem]^T, bf16 inputs, fp32 accumulate.
-__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t desc_lo,
+// D[tmem] (+)= A[tmem] * B[smem]^T, fp16 inputs, fp32 accumulate.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t desc_lo,
                                                uint32_t desc_hi, uint32_t idesc,
                                                uint32_t accumulate) {
   asm volatile(
@@ -145,16 +160,19 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* m, 
       : "memory");
 }
 
-// The column pairs of a word as bf16 s * (q - z): 0x4300 is 128.0 and a code is
-// the last four bits of the mantissa; 128 + q - (128 + z) is exact, the product
+// The column pairs of a word as fp16 s * (q - z): 0x6400 is 1024.0 and a code is
+// the last four bits of the mantissa; 1024 + q - (1024 + z) is exact, the product
 // is rounded once.
 __device__ __forceinline__ void w4_scaled_pairs(uint32_t w, uint32_t z, uint32_t s, uint32_t* r,
                                                 int stride) {
   uint32_t v[4];
-  w4_pairs(w, v);
+  w4_pairs<0x64006400u>(w, v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm("mul.bf16x2 %0, %1, %2;" : "=r"(r[i * stride]) : "r"(sub_bf16x2(v[i], z)), "r"(s));
+  for (int i = 0; i < 4; ++i) {
+    uint32_t d;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v[i]), "r"(z));
+    asm("mul.f16x2 %0, %1, %2;" : "=r"(r[i * stride]) : "r"(d), "r"(s));
+  }
 }
 
 // Which accumulator columns a unit uses.  Up to 64 records: one of two halves of
@@ -174,6 +192,27 @@ struct TcAcc {
     d1 = d0 + (small ? 64 : 128);
   }
 };
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Accumulator rows of this warp's lanes times `factor` of the lane's row: for the weight
+// rows that have a power of two of their own, which are rare.  (The same products in
+// the loop that takes the accumulators out cost it 15 % where there are none.)
+__device__ __noinline__ void tc_rescale(uint32_t taddr, int cols, float factor) {
+  for (int c = 0; c < cols; c += 16) {
+    uint32_t v[16];
+    tmem_ld16(taddr + c, v);
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
+    tmem_st_32x32b_x16(taddr + c, v);
+  }
+  tmem_wait_st();
+}
 
 // Units of the grid in turn: entry, 16-tile group, and whether there is work.
 struct TcUnit {
@@ -243,7 +282,7 @@ __device__ __forceinline__ void tc_block(uint32_t d, uint32_t at, uint32_t lo, u
                                          uint32_t idesc, bool add) {
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk)
-    tc_mma_bf16_ts(d, at + kk * 8, lo + 2 * kk, hi, idesc, kk != 0 || add ? 1u : 0u);
+    tc_mma_f16_ts(d, at + kk * 8, lo + 2 * kk, hi, idesc, kk != 0 || add ? 1u : 0u);
 }
 
 // HALVES: groups of 32, two to a block; ZEROS: zero points are kept.
@@ -368,13 +407,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               for (int i = 0; i < 2; ++i) {
                 if (HALVES || h == 0) {
                   const uint32_t r = rec + (tile0 + i) * args.rec_stride + h * (8 * kRec);
-                  uint32_t sv, zv = 0;  // scales of rows g, g + 8, and 128 + z
+                  uint32_t sv, zv = 0;  // scales of rows g, g + 8, and 1024 + z
                   if (ZEROS) lds64(r, sv, zv);
                   else sv = lds32(r);
                   sc[h][i][0] = __byte_perm(sv, 0, 0x1010);
                   sc[h][i][1] = __byte_perm(sv, 0, 0x3232);
-                  zp[h][i][0] = ZEROS ? __byte_perm(zv, 0, 0x1010) : 0x43084308u;
-                  zp[h][i][1] = ZEROS ? __byte_perm(zv, 0, 0x3232) : 0x43084308u;
+                  zp[h][i][0] = ZEROS ? __byte_perm(zv, 0, 0x1010) : 0x64086408u;
+                  zp[h][i][1] = ZEROS ? __byte_perm(zv, 0, 0x3232) : 0x64086408u;
                 } else {
 #pragma unroll
                   for (int k = 0; k < 2; ++k) {
@@ -447,7 +486,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       rows[r] = o;
-      s_scale[r] = !SWIGLU && o >= 0 && a.row_scale != nullptr ? a.row_scale[o] : 1.0f;
+      float scale = !SWIGLU && o >= 0 && a.row_scale != nullptr ? a.row_scale[o] : 1.0f;
+      if (o >= 0) {  // times the power of two of the record's activations
+        const int p = u.t.y + r, row = a.index != nullptr ? a.index[p] / a.index_div : p;
+        if (row >= 0 && row < a.act_rows)
+          scale *= a.act_factor[row] * a.row_factor[static_cast<size_t>(a.E) * a.m.tiles * 16 + u.t.x];
+      }
+      s_scale[r] = scale;
+      const bool wide = SWIGLU && a.out_f32 != nullptr;
+      // of this lane's two weight rows, gate and up or one of each operand
+      float own[2];
+#pragma unroll
+      for (int op = 0; op < 2; ++op) {
+        const int j = 32 * quarter + lane;
+        const int tile = u.m * kTcTiles + (SWIGLU ? j >> 3 : 8 * op + (j >> 4));
+        const int row = SWIGLU ? 8 * op + (j & 7) : j & 15;
+        own[op] = tile < a.m.tiles
+                      ? __ldg(a.row_factor + (static_cast<size_t>(u.t.x) * a.m.tiles + tile) * 16 + row)
+                      : 1.0f;
+      }
+      const bool rescale = __any_sync(0xffffffffu, own[0] != 1.0f || own[1] != 1.0f);
       ok = mbar_wait_idle(&acc_full[acc.first], acc.filled[acc.first] & 1u, abort_flag, a.status,
                      kErrTimeoutAccFull);
       ok = __all_sync(0xffffffffu, ok);
@@ -460,6 +518,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!ok) *store_stop = 1;
       named_barrier(1, 128);
       ok = *store_stop == 0;  // the four warps leave together: they meet at this barrier
+      if (rescale && ok) {
+        tc_rescale(tmem + lanes + acc.d0, cols, own[0]);
+        tc_rescale(tmem + lanes + acc.d1, cols, own[1]);
+      }
 #pragma unroll
       for (int part = 0; part < kOuts / 128; ++part) {
         if (ok && part * 128 < outs) {
@@ -467,10 +529,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // records down the staging rows: the fragments go through transposing stores
           const uint32_t dst = stage + ((lane >> 4) * 8 + (lane & 7)) * kOutRow +
                                (128 * part + 32 * quarter + ((lane >> 3) & 1) * 8) * 2;
+          // fp32 rows: this lane's first output in its column 2t of the record
+          float* to = a.out_f32 + static_cast<size_t>(u.t.y + 2 * (lane & 3)) * a.out_ld + first +
+                      32 * quarter + (lane >> 2);
+          if (wide && 32 * quarter >= outs) continue;  // outs is a multiple of 64
           for (int c = 0; c < cols; c += 16) {
             uint32_t v[2][8];
             tmem_ld_16x256b_x2(d + c, v[0]);
             tmem_ld_16x256b_x2(d + (16u << 16) + c, v[1]);
+            const float* sc = s_scale + c + 2 * (lane & 3);
+            const float2 s0 = *reinterpret_cast<const float2*>(sc);
+            const float2 s1 = *reinterpret_cast<const float2*>(sc + 8);
+            // value i of a fragment: column (i & 1) of 2t, 2t + 1, row g + 8 ((i >> 1) & 1),
+            // columns 8 on from i = 4
+            auto scaled = [&](uint32_t x, int i) {
+              const float2 sv = (i & 4) != 0 ? s1 : s0;
+              return __uint_as_float(x) * ((i & 1) != 0 ? sv.y : sv.x);
+            };
             if constexpr (SWIGLU) {
               uint32_t up[2][8];
               tmem_ld_16x256b_x2(tmem + lanes + acc.d1 + c, up[0]);
@@ -478,19 +553,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tc_wait_ld();
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                v[i >> 3][i & 7] = __float_as_uint(silu_f(__uint_as_float(v[i >> 3][i & 7])) *
-                                                   __uint_as_float(up[i >> 3][i & 7]));
+                v[i >> 3][i & 7] = __float_as_uint(silu_f(scaled(v[i >> 3][i & 7], i)) *
+                                                   scaled(up[i >> 3][i & 7], i));
+              if (wide) {
+                // straight from the registers: eight lanes write 32 bytes of a record's row
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // columns 2t, 2t + 1, 8 on
+                  const int col = (k & 1) + 8 * (k >> 1);
+                  if (c + 2 * (lane & 3) + col < n) {
+                    float* p = to + col * a.out_ld;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m)  // rows g, g + 8, 16 on
+                      p[8 * m] = __uint_as_float(v[m >> 1][(k & 1) + 2 * (m & 1) + 4 * (k >> 1)]);
+                  }
+                }
+                to += 16 * a.out_ld;
+                continue;
+              }
             } else {
-              const float* sc = s_scale + c + 2 * (lane & 3);
-              const float2 s0 = *reinterpret_cast<const float2*>(sc);
-              const float2 s1 = *reinterpret_cast<const float2*>(sc + 8);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 sv = (i & 4) != 0 ? s1 : s0;
-                v[i >> 3][i & 7] = __float_as_uint(__uint_as_float(v[i >> 3][i & 7]) *
-                                                   ((i & 1) != 0 ? sv.y : sv.x));
-              }
+              for (int i = 0; i < 16; ++i)
+                v[i >> 3][i & 7] = __float_as_uint(scaled(v[i >> 3][i & 7], i));
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -515,7 +599,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // gate/up, where nobody waits for the stores.)
       constexpr int kPer = kOuts / 8;
       const int v = r % kPer;
-      if (ok && v * 8 < outs) {
+      if (ok && v * 8 < outs && !wide) {
         const uint32_t src = stage + v * 16;
         __nv_bfloat16* dst = a.out + first + v * 8;
         for (int c = r / kPer; c < n; c += 4 * (128 / kPer)) {  // four rows in flight
@@ -687,7 +771,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!__all_sync(0xffffffffu, ok && *abort_flag == 0)) break;
       issued = acc.first;
       ++acc.filled[issued];
-      const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>(cols));
+      const uint32_t idesc = idesc_f16_f32(128, static_cast<uint32_t>(cols));
       const bool rows = op == 0 || SWIGLU || u.m * kTcTiles + 8 < a.m.tiles;  // of this operand
       const uint32_t d = tmem + (op == 0 ? acc.d0 : acc.d1);
       const uint32_t acc_bar = acc_full0 + issued * 8;
@@ -751,8 +835,90 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
+// Rows of activations as fp16 multiples of a power of two of the row, which puts its
+// largest value into [2^14, 2^15): a bf16 value down to 2^-31 of it stays exact, an fp32 one
+// is rounded by 2^-12 at most down to 2^-28, by 2^-39 of the largest below.  A row with an
+// infinity or a NaN keeps its values as they are.  dst may be src (fp32): a warp writes a
+// chunk of 4 KB below what it has read.  A warp for a row; HBM bounds it (6000 x 2048 bf16
+// 9 us, 49 MB).
+template <bool F32>
+__global__ void __launch_bounds__(256) w4_rows_f16(const uint8_t* src, long long src_pitch, int rows,
+                                                   const int* count, int vec, uint8_t* dst,
+                                                   long long dst_pitch, float* factor) {
+  constexpr int kHold = 8;  // 16-byte vectors of a lane at once
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int total = count != nullptr ? max(0, min(rows, *count)) : rows;
+  for (long long row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < total; row += gridDim.x * 8ll) {
+    const uint4* in = reinterpret_cast<const uint4*>(src + row * src_pitch);
+    uint8_t* out = dst + row * dst_pitch;
+    uint4 v[kHold];
+    auto load = [&](int base) {
+#pragma unroll
+      for (int j = 0; j < kHold; ++j) {
+        const int at = base + lane + 32 * j;
+        v[j] = at < vec ? in[at] : make_uint4(0, 0, 0, 0);
+      }
+    };
+    uint32_t top = 0;  // the largest magnitude's bits
+    for (int base = 0; base < vec; base += 32 * kHold) {
+      load(base);
+#pragma unroll
+      for (int j = 0; j < kHold; ++j) {
+        const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top = F32 ? max(top, w[i] & 0x7fffffffu) : __vmaxu2(top, w[i] & 0x7fff7fffu);
+      }
+    }
+    if (!F32) top = max(top & 0xffffu, top >> 16) << 16;
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int e = static_cast<int>(top >> 23);  // biased exponent
+    const int shift = e == 255 ? 0 : min(141 - e, 126);
+    const float mul = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+    if (lane == 0) factor[row] = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+    for (int base = 0; base < vec; base += 32 * kHold) {
+      if (vec > 32 * kHold) load(base);
+      __syncwarp();  // the whole chunk is read
+#pragma unroll
+      for (int j = 0; j < kHold; ++j) {
+        const int at = base + lane + 32 * j;
+        const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+        if (F32) {
+          if (at < vec)
+            *reinterpret_cast<uint2*>(out + at * 8) =
+                make_uint2(pack_f16x2(__uint_as_float(w[0]) * mul, __uint_as_float(w[1]) * mul),
+                           pack_f16x2(__uint_as_float(w[2]) * mul, __uint_as_float(w[3]) * mul));
+        } else if (at < vec) {
+          uint32_t o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            o[i] = pack_f16x2(__uint_as_float(w[i] << 16) * mul,
+                              __uint_as_float(w[i] & 0xffff0000u) * mul);
+          *reinterpret_cast<uint4*>(out + at * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+      __syncwarp();
+    }
+  }
+}
+
+template <bool F32>
+int rows_f16(const void* src, int rows, const int* count, int columns, void* dst,
+             long long dst_pitch, float* factor, cudaStream_t stream) {
+  const int vec = columns / (F32 ? 4 : 8);
+  const int grid = std::min((rows + 7) / 8, 8 * device_sm_count());
+  return note_cuda_error(launch_pdl(w4_rows_f16<F32>, dim3(grid), dim3(256), 0, stream,
+                                    static_cast<const uint8_t*>(src),
+                                    static_cast<long long>(columns) * (F32 ? 4 : 2), rows, count, vec,
+                                    static_cast<uint8_t*>(dst), dst_pitch, factor)) == cudaSuccess
+             ? kRcOk
+             : kRcCudaError;
+}
+
 template <bool SWIGLU, bool HALVES, bool ZEROS>
-int tc_launch(const W4Args& a, cudaStream_t stream) {
+int tc_launch(const W4Args& a, long long pitch, cudaStream_t stream) {
   TcArgs t{};
   t.a = a;
   t.rec_stride = (4 >> a.m.gshift) * 8 * a.m.rec;
@@ -771,7 +937,7 @@ int tc_launch(const W4Args& a, cudaStream_t stream) {
                     kTcBlocks * kW4BlockBytes / 8, kTcTiles);
   if (rc == kRcOk)
     rc = map_rows(&records, a.m.s, 4, a.m.ng * 8 * a.m.rec / 4, rows, t.rec_stride / 4, kTcTiles);
-  if (rc == kRcOk) rc = map_gather_rows(&act, a.act, a.act_rows, a.m.nb * 64);
+  if (rc == kRcOk) rc = map_gather_rows(&act, a.act, a.act_rows, a.m.nb * 64, pitch);
   if (rc != kRcOk) return rc;
   const long long units =
       static_cast<long long>(a.max_tiles) * ((a.m.tiles + kTcTiles - 1) / kTcTiles);
@@ -783,18 +949,29 @@ int tc_launch(const W4Args& a, cudaStream_t stream) {
 }
 
 template <bool SWIGLU>
-int tc_dispatch(const W4Args& a, cudaStream_t stream) {
+int tc_dispatch(const W4Args& a, long long pitch, cudaStream_t stream) {
   if (a.m.gshift == 0)
-    return a.m.rec == 8 ? tc_launch<SWIGLU, true, true>(a, stream)
-                        : tc_launch<SWIGLU, true, false>(a, stream);
-  return a.m.rec == 8 ? tc_launch<SWIGLU, false, true>(a, stream)
-                      : tc_launch<SWIGLU, false, false>(a, stream);
+    return a.m.rec == 8 ? tc_launch<SWIGLU, true, true>(a, pitch, stream)
+                        : tc_launch<SWIGLU, true, false>(a, pitch, stream);
+  return a.m.rec == 8 ? tc_launch<SWIGLU, false, true>(a, pitch, stream)
+                      : tc_launch<SWIGLU, false, false>(a, pitch, stream);
 }
 
 }  // namespace
 
-int w4_gemm(const W4Args& a, bool swiglu, cudaStream_t stream) {
-  return swiglu ? tc_dispatch<true>(a, stream) : tc_dispatch<false>(a, stream);
+int w4_gemm(W4Args a, bool swiglu, const W4Rows& rows, bool f32, cudaStream_t stream) {
+  const int columns = 64 * a.m.nb;
+  // fp32 rows turn into fp16 ones in the first half of their place
+  void* f16 = f32 ? const_cast<uint32_t*>(a.act) : rows.f16;
+  const long long pitch = static_cast<long long>(columns) * (f32 ? 4 : 2);
+  const int rc = f32 ? rows_f16<true>(a.act, a.act_rows, rows.count, columns, f16, pitch,
+                                      rows.factor, stream)
+                     : rows_f16<false>(a.act, a.act_rows, rows.count, columns, f16, pitch,
+                                       rows.factor, stream);
+  if (rc != kRcOk) return rc;
+  a.act = static_cast<const uint32_t*>(f16);
+  a.act_factor = rows.factor;
+  return swiglu ? tc_dispatch<true>(a, pitch, stream) : tc_dispatch<false>(a, pitch, stream);
 }
 
 }  // namespace moe

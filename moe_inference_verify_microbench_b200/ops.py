@@ -668,6 +668,15 @@ def _output(out: torch.Tensor | None, shape, device: torch.device) -> torch.Tens
     return out
 
 
+def _rows_workspace(M: int, bank, rows: int, columns: int, device: torch.device):
+    """Room for ``rows`` of activations in fp16, which products of at least 8 records per
+    expert read (kW4TcRecords)."""
+    if M // bank.num_experts < 8:
+        return None
+    need = _native.load().moe_w4_grouped_workspace_bytes(rows, columns)
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
 def grouped_w13_swiglu_w4(a: torch.Tensor, tiles: torch.Tensor, num_tiles: torch.Tensor,
                           max_tiles_: int, bank, index: torch.Tensor | None = None,
                           index_div: int = 1, M: int | None = None,
@@ -692,10 +701,12 @@ def grouped_w13_swiglu_w4(a: torch.Tensor, tiles: torch.Tensor, num_tiles: torch
             raise ValueError("a must hold at least M rows")
     _same_device(dev, tiles=tiles, num_tiles=num_tiles, index=index)
     h = _output(out, (M, bank.intermediate), dev)
+    ws = _rows_workspace(M, bank, *a.shape, dev)
     with _on(dev):
-        _rc(_native.load().moe_grouped_w13_swiglu_w4(
+        _rc(_native.load().moe_grouped_w13_swiglu_w4_ex(
             _p(a), a.shape[0], _p(index), index_div, M, _p(tiles), _p(num_tiles), max_tiles_,
-            bank.native, _p(h), _p(status_word(dev)), _stream(dev)), "moe_grouped_w13_swiglu_w4")
+            bank.native, _p(h), _p(ws), 0 if ws is None else ws.nbytes, _p(status_word(dev)),
+            _stream(dev)), "moe_grouped_w13_swiglu_w4_ex")
     return h
 
 
@@ -725,11 +736,12 @@ def grouped_w2_w4(h: torch.Tensor, tiles: torch.Tensor, num_tiles: torch.Tensor,
             raise ValueError("slot_scale must hold an entry for every row of out")
     _same_device(dev, tiles=tiles, num_tiles=num_tiles, row_map=row_map, slot_scale=slot_scale)
     out = _output(out, (rows, bank.hidden), dev)
+    ws = _rows_workspace(M, bank, M, I, dev)
     with _on(dev):
-        _rc(_native.load().moe_grouped_w2_w4(
+        _rc(_native.load().moe_grouped_w2_w4_ex(
             _p(h), M, _p(tiles), _p(num_tiles), max_tiles_, bank.native, _p(row_map),
-            _p(slot_scale), _p(out), rows, _p(status_word(dev)), _stream(dev)),
-            "moe_grouped_w2_w4")
+            _p(slot_scale), _p(out), rows, _p(ws), 0 if ws is None else ws.nbytes,
+            _p(status_word(dev)), _stream(dev)), "moe_grouped_w2_w4_ex")
     return out
 
 

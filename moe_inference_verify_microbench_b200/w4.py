@@ -7,11 +7,13 @@ and zero points in 0..15 (zero point 8 throughout where none are kept).  The
 bank holds the three projections in the layout the kernels stream
 (``moe_w4_pack`` in the C ABI): gate and up interleaved by eight rows, 16-row
 tiles of 64-column blocks.  It takes 0.5 byte and the group's share of a scale
-per weight (``3 * H * I * (1/2 + 2/group)`` bytes per expert without zero points).
+per weight, the scales twice, as bf16 and as fp16 multiples of powers of two
+(``3 * H * I * (1/2 + 4/group)`` bytes per expert without zero points, and 4 per row).
 
-The kernels multiply activations by 128 + code (or by the rounded weight) and sum in
-fp32, so K * 144 * |x| has to stay below 3.4e38; an infinity or a NaN in a row makes the
-outputs of that row NaN or infinite and no other's.
+The kernels multiply activations by 128 + code, or from 8 records per expert on by the
+weight in fp16 (rounded by 2^-12 of it at most), and sum in fp32, so K * 144 * |x| has to
+stay below 3.4e38; an infinity or a NaN in a row makes the outputs of that row NaN or
+infinite and no other's.
 
 Build it once when the weights are loaded, from codes (``from_codes``) or from
 bf16 weights (``quantize``); the ops that take it are ``ops.moe_layer_w4``,
@@ -84,13 +86,16 @@ class W4Experts:
 
     def __init__(self, w13, w2, num_experts: int, hidden: int, intermediate: int,
                  group_size: int, has_zeros: bool) -> None:
-        """Use ``from_codes`` or ``quantize``; w13 and w2 are packed (q, s)."""
+        """Use ``from_codes`` or ``quantize``; w13 and w2 are packed (q, s, f, r), codes and
+        scales and the scales again as products of many records read them."""
         self.w13, self.w2 = w13, w2
         self.num_experts, self.hidden, self.intermediate = num_experts, hidden, intermediate
         self.group_size, self.has_zeros = group_size, has_zeros
         self.device = w13[0].device
-        self._struct = _native.W4BankStruct(*(t.data_ptr() for t in (*w13, *w2)), num_experts,
-                                            hidden, intermediate, group_size, int(has_zeros))
+        fine = [t.data_ptr() for t in (*w13[2:], *w2[2:])]
+        self._struct = _native.W4BankStruct(
+            *(t.data_ptr() for t in (*w13[:2], *w2[:2])), num_experts, hidden, intermediate,
+            group_size, int(has_zeros) | (_native.W4_FINE if fine else 0), *fine)
         self.native = ctypes.addressof(self._struct)  # const moe_w4_bank*
 
     def __getstate__(self):
@@ -181,16 +186,20 @@ def _pack(first, second, group: int, status: torch.Tensor, into=None):
     E, N, K = codes.shape
     M = N if second is None else 2 * N
     dev = codes.device
-    q, s = into if into is not None else (
+    records = E * M * (K // group) * (1 if zeros is None else 2)
+    q, s, f, r = into if into is not None else (
         torch.empty(E * M * K // 2, dtype=torch.uint8, device=dev),
-        torch.empty(E * M * (K // group) * (1 if zeros is None else 2), dtype=torch.bfloat16,
-                    device=dev))
+        torch.empty(records, dtype=torch.bfloat16, device=dev),
+        torch.empty(records, dtype=torch.float16, device=dev),
+        torch.empty(E * (M + 1), dtype=torch.float32, device=dev))
     p = ops._p
     c1, s1, z1 = second if second is not None else (None, None, None)
     ops._rc(_native.load().moe_w4_pack(p(codes), p(scales), p(zeros), p(c1), p(s1), p(z1), E, N, K,
                                        group, p(q), p(s), p(status), ops._stream(dev)),
             "moe_w4_pack")
-    return q, s
+    ops._rc(_native.load().moe_w4_pack_fine(p(scales), p(zeros), p(s1), p(z1), E, N, K, group,
+                                            p(f), p(r), ops._stream(dev)), "moe_w4_pack_fine")
+    return q, s, f, r
 
 
 ops._W4Experts = W4Experts

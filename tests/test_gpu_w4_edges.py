@@ -9,7 +9,8 @@ import torch
 
 import test_gpu_w4 as w4
 import w4_reference as ref
-from moe_inference_verify_microbench_b200 import PermutedSparseMoE, fused_moe_forward_w4, ops, quantize_w4
+from moe_inference_verify_microbench_b200 import (PermutedSparseMoE, W4Experts,
+                                                  fused_moe_forward_w4, ops, quantize_w4)
 from test_gpu_w4 import bank_of, close, rms_close, rows
 from test_gpu_w4_layers import module
 
@@ -376,3 +377,160 @@ def test_non_finite_rows_in_the_layer(cuda, T):
     ops.check_status(cuda)
     assert torch.equal(y[1:T - 1], clean[1:T - 1])
     assert not bool(torch.isfinite(y[[0, T - 1]].float()).any())
+
+
+# ------------------------------------------------------------------ what the forms round
+
+
+FINE = 2.0 ** -12  # a weight, or a value of h, in fp16
+
+
+def fine_down(m, v, h, e):
+    """o = h Wd^T of expert e in 64 bits, and the bound of the tensor-memory form: fp32 sums,
+    weights in fp16, activations of which fp16 holds all that is 2^-25 of the row's largest."""
+    o = h.double() @ v[e].t()
+    top = h.double().abs().amax(1, keepdim=True)
+    return o, (ref.ACC * ref.operand_sums(m, h, e) + FINE * (h.double().abs() @ v[e].abs().t())
+               + 2.0 ** -39 * top * v[e].abs().sum(1) + 2.0 ** -133)
+
+
+def many(E, seed=0):
+    """Offsets of at least TC_RECORDS rows per expert on average, ragged."""
+    gen = torch.Generator().manual_seed(seed)
+    c = torch.randint(0, 150, (E,), generator=gen)
+    c[0], c[-1] = 129, 0
+    return torch.cat([c.new_zeros(1), c.cumsum(0)])
+
+
+@pytest.mark.parametrize("E,H,I,group,zeros", [(4, 256, 128, 64, True), (6, 2048, 768, 128, False),
+                                               (3, 512, 192, 32, True), (2, 1024, 8192, 64, False)])
+def test_many_records_do_not_round_the_weights_to_bf16(cuda, E, H, I, group, zeros):
+    """Each product of many records is as near to 64 bits as its output's type lets it be."""
+    p = ref.parts(E, H, I, group, zeros, seed=E, device=cuda)
+    bank = bank_of(p)
+    off = many(E).to(cuda)
+    M = int(off[-1])
+    assert M // E >= ref.TC_RECORDS
+    x, hin = rows(M, H, 7, cuda), rows(M, I, 8, cuda)
+    tiles, num, mt = ops.tiles_from_offsets(off, M)
+    h = ops.grouped_w13_swiglu_w4(x, tiles, num, mt, bank)
+    out = ops.grouped_w2_w4(hin, tiles, num, mt, bank)
+    y = ops.sorted_experts_w4(x, off, bank)
+    ops.check_status(cuda)
+    vg, vu, vd = (ref.values(m) for m in p)
+    for e in range(E):
+        a, z = int(off[e]), int(off[e + 1])
+        if a == z:
+            continue
+        g, u = x[a:z].double() @ vg[e].t(), x[a:z].double() @ vu[e].t()
+        want = g * torch.sigmoid(g) * u
+        rms_close(h[a:z], want, "h", False, f"h of expert {e}")
+        o, do = fine_down(p[2], vd, hin[a:z], e)
+        close(out[a:z], o, ref.BF16 * o.abs() + 1.01 * do, f"out of expert {e}")
+        rms_close(out[a:z], o, "out", False, f"out of expert {e}")
+        rms_close(y[a:z], want @ vd[e].t(), "out", False, f"rows of expert {e}")
+
+
+@pytest.mark.parametrize("T,k", [(60, 2), (700, 3)])
+def test_experts_of_many_records_round_twice(cuda, T, k):
+    """The slot rows and the result, but neither the weights nor h, are rounded to bf16."""
+    E, H, I = 4, 512, 256
+    p = ref.parts(E, H, I, 64, True, seed=T, device=cuda)
+    gen = torch.Generator().manual_seed(T)
+    ids = torch.rand((T, E), generator=gen).argsort(1)[:, :k].int().contiguous().to(cuda)
+    w = torch.rand((T, k), generator=gen).to(cuda)
+    x = rows(T, H, 2, cuda)
+    y = ops.experts_w4(x, ids, w, bank_of(p))
+    ops.check_status(cuda)
+    want, _ = ref.experts(p, x, ids, w)
+    rel = ((y.double() - want).norm() / want.norm()).item()
+    assert rel <= ref.BF16 * (2 / 3) ** 0.5 + 2.0 ** -12
+
+
+@pytest.mark.parametrize("peak", [1e-30, 1e-3, 3e4, 1e30])
+@pytest.mark.parametrize("group,zeros", [(64, False), (32, True)])
+def test_activation_range_of_many_records(cuda, peak, group, zeros):
+    """Rows of any magnitude that bf16 holds, rows of zeros, channels 2^20 times the others."""
+    E, H, I = 2, 512, 128
+    p = ref.parts(E, H, I, group, zeros, device=cuda)
+    off = torch.tensor([0, 50, 120], device=cuda)
+    h = rows(120, I, 8, cuda).float() * peak
+    h[3] = 0.0
+    h[6, 9] *= 2.0 ** 20 if peak < 1e10 else 1.0
+    h[7, ::2] *= 2.0 ** -20 if peak > 1e-10 else 1.0
+    h[60:70] *= 2.0 ** -60 if peak > 1e10 else 1.0
+    h = h.bfloat16()
+    tiles, num, mt = ops.tiles_from_offsets(off, 120)
+    out = ops.grouped_w2_w4(h, tiles, num, mt, bank_of(p))
+    ops.check_status(cuda)
+    vd = ref.values(p[2])
+    for e in range(E):
+        a, z = int(off[e]), int(off[e + 1])
+        o, do = fine_down(p[2], vd, h[a:z], e)
+        close(out[a:z], o, ref.BF16 * o.abs() + 1.01 * do, f"expert {e}")
+
+
+@pytest.mark.parametrize("T", [12, 120])
+@pytest.mark.parametrize("group,zeros", [(128, False), (64, True), (32, False)])
+def test_scales_of_any_size(cuda, T, group, zeros):
+    """Experts, rows and groups whose scales are powers of two apart, rows of zeros, negative
+    scales: every row keeps its own relative error in both forms of the products."""
+    E, H, I = 2, 512, 256
+    p = ref.parts(E, H, I, group, zeros, seed=group, device=cuda)
+    gen = torch.Generator().manual_seed(T)
+    for m in (0, 1, 2):
+        codes, s, z = p[m]
+        n = s.shape[1]
+        by_row = torch.randint(-40, 8, (1, n, 1), generator=gen).double()
+        by_row[:, ::3] = 0.0
+        by_group = torch.randint(-6, 3, (E, n, s.shape[2]), generator=gen).double()
+        by_expert = torch.tensor([0.0, -30.0 if m else 20.0]).view(E, 1, 1).double()
+        f = torch.exp2(by_row + by_group + by_expert).to(cuda)
+        f[:, 5] = 0.0
+        f[:, 7] *= -1.0
+        s.copy_((s.double() * f).bfloat16())
+    bank = bank_of(p)
+    off = torch.tensor([0, T // 2, T], device=cuda)
+    x, hin = rows(T, H, 7, cuda), rows(T, I, 8, cuda)
+    tiles, num, mt = ops.tiles_from_offsets(off, T)
+    h = ops.grouped_w13_swiglu_w4(x, tiles, num, mt, bank)
+    out = ops.grouped_w2_w4(hin, tiles, num, mt, bank)
+    y = ops.sorted_experts_w4(x, off, bank)
+    ops.check_status(cuda)
+    vg, vu, vd = (ref.values(m) for m in p)
+    for e in range(E):
+        a, z = int(off[e]), int(off[e + 1])
+        want, bound = ref.swiglu_rows(p[0], p[1], vg, vu, x[a:z], e, False)
+        g, u = x[a:z].double() @ vg[e].t(), x[a:z].double() @ vu[e].t()
+        fg, fu = (FINE * (x[a:z].double().abs() @ v[e].abs().t()) for v in (vg, vu))
+        wide = bound + 1.1 * fg * (u.abs() + fu) + (g * torch.sigmoid(g)).abs() * fu + 2.0 ** -133
+        close(h[a:z], want, wide * 1.01, f"h of expert {e}")
+        o, do = fine_down(p[2], vd, hin[a:z], e)
+        close(out[a:z], o, ref.BF16 * o.abs() + 1.01 * do, f"out of expert {e}")
+        # h in bf16 (few rows) or fp16 of the row's largest value (many), then the down product
+        dh = wide * 1.01 + 2.0 ** -39 * want.abs().amax(1, keepdim=True)
+        ws, ds = fine_down(p[2], vd, want, e)
+        close(y[a:z], ws, ref.BF16 * ws.abs() + 1.02 * (ds + dh @ vd[e].abs().t()), f"y of expert {e}")
+
+
+def test_many_records_on_a_bank_without_fine_scales(cuda):
+    """A bank of codes and scales alone, as a caller of the C ABI may pack it: products of
+    many records stream, with the weights exact."""
+    E, H, I = 4, 256, 192
+    p = ref.parts(E, H, I, 64, True, device=cuda)
+    full = bank_of(p)
+    plain = W4Experts(full.w13[:2], full.w2[:2], E, H, I, 64, True)
+    off = many(E).to(cuda)
+    M = int(off[-1])
+    x = rows(M, H, 3, cuda)
+    y, z = (ops.sorted_experts_w4(x, off, b) for b in (plain, full))
+    ops.check_status(cuda)
+    owner = torch.repeat_interleave(torch.arange(E, device=cuda), off.diff())
+    want, bound = ref.experts(p, x, owner[:, None], torch.ones((M, 1), device=cuda))
+    close(y, want, bound)
+    close(z, want, bound)
+    rms_close(y, z.double(), "y", False)
+    tiles, num, mt = ops.tiles_from_offsets(off, M)
+    h = ops.grouped_w13_swiglu_w4(x, tiles, num, mt, plain)
+    rms_close(h, ops.grouped_w13_swiglu_w4(x, tiles, num, mt, full).double(), "y", False)
+    ops.check_status(cuda)
