@@ -908,7 +908,7 @@ template <bool F32>
 int rows_f16(const void* src, int rows, const int* count, int columns, void* dst,
              long long dst_pitch, float* factor, cudaStream_t stream) {
   const int vec = columns / (F32 ? 4 : 8);
-  const int grid = std::min((rows + 7) / 8, 8 * device_sm_count());
+  const int grid = std::min(rows / 8 + 1, 8 * device_sm_count());
   return note_cuda_error(launch_pdl(w4_rows_f16<F32>, dim3(grid), dim3(256), 0, stream,
                                     static_cast<const uint8_t*>(src),
                                     static_cast<long long>(columns) * (F32 ? 4 : 2), rows, count, vec,

@@ -534,3 +534,32 @@ def test_many_records_on_a_bank_without_fine_scales(cuda):
     h = ops.grouped_w13_swiglu_w4(x, tiles, num, mt, plain)
     rms_close(h, ops.grouped_w13_swiglu_w4(x, tiles, num, mt, full).double(), "y", False)
     ops.check_status(cuda)
+    # the C calls without a workspace stream too, on any bank
+    q, lib = ops._p, ops._native.load()
+    again = torch.empty_like(h)
+    assert lib.moe_grouped_w13_swiglu_w4(q(x), M, None, 1, M, q(tiles), q(num), mt, full.native,
+                                         q(again), q(ops.status_word(cuda)), ops._stream(cuda)) == 0
+    assert torch.equal(again, h)
+    out = ops.grouped_w2_w4(h, tiles, num, mt, plain)
+    again = torch.empty_like(out)
+    assert lib.moe_grouped_w2_w4(q(h), M, q(tiles), q(num), mt, full.native, None, None, q(again),
+                                 M, q(ops.status_word(cuda)), ops._stream(cuda)) == 0
+    assert torch.equal(again, out)
+    ops.check_status(cuda)
+
+
+@pytest.mark.parametrize("T", [23, 24, 31, 32, 33])
+def test_shard_beside_the_choice_of_form(cuda, T):
+    """Many records for each expert that the bank holds, but few for each of all experts, and
+    the first batches on the other side: the workspace serves both."""
+    E, H, I, k = 4, 256, 128, 4
+    p = ref.parts(E, H, I, 64, True, seed=T, device=cuda)
+    bank = bank_of(p)
+    gen = torch.Generator().manual_seed(T)
+    ids = torch.rand((T, 16), generator=gen).argsort(1)[:, :k].int().contiguous().to(cuda)
+    w = torch.randn((T, k), generator=gen).to(cuda)
+    x = rows(T, H, 2, cuda)
+    ws = torch.empty(ops.experts_w4_workspace_bytes(T, k, bank), dtype=torch.uint8, device=cuda)
+    y = ops.experts_w4(x, ids, w, bank, num_experts=16, e_begin=6, workspace=ws)
+    ops.check_status(cuda)
+    close(y, *ref.experts(p, x, ids, w, e_begin=6, num_experts=16))
