@@ -199,8 +199,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 
-// Accumulator rows of this warp's lanes times `factor` of the lane's row: for the weight
-// rows that have a power of two of their own, which are rare.  (The same products in
+// Accumulator rows of this warp's lanes times `factor` of the lane's row: for weight rows
+// that have a power of two of their own, or an expert whose scales are all below 2^-26 or
+// reach 2^24, which are rare.  (The same products in
 // the loop that takes the accumulators out cost it 15 % where there are none.)
 __device__ __noinline__ void tc_rescale(uint32_t taddr, int cols, float factor) {
   for (int c = 0; c < cols; c += 16) {
@@ -487,10 +488,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       rows[r] = o;
       float scale = !SWIGLU && o >= 0 && a.row_scale != nullptr ? a.row_scale[o] : 1.0f;
-      if (o >= 0) {  // times the power of two of the record's activations
+      // Times the powers of two of the record's activations (2^-112 to 2^113) and of the
+      // expert's scales, unless the two might leave fp32's range together.
+      const float base = a.row_factor[static_cast<size_t>(a.E) * a.m.tiles * 16 + u.t.x];
+      const bool far = base < 0x1p-36f || base > 0x1p14f;
+      if (o >= 0) {
         const int p = u.t.y + r, row = a.index != nullptr ? a.index[p] / a.index_div : p;
-        if (row >= 0 && row < a.act_rows)
-          scale *= a.act_factor[row] * a.row_factor[static_cast<size_t>(a.E) * a.m.tiles * 16 + u.t.x];
+        if (row >= 0 && row < a.act_rows) scale *= a.act_factor[row] * (far ? 1.0f : base);
       }
       s_scale[r] = scale;
       const bool wide = SWIGLU && a.out_f32 != nullptr;
@@ -504,6 +508,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         own[op] = tile < a.m.tiles
                       ? __ldg(a.row_factor + (static_cast<size_t>(u.t.x) * a.m.tiles + tile) * 16 + row)
                       : 1.0f;
+        if (far) own[op] *= base;
       }
       const bool rescale = __any_sync(0xffffffffu, own[0] != 1.0f || own[1] != 1.0f);
       ok = mbar_wait_idle(&acc_full[acc.first], acc.filled[acc.first] & 1u, abort_flag, a.status,
@@ -836,7 +841,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // Rows of activations as fp16 multiples of a power of two of the row, which puts its
-// largest value into [2^14, 2^15): a bf16 value down to 2^-31 of it stays exact, an fp32 one
+// largest value into [2^14, 2^15) (if that is 2^-98 or more; the power is 2^-112 at least): a bf16 value down to 2^-31 of it stays exact, an fp32 one
 // is rounded by 2^-12 at most down to 2^-28, by 2^-39 of the largest below.  A row with an
 // infinity or a NaN keeps its values as they are.  dst may be src (fp32): a warp writes a
 // chunk of 4 KB below what it has read.  A warp for a row; HBM bounds it (6000 x 2048 bf16
@@ -875,7 +880,7 @@ __global__ void __launch_bounds__(256) w4_rows_f16(const uint8_t* src, long long
     if (!F32) top = max(top & 0xffffu, top >> 16) << 16;
     top = __reduce_max_sync(0xffffffffu, top);
     const int e = static_cast<int>(top >> 23);  // biased exponent
-    const int shift = e == 255 ? 0 : min(141 - e, 126);
+    const int shift = e == 255 ? 0 : min(141 - e, 112);
     const float mul = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
     if (lane == 0) factor[row] = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
     for (int base = 0; base < vec; base += 32 * kHold) {

@@ -152,7 +152,7 @@ class W4Experts:
             raise ValueError("codes, scales and zero points must be on one device")
         with torch.cuda.device(dev):
             status = torch.zeros(1, dtype=torch.int32, device=dev)
-            same = into is not None and (E, H, I, group, gz is not None, dev) == (
+            same = into is not None and len(into.w13) == 4 and (E, H, I, group, gz is not None, dev) == (
                 into.num_experts, into.hidden, into.intermediate, into.group_size,
                 into.has_zeros, into.device)
             w13 = _pack((gc, gs, gz), (uc, us, uz), group, status, into.w13 if same else None)

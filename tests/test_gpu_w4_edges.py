@@ -513,6 +513,35 @@ def test_scales_of_any_size(cuda, T, group, zeros):
         close(y[a:z], ws, ref.BF16 * ws.abs() + 1.02 * (ds + dh @ vd[e].abs().t()), f"y of expert {e}")
 
 
+@pytest.mark.parametrize("x_exp,s_exp", [(-112, 20), (-100, -8), (-108, -28), (-60, -60), (0, -90),
+                                         (0, 40), (90, 12), (118, -30), (60, 30)])
+def test_far_ranges_of_many_records(cuda, x_exp, s_exp):
+    """Activations and scales that lie far out on either side, together with rows of zeros on
+    both: results that bf16 holds are right, and zeros stay zeros."""
+    E, H, I = 2, 256, 128
+    p = ref.parts(E, H, I, 64, True, device=cuda)
+    codes, scales, zeros = p[2]
+    scales.copy_((scales.double() * 2.0 ** s_exp).bfloat16())
+    codes[:, 3] = zeros[:, 3].repeat_interleave(64, -1)  # weights of zero under large scales
+    scales[:, 9] = 0.0
+    bank = bank_of(p)
+    off = torch.tensor([0, 30, 70], device=cuda)
+    h = rows(70, I, 8, cuda).double() * 2.0 ** x_exp
+    h[2] = 0.0
+    h[33, 1:] = 0.0
+    h = h.bfloat16()
+    tiles, num, mt = ops.tiles_from_offsets(off, 70)
+    out = ops.grouped_w2_w4(h, tiles, num, mt, bank)
+    ops.check_status(cuda)
+    assert not bool(out[2].any()) and not bool(out[:, 3].any()) and not bool(out[:, 9].any())
+    vd = ref.values(p[2])
+    for e in range(E):
+        a, z = int(off[e]), int(off[e + 1])
+        o, do = fine_down(p[2], vd, h[a:z], e)
+        assert bool((o.abs() < 3e38).all())
+        close(out[a:z], o, ref.BF16 * o.abs() + 1.01 * do, f"expert {e}")
+
+
 def test_many_records_on_a_bank_without_fine_scales(cuda):
     """A bank of codes and scales alone, as a caller of the C ABI may pack it: products of
     many records stream, with the weights exact."""
@@ -563,3 +592,16 @@ def test_shard_beside_the_choice_of_form(cuda, T):
     y = ops.experts_w4(x, ids, w, bank, num_experts=16, e_begin=6, workspace=ws)
     ops.check_status(cuda)
     close(y, *ref.experts(p, x, ids, w, e_begin=6, num_experts=16))
+
+
+def test_bank_into_another(cuda):
+    """The memory of a bank of the same sizes and form is taken over; of any other it is not."""
+    p, q = (ref.parts(2, 128, 64, 32, True, seed=s, device=cuda) for s in (0, 1))
+    first, want = bank_of(p), bank_of(q)
+    plain = W4Experts(first.w13[:2], first.w2[:2], 2, 128, 64, 32, True)
+    other = bank_of(ref.parts(2, 128, 64, 32, False, device=cuda))
+    for into, takes in ((plain, False), (other, False), (first, True)):
+        was = [t.data_ptr() for t in (*into.w13, *into.w2)]
+        got = W4Experts.from_codes(*q, into=into)
+        assert ([t.data_ptr() for t in (*got.w13, *got.w2)] == was) == takes
+        assert all(torch.equal(a, b) for a, b in zip((*got.w13, *got.w2), (*want.w13, *want.w2)))
