@@ -46,6 +46,15 @@ def status_word(device: torch.device) -> torch.Tensor:
     return t
 
 
+def _status_ptr(device: torch.device) -> int | None:
+    """Address of the status word for a launch; None (the kernels then report nothing) where
+    the first call on a device happens under a graph capture: a word made there would belong
+    to the graph, hold anything before a replay and be cleared by each."""
+    if device.index not in _status and torch.cuda.is_current_stream_capturing():
+        return None
+    return status_word(device).data_ptr()
+
+
 def check_status(device: torch.device | None = None, reset: bool = True) -> None:
     """Synchronise and raise ``MoEKernelError`` if any kernel on ``device``
     reported an error (then the word is cleared unless ``reset`` is False).
@@ -479,7 +488,7 @@ def block_norm(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor,
         rc = _native_lib().moe_block_norm_ex(
             x.data_ptr(), delta.data_ptr(), post.data_ptr(), pre.data_ptr(), g_ptr, kind, g_f32,
             act, residual_scale, T, H, eps, h.data_ptr(), y.data_ptr(),
-            status_word(dev).data_ptr(), _raw_stream(dev))
+            _status_ptr(dev), _raw_stream(dev))
     if rc:
         _rc(rc, "moe_block_norm")
     return h, y
@@ -705,7 +714,7 @@ def grouped_w13_swiglu_w4(a: torch.Tensor, tiles: torch.Tensor, num_tiles: torch
     with _on(dev):
         _rc(_native.load().moe_grouped_w13_swiglu_w4_ex(
             _p(a), a.shape[0], _p(index), index_div, M, _p(tiles), _p(num_tiles), max_tiles_,
-            bank.native, _p(h), _p(ws), 0 if ws is None else ws.nbytes, _p(status_word(dev)),
+            bank.native, _p(h), _p(ws), 0 if ws is None else ws.nbytes, _status_ptr(dev),
             _stream(dev)), "moe_grouped_w13_swiglu_w4_ex")
     return h
 
@@ -741,7 +750,7 @@ def grouped_w2_w4(h: torch.Tensor, tiles: torch.Tensor, num_tiles: torch.Tensor,
         _rc(_native.load().moe_grouped_w2_w4_ex(
             _p(h), M, _p(tiles), _p(num_tiles), max_tiles_, bank.native, _p(row_map),
             _p(slot_scale), _p(out), rows, _p(ws), 0 if ws is None else ws.nbytes,
-            _p(status_word(dev)), _stream(dev)), "moe_grouped_w2_w4_ex")
+            _status_ptr(dev), _stream(dev)), "moe_grouped_w2_w4_ex")
     return out
 
 
@@ -780,7 +789,7 @@ def experts_w4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, bank,
     with _on(dev):
         rc = lib.moe_w4_experts_forward(x.data_ptr(), ids_p, weights_p, T, k, num_experts, e_begin,
                                         bank.native, ws.data_ptr(), ws.nbytes, y.data_ptr(),
-                                        status_word(dev).data_ptr(), _raw_stream(dev))
+                                        _status_ptr(dev), _raw_stream(dev))
     if rc:
         _rc(rc, "moe_w4_experts_forward")
     return y
@@ -807,7 +816,7 @@ def sorted_experts_w4(sorted_x: torch.Tensor, offsets: torch.Tensor, bank,
     with _on(dev):
         rc = lib.moe_w4_sorted_forward(sorted_x.data_ptr(), M, offsets_p, bank.native,
                                        ws.data_ptr(), ws.nbytes, y.data_ptr(),
-                                       status_word(dev).data_ptr(), _raw_stream(dev))
+                                       _status_ptr(dev), _raw_stream(dev))
     if rc:
         _rc(rc, "moe_w4_sorted_forward")
     return y
@@ -843,7 +852,7 @@ def moe_layer_w4(x: torch.Tensor, router_weight: torch.Tensor, bank, top_k: int,
     with _on(dev):
         rc = lib.moe_w4_layer_forward(x.data_ptr(), router_p, bias_p, bank.native, T, top_k,
                                       1 if norm_topk_prob else 0, ws.data_ptr(), ws.nbytes,
-                                      y.data_ptr(), status_word(dev).data_ptr(), _raw_stream(dev))
+                                      y.data_ptr(), _status_ptr(dev), _raw_stream(dev))
     if rc:
         _rc(rc, "moe_w4_layer_forward")
     return y

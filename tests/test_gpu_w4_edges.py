@@ -3,6 +3,9 @@ written after a forward, rows that no expert owns, tensors in place, rows and fo
 beside one another."""
 
 import copy
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -605,3 +608,12 @@ def test_bank_into_another(cuda):
         got = W4Experts.from_codes(*q, into=into)
         assert ([t.data_ptr() for t in (*got.w13, *got.w2)] == was) == takes
         assert all(torch.equal(a, b) for a, b in zip((*got.w13, *got.w2), (*want.w13, *want.w2)))
+
+
+def test_first_call_under_a_capture(cuda):
+    """The status word does not become the graph's: it is zero before any replay, and a replay
+    does not clear what was reported."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    run = subprocess.run([sys.executable, os.path.join(here, "first_in_capture.py")],
+                         capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and run.stdout.split()[-1:] == ["ok"], run.stdout + run.stderr
