@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(256) w4_pack_fine(const W4PackArgs a, float* r
     return bits == 0 ? 0 : 10 - ilogbf(__uint_as_float(static_cast<uint32_t>(bits) << 16));
   };
   const int base = shift_of(most);
-  if (threadIdx.x == 0 && blockIdx.y == 0) r[static_cast<size_t>(a.E) * tiles * 16 + e] = ldexpf(1.0f, -base);
+  if (threadIdx.x == 0 && blockIdx.y == 0)
+    r[static_cast<size_t>(a.E) * tiles * 16 + e] = ldexpf(1.0f, -base);
   for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < tiles * 16; i += gridDim.y * blockDim.x) {
     const int tile = i >> 4, g = i & 7, half = (i >> 3) & 1;  // packed row g, or g + 8
     const int m = pair ? half : 0;

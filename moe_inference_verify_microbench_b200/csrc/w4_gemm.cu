@@ -505,9 +505,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int j = 32 * quarter + lane;
         const int tile = u.m * kTcTiles + (SWIGLU ? j >> 3 : 8 * op + (j >> 4));
         const int row = SWIGLU ? 8 * op + (j & 7) : j & 15;
-        own[op] = tile < a.m.tiles
-                      ? __ldg(a.row_factor + (static_cast<size_t>(u.t.x) * a.m.tiles + tile) * 16 + row)
-                      : 1.0f;
+        const size_t et = static_cast<size_t>(u.t.x) * a.m.tiles + tile;
+        own[op] = tile < a.m.tiles ? __ldg(a.row_factor + et * 16 + row) : 1.0f;
         if (far) own[op] *= base;
       }
       const bool rescale = __any_sync(0xffffffffu, own[0] != 1.0f || own[1] != 1.0f);
@@ -841,11 +840,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // Rows of activations as fp16 multiples of a power of two of the row, which puts its
-// largest value into [2^14, 2^15) (if that is 2^-98 or more; the power is 2^-112 at least): a bf16 value down to 2^-31 of it stays exact, an fp32 one
-// is rounded by 2^-12 at most down to 2^-28, by 2^-39 of the largest below.  A row with an
-// infinity or a NaN keeps its values as they are.  dst may be src (fp32): a warp writes a
-// chunk of 4 KB below what it has read.  A warp for a row; HBM bounds it (6000 x 2048 bf16
-// 9 us, 49 MB).
+// largest value into [2^14, 2^15), or is 2^-112 where that value is below 2^-98.  A bf16
+// value down to 2^-31 of the largest stays exact; an fp32 one is rounded by 2^-12 at most
+// down to 2^-28 of the largest, and by 2^-39 of the largest below.  A row with an infinity
+// or a NaN keeps its values as they are.  dst may be src (fp32): a warp writes a chunk of
+// 4 KB below what it has read.  A warp for a row; HBM bounds it (6000 x 2048 bf16 9 us,
+// 49 MB).
 template <bool F32>
 __global__ void __launch_bounds__(256) w4_rows_f16(const uint8_t* src, long long src_pitch, int rows,
                                                    const int* count, int vec, uint8_t* dst,
